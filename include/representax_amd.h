@@ -575,6 +575,93 @@ int rpx_head_norm(const rpx_head_part* parts, int64_t count, const void* cosines
 int rpx_cast_many(const void* const* src, void* const* dst, const int64_t* counts, int64_t tensors,
                   void* stream);
 
+/* ---------------------------------------------------------------------------
+ * MXFP4: matrices of 4-bit e2m1 numbers with one power-of-two scale for every
+ * 32 consecutive columns of a row (OCP Microscaling Formats v1.0), and products
+ * that contract the columns of two of them. No reference counterpart: its
+ * low-bit matrices are INT4 weights and fp8 operands
+ * (src/representax/models/adapters.py:38-79, src/representax/precision.py:
+ * 127-221); this is a third choice of matrix type next to those.
+ *
+ * A block with largest magnitude a has the scale 2^e, e = max(floor(log2 a) - 2,
+ * -127) (-127 for zeros); a value is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * to |v| / 2^e, ties to the even code, with its sign. A block that holds an
+ * infinity or a NaN is NaN throughout.
+ *   codes  uint8 [rows, C / 2], C = columns rounded up to 256: column 2 j in
+ *          the low half of byte j, zeros past the end
+ *   scales uint8 [C / 256, R, 8], R = rows rounded up to 32: block b of row i
+ *          at [b / 8, i, b % 8], e + 127, or 255 for NaN
+ * Both 16-byte aligned. Products are summed in float32 and rounded once.
+ * ------------------------------------------------------------------------- */
+size_t rpx_mxfp4_code_bytes(int64_t rows, int64_t columns);
+size_t rpx_mxfp4_scale_bytes(int64_t rows, int64_t columns);
+
+/* One matrix to encode: t [rows, columns] (row_stride elements between rows,
+ * columns dense) along its columns into codes and scales, along its rows into
+ * codes_t and scales_t, which hold its transpose [columns, rows]; either pair
+ * may be NULL. code_stride and code_stride_t: bytes between rows of codes, 0
+ * for dense; multiples of 16. */
+typedef struct rpx_mxfp4_part {
+  const void* t;
+  int64_t rows, columns, row_stride;
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t code_stride;
+  uint8_t* codes_t;
+  uint8_t* scales_t;
+  int64_t code_stride_t;
+  int dtype;
+} rpx_mxfp4_part;
+
+/* Up to four matrices in one launch (a linear's input and weight). `parts` is
+ * a host array, read before the call returns. */
+int rpx_mxfp4_quantize(const rpx_mxfp4_part* parts, int64_t count, void* stream);
+
+/* out [rows, columns] = the values that the codes stand for. */
+int rpx_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                         int64_t columns, void* out, int dtype, void* stream);
+
+size_t rpx_mxfp4_gemm_workspace(int64_t m, int64_t n, int64_t k);
+
+/* out [m, n] = A B^T from a [m, k] and b [n, k]; zeros where k is 0. */
+int rpx_mxfp4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
+                   const uint8_t* b_scales, int64_t m, int64_t n, int64_t k, void* out,
+                   int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* h [m, n] = silu(A G^T) * (A U^T), both products rounded to `dtype` before the
+ * activation; z_gate and z_up receive them (both, or both NULL). */
+int rpx_mxfp4_gated_gemm(const uint8_t* a_codes, const uint8_t* a_scales,
+                         const uint8_t* gate_codes, const uint8_t* gate_scales,
+                         const uint8_t* up_codes, const uint8_t* up_scales, int64_t m, int64_t n,
+                         int64_t k, void* h, void* z_gate, void* z_up, int dtype, void* stream);
+
+/* The gradients of the gated block's two products for the gradient dh of h,
+ *   dz_gate = dh z_up silu'(z_gate),  dz_up = dh silu(z_gate)    (all [m, n]),
+ * encoded for the two products that take them; they are not stored otherwise.
+ *   codes, scales      [m, 2 N], N = n rounded up to 256: dz_gate in columns
+ *                      [0, n), dz_up in columns [N, N + n); for dx, against
+ *                      [G^T | U^T] with the same columns
+ *   codes_t, scales_t  [2 n, m]: dz_gate's transpose over dz_up's; for the two
+ *                      weight gradients, against x^T
+ * Either pair may be NULL. */
+int rpx_mxfp4_gated_backward(const void* dh, const void* z_gate, const void* z_up, int dtype,
+                             int64_t m, int64_t n, uint8_t* codes, uint8_t* scales,
+                             uint8_t* codes_t, uint8_t* scales_t, void* stream);
+
+/* y [m, n] = x W^T with x [m, k] encoded within the call (inference over a
+ * kept weight); row_stride elements between rows of x. */
+size_t rpx_mxfp4_linear_workspace(int64_t m, int64_t n, int64_t k);
+int rpx_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t k, int64_t row_stride,
+                     const uint8_t* codes, const uint8_t* scales, int64_t n, void* y,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* h [m, n] = silu(x G^T) * (x U^T), x encoded within the call. */
+size_t rpx_mxfp4_gated_workspace(int64_t m, int64_t n, int64_t k);
+int rpx_mxfp4_gated(const void* x, int dtype, int64_t m, int64_t k, int64_t row_stride,
+                    const uint8_t* gate_codes, const uint8_t* gate_scales,
+                    const uint8_t* up_codes, const uint8_t* up_scales, int64_t n, void* h,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,9 +16,17 @@ from .adapters import (
     matched_linear_paths,
     merge_quantized_lora,
 )
-from .components import Linear
+from .components import Linear, MXFP4Linear
 from .config import PrecisionConfig, QuantizedLoRAConfig
 from .mlp import gelu_mlp, shared_input_projections, swiglu_mlp
+from .mxfp4 import (
+    MXFP4Matrix,
+    mxfp4_gated,
+    mxfp4_linear,
+    mxfp4_matmul,
+    mxfp4_quantize,
+    mxfp4_quantize_both,
+)
 from .precision import (
     FP32_POLICY,
     DelayedScaling,
@@ -27,6 +35,7 @@ from .precision import (
     active_compute_dtype,
     active_model_for_compute,
     compute_parameter,
+    gated_matmul,
     linear_matmul,
     model_for_compute,
     precision_context,
@@ -38,6 +47,8 @@ __all__ = [
     "DelayedScaling",
     "FP32_POLICY",
     "Linear",
+    "MXFP4Linear",
+    "MXFP4Matrix",
     "PrecisionConfig",
     "PrecisionPolicy",
     "QuantizedLoRAConfig",
@@ -49,6 +60,7 @@ __all__ = [
     "apply_quantized_lora",
     "compute_parameter",
     "constrain_activation",
+    "gated_matmul",
     "gelu_mlp",
     "linear_matmul",
     "lora_parameter_filter",
@@ -56,6 +68,11 @@ __all__ = [
     "matched_linear_paths",
     "merge_quantized_lora",
     "model_for_compute",
+    "mxfp4_gated",
+    "mxfp4_linear",
+    "mxfp4_matmul",
+    "mxfp4_quantize",
+    "mxfp4_quantize_both",
     "precision_context",
     "replicate",
     "resolve_precision_policy",

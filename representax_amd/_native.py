@@ -144,6 +144,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rpx_cast_many": (_int, [_p, _p, _p, _i64, _p]),
     "rpx_norm_forward": (_int, [_p, _p, _p, _p, _int, _i64, _i64, _f32, _int, _p, _p, _p]),
     "rpx_norm_backward": (_int, [_p, _p, _p, _p, _int, _i64, _i64, _f32, _int, _p, _p]),
+    "rpx_mxfp4_code_bytes": (_size, [_i64, _i64]),
+    "rpx_mxfp4_scale_bytes": (_size, [_i64, _i64]),
+    "rpx_mxfp4_quantize": (_int, [_p, _i64, _p]),
+    "rpx_mxfp4_dequantize": (_int, [_p, _p, _i64, _i64, _p, _int, _p]),
+    "rpx_mxfp4_gemm_workspace": (_size, [_i64, _i64, _i64]),
+    "rpx_mxfp4_gemm": (
+        _int, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _int, _p, _size, _p]
+    ),
+    "rpx_mxfp4_gated_gemm": (
+        _int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _int, _p]
+    ),
+    "rpx_mxfp4_gated_backward": (
+        _int, [_p, _p, _p, _int, _i64, _i64, _p, _p, _p, _p, _p]
+    ),
+    "rpx_mxfp4_linear_workspace": (_size, [_i64, _i64, _i64]),
+    "rpx_mxfp4_linear": (
+        _int, [_p, _int, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _size, _p]
+    ),
+    "rpx_mxfp4_gated_workspace": (_size, [_i64, _i64, _i64]),
+    "rpx_mxfp4_gated": (
+        _int, [_p, _int, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p, _size, _p]
+    ),
     "rpx_head_norm": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _int, _p]),
 }
 
@@ -155,6 +177,24 @@ class HeadPart(ctypes.Structure):
     _fields_ += [(name, ctypes.c_int64)
                  for name in ("stride_b", "stride_s", "stride_h", "heads", "repeat")]
     _fields_ += [("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
+class Mxfp4Part(ctypes.Structure):
+    """``rpx_mxfp4_part`` of include/representax_amd.h."""
+
+    _fields_ = [
+        ("t", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("columns", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("code_stride", ctypes.c_int64),
+        ("codes_t", ctypes.c_void_p),
+        ("scales_t", ctypes.c_void_p),
+        ("code_stride_t", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+    ]
 
 
 class Int4LoraProjection(ctypes.Structure):

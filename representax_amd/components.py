@@ -1,10 +1,12 @@
 """The native projection that the adapter replaces
-(mirror of src/representax/models/components.py:58-94)."""
+(mirror of src/representax/models/components.py:58-94), and its form with a kept
+4-bit weight for inference."""
 
 from __future__ import annotations
 
 import torch
 
+from .mxfp4 import MXFP4Matrix, mxfp4_linear, mxfp4_quantize
 from .precision import activation_inputs, compute_parameter, linear_matmul
 
 
@@ -60,4 +62,51 @@ class Linear(torch.nn.Module):
         return output
 
 
-__all__ = ["Linear"]
+class MXFP4Linear(torch.nn.Module):
+    """A frozen projection ``y = x W^T (+ b)`` whose weight is kept in MXFP4 (0.53 bytes
+    a value), for inference (an extension): the input is cast to the activation dtype
+    and encoded within the call, so the result is that of a ``Linear`` under
+    ``PrecisionConfig.mxfp4_mixed()`` without encoding the weight on every call."""
+
+    def __init__(self, weight: MXFP4Matrix, bias: torch.Tensor | None = None) -> None:
+        super().__init__()
+        if bias is not None and tuple(bias.shape) != (weight.rows,):
+            raise ValueError(f"bias: shape {tuple(bias.shape)}, expected {(weight.rows,)}")
+        self.input_size = weight.columns
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_linear(cls, linear: Linear) -> "MXFP4Linear":
+        """Encodes the compute view of a native ``Linear``'s weight ``[N, K]``."""
+
+        weight = compute_parameter(linear.weight.detach())
+        bias = None if linear.bias is None else linear.bias.detach().clone()
+        return cls(mxfp4_quantize(weight), bias)
+
+    @property
+    def output_size(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def weight(self) -> MXFP4Matrix:
+        return MXFP4Matrix(self.codes, self.scales, self.input_size)
+
+    def inputs(self, value: torch.Tensor) -> torch.Tensor:
+        """``value`` as rows in the activation dtype."""
+
+        value = activation_inputs(value)
+        if torch.is_grad_enabled() and value.requires_grad:
+            raise RuntimeError("MXFP4Linear gives no gradients (its weight is kept for "
+                               "inference); train a Linear under PrecisionConfig.mxfp4_mixed()")
+        return value.reshape(-1, self.input_size)
+
+    def forward(self, value: torch.Tensor) -> torch.Tensor:
+        y = mxfp4_linear(self.inputs(value), self.weight)
+        if self.bias is not None:
+            y = y + compute_parameter(self.bias).to(y.dtype)
+        return y.reshape(*value.shape[:-1], self.output_size)
+
+
+__all__ = ["Linear", "MXFP4Linear"]

@@ -9,7 +9,7 @@ from typing import Literal
 from pydantic import BaseModel, ConfigDict, Field, PositiveFloat, PositiveInt, field_validator
 
 PrecisionDType = Literal["float32", "bfloat16"]
-MatrixDType = Literal["float32", "bfloat16", "float8_e4m3fn"]
+MatrixDType = Literal["float32", "bfloat16", "float8_e4m3fn", "float4_e2m1fn"]
 
 
 class FrozenConfig(BaseModel):
@@ -45,6 +45,15 @@ class PrecisionConfig(FrozenConfig):
         return cls(compute_dtype="bfloat16", activation_dtype="bfloat16",
                    matrix_dtype="float8_e4m3fn", fp8_scaling=fp8_scaling,
                    amax_history_len=amax_history_len)
+
+    @classmethod
+    def mxfp4_mixed(cls) -> "PrecisionConfig":
+        """MXFP4 matrices with bf16 everything else (an extension): every ``Linear``
+        product, gradients included, over 4-bit operands with a scale per 32 values.
+        INT4 + LoRA linears, whose weights have four bits already, run as under bf16."""
+
+        return cls(compute_dtype="bfloat16", activation_dtype="bfloat16",
+                   matrix_dtype="float4_e2m1fn")
 
     @property
     def resolved_matrix_dtype(self) -> MatrixDType:

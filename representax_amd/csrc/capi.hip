@@ -12,6 +12,7 @@
 #include "../../include/representax_amd.h"
 #include "common.h"
 #include "act.h"
+#include "capi.h"
 #include "kernels.h"
 #include "tuning.h"
 
@@ -19,45 +20,6 @@ namespace rpx {
 
 namespace {
 thread_local std::string g_last_error;
-
-// Bump allocator over a caller-provided workspace.
-struct Arena {
-  uint8_t* base;
-  size_t cap;
-  size_t used = 0;
-  bool overflow = false;
-  Arena(void* p, size_t c) : base(static_cast<uint8_t*>(p)), cap(c) {}
-  template <typename T>
-  T* take(int64_t count) {
-    const size_t bytes = (static_cast<size_t>(count) * sizeof(T) + 255) & ~static_cast<size_t>(255);
-    if (used + bytes > cap) {
-      overflow = true;
-      return nullptr;
-    }
-    T* p = reinterpret_cast<T*>(base + used);
-    used += bytes;
-    return p;
-  }
-};
-
-// Size-only twin of Arena.
-struct Sizer {
-  size_t used = 0;
-  template <typename T>
-  void take(int64_t count) {
-    used += (static_cast<size_t>(count) * sizeof(T) + 255) & ~static_cast<size_t>(255);
-  }
-};
-
-size_t elem_size(int dtype) { return dtype == kBF16 ? 2 : 4; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// Every non-null pointer 16-byte aligned.
-bool aligned16_all(std::initializer_list<const void*> ps) {
-  for (const void* p : ps)
-    if (p != nullptr && !aligned16(p)) return false;
-  return true;
-}
-bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 
 float round_to_dtype(float v, int dtype) {
   if (dtype != kBF16) return v;
@@ -84,23 +46,10 @@ int check_int4_shape(int64_t n, int64_t k, int64_t group_size, int64_t* n_groups
   return kOk;
 }
 
-int check_dtype(int dtype) {
-  if (dtype != kF32 && dtype != kBF16) return fail_invalid("dtype must be RPX_DTYPE_F32 or RPX_DTYPE_BF16");
-  return kOk;
-}
-
 int check_fmt(int fmt) {
   if (fmt != kE4M3FN && fmt != kE5M2) return fail_invalid("fp8 format must be RPX_FP8_E4M3FN or RPX_FP8_E5M2");
   return kOk;
 }
-
-#define RPX_TRY(expr)            \
-  do {                           \
-    const int _rc = (expr);      \
-    if (_rc != kOk) return _rc;  \
-  } while (0)
-
-#define RPX_HIP(expr, what) RPX_TRY(check_hip((expr), (what)))
 
 // --- INT4 + LoRA path selection -------------------------------------------
 bool lora_fast_shape(int dtype, int64_t k, int64_t n_groups, int64_t group, int64_t rank) {

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.h"
+#include "mxfp4.h"
 
 namespace rpx {
 
@@ -333,5 +334,36 @@ struct CastMany {
   int64_t first[kCastMany + 1];
 };
 hipError_t launch_cast_many(CastMany args, int tensors, hipStream_t stream);
+
+// MXFP4 (mxfp4.h) -----------------------------------------------------------
+constexpr int kMxParts = 8;  // encodings of one launch
+struct MxPart {
+  const void* t;
+  int dtype;
+  int64_t rows, columns, row_stride, column_stride;  // in elements
+  MxOut out;
+};
+struct MxParts {
+  MxPart part[kMxParts];
+  int64_t first[kMxParts + 1];  // part p has workgroups first[p] .. first[p + 1] - 1
+};
+// Zeros (a product over no columns); `bytes` even.
+hipError_t launch_mx_zero(void* out, int64_t bytes, hipStream_t stream);
+hipError_t launch_mx_quantize(MxParts parts, int count, hipStream_t stream);
+hipError_t launch_mx_gated_backward(const void* dh, const void* z_gate, const void* z_up, int dtype,
+                                    int64_t m, int64_t n, MxOut along, MxOut stacked,
+                                    hipStream_t stream);
+hipError_t launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                int64_t columns, void* out, int dtype, hipStream_t stream);
+// out [m, n] = A B^T over `slices` slices; with b2, out = silu(A B^T) * (A B2^T)
+// and z_gate, z_up (or null) the two products as rounded to dtype.
+struct MxGemm {
+  const uint8_t *a_codes, *a_scales, *b_codes, *b_scales, *b2_codes, *b2_scales;
+  int64_t m, n, slices;
+  void *out, *z_gate, *z_up;
+  int dtype;
+};
+int64_t mx_gemm_workspace_floats(int64_t m, int64_t n, int64_t slices);
+hipError_t launch_mx_gemm(const MxGemm& p, float* partials, hipStream_t stream);
 
 }  // namespace rpx

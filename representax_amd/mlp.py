@@ -11,6 +11,10 @@ float32 on the projections' bf16 outputs and is rounded once to bf16, the
 reading in which XLA evaluates a fused elementwise chain with its default
 excess precision. Under the fp8 policy, or with another compute dtype, the
 blocks are composed from the separate projections.
+
+``swiglu_mlp`` over native ``Linear`` projections under the MXFP4 policy, or over
+kept ``MXFP4Linear`` weights, runs both input projections, the activation and the
+product in one kernel (``gated_matmul``, ``mxfp4_gated``).
 """
 
 from __future__ import annotations
@@ -20,8 +24,10 @@ import torch.nn.functional as F
 
 from . import ops
 from .adapters import QuantizedLoRALinear
+from .components import Linear, MXFP4Linear
+from .mxfp4 import mxfp4_gated
 from .precision import (activation_inputs, active_compute_dtype, active_policy,
-                        compute_operands, compute_parameter_dtype)
+                        compute_operands, compute_parameter, compute_parameter_dtype, gated_matmul)
 
 
 def _fusable(value: torch.Tensor, *linears: QuantizedLoRALinear) -> bool:
@@ -58,12 +64,32 @@ def gelu_mlp(value: torch.Tensor, up: torch.nn.Module, down: torch.nn.Module) ->
     return y.reshape(*lead, down.output_size)
 
 
+def _gated(value: torch.Tensor, gate: torch.nn.Module, up: torch.nn.Module):
+    """``silu(gate(value)) * up(value)`` in one kernel where gate and up are MXFP4
+    projections without biases; None otherwise."""
+
+    kept = isinstance(gate, MXFP4Linear) and isinstance(up, MXFP4Linear)
+    native = (isinstance(gate, Linear) and isinstance(up, Linear) and gate.weight.ndim == 2
+              and up.weight.ndim == 2)
+    if not (kept or native) or gate.bias is not None or up.bias is not None:
+        return None
+    if kept:
+        h = mxfp4_gated(gate.inputs(value), gate.weight, up.weight)
+        return h.reshape(*value.shape[:-1], gate.output_size)
+    policy = active_policy()
+    if policy is None or policy.matrix_dtype != torch.float4_e2m1fn_x2:
+        return None
+    return gated_matmul(activation_inputs(value), compute_parameter(gate.weight).transpose(-1, -2),
+                        compute_parameter(up.weight).transpose(-1, -2))
+
+
 def swiglu_mlp(value: torch.Tensor, gate: torch.nn.Module, up: torch.nn.Module,
                down: torch.nn.Module) -> torch.Tensor:
     """``down(silu(gate(value)) * up(value))``."""
 
     if not _fusable(value, gate, up, down):
-        return down(F.silu(gate(value)) * up(value))
+        hidden = _gated(value, gate, up)
+        return down(F.silu(gate(value)) * up(value) if hidden is None else hidden)
     x = activation_inputs(value).to(torch.bfloat16)
     lead = x.shape[:-1]
     y = ops.Int4LoRASwiGLUMLPFn.apply(x.reshape(-1, up.input_size), *_adapters(gate, up, down),

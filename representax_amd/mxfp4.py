@@ -1,0 +1,423 @@
+"""MXFP4: matrices of 4-bit floating-point numbers with one power-of-two scale
+for every 32 consecutive columns of a row, products that contract the columns of
+two of them, and the first half of a gated feed-forward block over them.
+
+An extension next to the reference's INT4 weights and fp8 operands
+(src/representax/models/adapters.py:38-79, src/representax/precision.py:127-221):
+a third choice of matrix type, which gfx950's matrix cores multiply at twice the
+rate of fp8. The format is that of the OCP Microscaling Formats specification
+v1.0 (e2m1 numbers, e8m0 scales); ``include/representax_amd.h`` states it.
+
+* ``mxfp4_quantize``, ``mxfp4_quantize_both``, ``MXFP4Matrix.dequantize``: to the
+  format, along a matrix's columns or along both of its axes in one pass, and back.
+* ``mxfp4_matmul``: ``a b^T`` of two encoded matrices.
+* ``mxfp4_linear``, ``mxfp4_gated``: inference over kept weights, the input
+  encoded within the call; ``components.MXFP4Linear`` is the module that keeps one.
+* ``MXFP4LinearFn``, ``MXFP4GatedFn``: the autograd nodes that ``linear_matmul`` and
+  ``gated_matmul`` take under ``PrecisionConfig.mxfp4_mixed()``. Each of a linear's
+  three products has both of its operands encoded along the axis that it contracts:
+  ``y = x W^T`` along the inputs, ``dx = dy W`` along the outputs, ``dW = dy^T x``
+  along the tokens. The forward encodes its operands along both axes in one pass and
+  keeps the codes (about half a byte per value) in place of the values.
+
+A block that holds an infinity or a NaN stands for NaN throughout, so overflow
+stays visible. Empty operands follow a product's own rules: no rows give no rows,
+and a sum over nothing is zero.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+from .ops import BF16, F32, _aligned, _dtype_code, _on_device, _ptr, _stream, _workspace
+
+SLICE = 256  # columns are padded to this
+ROW_PAD = 32  # the scales' rows are padded to this
+
+
+def _slices(columns: int) -> int:
+    return -(-columns // SLICE)
+
+
+def _pad_rows(rows: int) -> int:
+    return -(-rows // ROW_PAD) * ROW_PAD
+
+
+def _scales_shape(rows: int, columns: int) -> tuple[int, int, int]:
+    return (_slices(columns), _pad_rows(rows), 8)
+
+
+class MXFP4Matrix:
+    """An encoded matrix ``[rows, columns]``: ``codes`` uint8 ``[rows, C / 2]`` and
+    ``scales`` uint8 ``[C / 256, R, 8]`` (C and R the columns and rows rounded up to
+    256 and 32), both dense and 16-byte aligned on one device."""
+
+    __slots__ = ("codes", "scales", "columns")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int) -> None:
+        columns = int(columns)
+        cs = codes.shape
+        if codes.dtype != torch.uint8 or len(cs) != 2 or cs[1] != _slices(columns) * (SLICE // 2):
+            raise ValueError(f"MXFP4 codes must be uint8 [rows, {_slices(columns) * (SLICE // 2)}] "
+                             f"for {columns} columns, got {codes.dtype} {tuple(cs)}")
+        if scales.dtype != torch.uint8 or scales.shape != _scales_shape(cs[0], columns):
+            raise ValueError(f"MXFP4 scales must be uint8 {_scales_shape(cs[0], columns)}, got "
+                             f"{scales.dtype} {tuple(scales.shape)}")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("MXFP4 codes and scales must be dense")
+        self.codes = codes
+        self.scales = scales
+        self.columns = columns
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return (self.codes.shape[0], self.columns)
+
+    @classmethod
+    def empty(cls, rows: int, columns: int, device: torch.device) -> "MXFP4Matrix":
+        """Room for an encoded matrix, contents undefined."""
+
+        return cls(torch.empty((rows, _slices(columns) * (SLICE // 2)), dtype=torch.uint8,
+                               device=device),
+                   torch.empty(_scales_shape(rows, columns), dtype=torch.uint8, device=device),
+                   columns)
+
+    def dequantize(self, dtype: torch.dtype = BF16) -> torch.Tensor:
+        """The values that the codes stand for (exact in bf16 and float32)."""
+
+        device = _on_device(self.codes, self.scales)
+        out = torch.empty(self.shape, dtype=dtype, device=device)
+        with _launches_on(device):
+            nat.call("rpx_mxfp4_dequantize", _ptr(self.codes), _ptr(self.scales), *self.shape,
+                     _ptr(out), _dtype_code(dtype), _stream(device))
+        return out
+
+    def __repr__(self) -> str:
+        return f"MXFP4Matrix({self.rows} x {self.columns}, {self.codes.device})"
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _launches_on(device: torch.device):
+    """Context in which launches go to ``device`` (they go to the current one)."""
+
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def _matrix_input(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
+    if t.dtype not in (BF16, F32):
+        raise TypeError(f"{what}: unsupported dtype {t.dtype}; expected float32 or bfloat16")
+    return t
+
+
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    """t with its columns dense and its rows apart (any row stride)."""
+
+    rows, columns = t.shape
+    if (t.stride(1) == 1 or columns == 1) and (t.stride(0) >= columns or rows <= 1):
+        return t
+    return t.contiguous()
+
+
+def _part(t, along: MXFP4Matrix | None, across: MXFP4Matrix | None):
+    """One matrix to encode, as the library takes it (``across``: its transpose)."""
+
+    rows, columns = t.shape
+    return nat.Mxfp4Part(_ptr(t), rows, columns, max(t.stride(0), columns),
+                         _ptr(along.codes) if along else None,
+                         _ptr(along.scales) if along else None, 0,
+                         _ptr(across.codes) if across else None,
+                         _ptr(across.scales) if across else None, 0, _dtype_code(t.dtype))
+
+
+def _encode(parts, device: torch.device) -> None:
+    count = len(parts)
+    with _launches_on(device):
+        nat.call("rpx_mxfp4_quantize", (nat.Mxfp4Part * count)(*parts), count, _stream(device))
+
+
+def mxfp4_quantize(t: torch.Tensor) -> MXFP4Matrix:
+    """``t [rows, columns]`` (bf16 or float32) encoded along its columns."""
+
+    device = _on_device(_matrix_input(t, "MXFP4 operand"))
+    if t.stride(0) == 1 and t.stride(1) > 1:  # a transpose: encode along its own rows
+        base = _dense_rows(t.t())
+        out = MXFP4Matrix.empty(*t.shape, device)
+        _encode([_part(base, None, out)], device)
+        return out
+    t = _dense_rows(t)
+    out = MXFP4Matrix.empty(*t.shape, device)
+    _encode([_part(t, out, None)], device)
+    return out
+
+
+def mxfp4_quantize_both(t: torch.Tensor) -> tuple[MXFP4Matrix, MXFP4Matrix]:
+    """``t`` encoded along its columns, and its transpose encoded along its own (the
+    rows of ``t``), from one pass over ``t``: the operands of the two products that
+    contract one axis of ``t`` each."""
+
+    device = _on_device(_matrix_input(t, "MXFP4 operand"))
+    if t.stride(0) == 1 and t.stride(1) > 1:
+        across, along = mxfp4_quantize_both(t.t())
+        return along, across
+    t = _dense_rows(t)
+    along = MXFP4Matrix.empty(*t.shape, device)
+    across = MXFP4Matrix.empty(t.shape[1], t.shape[0], device)
+    _encode([_part(t, along, across)], device)
+    return along, across
+
+
+def _gemm(a: MXFP4Matrix, b: MXFP4Matrix, out_dtype: torch.dtype, device) -> torch.Tensor:
+    m, n, k = a.rows, b.rows, a.columns
+    out = torch.empty((m, n), dtype=out_dtype, device=device)
+    ws = _workspace(nat.query("rpx_mxfp4_gemm_workspace", m, n, k), device)
+    nat.call("rpx_mxfp4_gemm", _ptr(a.codes), _ptr(a.scales), _ptr(b.codes), _ptr(b.scales), m, n,
+             k, _ptr(out), _dtype_code(out_dtype), _ptr(ws), ws.numel(), _stream(device))
+    return out
+
+
+def _check_contraction(a: MXFP4Matrix, b: MXFP4Matrix) -> None:
+    if a.columns != b.columns:
+        raise ValueError(f"MXFP4 product needs a [M, K] and b [N, K]; got {a.shape} and {b.shape}")
+
+
+def mxfp4_matmul(a: MXFP4Matrix, b: MXFP4Matrix, out_dtype: torch.dtype = BF16) -> torch.Tensor:
+    """``a [M, K] b^T [K, N]``, summed in float32 and rounded once."""
+
+    _check_contraction(a, b)
+    device = _on_device(a.codes, a.scales, b.codes, b.scales)
+    with _launches_on(device):
+        return _gemm(a, b, out_dtype, device)
+
+
+def _check_serving(x2d: torch.Tensor, *weights: MXFP4Matrix):
+    _matrix_input(x2d, "x")
+    for w in weights:
+        if w.columns != x2d.shape[1]:
+            raise ValueError(f"x has {x2d.shape[1]} columns, the MXFP4 weight {w.columns}")
+        if w.rows != weights[0].rows:
+            raise ValueError(f"gate and up must have the same rows, got {weights[0].rows} and "
+                             f"{w.rows}")
+    device = _on_device(x2d, *[t for w in weights for t in (w.codes, w.scales)])
+    return device, _dense_rows(x2d)
+
+
+def mxfp4_linear(x2d: torch.Tensor, weight: MXFP4Matrix) -> torch.Tensor:
+    """``x [M, K] W^T`` in x's dtype, ``weight`` the encoded ``W [N, K]``; x is encoded
+    within the call. Inference: no gradients."""
+
+    device, x2d = _check_serving(x2d, weight)
+    m, k = x2d.shape
+    n = weight.rows
+    y = torch.empty((m, n), dtype=x2d.dtype, device=device)
+    ws = _workspace(nat.query("rpx_mxfp4_linear_workspace", m, n, k), device)
+    with _launches_on(device):
+        nat.call("rpx_mxfp4_linear", _ptr(x2d), _dtype_code(x2d.dtype), m, k,
+                 max(x2d.stride(0), k), _ptr(weight.codes), _ptr(weight.scales), n, _ptr(y),
+                 _ptr(ws), ws.numel(), _stream(device))
+    return y
+
+
+def mxfp4_gated(x2d: torch.Tensor, gate: MXFP4Matrix, up: MXFP4Matrix) -> torch.Tensor:
+    """``silu(x G^T) * (x U^T)`` in x's dtype over two kept weights, in one pass over x;
+    both products are rounded to x's dtype before the activation. Inference."""
+
+    device, x2d = _check_serving(x2d, gate, up)
+    m, k = x2d.shape
+    n = gate.rows
+    h = torch.empty((m, n), dtype=x2d.dtype, device=device)
+    ws = _workspace(nat.query("rpx_mxfp4_gated_workspace", m, n, k), device)
+    with _launches_on(device):
+        nat.call("rpx_mxfp4_gated", _ptr(x2d), _dtype_code(x2d.dtype), m, k,
+                 max(x2d.stride(0), k), _ptr(gate.codes), _ptr(gate.scales), _ptr(up.codes),
+                 _ptr(up.scales), n, _ptr(h), _ptr(ws), ws.numel(), _stream(device))
+    return h
+
+
+# ---------------------------------------------------------------------------
+# autograd nodes
+# ---------------------------------------------------------------------------
+def _check_product(left: torch.Tensor, right: torch.Tensor, what: str) -> None:
+    _matrix_input(left, f"{what}: left")
+    _matrix_input(right, f"{what}: right")
+    if left.shape[1] != right.shape[0]:
+        raise ValueError(f"{what} needs left [M, K] and right [K, N]; got {tuple(left.shape)} "
+                         f"and {tuple(right.shape)}")
+
+
+def _weight_part(right: torch.Tensor, rows: MXFP4Matrix, across: MXFP4Matrix | None):
+    """The part that encodes ``right [K, N]`` along K into ``rows [N, K]`` and, where
+    given, along N into ``across [K, N]``, whichever way ``right`` lies in memory."""
+
+    if right.stride(0) == 1 and right.stride(1) >= right.shape[0]:
+        w = _dense_rows(right.t())
+        return w, _part(w, rows, across)
+    w = _dense_rows(right)
+    return w, _part(w, across, rows)
+
+
+class MXFP4LinearFn(torch.autograd.Function):
+    """``left [M, K] @ right [K, N]`` on MXFP4 operands, gradients included (see the
+    module's docstring). Gradients come in the operands' dtypes."""
+
+    @staticmethod
+    def forward(ctx, left, right, out_dtype):
+        _check_product(left, right, "MXFP4 linear")
+        device = _on_device(left, right)
+        m, k = left.shape
+        n = right.shape[1]
+        need_left, need_right = ctx.needs_input_grad[:2]
+        x = _dense_rows(left)
+        xq = MXFP4Matrix.empty(m, k, device)
+        xt = MXFP4Matrix.empty(k, m, device) if need_right else None
+        wq = MXFP4Matrix.empty(n, k, device)
+        wt = MXFP4Matrix.empty(k, n, device) if need_left else None
+        w, weight = _weight_part(right, wq, wt)
+        _encode([_part(x, xq, xt), weight], device)
+        with _launches_on(device):
+            out = _gemm(xq, wq, out_dtype, device)
+        if need_left or need_right:
+            ctx.save_for_backward(*[t for q in (xt, wt) if q is not None
+                                    for t in (q.codes, q.scales)])
+            ctx.cfg = (m, k, n, left.dtype, right.dtype)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        m, k, n, left_dtype, right_dtype = ctx.cfg
+        need_left, need_right = ctx.needs_input_grad[:2]
+        saved = list(ctx.saved_tensors)
+        device = grad.device
+        g = _dense_rows(grad)
+        gq = MXFP4Matrix.empty(m, n, device) if need_left else None
+        gt = MXFP4Matrix.empty(n, m, device) if need_right else None
+        _encode([_part(g, gq, gt)], device)
+        d_left = d_right = None
+        with _launches_on(device):
+            if need_right:
+                xt = MXFP4Matrix(saved.pop(0), saved.pop(0), m)
+                d_right = _gemm(gt, xt, right_dtype, device).t()
+            if need_left:
+                wt = MXFP4Matrix(saved.pop(0), saved.pop(0), n)
+                d_left = _gemm(gq, wt, left_dtype, device)
+        return d_left, d_right, None
+
+
+class MXFP4GatedFn(torch.autograd.Function):
+    """``silu(left @ gate) * (left @ up)``, ``left [M, K]``, ``gate`` and ``up [K, N]``:
+    both projections, the activation and the product in one kernel; the backward's
+    ``dx`` is one product over both projections' outputs, the two weight gradients
+    another. The projections are rounded to ``out_dtype`` before the activation, as
+    separate linears would leave them."""
+
+    @staticmethod
+    def forward(ctx, left, gate, up, out_dtype):
+        _check_product(left, gate, "MXFP4 gated block")
+        _check_product(left, up, "MXFP4 gated block")
+        if gate.shape != up.shape:
+            raise ValueError(f"gate and up must have one shape, got {tuple(gate.shape)} and "
+                             f"{tuple(up.shape)}")
+        device = _on_device(left, gate, up)
+        m, k = left.shape
+        n = gate.shape[1]
+        need_x, need_g, need_u = ctx.needs_input_grad[:3]
+        need_w = need_g or need_u
+        x = _dense_rows(left)
+        xq = MXFP4Matrix.empty(m, k, device)
+        xt = MXFP4Matrix.empty(k, m, device) if need_w else None
+        wide = _slices(n) * SLICE  # one projection's columns in the joint transpose
+        both = MXFP4Matrix.empty(k, 2 * wide, device) if need_x else None
+        weights, parts = [], [_part(x, xq, xt)]
+        for i, right in enumerate((gate, up)):
+            wq = MXFP4Matrix.empty(n, k, device)
+            w, part = _weight_part(right, wq, None)
+            if need_x:
+                codes = both.codes.data_ptr() + i * (wide // 2)
+                scales = both.scales.data_ptr() + i * _slices(n) * _pad_rows(k) * 8
+                if part.codes is not None:  # w is [N, K]: its transpose goes to the joint matrix
+                    part.codes_t, part.scales_t, part.code_stride_t = codes, scales, wide
+                else:
+                    part.codes, part.scales, part.code_stride = codes, scales, wide
+            weights.append(wq)
+            parts.append(part)
+            x = (x, w)  # keeps any copy alive until the launch
+        _encode(parts, device)
+        h = torch.empty((m, n), dtype=out_dtype, device=device)
+        z = [torch.empty((m, n), dtype=out_dtype, device=device) for _ in range(2)] \
+            if need_x or need_w else [None, None]
+        with _launches_on(device):
+            nat.call("rpx_mxfp4_gated_gemm", _ptr(xq.codes), _ptr(xq.scales),
+                     _ptr(weights[0].codes), _ptr(weights[0].scales), _ptr(weights[1].codes),
+                     _ptr(weights[1].scales), m, n, k, _ptr(h), _ptr(z[0]), _ptr(z[1]),
+                     _dtype_code(out_dtype), _stream(device))
+        if need_x or need_w:
+            ctx.save_for_backward(*z, *[t for q in (xt, both) if q is not None
+                                       for t in (q.codes, q.scales)])
+            ctx.cfg = (m, k, n, left.dtype, gate.dtype, up.dtype)
+        return h
+
+    @staticmethod
+    def backward(ctx, grad):
+        m, k, n, left_dtype, gate_dtype, up_dtype = ctx.cfg
+        need_x, need_g, need_u = ctx.needs_input_grad[:3]
+        need_w = need_g or need_u
+        z_gate, z_up, *saved = ctx.saved_tensors
+        device = grad.device
+        dh = _aligned(grad.to(z_gate.dtype))
+        wide = _slices(n) * SLICE
+        dz = MXFP4Matrix.empty(m, 2 * wide, device) if need_x else None
+        dzt = MXFP4Matrix.empty(2 * n, m, device) if need_w else None
+        d_x = d_gate = d_up = None
+        with _launches_on(device):
+            nat.call("rpx_mxfp4_gated_backward", _ptr(dh), _ptr(z_gate), _ptr(z_up),
+                     _dtype_code(dh.dtype), m, n, _ptr(dz.codes) if dz else None,
+                     _ptr(dz.scales) if dz else None, _ptr(dzt.codes) if dzt else None,
+                     _ptr(dzt.scales) if dzt else None, _stream(device))
+            if need_w:
+                xt = MXFP4Matrix(saved.pop(0), saved.pop(0), m)
+                wide_dtype = gate_dtype if gate_dtype == up_dtype else F32
+                d_w = _gemm(dzt, xt, wide_dtype, device)
+                d_gate = d_w[:n].to(gate_dtype).t() if need_g else None
+                d_up = d_w[n:].to(up_dtype).t() if need_u else None
+            if need_x:
+                both = MXFP4Matrix(saved.pop(0), saved.pop(0), 2 * wide)
+                d_x = _gemm(dz, both, left_dtype, device)
+        return d_x, d_gate, d_up, None
+
+
+def linear_product(left, right, out_dtype: torch.dtype) -> torch.Tensor:
+    """``MXFP4LinearFn``, without what only a backward reads where none will run."""
+
+    if not torch.is_grad_enabled():
+        left, right = left.detach(), right.detach()
+    return MXFP4LinearFn.apply(left, right, out_dtype)
+
+
+def gated_product(left, gate, up, out_dtype: torch.dtype) -> torch.Tensor:
+    """``MXFP4GatedFn``, without what only a backward reads where none will run."""
+
+    if not torch.is_grad_enabled():
+        left, gate, up = left.detach(), gate.detach(), up.detach()
+    return MXFP4GatedFn.apply(left, gate, up, out_dtype)
+
+
+__all__ = ["MXFP4GatedFn", "MXFP4LinearFn", "MXFP4Matrix", "gated_product", "linear_product",
+           "mxfp4_gated", "mxfp4_linear", "mxfp4_matmul", "mxfp4_quantize", "mxfp4_quantize_both"]

@@ -3,8 +3,9 @@
 Same names and meaning as the reference, over torch dtypes. A policy is made
 visible with ``precision_context``; ``linear_matmul`` routes projections
 through the fp8 kernels when the policy's ``matrix_dtype`` is
-``float8_e4m3fn`` (precision.py:224-239), and otherwise through an ordinary
-matmul, as the reference does with ``jnp.matmul``.
+``float8_e4m3fn`` (precision.py:224-239), through the MXFP4 kernels when it is
+``float4_e2m1fn`` (an extension), and otherwise through an ordinary matmul, as the
+reference does with ``jnp.matmul``.
 """
 
 from __future__ import annotations
@@ -17,8 +18,9 @@ from dataclasses import dataclass
 from typing import Any
 
 import torch
+import torch.nn.functional as F
 
-from . import ops
+from . import mxfp4, ops
 
 
 class DelayedScaling:
@@ -151,7 +153,10 @@ _DTYPES = {
     "float32": torch.float32,
     "bfloat16": torch.bfloat16,
     "float8_e4m3fn": torch.float8_e4m3fn,
+    "float4_e2m1fn": torch.float4_e2m1fn_x2,
 }
+# matrix types whose products run in this package's kernels
+_KERNEL_MATRIX_DTYPES = (torch.float8_e4m3fn, torch.float4_e2m1fn_x2)
 _ACTIVE_PRECISION: ContextVar[PrecisionPolicy | None] = ContextVar(
     "representax_amd_precision", default=None
 )
@@ -320,17 +325,33 @@ def linear_matmul(left: torch.Tensor, right: torch.Tensor, *, out_sharding: Any 
 
     del out_sharding  # single-device: sharding annotations are the identity
     policy = _ACTIVE_PRECISION.get()
-    if policy is None or policy.matrix_dtype != torch.float8_e4m3fn:
+    if policy is None or policy.matrix_dtype not in _KERNEL_MATRIX_DTYPES:
         return torch.matmul(left, right)
     leading = left.shape[:-1]
     flat = left.reshape(math.prod(leading), left.shape[-1])
-    if policy.fp8_state is not None and fp8_owner is not None:
+    if policy.matrix_dtype == torch.float4_e2m1fn_x2:
+        out = mxfp4.linear_product(flat, right, policy.activation_dtype)
+    elif policy.fp8_state is not None and fp8_owner is not None:
         slots = policy.fp8_state.slots_for(fp8_owner, LINEAR_FORMATS)
         out = ops.Fp8DelayedLinearFn.apply(flat, right, policy.activation_dtype,
                                            policy.fp8_state, slots)
     else:
         out = ops.Fp8LinearFn.apply(flat, right, policy.activation_dtype)
     return out.reshape(*leading, right.shape[-1]).to(policy.activation_dtype)
+
+
+def gated_matmul(left: torch.Tensor, gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """``silu(left @ gate) * (left @ up)`` under the active matrix policy, ``left
+    [..., K]``, ``gate`` and ``up [K, N]``: the first half of a gated feed-forward block.
+    One kernel under MXFP4, separate products otherwise."""
+
+    policy = _ACTIVE_PRECISION.get()
+    if policy is None or policy.matrix_dtype != torch.float4_e2m1fn_x2:
+        return F.silu(linear_matmul(left, gate)) * linear_matmul(left, up)
+    leading = left.shape[:-1]
+    flat = left.reshape(math.prod(leading), left.shape[-1])
+    out = mxfp4.gated_product(flat, gate, up, policy.activation_dtype)
+    return out.reshape(*leading, gate.shape[-1])
 
 
 def activation_inputs(inputs: Any) -> Any:
@@ -376,6 +397,7 @@ __all__ = [
     "active_compute_views",
     "compute_parameter",
     "compute_views",
+    "gated_matmul",
     "linear_matmul",
     "loss_value",
     "model_for_compute",
