@@ -92,6 +92,9 @@ int rpx_abi_version(void);
  *   RPX_TUNE_FP8_PAIR    fp8 linear backward's input and weight gradients in
  *                        one launch: -1 planner (where both products' tiles
  *                        allow it), 0 two launches (env RPX_FP8_PAIR)
+ *   RPX_TUNE_MX_TILE     MXFP4 GEMM tile: 0 planner, 1..7
+ *   RPX_TUNE_MX_SPLITS   MXFP4 GEMM split count over the contracted columns:
+ *                        0 planner, 1..64 (at least four slices each)
  * ------------------------------------------------------------------------- */
 #define RPX_TUNE_INT4_TILE 0
 #define RPX_TUNE_BF16_TILE 1
@@ -106,6 +109,8 @@ int rpx_abi_version(void);
 #define RPX_TUNE_RANK_NT_U 10
 #define RPX_TUNE_FP8_SPLITS 11
 #define RPX_TUNE_FP8_PAIR 12
+#define RPX_TUNE_MX_TILE 13
+#define RPX_TUNE_MX_SPLITS 14
 
 /* RPX_ERR_INVALID for an unknown knob or value. */
 int rpx_set_tuning(int knob, int value);

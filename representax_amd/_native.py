@@ -46,6 +46,8 @@ TUNE_RANK_BLOCKS = 9
 TUNE_RANK_NT_U = 10
 TUNE_FP8_SPLITS = 11
 TUNE_FP8_PAIR = 12
+TUNE_MX_TILE = 13
+TUNE_MX_SPLITS = 14
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64

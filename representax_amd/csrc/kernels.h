@@ -363,6 +363,7 @@ struct MxGemm {
   void *out, *z_gate, *z_up;
   int dtype;
 };
+int mx_tile_count();
 int64_t mx_gemm_workspace_floats(int64_t m, int64_t n, int64_t slices);
 hipError_t launch_mx_gemm(const MxGemm& p, float* partials, hipStream_t stream);
 

@@ -1,94 +1,533 @@
 // Products of MXFP4 matrices: out[i, j] = sum_c A[i, c] B[j, c], and the first
 // half of a gated feed-forward block, silu(A G^T) * (A U^T), from one pass over
 // A. mxfp4.h states the format and the order in which a slice's blocks meet.
+#include <atomic>
+
 #include <hip/hip_runtime.h>
 
 #include "act.h"
 #include "kernels.h"
+#include "lds_pipeline.h"
 #include "mxfp4.h"
+#include "tuning.h"
 
 namespace rpx {
 
 namespace {
 
-__device__ __forceinline__ void store_as(void* out, int dtype, int64_t i, float v) {
-  if (dtype == kBF16)
-    static_cast<uint16_t*>(out)[i] = f32_to_bf16(v);
-  else
-    static_cast<float*>(out)[i] = v;
-}
-
-// One wave per 32 x 32 tile, fragments straight from memory. GATED: B is the
-// gate's weight and B2 the up projection's.
-template <bool GATED>
-__global__ void __launch_bounds__(64) k_mx_gemm_simple(MxGemm p) {
-  const int64_t tile = block_of_grid();
-  const int64_t tiles_n = ceil_div(p.n, 32);
-  if (tile >= ceil_div(p.m, 32) * tiles_n) return;
-  const int64_t m0 = tile / tiles_n * 32;
-  const int64_t n0 = tile % tiles_n * 32;
-  const int lane = threadIdx.x;
-  const int half = lane >> 5;
-  int64_t ra = m0 + (lane & 31), rb = n0 + (lane & 31);
-  ra = ra < p.m ? ra : p.m - 1;
-  rb = rb < p.n ? rb : p.n - 1;
-  const int64_t row_bytes = p.slices * kMxSliceBytes;
-  const int64_t ra_pad = mx_pad_rows(p.m), rb_pad = mx_pad_rows(p.n);
-  f32x16_t acc, acc2;
+// Writes a wave's sub-tile of ROWS x COLS bf16 values, staged in LDS with a row
+// pitch of 2 COLS + 16 bytes, as 16-byte pieces of whole row segments. m0, n0:
+// its first row and column in the output.
+template <int ROWS, int COLS>
+__device__ __forceinline__ void store_staged(const uint8_t* reg, uint16_t* out, int64_t m0,
+                                             int64_t n0, int64_t M, int64_t N, int lane) {
+  constexpr int P = COLS * 2 + 16;
+  constexpr int CPR = COLS / 8;
+  constexpr int ITS = ROWS * CPR / 64;
+  constexpr int UN = ITS % 8 == 0 ? 8 : ITS % 4 == 0 ? 4 : 1;
+  // other lanes' staged values: every write of this wave before its reads
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if ((N & 7) == 0 && m0 + ROWS <= M && n0 + COLS <= N) {
+    for (int i0 = 0; i0 < ITS; i0 += UN) {
+      u32x4_t v[UN];
 #pragma unroll
-  for (int v = 0; v < 16; ++v) acc[v] = acc2[v] = 0.0f;
-  for (int64_t s = 0; s < p.slices; ++s) {
-    const int64_t ca = ra * row_bytes + s * kMxSliceBytes + 64 * half;
-    const int64_t cb = rb * row_bytes + s * kMxSliceBytes + 64 * half;
-    const int64_t sb_at = (s * rb_pad + rb) * kMxSliceBlocks + 4 * half;
-    const uint32_t sa = *reinterpret_cast<const uint32_t*>(
-        p.a_scales + (s * ra_pad + ra) * kMxSliceBlocks + 4 * half);
-    auto a = [&](int j) { return *reinterpret_cast<const u32x4_t*>(p.a_codes + ca + 16 * j); };
-    auto run = [&](const uint8_t* codes, const uint8_t* scales, f32x16_t c) {
-      const uint32_t sb = *reinterpret_cast<const uint32_t*>(scales + sb_at);
-      auto b = [&](int j) { return *reinterpret_cast<const u32x4_t*>(codes + cb + 16 * j); };
-      c = mx_mfma32<0, 0>(b(0), sb, a(0), sa, c);
-      c = mx_mfma32<1, 1>(b(1), sb, a(1), sa, c);
-      c = mx_mfma32<2, 2>(b(2), sb, a(2), sa, c);
-      return mx_mfma32<3, 3>(b(3), sb, a(3), sa, c);
-    };
-    acc = run(p.b_codes, p.b_scales, acc);
-    if constexpr (GATED) acc2 = run(p.b2_codes, p.b2_scales, acc2);
-  }
-  // lane l holds row m0 + l % 32 and columns n0 + 8 g + 4 (l / 32) + e in acc[4 g + e]
-  const int64_t m = m0 + (lane & 31);
-  if (m >= p.m) return;
-#pragma unroll
-  for (int v = 0; v < 16; ++v) {
-    const int64_t n = n0 + 8 * (v / 4) + 4 * half + v % 4;
-    if (n >= p.n) continue;
-    const int64_t at = m * p.n + n;
-    if constexpr (GATED) {
-      const float g = p.dtype == kBF16 ? round_bf16(acc[v]) : acc[v];
-      const float u = p.dtype == kBF16 ? round_bf16(acc2[v]) : acc2[v];
-      store_as(p.out, p.dtype, at, act_apply<kActSiluMulFwd>(u, g, 0.0f, nullptr));
-      if (p.z_gate != nullptr) {
-        store_as(p.z_gate, p.dtype, at, g);
-        store_as(p.z_up, p.dtype, at, u);
+      for (int i = 0; i < UN; ++i) {
+        const int idx = (i0 + i) * 64 + lane;
+        v[i] = *reinterpret_cast<const u32x4_t*>(reg + (idx / CPR) * P + (idx % CPR) * 16);
       }
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        const int idx = (i0 + i) * 64 + lane;
+        *reinterpret_cast<u32x4_t*>(out + (m0 + idx / CPR) * N + n0 + 8 * (idx % CPR)) = v[i];
+      }
+    }
+    return;
+  }
+  for (int it = 0; it < ITS; ++it) {
+    const int idx = it * 64 + lane;
+    const int r = idx / CPR;
+    const int c = idx % CPR;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(reg + r * P + c * 16);
+    const int64_t m = m0 + r;
+    const int64_t n = n0 + 8 * c;
+    if (m >= M) continue;
+    uint16_t* d = out + m * N + n;
+    if ((N & 7) == 0 && n + 7 < N) {
+      *reinterpret_cast<u32x4_t*>(d) = v;
     } else {
-      store_as(p.out, p.dtype, at, acc[v]);
+      for (int e = 0; e < 8; ++e)
+        if (n + e < N) d[e] = static_cast<uint16_t>((v[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
     }
   }
 }
 
+// Four float32 values at columns n .. n + 3 of a row.
+__device__ __forceinline__ void store4(float* d, int64_t n, int64_t N, const float* y) {
+  if (n + 3 < N && (N & 3) == 0) {
+    *reinterpret_cast<f32x4_t*>(d) = f32x4_t{y[0], y[1], y[2], y[3]};
+  } else {
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) d[e] = y[e];
+  }
+}
+
+// A workgroup of WM x WN waves computes a BM x BN tile (a wave: BM / WM x
+// BN / WN, in blocks of 32 x 32) over the slices of its split. A slice (256
+// columns of every row of the tile, 128 bytes each, and eight scale bytes each)
+// goes from memory to LDS by direct-to-LDS loads, into NS rotating stages. A
+// slice is four MFMA steps; the fragments of a step are read from LDS while the
+// step before it runs, and after the last reads of a stage its refill is issued
+// under the last step's MFMAs:
+//   steps 0, 1, 2   MFMAs, each followed by LDS reads of the next step's fragments
+//   barrier         slice t + 1 has landed, every wave is done with stage t
+//   step 3          MFMAs, with the loads of slice t + NS into stage t, and the
+//                   reads of slice t + 1's first fragments and scales
+// Refills past the end re-read the last slice, which keeps the count of loads in
+// flight a constant. The weight's fragments are the MFMA's first operand, so a
+// lane ends up with four consecutive output columns of one row.
+//
+// GATED: B's BN rows are, for each wave, half gate and half up projections of the
+// same output columns, so that both meet in the wave's registers.
+template <int BM, int BN, int WM, int WN, int NS, bool GATED>
+__device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t slices_per_split,
+                                             int tile_m, int tile_n, int tiles, int tile,
+                                             float* partials) {
+  constexpr int NW = WM * WN;
+  constexpr int TM = BM / WM;
+  constexpr int TN = BN / WN;
+  constexpr int FM = TM / 32;
+  constexpr int FN = TN / 32;
+  static_assert(TM % 32 == 0 && TN % 32 == 0 && (!GATED || FN % 2 == 0), "wave tile");
+  constexpr int SEGS = (BM + BN) / 8;
+  static_assert(SEGS % NW == 0, "segments must split evenly over the waves");
+  constexpr int CODE_LPW = SEGS / NW;
+  constexpr int SCALE_SEGS = (BM + BN + 127) / 128;
+  static_assert(SCALE_SEGS <= NW, "a wave loads one segment of scales");
+  constexpr int LPW = CODE_LPW + 1;
+  static_assert(NS >= 2 && LPW * (NS - 1) < 64, "vmcnt range");
+  constexpr int SCALES = (BM + BN) * kMxSliceBytes;
+  constexpr int STAGE = SCALES + SCALE_SEGS * 1024;
+  constexpr int OUT_N = GATED ? BN / 2 : BN;  // output columns of the tile
+  extern __shared__ __align__(16) uint8_t smem[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM;
+  const int wn = wave / WM;
+  const int64_t m0 = static_cast<int64_t>(tile_m) * BM;
+  const int64_t n0 = static_cast<int64_t>(tile_n) * OUT_N;
+  const int64_t sbeg = split * slices_per_split;
+  const int64_t send = sbeg + slices_per_split < p.slices ? sbeg + slices_per_split : p.slices;
+  const int ns = static_cast<int>(send - sbeg);
+
+  // Row r of the tile's B operand: which matrix, and which of its rows.
+  auto b_row = [&](int r, bool* up) {
+    if constexpr (GATED) {
+      const int w = r / TN, q = r % TN;
+      *up = q >= TN / 2;
+      return n0 + w * (TN / 2) + q % (TN / 2);
+    } else {
+      *up = false;
+      return n0 + r;
+    }
+  };
+
+  // Sources of the wave's segments: 8 rows of codes each (lane l brings chunk
+  // l % 8 of row l / 8, swizzled), and 128 rows of scales (two rows a lane). Rows
+  // past the end re-read the last; they only feed outputs that are not stored.
+  const uint8_t* src[LPW];
+#pragma unroll
+  for (int i = 0; i < CODE_LPW; ++i) {
+    const int r = 8 * (wave + i * NW) + (lane >> 3);
+    const int chunk = ((lane & 7) ^ swz(r)) << 4;
+    const uint8_t* base = p.a_codes;
+    int64_t row = m0 + r, lim = p.m;
+    if (r >= BM) {
+      bool up;
+      row = b_row(r - BM, &up);
+      lim = p.n;
+      base = GATED && up ? p.b2_codes : p.b_codes;
+    }
+    row = row < lim ? row : lim - 1;
+    src[i] = base + (row * p.slices + sbeg) * kMxSliceBytes + chunk;
+  }
+  int64_t scale_step;
+  {
+    const int r = 128 * (wave % SCALE_SEGS) + 2 * lane;
+    const uint8_t* base = p.a_scales;
+    int64_t row = m0 + r, lim = mx_pad_rows(p.m);
+    if (r >= BM) {
+      bool up;
+      row = b_row(r - BM < BN ? r - BM : 0, &up);
+      lim = mx_pad_rows(p.n);
+      base = GATED && up ? p.b2_scales : p.b_scales;
+    }
+    row = row < lim ? row : lim - 2;
+    src[CODE_LPW] = base + (sbeg * lim + row) * kMxSliceBlocks;
+    scale_step = lim * kMxSliceBlocks;
+  }
+  auto dma_one = [&](uint8_t* st, int64_t slice, int i) {
+    if (i < CODE_LPW)
+      dma_seg(st, src[i], slice * kMxSliceBytes, wave + i * NW);
+    else
+      dma_seg(st + SCALES, src[CODE_LPW], slice * scale_step, wave % SCALE_SEGS);
+  };
+
+  f32x16_t acc[FN][FM];
+#pragma unroll
+  for (int fn = 0; fn < FN; ++fn)
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[fn][fm][v] = 0.0f;
+
+  const int frow = lane & 31;
+  const int half = lane >> 5;
+  constexpr int NMF = FM * FN;
+  constexpr int NFR = FM + FN;
+  u32x4_t fx[NFR], fy[NFR];       // fragments of two consecutive steps: A's, then B's
+  uint32_t sc[NFR], sc_next[NFR];  // scale words of a slice
+  auto frag_row = [&](int j) {
+    return j < FM ? wm * TM + j * 32 + frow : BM + wn * TN + (j - FM) * 32 + frow;
+  };
+  auto frag_one = [&](const uint8_t* st, int step, int j, u32x4_t* f) {
+    f[j] = lds_chunk(st, frag_row(j), 4 * half + step);
+  };
+  auto scale_one = [&](const uint8_t* st, int j, uint32_t* s) {
+    s[j] = *reinterpret_cast<const uint32_t*>(st + SCALES + frag_row(j) * kMxSliceBlocks + 4 * half);
+  };
+
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) dma_one(smem + s * STAGE, s < ns ? s : ns - 1, i);
+  wait_sync<(NS - 1) * LPW>();
+#pragma unroll
+  for (int j = 0; j < NFR; ++j) frag_one(smem, 0, j, fx);
+#pragma unroll
+  for (int j = 0; j < NFR; ++j) scale_one(smem, j, sc);
+
+#define RPX_MX_STEP(STEP, F, MORE)                                                               \
+  _Pragma("unroll") for (int i = 0; i < NMF; ++i) {                                              \
+    acc[i / FM][i % FM] = mx_mfma32<STEP, STEP>(F[FM + i / FM], sc[FM + i / FM], F[i % FM],      \
+                                                sc[i % FM], acc[i / FM][i % FM]);                \
+    __builtin_amdgcn_sched_barrier(0);                                                           \
+    MORE __builtin_amdgcn_sched_barrier(0);                                                      \
+  }
+#define RPX_MX_READS(ST, STEP, F)                                                                \
+  _Pragma("unroll") for (int j = i * NFR / NMF; j < (i + 1) * NFR / NMF; ++j)                    \
+      frag_one(ST, STEP, j, F);
+
+  int stage = 0;
+  for (int t = 0; t < ns; ++t) {
+    const int next = stage + 1 == NS ? 0 : stage + 1;
+    uint8_t* st = smem + stage * STAGE;
+    const uint8_t* nst = smem + next * STAGE;
+    RPX_MX_STEP(0, fx, RPX_MX_READS(st, 1, fy))
+    RPX_MX_STEP(1, fy, RPX_MX_READS(st, 2, fx))
+    RPX_MX_STEP(2, fx, RPX_MX_READS(st, 3, fy))
+    wait_sync<(NS - 2) * LPW>();
+    const int64_t refill = t + NS < ns ? t + NS : ns - 1;
+    RPX_MX_STEP(3, fy, {
+      _Pragma("unroll") for (int d = i * LPW / NMF; d < (i + 1) * LPW / NMF; ++d)
+          dma_one(st, refill, d);
+      RPX_MX_READS(nst, 0, fx)
+      _Pragma("unroll") for (int j = i * NFR / NMF; j < (i + 1) * NFR / NMF; ++j)
+          scale_one(nst, j, sc_next);
+    })
+#pragma unroll
+    for (int j = 0; j < NFR; ++j) sc[j] = sc_next[j];
+    stage = next;
+  }
+#undef RPX_MX_STEP
+#undef RPX_MX_READS
+  // no load may be in flight to an LDS that the epilogue, or the workgroup after
+  // this one, writes
+  wait_sync<0>();
+
+  // Block (fn, fm): the lane holds row 32 fm + l % 32 and columns 32 fn + 8 g +
+  // 4 (l / 32) + e of the wave's sub-tile in acc[fn][fm][4 g + e].
+  const int64_t mw = m0 + wm * TM;
+  const int64_t nw = n0 + wn * (OUT_N / WN);
+  if (!GATED && partials != nullptr) {
+    f32x4_t* dst = reinterpret_cast<f32x4_t*>(
+        partials + (static_cast<int64_t>(split) * tiles + tile) * (BM * BN));
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn)
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x16_t& a = acc[fn][fm];
+          dst[(((wave * FN + fn) * FM + fm) * 4 + g) * 64 + lane] =
+              f32x4_t{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+        }
+    return;
+  }
+  constexpr int FO = GATED ? FN / 2 : FN;  // output blocks along the columns
+  if (p.dtype != kBF16) {
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      const int64_t m = mw + fm * 32 + frow;
+      if (m >= p.m) continue;
+#pragma unroll
+      for (int fn = 0; fn < FO; ++fn)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int64_t n = nw + fn * 32 + 8 * g + 4 * half;
+          const int64_t at = m * p.n + n;
+          float y[4], z[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[e] = acc[fn][fm][4 * g + e];
+            if constexpr (GATED) z[e] = acc[FO + fn][fm][4 * g + e];
+          }
+          if constexpr (GATED) {
+            float h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              h[e] = act_apply<kActSiluMulFwd>(z[e], y[e], 0.0f, nullptr);
+            store4(static_cast<float*>(p.out) + at, n, p.n, h);
+            if (p.z_gate != nullptr) {
+              store4(static_cast<float*>(p.z_gate) + at, n, p.n, y);
+              store4(static_cast<float*>(p.z_up) + at, n, p.n, z);
+            }
+          } else {
+            store4(static_cast<float*>(p.out) + at, n, p.n, y);
+          }
+        }
+    }
+    return;
+  }
+  // bf16: the wave's sub-tile through LDS. Its region is the wave's own, so its
+  // own order of LDS operations is all that the passes need.
+  constexpr int P = OUT_N / WN * 2 + 16;
+  uint8_t* reg = smem + wave * (TM * P);
+  auto stage_block = [&](int fm, int fn, int g, uint32_t lo, uint32_t hi) {
+    *reinterpret_cast<u32x2_t*>(reg + (fm * 32 + frow) * P + (fn * 32 + 8 * g + 4 * half) * 2) =
+        u32x2_t{lo, hi};
+  };
+  if constexpr (GATED) {
+    // pass 0 leaves the rounded projections in acc's low words, pass 1 and 2 (if
+    // asked for) store them
+#pragma unroll
+    for (int fn = 0; fn < FO; ++fn)
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float zg = round_bf16(acc[fn][fm][4 * g + e]);
+            const float zu = round_bf16(acc[FO + fn][fm][4 * g + e]);
+            h[e] = act_apply<kActSiluMulFwd>(zu, zg, 0.0f, nullptr);
+          }
+          stage_block(fm, fn, g, pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3]));
+        }
+    store_staged<TM, OUT_N / WN>(reg, static_cast<uint16_t*>(p.out), mw, nw, p.m, p.n, lane);
+    if (p.z_gate == nullptr) return;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+#pragma unroll
+      for (int fn = 0; fn < FO; ++fn)
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x16_t& a = acc[z * FO + fn][fm];
+            stage_block(fm, fn, g, pack_bf16x2(a[4 * g], a[4 * g + 1]),
+                        pack_bf16x2(a[4 * g + 2], a[4 * g + 3]));
+          }
+      store_staged<TM, OUT_N / WN>(reg, static_cast<uint16_t*>(z == 0 ? p.z_gate : p.z_up), mw, nw,
+                                   p.m, p.n, lane);
+    }
+  } else {
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn)
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x16_t& a = acc[fn][fm];
+          stage_block(fm, fn, g, pack_bf16x2(a[4 * g], a[4 * g + 1]),
+                      pack_bf16x2(a[4 * g + 2], a[4 * g + 3]));
+        }
+    store_staged<TM, TN>(reg, static_cast<uint16_t*>(p.out), mw, nw, p.m, p.n, lane);
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int NS, int WPE, bool GATED>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
+    k_mx_gemm(MxGemm p, int64_t slices_per_split, int tiles_m, int tiles_n, int band,
+              float* partials) {
+  // Tiles are dealt to the XCDs in contiguous ranges of a banded order, so the
+  // tiles that an XCD runs at once share few rows of A and B in its L2; splits are
+  // outermost.
+  const int tiles = tiles_m * tiles_n;
+  const int b = xcd_block(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+  int tile_m, tile_n;
+  band_tile(b % tiles, tiles_m, tiles_n, band, tile_m, tile_n);
+  mx_gemm_tile<BM, BN, WM, WN, NS, GATED>(p, b / tiles, slices_per_split, tile_m, tile_n, tiles,
+                                          tile_m * tiles_n + tile_n, partials);
+}
+
+// Sums the partial tiles of a split product in split order. One thread per
+// 16-byte chunk: consecutive threads read consecutive chunks of every split.
+template <int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(256)
+    k_mx_split_reduce(const float* __restrict__ partials, int splits, int64_t M, int64_t N,
+                      int tiles_n, int64_t tiles, void* __restrict__ out, int dtype) {
+  constexpr int TM = BM / WM;
+  constexpr int TN = BN / WN;
+  constexpr int FM = TM / 32;
+  constexpr int FN = TN / 32;
+  constexpr int CHUNKS = BM * BN / 4;
+  const int64_t q = block_of_grid() * 256 + threadIdx.x;
+  if (q >= tiles * CHUNKS) return;
+  const f32x4_t* p = reinterpret_cast<const f32x4_t*>(partials);
+  f32x4_t s = p[q];
+  for (int i = 1; i < splits; ++i) s += p[i * tiles * CHUNKS + q];
+  const int64_t tile = q / CHUNKS;
+  int r = static_cast<int>(q % CHUNKS);
+  const int lane = r & 63;
+  r >>= 6;
+  const int g = r & 3;
+  r >>= 2;
+  const int fm = r % FM;
+  r /= FM;
+  const int fn = r % FN;
+  const int wave = r / FN;
+  const int64_t m = (tile / tiles_n) * BM + (wave % WM) * TM + fm * 32 + (lane & 31);
+  const int64_t n = (tile % tiles_n) * BN + (wave / WM) * TN + fn * 32 + 8 * g + 4 * (lane >> 5);
+  if (m >= M) return;
+  const float y[4] = {s[0], s[1], s[2], s[3]};
+  if (dtype != kBF16) {
+    store4(static_cast<float*>(out) + m * N + n, n, N, y);
+    return;
+  }
+  uint16_t* d = static_cast<uint16_t*>(out) + m * N + n;
+  if (n + 3 < N && (N & 3) == 0) {
+    *reinterpret_cast<u32x2_t*>(d) = u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  } else {
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) d[e] = f32_to_bf16(y[e]);
+  }
+}
+
+// Tiles: id, rows of A, rows of B, waves along each, stages, waves per SIMD.
+#define RPX_MX_CONFIGS(X)     \
+  X(1, 256, 256, 2, 2, 2, 1)  \
+  X(2, 256, 256, 4, 2, 2, 2)  \
+  X(3, 256, 128, 2, 2, 3, 1)  \
+  X(4, 128, 128, 2, 2, 2, 2)  \
+  X(5, 128, 128, 2, 2, 4, 1)  \
+  X(6, 64, 128, 2, 2, 2, 2)   \
+  X(7, 64, 64, 2, 1, 2, 2)
+
+struct Plan {
+  int id, bm, bn;
+  int64_t tiles_m, tiles_n;
+  int splits;
+  int64_t per_split;
+};
+
+Plan plan_for(int id, int64_t m, int64_t n, int64_t slices, bool gated) {
+  Plan p{};
+  p.id = id;
+  switch (id) {
+#define X(ID, BM, BN, WM, WN, NS, WPE) \
+  case ID:                             \
+    p.bm = BM;                         \
+    p.bn = BN;                         \
+    break;
+    RPX_MX_CONFIGS(X)
+#undef X
+  }
+  p.tiles_m = ceil_div(m, p.bm);
+  p.tiles_n = ceil_div(n, gated ? p.bn / 2 : p.bn);
+  p.splits = 1;
+  p.per_split = slices;
+  return p;
+}
+
+Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {
+  int id = tune(kTuneMxTile);
+  if (id == 0) {
+    id = 1;
+    for (int c : {1, 4, 6}) {
+      id = c;
+      const Plan p = plan_for(c, m, n, slices, gated);
+      if (p.tiles_m * p.tiles_n >= 192) break;
+    }
+  }
+  Plan p = plan_for(id, m, n, slices, gated);
+  const int64_t tiles = p.tiles_m * p.tiles_n;
+  int64_t splits = tune(kTuneMxSplits);
+  if (splits == 0) splits = tiles >= 128 ? 1 : 256 / (tiles > 0 ? tiles : 1);
+  if (gated) splits = 1;
+  if (splits > slices / 4) splits = slices / 4;
+  if (splits > 1) {
+    p.per_split = ceil_div(slices, splits);
+    p.splits = static_cast<int>(ceil_div(slices, p.per_split));
+  }
+  return p;
+}
+
+template <int BM, int BN, int WM, int WN, int NS, int WPE, bool GATED>
+hipError_t launch_config(const MxGemm& g, const Plan& p, float* partials, hipStream_t stream) {
+  constexpr int SCALE_SEGS = (BM + BN + 127) / 128;
+  constexpr int STAGES = NS * ((BM + BN) * kMxSliceBytes + SCALE_SEGS * 1024);
+  constexpr int OUT = WM * WN * (BM / WM) * ((GATED ? BN / 2 : BN) / WN * 2 + 16);
+  constexpr int LDS = STAGES > OUT ? STAGES : OUT;
+  static_assert(LDS <= 160 * 1024, "LDS");
+  const void* kernel = reinterpret_cast<const void*>(k_mx_gemm<BM, BN, WM, WN, NS, WPE, GATED>);
+  static std::atomic<unsigned> done{0};
+  if (hipError_t e = ensure_lds_limit(kernel, LDS, done); e != hipSuccess) return e;
+  const int64_t tiles = p.tiles_m * p.tiles_n;
+  if (tiles * p.splits > (int64_t{1} << 30)) return hipErrorInvalidValue;
+  const int band = tune(kTuneBand) > 0 ? tune(kTuneBand) : 4;
+  k_mx_gemm<BM, BN, WM, WN, NS, WPE, GATED>
+      <<<dim3(static_cast<unsigned>(tiles * p.splits)), dim3(64 * WM * WN), LDS, stream>>>(
+          g, p.per_split, static_cast<int>(p.tiles_m), static_cast<int>(p.tiles_n), band,
+          p.splits > 1 ? partials : nullptr);
+  if (p.splits > 1) {
+    const int64_t chunks = tiles * (BM * BN / 4);
+    k_mx_split_reduce<BM, BN, WM, WN><<<grid_of(ceil_div(chunks, 256)), dim3(256), 0, stream>>>(
+        partials, p.splits, g.m, g.n, static_cast<int>(p.tiles_n), tiles, g.out, g.dtype);
+  }
+  return hipGetLastError();
+}
+
 }  // namespace
 
-int64_t mx_gemm_workspace_floats(int64_t m, int64_t n, int64_t slices) { return 0; }
+int mx_tile_count() {
+  int count = 0;
+#define X(...) ++count;
+  RPX_MX_CONFIGS(X)
+#undef X
+  return count;
+}
 
-hipError_t launch_mx_gemm(const MxGemm& p, float* partials, hipStream_t stream) {
-  const int64_t tiles = ceil_div(p.m, 32) * ceil_div(p.n, 32);
-  if (tiles == 0) return hipSuccess;
-  if (p.b2_codes != nullptr)
-    hipLaunchKernelGGL(k_mx_gemm_simple<true>, grid_of(tiles), dim3(64), 0, stream, p);
-  else
-    hipLaunchKernelGGL(k_mx_gemm_simple<false>, grid_of(tiles), dim3(64), 0, stream, p);
-  return hipGetLastError();
+int64_t mx_gemm_workspace_floats(int64_t m, int64_t n, int64_t slices) {
+  const Plan p = choose(m, n, slices, false);
+  return p.splits > 1 ? p.tiles_m * p.tiles_n * p.splits * p.bm * p.bn : 0;
+}
+
+hipError_t launch_mx_gemm(const MxGemm& g, float* partials, hipStream_t stream) {
+  if (g.m == 0 || g.n == 0) return hipSuccess;
+  const bool gated = g.b2_codes != nullptr;
+  const Plan p = choose(g.m, g.n, g.slices, gated);
+  switch (p.id) {
+#define X(ID, BM, BN, WM, WN, NS, WPE)                                            \
+  case ID:                                                                        \
+    return gated ? launch_config<BM, BN, WM, WN, NS, WPE, true>(g, p, partials, stream) \
+                 : launch_config<BM, BN, WM, WN, NS, WPE, false>(g, p, partials, stream);
+    RPX_MX_CONFIGS(X)
+#undef X
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace rpx

@@ -26,7 +26,9 @@ enum TuneKnob : int {
   kTuneRankNtU = 10,    // rank_nt 128-column steps in flight per wave (0: planner; 4, 8, 16)
   kTuneFp8Splits = 11,  // fp8 GEMM split-K count (0: planner; else forced where it divides K)
   kTuneFp8Pair = 12,    // fp8 backward's two products in one launch: -1 planner, 0 never  RPX_FP8_PAIR
-  kTuneCount = 13
+  kTuneMxTile = 13,     // MXFP4 GEMM tile (0: planner)
+  kTuneMxSplits = 14,   // MXFP4 GEMM split count (0: planner)
+  kTuneCount = 15
 };
 
 // Current value of a knob.

@@ -242,6 +242,8 @@ TUNING_KNOBS = {
     "rank_nt_u": nat.TUNE_RANK_NT_U,
     "fp8_splits": nat.TUNE_FP8_SPLITS,
     "fp8_pair": nat.TUNE_FP8_PAIR,
+    "mx_tile": nat.TUNE_MX_TILE,
+    "mx_splits": nat.TUNE_MX_SPLITS,
 }
 
 

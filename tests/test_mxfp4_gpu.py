@@ -160,6 +160,53 @@ def test_products_over_long_sums(m, n, k):
     _check_product(got, a, b, F32)
 
 
+TILES = range(1, 8)
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_every_tile(tile):
+    """Ragged edges, one slice to more than the pipeline holds, several bands of tiles."""
+
+    g = rng(tile)
+    for m, n, k in ((1, 1, 200), (300, 513, 256), (257, 300, 512), (513, 130, 1500),
+                    (1300, 777, 700)):
+        a, b = _data(g, m, k), _data(g, n, k, 0.05)
+        aq, bq = rx.mxfp4_quantize(to_dev_bf16(a)), rx.mxfp4_quantize(to_dev_bf16(b))
+        with ops.tuning(mx_tile=tile):
+            for out in (BF16, F32):
+                _check_product(rx.mxfp4_matmul(aq, bq, out), a, b, out, (tile, m, n, k))
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_every_tile_of_the_gated_block(tile):
+    g = rng(20 + tile)
+    for m, n, k in ((70, 33, 200), (300, 513, 512), (700, 260, 1500)):
+        x, wg, wu = _data(g, m, k), _data(g, n, k, 0.05), _data(g, n, k, 0.05)
+        xd, gd, ud = to_dev_bf16(x), to_dev_bf16(wg).requires_grad_(), to_dev_bf16(wu)
+        for out in (BF16, F32):
+            with ops.tuning(mx_tile=tile):
+                h = mxfp4.gated_product(xd, gd.t(), ud.t(), out)
+            z = h.grad_fn.saved_tensors[:2]
+            _check_product(z[0], x, wg, out, "gate")
+            _check_product(z[1], x, wu, out, "up")
+            zg, zu = (from_dev(t).astype(np.float64) for t in z)
+            want = omx.gated(zg, zu)
+            bound = _silu_bound(zg, zu) + np.abs(want) * (2.0 ** -8 if out == BF16 else 2.0 ** -24)
+            assert np.all(np.abs(from_dev(h.detach()) - want) <= bound)
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("splits", [2, 3, 5, 64])
+def test_split_sums(tile, splits):
+    g = rng(tile + splits)
+    m, n, k = 200, 333, 5000
+    a, b = _data(g, m, k), _data(g, n, k, 0.05)
+    aq, bq = rx.mxfp4_quantize(to_dev_bf16(a)), rx.mxfp4_quantize(to_dev_bf16(b))
+    with ops.tuning(mx_tile=tile, mx_splits=splits):
+        for out in (BF16, F32):
+            _check_product(rx.mxfp4_matmul(aq, bq, out), a, b, out)
+
+
 @pytest.mark.parametrize("m", [2, 40, 300])
 def test_nan_blocks_reach_their_sums_only(m):
     g = rng(2)
