@@ -85,8 +85,9 @@ int serve(const char* who, const void* x, int dtype, int64_t m, int64_t k, int64
   if (arena.overflow) return fail_invalid(std::string(who) + ": workspace too small");
   RPX_TRY(check_pointers(who, {workspace}));
   MxParts parts{};
-  parts.part[0] = MxPart{x, dtype, m, k, row_stride, 1,
-                         MxOut{e.codes, e.scales, mx_slices(k) * kMxSliceBytes, mx_pad_rows(m)}};
+  parts.part[0] = MxPart{x, dtype, m, k, row_stride,
+                         MxOut{e.codes, e.scales, mx_slices(k) * kMxSliceBytes, mx_pad_rows(m)},
+                         MxOut{}, false, 0};
   RPX_HIP(launch_mx_quantize(parts, 1, st), who);
   const MxGemm g{e.codes, e.scales, codes, scales, up_codes, up_scales, m, n, mx_slices(k),
                  y, nullptr, nullptr, dtype};
@@ -113,7 +114,7 @@ size_t rpx_mxfp4_scale_bytes(int64_t rows, int64_t columns) {
 
 int rpx_mxfp4_quantize(const rpx_mxfp4_part* parts, int64_t count, void* stream) {
   const char* who = "rpx_mxfp4_quantize";
-  if (count < 0 || count > kMxParts / 2)
+  if (count < 0 || count > kMxParts)
     return fail_invalid("rpx_mxfp4_quantize: need 0 <= count <= 4");
   if (count > 0 && parts == nullptr) return fail_invalid("rpx_mxfp4_quantize: null pointer");
   MxParts args{};
@@ -137,16 +138,12 @@ int rpx_mxfp4_quantize(const rpx_mxfp4_part* parts, int64_t count, void* stream)
     const int64_t stride_t = in.code_stride_t == 0 ? dense_t : in.code_stride_t;
     if (stride < dense || stride_t < dense_t || stride % 16 != 0 || stride_t % 16 != 0)
       return fail_invalid("rpx_mxfp4_quantize: invalid code stride");
-    if (in.codes != nullptr) {
-      RPX_TRY(check_pointers(who, {in.codes, in.scales}));
-      args.part[jobs++] = MxPart{in.t, in.dtype, in.rows, in.columns, in.row_stride, 1,
-                                 MxOut{in.codes, in.scales, stride, mx_pad_rows(in.rows)}};
-    }
-    if (in.codes_t != nullptr) {
-      RPX_TRY(check_pointers(who, {in.codes_t, in.scales_t}));
-      args.part[jobs++] = MxPart{in.t, in.dtype, in.columns, in.rows, 1, in.row_stride,
-                                 MxOut{in.codes_t, in.scales_t, stride_t, mx_pad_rows(in.columns)}};
-    }
+    if (in.codes != nullptr) RPX_TRY(check_pointers(who, {in.codes, in.scales}));
+    if (in.codes_t != nullptr) RPX_TRY(check_pointers(who, {in.codes_t, in.scales_t}));
+    args.part[jobs++] =
+        MxPart{in.t, in.dtype, in.rows, in.columns, in.row_stride,
+               MxOut{in.codes, in.scales, stride, mx_pad_rows(in.rows)},
+               MxOut{in.codes_t, in.scales_t, stride_t, mx_pad_rows(in.columns)}, false, 0};
   }
   RPX_HIP(launch_mx_quantize(args, jobs, static_cast<hipStream_t>(stream)), who);
   return kOk;
@@ -233,8 +230,8 @@ int rpx_mxfp4_gated_backward(const void* dh, const void* z_gate, const void* z_u
   if (codes != nullptr) RPX_TRY(check_pointers(who, {codes, scales}));
   if (codes_t != nullptr) RPX_TRY(check_pointers(who, {codes_t, scales_t}));
   MxOut along{codes, scales, 2 * mx_slices(n) * kMxSliceBytes, mx_pad_rows(m)};
-  MxOut stacked{codes_t, scales_t, mx_slices(m) * kMxSliceBytes, mx_pad_rows(2 * n)};
-  RPX_HIP(launch_mx_gated_backward(dh, z_gate, z_up, dtype, m, n, along, stacked,
+  MxOut across{codes_t, scales_t, mx_slices(m) * kMxSliceBytes, mx_pad_rows(2 * n)};
+  RPX_HIP(launch_mx_gated_backward(dh, z_gate, z_up, dtype, m, n, along, across,
                                    static_cast<hipStream_t>(stream)),
           who);
   return kOk;

@@ -336,12 +336,14 @@ struct CastMany {
 hipError_t launch_cast_many(CastMany args, int tensors, hipStream_t stream);
 
 // MXFP4 (mxfp4.h) -----------------------------------------------------------
-constexpr int kMxParts = 8;  // encodings of one launch
+constexpr int kMxParts = 4;  // matrices of one launch
 struct MxPart {
   const void* t;
   int dtype;
-  int64_t rows, columns, row_stride, column_stride;  // in elements
-  MxOut out;
+  int64_t rows, columns, row_stride;  // in elements, columns dense
+  MxOut along, across;  // its encoding along its columns, its transpose's (codes null: none)
+  bool aligned;         // set by the launcher, as `tiles`
+  int64_t tiles;
 };
 struct MxParts {
   MxPart part[kMxParts];
@@ -351,7 +353,7 @@ struct MxParts {
 hipError_t launch_mx_zero(void* out, int64_t bytes, hipStream_t stream);
 hipError_t launch_mx_quantize(MxParts parts, int count, hipStream_t stream);
 hipError_t launch_mx_gated_backward(const void* dh, const void* z_gate, const void* z_up, int dtype,
-                                    int64_t m, int64_t n, MxOut along, MxOut stacked,
+                                    int64_t m, int64_t n, MxOut along, MxOut across,
                                     hipStream_t stream);
 hipError_t launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
                                 int64_t columns, void* out, int dtype, hipStream_t stream);

@@ -86,12 +86,16 @@ __device__ __forceinline__ uint32_t mx_encode8(const float* v, float scale) {
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
   return w;
 }
+// By value: a bit cast of a vector's element would read the vector's first.
+__device__ __forceinline__ bf16x2_t mx_as_bf16x2(uint32_t w) {
+  return __builtin_bit_cast(bf16x2_t, w);
+}
 __device__ __forceinline__ uint32_t mx_encode8(u32x4_t bf16s, float scale) {
   uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, bf16s[0]), scale, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, bf16s[1]), scale, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, bf16s[2]), scale, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, bf16s[3]), scale, 3);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_as_bf16x2(bf16s[0]), scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_as_bf16x2(bf16s[1]), scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_as_bf16x2(bf16s[2]), scale, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_as_bf16x2(bf16s[3]), scale, 3);
   return w;
 }
 

@@ -186,6 +186,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
   const int half = lane >> 5;
   constexpr int NMF = FM * FN;
   constexpr int NFR = FM + FN;
+  constexpr int RPM = NFR * 2 <= NMF ? 2 : NFR <= NMF ? 2 : NFR;
   u32x4_t fx[NFR], fy[NFR];       // fragments of two consecutive steps: A's, then B's
   uint32_t sc[NFR], sc_next[NFR];  // scale words of a slice
   auto frag_row = [&](int j) {
@@ -208,6 +209,9 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
 #pragma unroll
   for (int j = 0; j < NFR; ++j) scale_one(smem, j, sc);
 
+  // the reads that follow MFMA i of a step: all of them behind the first MFMAs, RPM
+  // behind each
+  auto read_from = [](int i) { return i * RPM < NFR ? i * RPM : NFR; };
 #define RPX_MX_STEP(STEP, F, MORE)                                                               \
   _Pragma("unroll") for (int i = 0; i < NMF; ++i) {                                              \
     acc[i / FM][i % FM] = mx_mfma32<STEP, STEP>(F[FM + i / FM], sc[FM + i / FM], F[i % FM],      \
@@ -216,8 +220,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
     MORE __builtin_amdgcn_sched_barrier(0);                                                      \
   }
 #define RPX_MX_READS(ST, STEP, F)                                                                \
-  _Pragma("unroll") for (int j = i * NFR / NMF; j < (i + 1) * NFR / NMF; ++j)                    \
-      frag_one(ST, STEP, j, F);
+  _Pragma("unroll") for (int j = read_from(i); j < read_from(i + 1); ++j) frag_one(ST, STEP, j, F);
 
   int stage = 0;
   for (int t = 0; t < ns; ++t) {
@@ -233,7 +236,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
       _Pragma("unroll") for (int d = i * LPW / NMF; d < (i + 1) * LPW / NMF; ++d)
           dma_one(st, refill, d);
       RPX_MX_READS(nst, 0, fx)
-      _Pragma("unroll") for (int j = i * NFR / NMF; j < (i + 1) * NFR / NMF; ++j)
+      _Pragma("unroll") for (int j = read_from(i); j < read_from(i + 1); ++j)
           scale_one(nst, j, sc_next);
     })
 #pragma unroll
