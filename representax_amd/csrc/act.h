@@ -75,6 +75,17 @@ __device__ __forceinline__ float act_silu_grad(float g, float s) {
   return s * (1.0f + g * act_sigmoid(-g));
 }
 
+// Both gradients of silu(g) u from one exponential: with s = sigmoid(g) and
+// h = g s, silu'(g) = s + h (1 - s). 1 - s loses its relative precision only where
+// s is near 1 and the sum does not need it.
+__device__ __forceinline__ void act_silu_mul_grads(float dh, float g, float u, float* dg,
+                                                   float* du) {
+  const float s = act_sigmoid(g);
+  const float h = g * s;
+  *du = dh * h;
+  *dg = dh * u * __builtin_fmaf(h, 1.0f - s, s);
+}
+
 // One output element (two for kActSiluMulBwd) from v and the auxiliary
 // operands a0 (z or gate) and a1 (up).
 template <int ACT>

@@ -87,7 +87,7 @@ int serve(const char* who, const void* x, int dtype, int64_t m, int64_t k, int64
   MxParts parts{};
   parts.part[0] = MxPart{x, dtype, m, k, row_stride,
                          MxOut{e.codes, e.scales, mx_slices(k) * kMxSliceBytes, mx_pad_rows(m)},
-                         MxOut{}, false, 0};
+                         MxOut{}, 0};
   RPX_HIP(launch_mx_quantize(parts, 1, st), who);
   const MxGemm g{e.codes, e.scales, codes, scales, up_codes, up_scales, m, n, mx_slices(k),
                  y, nullptr, nullptr, dtype};
@@ -114,7 +114,7 @@ size_t rpx_mxfp4_scale_bytes(int64_t rows, int64_t columns) {
 
 int rpx_mxfp4_quantize(const rpx_mxfp4_part* parts, int64_t count, void* stream) {
   const char* who = "rpx_mxfp4_quantize";
-  if (count < 0 || count > kMxParts)
+  if (count < 0 || count > kMxParts / 2)
     return fail_invalid("rpx_mxfp4_quantize: need 0 <= count <= 4");
   if (count > 0 && parts == nullptr) return fail_invalid("rpx_mxfp4_quantize: null pointer");
   MxParts args{};
@@ -143,7 +143,7 @@ int rpx_mxfp4_quantize(const rpx_mxfp4_part* parts, int64_t count, void* stream)
     args.part[jobs++] =
         MxPart{in.t, in.dtype, in.rows, in.columns, in.row_stride,
                MxOut{in.codes, in.scales, stride, mx_pad_rows(in.rows)},
-               MxOut{in.codes_t, in.scales_t, stride_t, mx_pad_rows(in.columns)}, false, 0};
+               MxOut{in.codes_t, in.scales_t, stride_t, mx_pad_rows(in.columns)}, 0};
   }
   RPX_HIP(launch_mx_quantize(args, jobs, static_cast<hipStream_t>(stream)), who);
   return kOk;

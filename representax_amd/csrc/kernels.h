@@ -336,14 +336,13 @@ struct CastMany {
 hipError_t launch_cast_many(CastMany args, int tensors, hipStream_t stream);
 
 // MXFP4 (mxfp4.h) -----------------------------------------------------------
-constexpr int kMxParts = 4;  // matrices of one launch
+constexpr int kMxParts = 8;  // encodings of one launch: two of each of four matrices
 struct MxPart {
   const void* t;
   int dtype;
   int64_t rows, columns, row_stride;  // in elements, columns dense
   MxOut along, across;  // its encoding along its columns, its transpose's (codes null: none)
-  bool aligned;         // set by the launcher, as `tiles`
-  int64_t tiles;
+  int64_t tiles;  // set by the launcher
 };
 struct MxParts {
   MxPart part[kMxParts];

@@ -10,15 +10,24 @@ namespace rpx {
 namespace {
 
 constexpr int kThreads = 256;
+// Waves of the fused form (32 KB read each) from which both encodings come from one
+// read; below, each from its own. Measured, fused against apart: 12.3 / 8.1 us at
+// 8192 x 768 bf16 (384 waves), 15.5 / 14.7 at 6144 x 2048 (768), 23.2 / 34.3 at
+// 16384 x 2048 (2048); 11.5 / 12.2 at 5003 x 1000 float32 (640), 12.2 / 13.3 at
+// 8192 x 768 (768), 12.9 / 16.7 at 2048 x 4096 (1024).
+constexpr int64_t kMxFusedWaves = 768;
 
-// Maximum over the four (or, EIGHT, eight) neighbouring lanes that share a block.
-template <bool EIGHT>
+// Maximum over the LANES neighbouring lanes that share a block.
+template <int LANES>
 __device__ __forceinline__ uint32_t block_max(uint32_t v) {
+  static_assert(LANES == 4 || LANES == 8 || LANES == 16, "lanes of a block");
   auto with = [](uint32_t x, uint32_t y) { return y > x ? y : x; };
   v = with(v, __builtin_amdgcn_update_dpp(0u, v, 0xB1, 0xF, 0xF, false));  // lane ^ 1
   v = with(v, __builtin_amdgcn_update_dpp(0u, v, 0x4E, 0xF, 0xF, false));  // lane ^ 2
-  if constexpr (EIGHT)
+  if constexpr (LANES >= 8)
     v = with(v, __builtin_amdgcn_update_dpp(0u, v, 0x141, 0xF, 0xF, false));  // 7 - lane
+  if constexpr (LANES >= 16)
+    v = with(v, __builtin_amdgcn_update_dpp(0u, v, 0x140, 0xF, 0xF, false));  // 15 - lane
   return v;
 }
 
@@ -28,87 +37,136 @@ __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
                                                                 __builtin_bit_cast(u16x2_t, b)));
 }
 
-// What a thread reads of one row: 16 bytes, VPT values.
-template <int DTYPE>
-struct Piece {
-  static constexpr int VPT = DTYPE == kBF16 ? 8 : 4;
-  static constexpr bool EIGHT = DTYPE != kBF16;  // lanes per block: 32 / VPT
-  u32x4_t w;
+__device__ __forceinline__ float as_f32(uint32_t v) { return __builtin_bit_cast(float, v); }
 
-  // Columns c .. c + VPT - 1; zeros outside [0, columns). ALIGNED: 16-byte loads
-  // may be used.
-  __device__ __forceinline__ void load(const void* row, int64_t c, int64_t columns, bool aligned) {
-    const uint8_t* p = static_cast<const uint8_t*>(row) + c * (16 / VPT);
-    if (aligned && c + VPT <= columns) {
-      w = *reinterpret_cast<const u32x4_t*>(p);
-      return;
-    }
-    w = u32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < VPT; ++e) {
-      if (c + e >= columns) continue;
-      if constexpr (DTYPE == kBF16)
-        w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
-      else
-        w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-    }
-  }
+// What a thread holds of one row: W words, COLS consecutive columns.
+template <int DTYPE, int W>
+struct Piece {
+  static constexpr int COLS = DTYPE == kBF16 ? 2 * W : W;
+  static constexpr int LANES = kMxBlock / COLS;  // that share a block
+  static constexpr int SIZE = DTYPE == kBF16 ? 2 : 4;
+  uint32_t w[W];
 
   // Largest magnitude's float32 bits (an integer maximum: infinities and NaN on top).
   __device__ __forceinline__ uint32_t amax() const {
+    uint32_t a = 0;
     if constexpr (DTYPE == kBF16) {
-      const uint32_t m = 0x7FFF7FFFu;
-      const uint32_t a = pk_max(pk_max(w[0] & m, w[1] & m), pk_max(w[2] & m, w[3] & m));
+#pragma unroll
+      for (int i = 0; i < W; ++i) a = pk_max(a, w[i] & 0x7FFF7FFFu);
       return (a << 16) > (a & 0xFFFF0000u) ? a << 16 : a & 0xFFFF0000u;
     } else {
-      uint32_t a = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) a = (w[e] & 0x7FFFFFFFu) > a ? w[e] & 0x7FFFFFFFu : a;
+      for (int i = 0; i < W; ++i) a = (w[i] & 0x7FFFFFFFu) > a ? w[i] & 0x7FFFFFFFu : a;
       return a;
     }
   }
 
-  // VPT codes (4 VPT bits).
-  __device__ __forceinline__ uint32_t encode(uint32_t byte) const {
+  // The codes of the block with scale `byte`, stored at column c of a row of codes.
+  __device__ __forceinline__ void store(uint8_t* codes, int64_t c, uint32_t byte) const {
     const float scale = mx_scale_operand(byte);
-    uint32_t c;
+    uint32_t code = 0;
     if constexpr (DTYPE == kBF16) {
-      c = mx_encode8(w, scale);
+      code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, mx_as_bf16x2(w[0]), scale, 0);
+      if constexpr (W > 1)
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, mx_as_bf16x2(w[1]), scale, 1);
+      if constexpr (W > 2) {
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, mx_as_bf16x2(w[2]), scale, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, mx_as_bf16x2(w[3]), scale, 3);
+      }
     } else {
-      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, as_f32(w[0]), as_f32(w[1]), scale, 0);
-      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, as_f32(w[2]), as_f32(w[3]), scale, 1);
+      static_assert(W > 1, "a byte of codes holds two columns");
+      code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, as_f32(w[0]), as_f32(w[1]), scale, 0);
+      if constexpr (W > 2)
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, as_f32(w[2]), as_f32(w[3]), scale, 1);
     }
-    return byte == 255u ? 0u : c;
+    code = byte == 255u ? 0u : code;
+    if constexpr (COLS == 8)
+      *reinterpret_cast<uint32_t*>(codes + c / 2) = code;
+    else if constexpr (COLS == 4)
+      *reinterpret_cast<uint16_t*>(codes + c / 2) = static_cast<uint16_t>(code);
+    else
+      codes[c / 2] = static_cast<uint8_t>(code);
   }
-
-  static __device__ __forceinline__ float as_f32(uint32_t v) { return __builtin_bit_cast(float, v); }
 };
 
-template <int DTYPE>
-__device__ __forceinline__ void store_piece(uint8_t* codes, int64_t c, uint32_t code) {
-  if constexpr (DTYPE == kBF16)
-    *reinterpret_cast<uint32_t*>(codes + c / 2) = code;
-  else
-    *reinterpret_cast<uint16_t*>(codes + c / 2) = static_cast<uint16_t>(code);
-}
+// The loads of a thread's column: whole words wherever the row has them, also at
+// addresses that are not aligned (the hardware takes any), with the columns past
+// the end masked off. Reading past a row's end runs into the next row, so the
+// last row, and rows narrower than a piece, are read element by element.
+template <int DTYPE, int W>
+struct Column {
+  using P = Piece<DTYPE, W>;
+  const uint8_t* base;
+  int64_t stride, c, columns;
+  uint32_t mask[W];
+
+  __device__ __forceinline__ Column(const MxPart& part, int64_t col)
+      : base(static_cast<const uint8_t*>(part.t)), stride(part.row_stride * P::SIZE), c(col),
+        columns(part.columns) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (DTYPE == kBF16)
+        mask[i] = (c + 2 * i < columns ? 0xFFFFu : 0u) | (c + 2 * i + 1 < columns ? 0xFFFF0000u : 0u);
+      else
+        mask[i] = c + i < columns ? ~0u : 0u;
+    }
+  }
+
+  __device__ __forceinline__ P whole(int64_t row) const {
+    struct Words {
+      uint32_t w[W];
+    };
+    Words x;
+    __builtin_memcpy(&x, base + row * stride + (c < columns ? c : 0) * P::SIZE, sizeof(x));
+    P v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] = x.w[i] & mask[i];
+    return v;
+  }
+  // Element by element, the columns past the end re-reading the last.
+  __device__ __forceinline__ P some(int64_t row) const {
+    P v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < P::COLS; ++e) {
+      const int64_t at = c + e < columns ? c + e : columns - 1;
+      if constexpr (DTYPE == kBF16)
+        v.w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(base + row * stride)[at])
+                      << (16 * (e & 1));
+      else
+        v.w[e] = reinterpret_cast<const uint32_t*>(base + row * stride)[at];
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] &= mask[i];
+    return v;
+  }
+};
 
 // Along the columns only: a thread takes 16 bytes of a row, neighbouring lanes a
 // block. A pass over memory (serving: the input of a product).
 template <int DTYPE>
 __device__ __forceinline__ void quantize_rows(const MxPart& part, int64_t i) {
-  using P = Piece<DTYPE>;
-  const int64_t per = mx_slices(part.columns) * (kMxSlice / P::VPT);
+  using P = Piece<DTYPE, 4>;
+  const int64_t per = mx_slices(part.columns) * (kMxSlice / P::COLS);
   const int64_t row = i / per;
-  const int64_t c = (i % per) * P::VPT;
+  const int64_t c = (i % per) * P::COLS;
   if (row >= part.along.scale_rows) return;  // whole blocks: `per` is a multiple of their lanes
-  P v;
-  v.w = u32x4_t{0, 0, 0, 0};
-  if (row < part.rows)
-    v.load(static_cast<const uint8_t*>(part.t) + row * part.row_stride * (16 / P::VPT), c,
-           part.columns, part.aligned);
-  const uint32_t byte = row < part.rows ? mx_scale_byte(block_max<P::EIGHT>(v.amax())) : 0u;
-  if (row < part.rows)
-    store_piece<DTYPE>(part.along.codes + row * part.along.row_bytes, c, v.encode(byte));
+  uint32_t byte = 0;
+  if (row < part.rows) {
+    P v;
+    if (c + P::COLS <= part.columns) {
+      __builtin_memcpy(&v,
+                       static_cast<const uint8_t*>(part.t) + (row * part.row_stride + c) * P::SIZE,
+                       sizeof(v));
+    } else if (c < part.columns) {
+      v = Column<DTYPE, 4>(part, c).some(row);
+    } else {
+      v = P{};
+    }
+    byte = mx_scale_byte(block_max<P::LANES>(v.amax()));
+    v.store(part.along.codes + row * part.along.row_bytes, c, byte);
+  }
   if (c % kMxBlock == 0) *mx_scale_at(part.along, row, c / kMxBlock) = static_cast<uint8_t>(byte);
 }
 
@@ -124,53 +182,72 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_rows(MxParts parts) {
     quantize_rows<kF32>(parts.part[p], i);
 }
 
-// Along both axes from one read. A thread owns 32 rows of its 16 bytes: whole
+// Along both axes from one read. A thread owns 32 rows of its W words: whole
 // blocks of the transpose, in registers, so nothing goes through LDS; a block
 // along the columns is shared by neighbouring lanes as above. A wave covers 128
-// rows of 16 pieces, so that its stores of either encoding are 64 contiguous bytes
+// rows of 16 pieces, so that its stores of the transpose are 64 contiguous bytes
 // of a row of codes.
-template <int DTYPE>
+template <int DTYPE, int W>
 __device__ __forceinline__ void quantize_both(const MxPart& part, int64_t tile, int lane) {
-  using P = Piece<DTYPE>;
-  constexpr int COLS = 16 * P::VPT;
+  using P = Piece<DTYPE, W>;
+  constexpr int COLS = 16 * P::COLS;
   const int64_t per = ceil_div(part.along.codes != nullptr ? mx_slices(part.columns) * kMxSlice
-                                                           : part.columns, COLS);
+                                                           : part.across.scale_rows,
+                               COLS);
   const int64_t r0 = (tile / per) * 128 + (lane >> 4) * 32;
-  const int64_t c = (tile % per) * COLS + (lane & 15) * P::VPT;
+  const int64_t c = (tile % per) * COLS + (lane & 15) * P::COLS;
+  const Column<DTYPE, W> col(part, c);
   P v[32];
-  const uint8_t* base =
-      static_cast<const uint8_t*>(part.t) + r0 * part.row_stride * (16 / P::VPT);
+  const int64_t last = part.rows - 1;
+  if (last > 0 && part.columns >= P::COLS) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    v[i].w = u32x4_t{0, 0, 0, 0};
-    if (r0 + i < part.rows)
-      v[i].load(base + i * part.row_stride * (16 / P::VPT), c, part.columns, part.aligned);
-  }
-  if (part.along.codes != nullptr && r0 < part.along.scale_rows) {
-    uint32_t kept = 0;  // the scale of this lane's share of four (eight) rows
-    constexpr int LANES = kMxBlock / P::VPT;
+    for (int i = 0; i < 32; ++i) v[i] = col.whole(r0 + i < last ? r0 + i : last - 1);
+    if (r0 + 31 >= last) {
+      const P end = col.some(last);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+#pragma unroll
+        for (int q = 0; q < W; ++q)
+          v[i].w[q] = r0 + i < last ? v[i].w[q] : r0 + i == last ? end.w[q] : 0u;
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const uint32_t byte = mx_scale_byte(block_max<P::EIGHT>(v[i].amax()));
+      v[i] = col.some(r0 + i < last ? r0 + i : last);
+#pragma unroll
+      for (int q = 0; q < W; ++q) v[i].w[q] = r0 + i <= last ? v[i].w[q] : 0u;
+    }
+  }
+  constexpr int LANES = P::LANES;
+  if constexpr (LANES > 16) {  // across only
+  } else if (part.along.codes != nullptr && r0 < part.along.scale_rows) {
+    uint32_t kept = 0;  // the scale of this lane's share of LANES rows
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint32_t byte = mx_scale_byte(block_max<LANES>(v[i].amax()));
       if (r0 + i < part.rows)
-        store_piece<DTYPE>(part.along.codes + (r0 + i) * part.along.row_bytes, c,
-                           v[i].encode(byte));
-      if ((lane & (LANES - 1)) == i % LANES) kept = byte;
+        v[i].store(part.along.codes + (r0 + i) * part.along.row_bytes, c, byte);
+      kept = (lane & (LANES - 1)) == i % LANES ? byte : kept;
       if (i % LANES == LANES - 1)
         *mx_scale_at(part.along, r0 + i - (LANES - 1) + (lane & (LANES - 1)), c / kMxBlock) =
             static_cast<uint8_t>(kept);
     }
   }
   if (part.across.codes == nullptr) return;
-  if constexpr (DTYPE == kBF16) {
+  auto store = [&](int64_t at, u32x4_t code, uint32_t byte) {
+    if (at < part.columns)
+      *reinterpret_cast<u32x4_t*>(part.across.codes + at * part.across.row_bytes + r0 / 2) = code;
+    if (at < part.across.scale_rows)
+      *mx_scale_at(part.across, at, r0 / kMxBlock) = static_cast<uint8_t>(byte);
+  };
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {  // columns c + 2 q and c + 2 q + 1
+  for (int q = 0; q < W; ++q) {
+    if constexpr (DTYPE == kBF16) {  // columns c + 2 q and c + 2 q + 1
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 32; ++i) top = pk_max(top, v[i].w[q] & 0x7FFF7FFFu);
 #pragma unroll
       for (int odd = 0; odd < 2; ++odd) {
-        const int64_t col = c + 2 * q + odd;
         const uint32_t byte = mx_scale_byte(odd ? top & 0xFFFF0000u : top << 16);
         const float scale = mx_scale_operand(byte);
         u32x4_t code;
@@ -183,26 +260,15 @@ __device__ __forceinline__ void quantize_both(const MxPart& part, int64_t tile, 
                                              odd ? 0x07060302u : 0x05040100u);
           code[g] = byte == 255u ? 0u : mx_encode8(pairs, scale);
         }
-        if (col < part.columns)
-          *reinterpret_cast<u32x4_t*>(part.across.codes + col * part.across.row_bytes + r0 / 2) =
-              code;
-        if (col < part.across.scale_rows)
-          *mx_scale_at(part.across, col, r0 / kMxBlock) = static_cast<uint8_t>(byte);
+        store(c + 2 * q + odd, code, byte);
       }
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t col = c + q;
+    } else {
       float x[kMxBlock];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = P::as_f32(v[i].w[q]);
+      for (int i = 0; i < 32; ++i) x[i] = as_f32(v[i].w[q]);
       uint32_t byte;
       const u32x4_t code = mx_encode_block(x, &byte);
-      if (col < part.columns)
-        *reinterpret_cast<u32x4_t*>(part.across.codes + col * part.across.row_bytes + r0 / 2) = code;
-      if (col < part.across.scale_rows)
-        *mx_scale_at(part.across, col, r0 / kMxBlock) = static_cast<uint8_t>(byte);
+      store(c + q, code, byte);
     }
   }
 }
@@ -215,7 +281,35 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_both(MxParts parts) {
   while (blk >= parts.first[p + 1]) ++p;
   const int64_t wave = (blk - parts.first[p]) * (kThreads / 64) + (threadIdx.x >> 6);
   if (wave >= parts.part[p].tiles) return;
-  quantize_both<DTYPE>(parts.part[p], wave, threadIdx.x & 63);
+  quantize_both<DTYPE, 4>(parts.part[p], wave, threadIdx.x & 63);
+}
+
+// The two encodings of a small matrix by different workgroups, each from its own
+// read: a part is along its columns or across them. A wave of the fused form above
+// is a chain of 5 us of instructions in a launch of few waves; the two halves of it
+// run side by side instead.
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
+    k_mx_quantize_apart(MxParts parts) {
+  const int64_t blk = block_of_grid();
+  if (blk >= parts.first[kMxParts]) return;
+  int p = 0;
+  while (blk >= parts.first[p + 1]) ++p;
+  const MxPart& part = parts.part[p];
+  const int64_t first = blk - parts.first[p];
+  if (part.across.codes == nullptr) {
+    const int64_t i = first * kThreads + threadIdx.x;
+    if (part.dtype == kBF16)
+      quantize_rows<kBF16>(part, i);
+    else
+      quantize_rows<kF32>(part, i);
+    return;
+  }
+  const int64_t wave = first * (kThreads / 64) + (threadIdx.x >> 6);
+  if (wave >= part.tiles) return;
+  if (part.dtype == kBF16)
+    quantize_both<kBF16, 1>(part, wave, threadIdx.x & 63);
+  else
+    quantize_both<kF32, 1>(part, wave, threadIdx.x & 63);
 }
 
 // The gradients of a gated block's projections, z_gate and z_up [m, n]:
@@ -239,13 +333,19 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   constexpr int CHUNK = 4;  // rows whose loads are in flight at once
   constexpr int WORDS = DTYPE == kBF16 ? 1 : 2;
   uint32_t raw[2][CHUNK][3][WORDS];
-  // columns past the end read the last ones and rows past the end the last row;
-  // their gradients are set to zero below
+  // columns past the end read the last ones and rows past the end the last row; they
+  // are set to zero before use, which makes their gradients zero
   const bool pair = (n & 1) == 0;
   const uint32_t c0 = static_cast<uint32_t>(c < n ? c : n - 1);
   const uint32_t c1 = static_cast<uint32_t>(c + 1 < n ? c + 1 : n - 1);
   const uint32_t cp = static_cast<uint32_t>(c < n ? c : n - 2);
-  const uint32_t in_column[2] = {c < n ? ~0u : 0u, c + 1 < n ? ~0u : 0u};
+  uint32_t in_column[WORDS];
+  if constexpr (DTYPE == kBF16) {
+    in_column[0] = (c < n ? 0xFFFFu : 0u) | (c + 1 < n ? 0xFFFF0000u : 0u);
+  } else {
+    in_column[0] = c < n ? ~0u : 0u;
+    in_column[1] = c + 1 < n ? ~0u : 0u;
+  }
   const int left = static_cast<int>(m - r0 < 32 ? m - r0 : 32);
   auto load = [&](int chunk) {
 #pragma unroll
@@ -279,9 +379,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   auto along_byte = [](float x, float y) {
     const uint32_t a = __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu;
     const uint32_t b = __builtin_bit_cast(uint32_t, y) & 0x7FFFFFFFu;
-    const uint32_t h = block_max<true>(a > b ? a : b);
-    const uint32_t o = __builtin_amdgcn_update_dpp(0u, h, 0x140, 0xF, 0xF, false);  // 15 - lane
-    return mx_scale_byte(o > h ? o : h);
+    return mx_scale_byte(block_max<16>(a > b ? a : b));
   };
   uint32_t kept[2] = {0, 0};  // this lane's share of the scales of sixteen rows
   load(0);
@@ -290,19 +388,19 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     if (chunk + 1 < 32 / CHUNK) load(chunk + 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < CHUNK; ++i)
+    for (int i = 0; i < CHUNK; ++i) {
+      const int row = chunk * CHUNK + i;
+      const uint32_t in_row = static_cast<uint32_t>((row - left) >> 31);  // all ones below m
+      uint32_t(&w)[3][WORDS] = raw[chunk & 1][i];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = chunk * CHUNK + i;
-        float gate;
-        const float up =
-            act_apply<kActSiluMulBwd>(value(raw[chunk & 1][i][0], e), value(raw[chunk & 1][i][1], e),
-                                      value(raw[chunk & 1][i][2], e), &gate);
-        // all ones where the row is below m and the column below n
-        const uint32_t in = static_cast<uint32_t>((row - left) >> 31) & in_column[e];
-        d[0][e][row] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, gate) & in);
-        d[1][e][row] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, up) & in);
-      }
+      for (int t = 0; t < 3; ++t)
+#pragma unroll
+        for (int e = 0; e < WORDS; ++e) w[t][e] &= in_row & in_column[e];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        act_silu_mul_grads(value(w[0], e), value(w[1], e), value(w[2], e), &d[0][e][row],
+                           &d[1][e][row]);
+    }
     if (along.codes != nullptr && left > 0) {
 #pragma unroll
       for (int i = 0; i < CHUNK; ++i)
@@ -399,43 +497,64 @@ hipError_t launch_mx_zero(void* out, int64_t bytes, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// One launch for the parts encoded along both axes of each type and size class, one
+// for those along their columns only.
 hipError_t launch_mx_quantize(MxParts parts, int count, hipStream_t stream) {
-  // Parts along both axes (or across only) go to one launch per type, the others
-  // to one more.
-  for (int kind = 0; kind < 3; ++kind) {
-    MxParts some{};
-    int jobs = 0;
-    for (int p = 0; p < count; ++p) {
-      MxPart part = parts.part[p];
-      const bool both = part.across.codes != nullptr;
-      if (kind != (both ? (part.dtype == kBF16 ? 0 : 1) : 2)) continue;
-      const int vpt = part.dtype == kBF16 ? 8 : 4;
-      const int size = part.dtype == kBF16 ? 2 : 4;
-      part.aligned = (reinterpret_cast<uintptr_t>(part.t) & 15) == 0 &&
-                     (part.row_stride * size) % 16 == 0;
-      int64_t blocks;
-      if (both) {
-        const int64_t columns =
-            part.along.codes != nullptr ? mx_slices(part.columns) * kMxSlice : part.columns;
-        part.tiles = mx_slices(part.rows) * 2 * ceil_div(columns, 16 * vpt);
-        blocks = ceil_div(part.tiles, kThreads / 64);
-      } else {
-        blocks = ceil_div(part.along.scale_rows * mx_slices(part.columns) * (kMxSlice / vpt),
-                          kThreads);
+  // waves of 128 rows of 16 pieces of `cols` columns
+  auto tiles_of = [](const MxPart& part, int cols) {
+    const int64_t columns =
+        part.along.codes != nullptr ? mx_slices(part.columns) * kMxSlice : part.across.scale_rows;
+    return mx_slices(part.rows) * 2 * ceil_div(columns, 16 * cols);
+  };
+  int64_t waves = 0;
+  for (int p = 0; p < count; ++p)
+    if (parts.part[p].across.codes != nullptr)
+      waves += tiles_of(parts.part[p], parts.part[p].dtype == kBF16 ? 8 : 4);
+  const bool fused = waves >= kMxFusedWaves;
+  enum { kRows, kFusedF32, kFusedBF16, kApart, kKinds };
+  MxParts some[kKinds] = {};
+  int jobs[kKinds] = {};
+  auto add = [&](int kind, const MxPart& part, int64_t blocks) {
+    MxParts& to = some[kind];
+    int& j = jobs[kind];
+    to.part[j] = part;
+    to.first[j + 1] = to.first[j] + blocks;
+    ++j;
+  };
+  auto row_blocks = [](const MxPart& part) {
+    return ceil_div(part.along.scale_rows * mx_slices(part.columns) *
+                        (kMxSlice / (part.dtype == kBF16 ? 8 : 4)),
+                    kThreads);
+  };
+  for (int p = 0; p < count; ++p) {
+    MxPart part = parts.part[p];
+    const bool bf16 = part.dtype == kBF16;
+    if (part.across.codes == nullptr) {
+      // beside encodings along both axes it costs no launch of its own
+      add(waves > 0 && !fused ? kApart : kRows, part, row_blocks(part));
+    } else if (fused && part.along.codes != nullptr) {
+      part.tiles = tiles_of(part, bf16 ? 8 : 4);
+      add(bf16 ? kFusedBF16 : kFusedF32, part, ceil_div(part.tiles, kThreads / 64));
+    } else {
+      MxPart across = part;
+      across.along = MxOut{};
+      across.tiles = tiles_of(across, bf16 ? 2 : 1);
+      add(kApart, across, ceil_div(across.tiles, kThreads / 64));
+      if (part.along.codes != nullptr) {
+        part.across = MxOut{};
+        add(kApart, part, row_blocks(part));
       }
-      some.part[jobs] = part;
-      some.first[jobs + 1] = some.first[jobs] + blocks;
-      ++jobs;
     }
-    if (jobs == 0) continue;
-    const int64_t total = some.first[jobs];
-    for (int j = jobs; j < kMxParts; ++j) some.first[j + 1] = total;
-    if (kind == 0)
-      hipLaunchKernelGGL(k_mx_quantize_both<kBF16>, grid_of(total), dim3(kThreads), 0, stream, some);
-    else if (kind == 1)
-      hipLaunchKernelGGL(k_mx_quantize_both<kF32>, grid_of(total), dim3(kThreads), 0, stream, some);
-    else
-      hipLaunchKernelGGL(k_mx_quantize_rows, grid_of(total), dim3(kThreads), 0, stream, some);
+  }
+  for (int kind = 0; kind < kKinds; ++kind) {
+    if (jobs[kind] == 0) continue;
+    const int64_t total = some[kind].first[jobs[kind]];
+    for (int j = jobs[kind]; j < kMxParts; ++j) some[kind].first[j + 1] = total;
+    auto* kernel = kind == kRows        ? k_mx_quantize_rows
+                   : kind == kFusedF32  ? k_mx_quantize_both<kF32>
+                   : kind == kFusedBF16 ? k_mx_quantize_both<kBF16>
+                                        : k_mx_quantize_apart;
+    hipLaunchKernelGGL(kernel, grid_of(total), dim3(kThreads), 0, stream, some[kind]);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;
