@@ -653,6 +653,61 @@ int rpx_mxfp4_gated_backward(const void* dh, const void* z_gate, const void* z_u
                              int64_t m, int64_t n, uint8_t* codes, uint8_t* scales,
                              uint8_t* codes_t, uint8_t* scales_t, void* stream);
 
+/* A linear's training step: y [m, n] = left [m, k] right [k, n] with both
+ * operands encoded along k, and (for the gradients that are asked for) left's
+ * transpose along m and right along n, which `saved` keeps for the backward
+ * (rpx_mxfp4_linear_saved_bytes; NULL where neither is needed). left has
+ * left_stride elements between rows; of right's strides one is 1 and the other
+ * spans it (a row-major operand, or the transposed view of a row-major weight).
+ * Operands may lie at any alignment of their elements; up to 14 bytes past the
+ * end of a row but the last are read (the next row, or the gap before it). */
+size_t rpx_mxfp4_linear_saved_bytes(int64_t m, int64_t n, int64_t k, int need_left,
+                                    int need_right);
+size_t rpx_mxfp4_linear_forward_workspace(int64_t m, int64_t n, int64_t k);
+int rpx_mxfp4_linear_forward(const void* left, int left_dtype, int64_t m, int64_t k,
+                             int64_t left_stride, const void* right, int right_dtype, int64_t n,
+                             int64_t right_row_stride, int64_t right_col_stride, void* y,
+                             int out_dtype, void* saved, size_t saved_bytes, int need_left,
+                             int need_right, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* d_left [m, k] = grad right^T and d_right, as [n, k], = grad^T left, from
+ * grad [m, n] and the forward's `saved` (with its need_left and need_right);
+ * either may be NULL. */
+size_t rpx_mxfp4_linear_backward_workspace(int64_t m, int64_t n, int64_t k, int need_left,
+                                           int need_right);
+int rpx_mxfp4_linear_backward(const void* grad, int grad_dtype, int64_t m, int64_t n,
+                              int64_t grad_stride, const void* saved, size_t saved_bytes,
+                              int64_t k, int need_left, int need_right, void* d_left,
+                              int left_dtype, void* d_right, int right_dtype, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* The gated block's training step: h [m, n] = silu(left gate) * (left up),
+ * gate and up [k, n] with strides as the linear's right operand. z_gate and z_up
+ * [m, n] (both or neither) receive the rounded products, `saved` what the
+ * backward's products read. */
+size_t rpx_mxfp4_gated_saved_bytes(int64_t m, int64_t n, int64_t k, int need_left,
+                                   int need_weights);
+size_t rpx_mxfp4_gated_forward_workspace(int64_t m, int64_t n, int64_t k);
+int rpx_mxfp4_gated_forward(const void* left, int left_dtype, int64_t m, int64_t k,
+                            int64_t left_stride, const void* gate, int gate_dtype,
+                            int64_t gate_row_stride, int64_t gate_col_stride, const void* up,
+                            int up_dtype, int64_t up_row_stride, int64_t up_col_stride, int64_t n,
+                            void* h, void* z_gate, void* z_up, int out_dtype, void* saved,
+                            size_t saved_bytes, int need_left, int need_weights, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* d_left [m, k] and d_weights [2 n, k] (the gate's gradient over the up
+ * projection's) for the gradient dh [m, n] of h; either may be NULL. */
+size_t rpx_mxfp4_gated_backward_workspace(int64_t m, int64_t n, int64_t k, int need_left,
+                                          int need_weights);
+int rpx_mxfp4_gated_backward_products(const void* dh, const void* z_gate, const void* z_up,
+                                      int dtype, int64_t m, int64_t n, const void* saved,
+                                      size_t saved_bytes, int64_t k, int need_left,
+                                      int need_weights, void* d_left, int left_dtype,
+                                      void* d_weights, int weights_dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
 /* y [m, n] = x W^T with x [m, k] encoded within the call (inference over a
  * kept weight); row_stride elements between rows of x. */
 size_t rpx_mxfp4_linear_workspace(int64_t m, int64_t n, int64_t k);

@@ -160,6 +160,32 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rpx_mxfp4_gated_backward": (
         _int, [_p, _p, _p, _int, _i64, _i64, _p, _p, _p, _p, _p]
     ),
+    "rpx_mxfp4_linear_saved_bytes": (_size, [_i64, _i64, _i64, _int, _int]),
+    "rpx_mxfp4_linear_forward_workspace": (_size, [_i64, _i64, _i64]),
+    "rpx_mxfp4_linear_forward": (
+        _int,
+        [_p, _int, _i64, _i64, _i64, _p, _int, _i64, _i64, _i64, _p, _int, _p, _size, _int, _int,
+         _p, _size, _p],
+    ),
+    "rpx_mxfp4_linear_backward_workspace": (_size, [_i64, _i64, _i64, _int, _int]),
+    "rpx_mxfp4_linear_backward": (
+        _int,
+        [_p, _int, _i64, _i64, _i64, _p, _size, _i64, _int, _int, _p, _int, _p, _int, _p, _size,
+         _p],
+    ),
+    "rpx_mxfp4_gated_saved_bytes": (_size, [_i64, _i64, _i64, _int, _int]),
+    "rpx_mxfp4_gated_forward_workspace": (_size, [_i64, _i64, _i64]),
+    "rpx_mxfp4_gated_forward": (
+        _int,
+        [_p, _int, _i64, _i64, _i64, _p, _int, _i64, _i64, _p, _int, _i64, _i64, _i64, _p, _p, _p,
+         _int, _p, _size, _int, _int, _p, _size, _p],
+    ),
+    "rpx_mxfp4_gated_backward_workspace": (_size, [_i64, _i64, _i64, _int, _int]),
+    "rpx_mxfp4_gated_backward_products": (
+        _int,
+        [_p, _p, _p, _int, _i64, _i64, _p, _size, _i64, _int, _int, _p, _int, _p, _int, _p, _size,
+         _p],
+    ),
     "rpx_mxfp4_linear_workspace": (_size, [_i64, _i64, _i64]),
     "rpx_mxfp4_linear": (
         _int, [_p, _int, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _size, _p]

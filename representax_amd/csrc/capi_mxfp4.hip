@@ -30,31 +30,81 @@ int check_pointers(const char* who, std::initializer_list<const void*> pointers)
   return kOk;
 }
 
-// The encoded forms of x that a call makes in its workspace.
+// An encoded matrix in a buffer.
 struct Encoded {
-  uint8_t* codes;
-  uint8_t* scales;
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
+  int64_t rows = 0, columns = 0;
+  MxOut out() const {
+    return codes == nullptr ? MxOut{}
+                            : MxOut{codes, scales, mx_slices(columns) * kMxSliceBytes,
+                                    mx_pad_rows(rows)};
+  }
 };
 
-Encoded take_encoded(Arena* arena, int64_t rows, int64_t columns) {
+// Carves an encoded matrix (or, not wanted, nothing) from an Arena, or counts its
+// bytes in a Sizer.
+Encoded take(Arena* a, bool wanted, int64_t rows, int64_t columns) {
   Encoded e;
-  e.codes = arena->take<uint8_t>(mx_code_bytes(rows, columns));
-  e.scales = arena->take<uint8_t>(mx_scale_bytes(rows, columns));
+  e.rows = rows;
+  e.columns = columns;
+  if (!wanted || rows == 0 || columns == 0) return e;
+  e.codes = a->take<uint8_t>(mx_code_bytes(rows, columns));
+  e.scales = a->take<uint8_t>(mx_scale_bytes(rows, columns));
   return e;
+}
+void take(Sizer* s, bool wanted, int64_t rows, int64_t columns) {
+  if (!wanted || rows == 0 || columns == 0) return;
+  s->take<uint8_t>(mx_code_bytes(rows, columns));
+  s->take<uint8_t>(mx_scale_bytes(rows, columns));
 }
 
 size_t encoded_bytes(int64_t rows, int64_t columns) {
   Sizer s;
-  s.take<uint8_t>(mx_code_bytes(rows, columns));
-  s.take<uint8_t>(mx_scale_bytes(rows, columns));
+  take(&s, true, rows, columns);
   return s.used;
+}
+
+// A B^T into out, zeros where nothing is summed; nothing for an empty output.
+int product(const char* who, const Encoded& a, const Encoded& b, void* out, int dtype,
+            float* partials, hipStream_t st) {
+  if (a.rows == 0 || b.rows == 0) return kOk;
+  if (a.columns == 0) {
+    RPX_HIP(launch_mx_zero(out, a.rows * b.rows * static_cast<int64_t>(elem_size(dtype)), st), who);
+    return kOk;
+  }
+  const MxGemm g{a.codes, a.scales, b.codes, b.scales, nullptr, nullptr, a.rows, b.rows,
+                 mx_slices(a.columns), out, nullptr, nullptr, dtype};
+  RPX_HIP(launch_mx_gemm(g, partials, st), who);
+  return kOk;
+}
+
+int64_t product_floats(int64_t m, int64_t n, int64_t k) {
+  return m <= 0 || n <= 0 || k <= 0 ? 0 : mx_gemm_workspace_floats(m, n, mx_slices(k));
+}
+
+// A weight as its product's right operand [k, n]: row-major, or (a transposed
+// view of a row-major weight [n, k]) column-major. Fills the part that encodes it
+// along k into w [n, k] and, where wanted, along n into wt [k, n].
+int weight_part(const char* who, const void* right, int dtype, int64_t k, int64_t n,
+                int64_t row_stride, int64_t col_stride, const Encoded& w, MxOut wt, MxPart* part) {
+  if (right == nullptr) return fail_invalid(std::string(who) + ": null pointer");
+  if (row_stride == 1 && (col_stride >= k || n <= 1)) {
+    *part = MxPart{right, dtype, n, k, n <= 1 ? k : col_stride, w.out(), wt, 0};
+  } else if (col_stride == 1 && (row_stride >= n || k <= 1)) {
+    *part = MxPart{right, dtype, k, n, k <= 1 ? n : row_stride, wt, w.out(), 0};
+  } else {
+    return fail_invalid(std::string(who) + ": one stride of the right operand must be 1, the "
+                                           "other span it");
+  }
+  return kOk;
 }
 
 size_t linear_workspace(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
   Sizer s;
-  s.used = encoded_bytes(m, k);
-  s.take<float>(mx_gemm_workspace_floats(m, n, mx_slices(k)));
+  take(&s, true, m, k);
+  s.take<float>(product_floats(m, n, k));
   return s.used;
 }
 
@@ -80,14 +130,12 @@ int serve(const char* who, const void* x, int dtype, int64_t m, int64_t k, int64
   RPX_TRY(check_pointers(who, {codes, scales, y}));
   if (gated) RPX_TRY(check_pointers(who, {up_codes, up_scales}));
   Arena arena(workspace, workspace == nullptr ? 0 : workspace_bytes);
-  const Encoded e = take_encoded(&arena, m, k);
+  const Encoded e = take(&arena, true, m, k);
   float* partials = gated ? nullptr : arena.take<float>(mx_gemm_workspace_floats(m, n, mx_slices(k)));
   if (arena.overflow) return fail_invalid(std::string(who) + ": workspace too small");
   RPX_TRY(check_pointers(who, {workspace}));
   MxParts parts{};
-  parts.part[0] = MxPart{x, dtype, m, k, row_stride,
-                         MxOut{e.codes, e.scales, mx_slices(k) * kMxSliceBytes, mx_pad_rows(m)},
-                         MxOut{}, 0};
+  parts.part[0] = MxPart{x, dtype, m, k, row_stride, e.out(), MxOut{}, 0};
   RPX_HIP(launch_mx_quantize(parts, 1, st), who);
   const MxGemm g{e.codes, e.scales, codes, scales, up_codes, up_scales, m, n, mx_slices(k),
                  y, nullptr, nullptr, dtype};
@@ -259,6 +307,246 @@ int rpx_mxfp4_gated(const void* x, int dtype, int64_t m, int64_t k, int64_t row_
   return serve("rpx_mxfp4_gated", x, dtype, m, k, row_stride, gate_codes, gate_scales, up_codes,
                up_scales, true, n, h, workspace, workspace_bytes,
                static_cast<hipStream_t>(stream));
+}
+
+// --- a linear's training step -------------------------------------------------
+namespace {
+
+int check_operand(const char* who, const void* t, int64_t rows, int64_t columns, int64_t stride) {
+  if (rows > 0 && columns > 0 && t == nullptr)
+    return fail_invalid(std::string(who) + ": null pointer");
+  if (stride < columns && rows > 1) return fail_invalid(std::string(who) + ": rows overlap");
+  return kOk;
+}
+
+}  // namespace
+
+size_t rpx_mxfp4_linear_saved_bytes(int64_t m, int64_t n, int64_t k, int need_left,
+                                    int need_right) {
+  if (m < 0 || n < 0 || k < 0) return 0;
+  Sizer s;
+  take(&s, need_right != 0, k, m);
+  take(&s, need_left != 0, k, n);
+  return s.used;
+}
+
+size_t rpx_mxfp4_linear_forward_workspace(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return 0;
+  Sizer s;
+  take(&s, true, m, k);
+  take(&s, true, n, k);
+  s.take<float>(product_floats(m, n, k));
+  return s.used;
+}
+
+int rpx_mxfp4_linear_forward(const void* left, int left_dtype, int64_t m, int64_t k,
+                             int64_t left_stride, const void* right, int right_dtype, int64_t n,
+                             int64_t right_row_stride, int64_t right_col_stride, void* y,
+                             int out_dtype, void* saved, size_t saved_bytes, int need_left,
+                             int need_right, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  const char* who = "rpx_mxfp4_linear_forward";
+  RPX_TRY(check_dtype(left_dtype));
+  RPX_TRY(check_dtype(right_dtype));
+  RPX_TRY(check_dtype(out_dtype));
+  RPX_TRY(check_extents(who, {m, n, k}));
+  RPX_TRY(check_operand(who, left, m, k, left_stride));
+  if (m > 0 && n > 0) RPX_TRY(check_pointers(who, {y}));
+  if ((saved != nullptr && !aligned16(saved)) || (workspace != nullptr && !aligned16(workspace)))
+    return fail_invalid("rpx_mxfp4_linear_forward: pointers must be 16-byte aligned");
+  Arena keep(saved, saved == nullptr ? 0 : saved_bytes);
+  const Encoded xt = take(&keep, need_right != 0, k, m);
+  const Encoded wt = take(&keep, need_left != 0, k, n);
+  if (keep.overflow) return fail_invalid("rpx_mxfp4_linear_forward: saved buffer too small");
+  Arena arena(workspace, workspace == nullptr ? 0 : workspace_bytes);
+  const Encoded xq = take(&arena, true, m, k);
+  const Encoded wq = take(&arena, true, n, k);
+  float* partials = arena.take<float>(product_floats(m, n, k));
+  if (arena.overflow) return fail_invalid("rpx_mxfp4_linear_forward: workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  MxParts parts{};
+  int jobs = 0;
+  if (m > 0 && k > 0)
+    parts.part[jobs++] = MxPart{left, left_dtype, m, k, m > 1 ? left_stride : k, xq.out(), xt.out(), 0};
+  if (n > 0 && k > 0)
+    RPX_TRY(weight_part(who, right, right_dtype, k, n, right_row_stride, right_col_stride, wq,
+                        wt.out(), &parts.part[jobs++]));
+  RPX_HIP(launch_mx_quantize(parts, jobs, st), who);
+  return product(who, xq, wq, y, out_dtype, partials, st);
+}
+
+size_t rpx_mxfp4_linear_backward_workspace(int64_t m, int64_t n, int64_t k, int need_left,
+                                           int need_right) {
+  if (m < 0 || n < 0 || k < 0) return 0;
+  Sizer s;
+  take(&s, need_left != 0, m, n);
+  take(&s, need_right != 0, n, m);
+  const int64_t left = need_left != 0 ? product_floats(m, k, n) : 0;
+  const int64_t right = need_right != 0 ? product_floats(n, k, m) : 0;
+  s.take<float>(left > right ? left : right);
+  return s.used;
+}
+
+int rpx_mxfp4_linear_backward(const void* grad, int grad_dtype, int64_t m, int64_t n,
+                              int64_t grad_stride, const void* saved, size_t saved_bytes,
+                              int64_t k, int need_left, int need_right, void* d_left,
+                              int left_dtype, void* d_right, int right_dtype, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  const char* who = "rpx_mxfp4_linear_backward";
+  RPX_TRY(check_dtype(grad_dtype));
+  RPX_TRY(check_dtype(left_dtype));
+  RPX_TRY(check_dtype(right_dtype));
+  RPX_TRY(check_extents(who, {m, n, k}));
+  RPX_TRY(check_operand(who, grad, m, n, grad_stride));
+  if (d_left == nullptr && d_right == nullptr) return kOk;
+  if ((d_left != nullptr && need_left == 0) || (d_right != nullptr && need_right == 0))
+    return fail_invalid("rpx_mxfp4_linear_backward: the forward saved nothing for this gradient");
+  for (const void* p : {static_cast<const void*>(d_left), static_cast<const void*>(d_right), saved,
+                        static_cast<const void*>(workspace)})
+    if (!aligned16(p))
+      return fail_invalid("rpx_mxfp4_linear_backward: pointers must be 16-byte aligned");
+  Arena keep(const_cast<void*>(saved), saved == nullptr ? 0 : saved_bytes);
+  const Encoded xt = take(&keep, need_right != 0, k, m);
+  const Encoded wt = take(&keep, need_left != 0, k, n);
+  if (keep.overflow) return fail_invalid("rpx_mxfp4_linear_backward: saved buffer too small");
+  Arena arena(workspace, workspace == nullptr ? 0 : workspace_bytes);
+  const Encoded gq = take(&arena, d_left != nullptr, m, n);
+  const Encoded gt = take(&arena, d_right != nullptr, n, m);
+  const int64_t left = d_left != nullptr ? product_floats(m, k, n) : 0;
+  const int64_t right = d_right != nullptr ? product_floats(n, k, m) : 0;
+  float* partials = arena.take<float>(left > right ? left : right);
+  if (arena.overflow) return fail_invalid("rpx_mxfp4_linear_backward: workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (m > 0 && n > 0) {
+    MxParts parts{};
+    parts.part[0] = MxPart{grad, grad_dtype, m, n, m > 1 ? grad_stride : n, gq.out(), gt.out(), 0};
+    RPX_HIP(launch_mx_quantize(parts, 1, st), who);
+  }
+  if (d_right != nullptr) RPX_TRY(product(who, gt, xt, d_right, right_dtype, partials, st));
+  if (d_left != nullptr) RPX_TRY(product(who, gq, wt, d_left, left_dtype, partials, st));
+  return kOk;
+}
+
+// --- the gated block's training step --------------------------------------------
+size_t rpx_mxfp4_gated_saved_bytes(int64_t m, int64_t n, int64_t k, int need_left,
+                                   int need_weights) {
+  if (m < 0 || n < 0 || k < 0) return 0;
+  Sizer s;
+  take(&s, need_weights != 0, k, m);
+  take(&s, need_left != 0, k, 2 * mx_slices(n) * kMxSlice);
+  return s.used;
+}
+
+size_t rpx_mxfp4_gated_forward_workspace(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return 0;
+  Sizer s;
+  take(&s, true, m, k);
+  take(&s, true, n, k);
+  take(&s, true, n, k);
+  return s.used;
+}
+
+int rpx_mxfp4_gated_forward(const void* left, int left_dtype, int64_t m, int64_t k,
+                            int64_t left_stride, const void* gate, int gate_dtype,
+                            int64_t gate_row_stride, int64_t gate_col_stride, const void* up,
+                            int up_dtype, int64_t up_row_stride, int64_t up_col_stride, int64_t n,
+                            void* h, void* z_gate, void* z_up, int out_dtype, void* saved,
+                            size_t saved_bytes, int need_left, int need_weights, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const char* who = "rpx_mxfp4_gated_forward";
+  for (int d : {left_dtype, gate_dtype, up_dtype, out_dtype}) RPX_TRY(check_dtype(d));
+  RPX_TRY(check_extents(who, {m, n, k}));
+  RPX_TRY(check_operand(who, left, m, k, left_stride));
+  if ((z_gate == nullptr) != (z_up == nullptr))
+    return fail_invalid("rpx_mxfp4_gated_forward: z_gate and z_up come together");
+  for (const void* p : {static_cast<const void*>(h), static_cast<const void*>(z_gate),
+                        static_cast<const void*>(z_up), static_cast<const void*>(saved),
+                        static_cast<const void*>(workspace)})
+    if (!aligned16(p))
+      return fail_invalid("rpx_mxfp4_gated_forward: pointers must be 16-byte aligned");
+  if (m > 0 && n > 0) RPX_TRY(check_pointers(who, {h}));
+  Arena keep(saved, saved == nullptr ? 0 : saved_bytes);
+  const int64_t wide = mx_slices(n) * kMxSlice;  // a projection's columns in the joint transpose
+  const Encoded xt = take(&keep, need_weights != 0, k, m);
+  const Encoded both = take(&keep, need_left != 0, k, 2 * wide);
+  if (keep.overflow) return fail_invalid("rpx_mxfp4_gated_forward: saved buffer too small");
+  Arena arena(workspace, workspace == nullptr ? 0 : workspace_bytes);
+  const Encoded xq = take(&arena, true, m, k);
+  const Encoded gq = take(&arena, true, n, k);
+  const Encoded uq = take(&arena, true, n, k);
+  if (arena.overflow) return fail_invalid("rpx_mxfp4_gated_forward: workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  MxParts parts{};
+  int jobs = 0;
+  if (m > 0 && k > 0)
+    parts.part[jobs++] = MxPart{left, left_dtype, m, k, m > 1 ? left_stride : k, xq.out(), xt.out(), 0};
+  if (n > 0 && k > 0) {
+    MxOut halves[2] = {both.out(), both.out()};
+    if (both.codes != nullptr) {
+      halves[1].codes += wide / 2;
+      halves[1].scales += mx_slices(n) * mx_pad_rows(k) * kMxSliceBlocks;
+    }
+    RPX_TRY(weight_part(who, gate, gate_dtype, k, n, gate_row_stride, gate_col_stride, gq,
+                        halves[0], &parts.part[jobs++]));
+    RPX_TRY(weight_part(who, up, up_dtype, k, n, up_row_stride, up_col_stride, uq, halves[1],
+                        &parts.part[jobs++]));
+  }
+  RPX_HIP(launch_mx_quantize(parts, jobs, st), who);
+  return rpx_mxfp4_gated_gemm(xq.codes, xq.scales, gq.codes, gq.scales, uq.codes, uq.scales, m, n,
+                              k, h, z_gate, z_up, out_dtype, stream);
+}
+
+size_t rpx_mxfp4_gated_backward_workspace(int64_t m, int64_t n, int64_t k, int need_left,
+                                          int need_weights) {
+  if (m < 0 || n < 0 || k < 0) return 0;
+  const int64_t wide = 2 * mx_slices(n) * kMxSlice;
+  Sizer s;
+  take(&s, need_left != 0, m, wide);
+  take(&s, need_weights != 0, 2 * n, m);
+  const int64_t left = need_left != 0 ? product_floats(m, k, wide) : 0;
+  const int64_t weights = need_weights != 0 ? product_floats(2 * n, k, m) : 0;
+  s.take<float>(left > weights ? left : weights);
+  return s.used;
+}
+
+int rpx_mxfp4_gated_backward_products(const void* dh, const void* z_gate, const void* z_up,
+                                      int dtype, int64_t m, int64_t n, const void* saved,
+                                      size_t saved_bytes, int64_t k, int need_left,
+                                      int need_weights, void* d_left, int left_dtype,
+                                      void* d_weights, int weights_dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  const char* who = "rpx_mxfp4_gated_backward_products";
+  RPX_TRY(check_dtype(left_dtype));
+  RPX_TRY(check_dtype(weights_dtype));
+  RPX_TRY(check_extents(who, {m, n, k}));
+  if (d_left == nullptr && d_weights == nullptr) return kOk;
+  if ((d_left != nullptr && need_left == 0) || (d_weights != nullptr && need_weights == 0))
+    return fail_invalid(
+        "rpx_mxfp4_gated_backward_products: the forward saved nothing for this gradient");
+  for (const void* p : {static_cast<const void*>(d_left), static_cast<const void*>(d_weights),
+                        saved, static_cast<const void*>(workspace)})
+    if (!aligned16(p))
+      return fail_invalid("rpx_mxfp4_gated_backward_products: pointers must be 16-byte aligned");
+  const int64_t wide = 2 * mx_slices(n) * kMxSlice;
+  Arena keep(const_cast<void*>(saved), saved == nullptr ? 0 : saved_bytes);
+  const Encoded xt = take(&keep, need_weights != 0, k, m);
+  const Encoded both = take(&keep, need_left != 0, k, wide);
+  if (keep.overflow)
+    return fail_invalid("rpx_mxfp4_gated_backward_products: saved buffer too small");
+  Arena arena(workspace, workspace == nullptr ? 0 : workspace_bytes);
+  const Encoded dz = take(&arena, d_left != nullptr, m, wide);
+  const Encoded dzt = take(&arena, d_weights != nullptr, 2 * n, m);
+  const int64_t left = d_left != nullptr ? product_floats(m, k, wide) : 0;
+  const int64_t weights = d_weights != nullptr ? product_floats(2 * n, k, m) : 0;
+  float* partials = arena.take<float>(left > weights ? left : weights);
+  if (arena.overflow)
+    return fail_invalid("rpx_mxfp4_gated_backward_products: workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  RPX_TRY(rpx_mxfp4_gated_backward(dh, z_gate, z_up, dtype, m, n, dz.codes, dz.scales, dzt.codes,
+                                   dzt.scales, stream));
+  if (d_weights != nullptr) RPX_TRY(product(who, dzt, xt, d_weights, weights_dtype, partials, st));
+  if (d_left != nullptr) RPX_TRY(product(who, dz, both, d_left, left_dtype, partials, st));
+  return kOk;
 }
 
 }  // extern "C"

@@ -28,9 +28,10 @@ and a sum over nothing is zero.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .ops import BF16, F32, _aligned, _dtype_code, _on_device, _ptr, _stream, _workspace
+from .ops import BF16, F32, _aligned, _as, _dtype_code, _on_device, _ptr, _stream, _workspace
 
 SLICE = 256  # columns are padded to this
 ROW_PAD = 32  # the scales' rows are padded to this
@@ -263,15 +264,24 @@ def _check_product(left: torch.Tensor, right: torch.Tensor, what: str) -> None:
                          f"and {tuple(right.shape)}")
 
 
-def _weight_part(right: torch.Tensor, rows: MXFP4Matrix, across: MXFP4Matrix | None):
-    """The part that encodes ``right [K, N]`` along K into ``rows [N, K]`` and, where
-    given, along N into ``across [K, N]``, whichever way ``right`` lies in memory."""
+def _right(t: torch.Tensor) -> torch.Tensor:
+    """``t [K, N]`` as the library takes a right operand: one stride 1, the other
+    spanning it (row-major, or the transposed view of a row-major weight)."""
 
-    if right.stride(0) == 1 and right.stride(1) >= right.shape[0]:
-        w = _dense_rows(right.t())
-        return w, _part(w, rows, across)
-    w = _dense_rows(right)
-    return w, _part(w, across, rows)
+    k, n = t.shape
+    s0, s1 = t.stride()
+    if (s1 == 1 and (s0 >= n or k <= 1)) or (s0 == 1 and (s1 >= k or n <= 1)):
+        return t
+    return t.contiguous()
+
+
+def _saved(name: str, m: int, n: int, k: int, need_left: bool, need_right: bool, device):
+    """The buffer that a forward keeps for its backward, or None."""
+
+    if not (need_left or need_right):
+        return None
+    return torch.empty(nat.query(name, m, n, k, need_left, need_right), dtype=torch.uint8,
+                       device=device)
 
 
 class MXFP4LinearFn(torch.autograd.Function):
@@ -285,40 +295,41 @@ class MXFP4LinearFn(torch.autograd.Function):
         m, k = left.shape
         n = right.shape[1]
         need_left, need_right = ctx.needs_input_grad[:2]
-        x = _dense_rows(left)
-        xq = MXFP4Matrix.empty(m, k, device)
-        xt = MXFP4Matrix.empty(k, m, device) if need_right else None
-        wq = MXFP4Matrix.empty(n, k, device)
-        wt = MXFP4Matrix.empty(k, n, device) if need_left else None
-        w, weight = _weight_part(right, wq, wt)
-        _encode([_part(x, xq, xt), weight], device)
+        x, w = _dense_rows(left), _right(right)
+        y = torch.empty((m, n), dtype=out_dtype, device=device)
+        saved = _saved("rpx_mxfp4_linear_saved_bytes", m, n, k, need_left, need_right, device)
+        stream = _stream(device)
+        ws = _workspace(nat.query("rpx_mxfp4_linear_forward_workspace", m, n, k), device, stream)
         with _launches_on(device):
-            out = _gemm(xq, wq, out_dtype, device)
-        if need_left or need_right:
-            ctx.save_for_backward(*[t for q in (xt, wt) if q is not None
-                                    for t in (q.codes, q.scales)])
-            ctx.cfg = (m, k, n, left.dtype, right.dtype)
-        return out
+            nat.call("rpx_mxfp4_linear_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
+                     x.stride(0), w.data_ptr(), _dtype_code(w.dtype), n, *w.stride(),
+                     y.data_ptr(), _dtype_code(out_dtype), _ptr(saved),
+                     0 if saved is None else saved.numel(), need_left, need_right, ws.data_ptr(),
+                     ws.numel(), stream)
+        if saved is not None:
+            ctx.save_for_backward(saved)
+            ctx.cfg = (m, k, n, left.dtype, right.dtype, need_left, need_right)
+        return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
-        m, k, n, left_dtype, right_dtype = ctx.cfg
+        m, k, n, left_dtype, right_dtype, saved_left, saved_right = ctx.cfg
         need_left, need_right = ctx.needs_input_grad[:2]
-        saved = list(ctx.saved_tensors)
+        (saved,) = ctx.saved_tensors
         device = grad.device
         g = _dense_rows(grad)
-        gq = MXFP4Matrix.empty(m, n, device) if need_left else None
-        gt = MXFP4Matrix.empty(n, m, device) if need_right else None
-        _encode([_part(g, gq, gt)], device)
-        d_left = d_right = None
+        d_left = torch.empty((m, k), dtype=left_dtype, device=device) if need_left else None
+        d_right = torch.empty((n, k), dtype=right_dtype, device=device) if need_right else None
+        stream = _stream(device)
+        ws = _workspace(nat.query("rpx_mxfp4_linear_backward_workspace", m, n, k, need_left,
+                                  need_right), device, stream)
         with _launches_on(device):
-            if need_right:
-                xt = MXFP4Matrix(saved.pop(0), saved.pop(0), m)
-                d_right = _gemm(gt, xt, right_dtype, device).t()
-            if need_left:
-                wt = MXFP4Matrix(saved.pop(0), saved.pop(0), n)
-                d_left = _gemm(gq, wt, left_dtype, device)
-        return d_left, d_right, None
+            nat.call("rpx_mxfp4_linear_backward", g.data_ptr(), _dtype_code(g.dtype), m, n,
+                     g.stride(0), saved.data_ptr(), saved.numel(), k, saved_left, saved_right,
+                     _ptr(d_left), _dtype_code(left_dtype), _ptr(d_right),
+                     _dtype_code(right_dtype), ws.data_ptr(), ws.numel(), stream)
+        return d_left, None if d_right is None else d_right.t(), None
 
 
 class MXFP4GatedFn(torch.autograd.Function):
@@ -338,69 +349,50 @@ class MXFP4GatedFn(torch.autograd.Function):
         device = _on_device(left, gate, up)
         m, k = left.shape
         n = gate.shape[1]
-        need_x, need_g, need_u = ctx.needs_input_grad[:3]
+        need_left, need_g, need_u = ctx.needs_input_grad[:3]
         need_w = need_g or need_u
-        x = _dense_rows(left)
-        xq = MXFP4Matrix.empty(m, k, device)
-        xt = MXFP4Matrix.empty(k, m, device) if need_w else None
-        wide = _slices(n) * SLICE  # one projection's columns in the joint transpose
-        both = MXFP4Matrix.empty(k, 2 * wide, device) if need_x else None
-        weights, parts = [], [_part(x, xq, xt)]
-        for i, right in enumerate((gate, up)):
-            wq = MXFP4Matrix.empty(n, k, device)
-            w, part = _weight_part(right, wq, None)
-            if need_x:
-                codes = both.codes.data_ptr() + i * (wide // 2)
-                scales = both.scales.data_ptr() + i * _slices(n) * _pad_rows(k) * 8
-                if part.codes is not None:  # w is [N, K]: its transpose goes to the joint matrix
-                    part.codes_t, part.scales_t, part.code_stride_t = codes, scales, wide
-                else:
-                    part.codes, part.scales, part.code_stride = codes, scales, wide
-            weights.append(wq)
-            parts.append(part)
-            x = (x, w)  # keeps any copy alive until the launch
-        _encode(parts, device)
+        x, wg, wu = _dense_rows(left), _right(gate), _right(up)
         h = torch.empty((m, n), dtype=out_dtype, device=device)
-        z = [torch.empty((m, n), dtype=out_dtype, device=device) for _ in range(2)] \
-            if need_x or need_w else [None, None]
+        z_gate = z_up = None
+        if need_left or need_w:
+            z_gate, z_up = (torch.empty((m, n), dtype=out_dtype, device=device) for _ in range(2))
+        saved = _saved("rpx_mxfp4_gated_saved_bytes", m, n, k, need_left, need_w, device)
+        stream = _stream(device)
+        ws = _workspace(nat.query("rpx_mxfp4_gated_forward_workspace", m, n, k), device, stream)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_gated_gemm", _ptr(xq.codes), _ptr(xq.scales),
-                     _ptr(weights[0].codes), _ptr(weights[0].scales), _ptr(weights[1].codes),
-                     _ptr(weights[1].scales), m, n, k, _ptr(h), _ptr(z[0]), _ptr(z[1]),
-                     _dtype_code(out_dtype), _stream(device))
-        if need_x or need_w:
-            ctx.save_for_backward(*z, *[t for q in (xt, both) if q is not None
-                                       for t in (q.codes, q.scales)])
-            ctx.cfg = (m, k, n, left.dtype, gate.dtype, up.dtype)
+            nat.call("rpx_mxfp4_gated_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
+                     x.stride(0), wg.data_ptr(), _dtype_code(wg.dtype), *wg.stride(),
+                     wu.data_ptr(), _dtype_code(wu.dtype), *wu.stride(), n, h.data_ptr(),
+                     _ptr(z_gate), _ptr(z_up), _dtype_code(out_dtype), _ptr(saved),
+                     0 if saved is None else saved.numel(), need_left, need_w, ws.data_ptr(),
+                     ws.numel(), stream)
+        if saved is not None:
+            ctx.save_for_backward(z_gate, z_up, saved)
+            ctx.cfg = (m, k, n, left.dtype, gate.dtype, up.dtype, need_left, need_w)
         return h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
-        m, k, n, left_dtype, gate_dtype, up_dtype = ctx.cfg
-        need_x, need_g, need_u = ctx.needs_input_grad[:3]
+        m, k, n, left_dtype, gate_dtype, up_dtype, saved_left, saved_w = ctx.cfg
+        need_left, need_g, need_u = ctx.needs_input_grad[:3]
         need_w = need_g or need_u
-        z_gate, z_up, *saved = ctx.saved_tensors
+        z_gate, z_up, saved = ctx.saved_tensors
         device = grad.device
-        dh = _aligned(grad.to(z_gate.dtype))
-        wide = _slices(n) * SLICE
-        dz = MXFP4Matrix.empty(m, 2 * wide, device) if need_x else None
-        dzt = MXFP4Matrix.empty(2 * n, m, device) if need_w else None
-        d_x = d_gate = d_up = None
+        dh = _aligned(_as(grad, z_gate.dtype))
+        wide = gate_dtype if gate_dtype == up_dtype else F32
+        d_x = torch.empty((m, k), dtype=left_dtype, device=device) if need_left else None
+        d_w = torch.empty((2 * n, k), dtype=wide, device=device) if need_w else None
+        stream = _stream(device)
+        ws = _workspace(nat.query("rpx_mxfp4_gated_backward_workspace", m, n, k, need_left,
+                                  need_w), device, stream)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_gated_backward", _ptr(dh), _ptr(z_gate), _ptr(z_up),
-                     _dtype_code(dh.dtype), m, n, _ptr(dz.codes) if dz else None,
-                     _ptr(dz.scales) if dz else None, _ptr(dzt.codes) if dzt else None,
-                     _ptr(dzt.scales) if dzt else None, _stream(device))
-            if need_w:
-                xt = MXFP4Matrix(saved.pop(0), saved.pop(0), m)
-                wide_dtype = gate_dtype if gate_dtype == up_dtype else F32
-                d_w = _gemm(dzt, xt, wide_dtype, device)
-                d_gate = d_w[:n].to(gate_dtype).t() if need_g else None
-                d_up = d_w[n:].to(up_dtype).t() if need_u else None
-            if need_x:
-                both = MXFP4Matrix(saved.pop(0), saved.pop(0), 2 * wide)
-                d_x = _gemm(dz, both, left_dtype, device)
-        return d_x, d_gate, d_up, None
+            nat.call("rpx_mxfp4_gated_backward_products", dh.data_ptr(), z_gate.data_ptr(),
+                     z_up.data_ptr(), _dtype_code(dh.dtype), m, n, saved.data_ptr(),
+                     saved.numel(), k, saved_left, saved_w, _ptr(d_x), _dtype_code(left_dtype),
+                     _ptr(d_w), _dtype_code(wide), ws.data_ptr(), ws.numel(), stream)
+        return (d_x, _as(d_w[:n], gate_dtype).t() if need_g else None,
+                _as(d_w[n:], up_dtype).t() if need_u else None, None)
 
 
 def linear_product(left, right, out_dtype: torch.dtype) -> torch.Tensor:

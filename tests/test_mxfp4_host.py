@@ -124,3 +124,52 @@ def test_c_entries_refuse_before_any_launch():
     with pytest.raises(ValueError, match="workspace too small"):
         nat.call("rpx_mxfp4_gated", P, BF16, m, k, k, P, P, P, P, n, P, P, need - 1, None)
     assert ctypes.sizeof(nat.Mxfp4Part) == 88
+
+
+def test_training_entries_refuse_before_any_launch():
+    big = 1 << 30
+
+    def forward(left=P, right=P, y=P, left_stride=64, strides=(1, 64), saved=P, saved_bytes=big,
+                ws=P, ws_bytes=big, dtype=BF16):
+        nat.call("rpx_mxfp4_linear_forward", left, dtype, 40, 64, left_stride, right, BF16, 48,
+                 *strides, y, BF16, saved, saved_bytes, 1, 1, ws, ws_bytes, None)
+
+    need = nat.query("rpx_mxfp4_linear_saved_bytes", 40, 48, 64, 1, 1)
+    assert need > nat.query("rpx_mxfp4_linear_saved_bytes", 40, 48, 64, 1, 0) > 0
+    assert nat.query("rpx_mxfp4_linear_saved_bytes", 40, 48, 64, 0, 0) == 0
+    for over, match in ((dict(dtype=5), "dtype"), (dict(left=None), "null"), (dict(y=None), "null"),
+                        (dict(left_stride=63), "overlap"), (dict(strides=(2, 64)), "stride"),
+                        (dict(strides=(1, 63)), "stride"), (dict(right=None), "null"),
+                        (dict(saved=None), "saved buffer"), (dict(saved_bytes=need - 1), "saved"),
+                        (dict(saved=8), "aligned"), (dict(ws_bytes=100), "workspace too small"),
+                        (dict(ws=None), "workspace too small")):
+        with pytest.raises(ValueError, match=match):
+            forward(**over)
+
+    def backward(grad=P, saved=P, saved_bytes=big, d_left=P, d_right=P, need=(1, 1), ws_bytes=big):
+        nat.call("rpx_mxfp4_linear_backward", grad, BF16, 40, 48, 48, saved, saved_bytes, 64, *need,
+                 d_left, BF16, d_right, BF16, P, ws_bytes, None)
+
+    for over, match in ((dict(grad=None), "null"), (dict(need=(0, 1)), "saved nothing"),
+                        (dict(saved_bytes=need - 1), "saved"), (dict(d_left=8), "aligned"),
+                        (dict(ws_bytes=100), "workspace too small")):
+        with pytest.raises(ValueError, match=match):
+            backward(**over)
+    backward(d_left=None, d_right=None)  # nothing asked for
+
+    def gated(z_gate=P, z_up=P, saved_bytes=big, ws_bytes=big, up=P):
+        nat.call("rpx_mxfp4_gated_forward", P, BF16, 40, 64, 64, P, BF16, 1, 64, up, BF16, 1, 64,
+                 48, P, z_gate, z_up, BF16, P, saved_bytes, 1, 1, P, ws_bytes, None)
+
+    need = nat.query("rpx_mxfp4_gated_saved_bytes", 40, 48, 64, 1, 1)
+    for over, match in ((dict(z_up=None), "together"), (dict(z_gate=8), "aligned"),
+                        (dict(saved_bytes=need - 1), "saved"), (dict(up=None), "null"),
+                        (dict(ws_bytes=100), "workspace too small")):
+        with pytest.raises(ValueError, match=match):
+            gated(**over)
+    with pytest.raises(ValueError, match="saved nothing"):
+        nat.call("rpx_mxfp4_gated_backward_products", P, P, P, BF16, 40, 48, P, big, 64, 1, 0, P,
+                 BF16, P, BF16, P, big, None)
+    with pytest.raises(ValueError, match="null"):
+        nat.call("rpx_mxfp4_gated_backward_products", None, P, P, BF16, 40, 48, P, big, 64, 1, 1, P,
+                 BF16, P, BF16, P, big, None)
