@@ -59,12 +59,6 @@ void take(Sizer* s, bool wanted, int64_t rows, int64_t columns) {
   s->take<uint8_t>(mx_scale_bytes(rows, columns));
 }
 
-size_t encoded_bytes(int64_t rows, int64_t columns) {
-  Sizer s;
-  take(&s, true, rows, columns);
-  return s.used;
-}
-
 // A B^T into out, zeros where nothing is summed; nothing for an empty output.
 int product(const char* who, const Encoded& a, const Encoded& b, void* out, int dtype,
             float* partials, hipStream_t st) {
@@ -100,11 +94,23 @@ int weight_part(const char* who, const void* right, int dtype, int64_t k, int64_
   return kOk;
 }
 
-size_t linear_workspace(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
+// Whether a serving call encodes x within its product's launch: up to 16 rows,
+// which every workgroup (16 rows of the weight) reads, 16 MB of such reads in all.
+// One launch against two, bf16 and float32 (graph replays, cold weights): 4 rows of
+// 2048 to 6144, 6 MB, 5.8 / 7.4 us; 16 rows of 2048 to 2048, 8 MB, 5.3 / 6.7; 13 of
+// 2048 to 6144, 20 MB, 7.4 / 7.4; 13 of 6144 to 2048, 20 MB, 9.2 / 8.4; 13 float32
+// rows of 2048 to 6144, 41 MB, 9.7 / 7.5.
+constexpr int64_t kMxSkinnyReads = int64_t{16} << 20;
+bool encodes_on_the_way(int64_t m, int64_t n, int64_t k, int dtype) {
+  return m <= kMxSkinnyRows &&
+         m * k * static_cast<int64_t>(elem_size(dtype)) <= kMxSkinnyReads / ceil_div(n, 16);
+}
+
+size_t serve_workspace(int64_t m, int64_t n, int64_t k, bool gated) {
+  if (m <= 0 || n <= 0 || k <= 0 || encodes_on_the_way(m, n, k, kF32)) return 0;
   Sizer s;
   take(&s, true, m, k);
-  s.take<float>(product_floats(m, n, k));
+  if (!gated && m > kMxThinRows) s.take<float>(product_floats(m, n, k));
   return s.used;
 }
 
@@ -129,14 +135,26 @@ int serve(const char* who, const void* x, int dtype, int64_t m, int64_t k, int64
   if (x == nullptr) return fail_invalid(std::string(who) + ": null pointer");
   RPX_TRY(check_pointers(who, {codes, scales, y}));
   if (gated) RPX_TRY(check_pointers(who, {up_codes, up_scales}));
+  MxSkinny few{x, nullptr, m, k, row_stride, codes, scales, up_codes, up_scales, n, mx_slices(k), y};
+  if (encodes_on_the_way(m, n, k, dtype)) {
+    RPX_HIP(launch_mx_skinny(few, dtype, st), who);
+    return kOk;
+  }
   Arena arena(workspace, workspace == nullptr ? 0 : workspace_bytes);
   const Encoded e = take(&arena, true, m, k);
-  float* partials = gated ? nullptr : arena.take<float>(mx_gemm_workspace_floats(m, n, mx_slices(k)));
+  float* partials =
+      gated || m <= kMxThinRows ? nullptr : arena.take<float>(product_floats(m, n, k));
   if (arena.overflow) return fail_invalid(std::string(who) + ": workspace too small");
   RPX_TRY(check_pointers(who, {workspace}));
   MxParts parts{};
   parts.part[0] = MxPart{x, dtype, m, k, row_stride, e.out(), MxOut{}, 0};
   RPX_HIP(launch_mx_quantize(parts, 1, st), who);
+  if (m <= kMxThinRows) {
+    few.x = e.codes;
+    few.x_scales = e.scales;
+    RPX_HIP(launch_mx_skinny(few, dtype, st), who);
+    return kOk;
+  }
   const MxGemm g{e.codes, e.scales, codes, scales, up_codes, up_scales, m, n, mx_slices(k),
                  y, nullptr, nullptr, dtype};
   RPX_HIP(launch_mx_gemm(g, partials, st), who);
@@ -286,7 +304,7 @@ int rpx_mxfp4_gated_backward(const void* dh, const void* z_gate, const void* z_u
 }
 
 size_t rpx_mxfp4_linear_workspace(int64_t m, int64_t n, int64_t k) {
-  return linear_workspace(m, n, k);
+  return serve_workspace(m, n, k, false);
 }
 
 int rpx_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t k, int64_t row_stride,
@@ -297,7 +315,7 @@ int rpx_mxfp4_linear(const void* x, int dtype, int64_t m, int64_t k, int64_t row
 }
 
 size_t rpx_mxfp4_gated_workspace(int64_t m, int64_t n, int64_t k) {
-  return m <= 0 || n <= 0 || k <= 0 ? 0 : encoded_bytes(m, k);
+  return serve_workspace(m, n, k, true);
 }
 
 int rpx_mxfp4_gated(const void* x, int dtype, int64_t m, int64_t k, int64_t row_stride,

@@ -368,4 +368,19 @@ int mx_tile_count();
 int64_t mx_gemm_workspace_floats(int64_t m, int64_t n, int64_t slices);
 hipError_t launch_mx_gemm(const MxGemm& p, float* partials, hipStream_t stream);
 
+// The same for few rows over kept weights (codes2: the up projection's, or null):
+// from x itself, m <= 16 rows of k columns of `dtype`, or (x_scales given) from its
+// codes, m <= 64.
+constexpr int64_t kMxSkinnyRows = 16;
+constexpr int64_t kMxThinRows = 64;
+struct MxSkinny {
+  const void* x;
+  const uint8_t* x_scales;
+  int64_t m, k, row_stride;
+  const uint8_t *codes, *scales, *codes2, *scales2;
+  int64_t n, slices;
+  void* y;
+};
+hipError_t launch_mx_skinny(const MxSkinny& p, int dtype, hipStream_t stream);
+
 }  // namespace rpx
