@@ -370,7 +370,7 @@ hipError_t launch_mx_gemm(const MxGemm& p, float* partials, hipStream_t stream);
 
 // The same for few rows over kept weights (codes2: the up projection's, or null):
 // from x itself, m <= 16 rows of k columns of `dtype`, or (x_scales given) from its
-// codes, m <= 64.
+// codes (any m; meant for kMxThinRows).
 constexpr int64_t kMxSkinnyRows = 16;
 constexpr int64_t kMxThinRows = 64;
 struct MxSkinny {

@@ -1,4 +1,6 @@
 // Encoding to MXFP4 and back (mxfp4.h states the format).
+#include <type_traits>
+
 #include <hip/hip_runtime.h>
 
 #include "act.h"
@@ -312,131 +314,211 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4
     quantize_both<kF32, 1>(part, wave, threadIdx.x & 63);
 }
 
+// max(|a|, |b|, |c|), NaN if any is one.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // The gradients of a gated block's projections, z_gate and z_up [m, n]:
 //   dz_gate = dh z_up silu'(z_gate),  dz_up = dh silu(z_gate)
 // encoded along their columns as [dz_gate | dz_up] (`along`) and along their rows
-// as their transposes, stacked (`across`). A thread owns 32 rows of two columns of
-// both, as above: sixteen lanes share a block along the columns.
-template <int DTYPE>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-    k_mx_gated_backward(const void* __restrict__ dh, const void* __restrict__ z_gate,
-                        const void* __restrict__ z_up, int64_t m, int64_t n, int64_t per,
-                        int64_t tiles, MxOut along, MxOut across) {
-  // uniform over the wave, so rows are addressed from scalar registers
-  const int64_t tile = block_of_grid() * (kThreads / 64) +
-                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  if (tile >= tiles) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t r0 = (tile / per) * 32;
-  const int64_t c = (tile % per) * 128 + 2 * lane;
-  float d[2][2][32];  // [gate, up][column][row]
-  constexpr int CHUNK = 4;  // rows whose loads are in flight at once
-  constexpr int WORDS = DTYPE == kBF16 ? 1 : 2;
-  uint32_t raw[2][CHUNK][3][WORDS];
-  // columns past the end read the last ones and rows past the end the last row; they
-  // are set to zero before use, which makes their gradients zero
-  const bool pair = (n & 1) == 0;
-  const uint32_t c0 = static_cast<uint32_t>(c < n ? c : n - 1);
-  const uint32_t c1 = static_cast<uint32_t>(c + 1 < n ? c + 1 : n - 1);
-  const uint32_t cp = static_cast<uint32_t>(c < n ? c : n - 2);
+// as their transposes, stacked (`across`). A wave takes 32 rows of 128 columns, a
+// thread two columns of them: whole blocks of the transposes, in registers; sixteen
+// lanes share a block along the columns, row by row.
+//
+// What bounds it is both memory (6 bytes read and 2.1 written a pair of gradients)
+// and the 55 VALU operations that a pair takes here, four of them transcendental,
+// so the bookkeeping is kept small: one exponential a pair, a maximum that takes two
+// new values an operation, no test for infinities and NaN but one of the whole tile
+// (the tile is then encoded again, with the tests).
+template <int DTYPE, bool WHOLE, bool PAIRS>
+struct GatedTile {
+  static constexpr int WORDS = DTYPE == kBF16 ? 1 : 2;
+  static constexpr int CHUNK = 4;  // rows loaded at a time, one chunk ahead
+  const uint8_t* src[3];  // row 0 of the tile of dh, z_gate and z_up
+  int64_t stride;         // bytes
+  int left;               // rows of the tile
+  uint32_t at[2];         // byte offsets of the thread's columns
   uint32_t in_column[WORDS];
-  if constexpr (DTYPE == kBF16) {
-    in_column[0] = (c < n ? 0xFFFFu : 0u) | (c + 1 < n ? 0xFFFF0000u : 0u);
-  } else {
-    in_column[0] = c < n ? ~0u : 0u;
-    in_column[1] = c + 1 < n ? ~0u : 0u;
-  }
-  const int left = static_cast<int>(m - r0 < 32 ? m - r0 : 32);
-  auto load = [&](int chunk) {
+  uint32_t raw[2][CHUNK][3][WORDS];
+  float d[2][2][32];  // [gate, up][column][row]
+
+  __device__ __forceinline__ void load(int chunk) {
 #pragma unroll
     for (int i = 0; i < CHUNK; ++i) {
-      const int64_t r = r0 + chunk * CHUNK + i < m ? r0 + chunk * CHUNK + i : m - 1;
+      int row = chunk * CHUNK + i;
+      if (!WHOLE) row = row < left ? row : left > 0 ? left - 1 : 0;  // past the end: the last
 #pragma unroll
       for (int t = 0; t < 3; ++t) {
-        const void* src = t == 0 ? dh : t == 1 ? z_gate : z_up;
+        const uint8_t* p = src[t] + row * stride;
         uint32_t(&to)[WORDS] = raw[chunk & 1][i][t];
-        if constexpr (DTYPE == kBF16) {
-          const uint16_t* p = static_cast<const uint16_t*>(src) + r * n;
-          if (pair)
-            to[0] = *reinterpret_cast<const uint32_t*>(p + cp);
-          else
-            to[0] = p[c0] | static_cast<uint32_t>(p[c1]) << 16;
+        if constexpr (DTYPE != kBF16) {
+          to[0] = *reinterpret_cast<const uint32_t*>(p + at[0]);
+          to[1] = *reinterpret_cast<const uint32_t*>(p + at[1]);
+        } else if constexpr (PAIRS) {
+          to[0] = *reinterpret_cast<const uint32_t*>(p + at[0]);
         } else {
-          const uint32_t* p = static_cast<const uint32_t*>(src) + r * n;
-          to[0] = p[c0];
-          to[1] = p[c1];
+          to[0] = *reinterpret_cast<const uint16_t*>(p + at[0]) |
+                  static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + at[1])) << 16;
         }
       }
     }
-  };
-  auto value = [](const uint32_t(&w)[WORDS], int e) {
-    if constexpr (DTYPE == kBF16)
-      return e == 0 ? bf16lo_to_f32(w[0]) : bf16hi_to_f32(w[0]);
-    else
-      return __builtin_bit_cast(float, w[e]);
-  };
-  // scale byte of a block of sixteen lanes
-  auto along_byte = [](float x, float y) {
-    const uint32_t a = __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu;
-    const uint32_t b = __builtin_bit_cast(uint32_t, y) & 0x7FFFFFFFu;
-    return mx_scale_byte(block_max<16>(a > b ? a : b));
-  };
-  uint32_t kept[2] = {0, 0};  // this lane's share of the scales of sixteen rows
-  load(0);
-#pragma unroll
-  for (int chunk = 0; chunk < 32 / CHUNK; ++chunk) {
-    if (chunk + 1 < 32 / CHUNK) load(chunk + 1);
-    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  __device__ __forceinline__ void gradients(int chunk) {
+    auto value = [](const uint32_t(&w)[WORDS], int e) {
+      if constexpr (DTYPE == kBF16)
+        return e == 0 ? bf16lo_to_f32(w[0]) : bf16hi_to_f32(w[0]);
+      else
+        return as_f32(w[e]);
+    };
 #pragma unroll
     for (int i = 0; i < CHUNK; ++i) {
       const int row = chunk * CHUNK + i;
-      const uint32_t in_row = static_cast<uint32_t>((row - left) >> 31);  // all ones below m
       uint32_t(&w)[3][WORDS] = raw[chunk & 1][i];
+      if constexpr (!WHOLE) {  // zeros where the tile ends, which have zero gradients
+        const uint32_t in_row = static_cast<uint32_t>((row - left) >> 31);
 #pragma unroll
-      for (int t = 0; t < 3; ++t)
+        for (int t = 0; t < 3; ++t)
 #pragma unroll
-        for (int e = 0; e < WORDS; ++e) w[t][e] &= in_row & in_column[e];
+          for (int e = 0; e < WORDS; ++e) w[t][e] &= in_row & in_column[e];
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         act_silu_mul_grads(value(w[0], e), value(w[1], e), value(w[2], e), &d[0][e][row],
                            &d[1][e][row]);
     }
-    if (along.codes != nullptr && left > 0) {
-#pragma unroll
-      for (int i = 0; i < CHUNK; ++i)
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int row = chunk * CHUNK + i;
-          const uint32_t byte = along_byte(d[z][0][row], d[z][1][row]);
-          const uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(
-              0u, d[z][0][row], d[z][1][row], mx_scale_operand(byte), 0);
-          if (row < left)
-            along.codes[(r0 + row) * along.row_bytes + z * (along.row_bytes / 2) + c / 2] =
-                static_cast<uint8_t>(byte == 255u ? 0u : code);
-          kept[z] = (lane & 15) == row % 16 ? byte : kept[z];
-          if (row % 16 == 15)
-            *mx_scale_at(along, r0 + row - 15 + (lane & 15), (z * along.row_bytes + c) / kMxBlock) =
-                static_cast<uint8_t>(kept[z]);
-        }
-    }
-    __builtin_amdgcn_sched_barrier(0);
   }
-  if (across.codes == nullptr) return;
+
+  // Rows `from` ... `from` + ROWS - 1 along the columns. TEST: with the scale NaN for
+  // blocks that are not finite. Returns the largest magnitude's bits of the blocks.
+  template <int ROWS, bool TEST>
+  __device__ __forceinline__ uint32_t encode_along(const MxOut& o, int64_t r0, int64_t c, int lane,
+                                                   int from, uint32_t (&kept)[2]) const {
+    uint32_t seen = 0;
 #pragma unroll
-  for (int z = 0; z < 2; ++z)
+    for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint32_t byte;
-      const u32x4_t code = mx_encode_block(d[z][e], &byte);
-      if (c + e < n) {
-        const int64_t row = z * n + c + e;
-        *reinterpret_cast<u32x4_t*>(across.codes + row * across.row_bytes + r0 / 2) = code;
-        *mx_scale_at(across, row, r0 / kMxBlock) = static_cast<uint8_t>(byte);
+      for (int z = 0; z < 2; ++z) {
+        const int row = from + i;
+        const float x = d[z][0][row], y = d[z][1][row];
+        const uint32_t top = block_max<16>(__builtin_bit_cast(uint32_t, max_abs(x, y, y)));
+        seen = top > seen ? top : seen;
+        // the scale's exponent field, in place
+        uint32_t field = top & 0x7F800000u;
+        field = (field > 0x01000000u ? field : 0x01000000u) - 0x01000000u;
+        uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x, y, as_f32(field), 0);
+        uint32_t byte = field >> 23;
+        if (TEST && top >= 0x7F800000u) {
+          code = 0;
+          byte = 255;
+        }
+        const int64_t half = o.row_bytes / 2;  // bytes of one projection's columns
+        if (WHOLE || row < left)
+          (o.codes + (r0 + row) * o.row_bytes + z * half)[static_cast<uint32_t>(c) / 2] =
+              static_cast<uint8_t>(code);
+        kept[z] = (lane & 15) == row % 16 ? byte : kept[z];
+        if (row % 16 == 15)
+          *mx_scale_at(o, r0 + row - 15 + (lane & 15), (z * 2 * half + c) / kMxBlock) =
+              static_cast<uint8_t>(kept[z]);
+      }
+    return seen;
+  }
+
+  __device__ __forceinline__ void run(const MxOut& along, const MxOut& across, int64_t r0,
+                                      int64_t c, int64_t n, int lane) {
+    uint32_t kept[2] = {0, 0};  // this lane's share of the scales of sixteen rows
+    uint32_t seen = 0;
+    const bool to_along = along.codes != nullptr && left > 0;
+    load(0);
+#pragma unroll
+    for (int chunk = 0; chunk < 32 / CHUNK; ++chunk) {
+      if (chunk + 1 < 32 / CHUNK) load(chunk + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      gradients(chunk);
+      if (to_along) {
+        const uint32_t top =
+            encode_along<CHUNK, false>(along, r0, c, lane, chunk * CHUNK, kept);
+        seen = top > seen ? top : seen;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (to_along && __any(seen >= 0x7F800000u)) encode_along<32, true>(along, r0, c, lane, 0, kept);
+    if (across.codes == nullptr) return;
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float* v = d[z][e];
+        float top = max_abs(v[0], v[1], v[1]);
+#pragma unroll
+        for (int i = 2; i < kMxBlock; i += 2) top = max_abs(top, v[i], v[i + 1]);
+        const uint32_t byte = mx_scale_byte(__builtin_bit_cast(uint32_t, top));
+        const float scale = mx_scale_operand(byte);
+        u32x4_t code = {mx_encode8(v, scale), mx_encode8(v + 8, scale), mx_encode8(v + 16, scale),
+                        mx_encode8(v + 24, scale)};
+        if (byte == 255u) code = u32x4_t{0, 0, 0, 0};
+        if (WHOLE || c + e < n) {
+          const int64_t row = z * n + c + e;
+          *reinterpret_cast<u32x4_t*>(across.codes + row * across.row_bytes + r0 / 2) = code;
+          *mx_scale_at(across, row, r0 / kMxBlock) = static_cast<uint8_t>(byte);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+};
+
+constexpr int kGatedWaves = 4;
+constexpr int kGatedThreads = 64 * kGatedWaves;
+
+template <int DTYPE, bool PAIRS>
+__global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per_eu(2)))
+    k_mx_gated_backward(const void* __restrict__ dh, const void* __restrict__ z_gate,
+                        const void* __restrict__ z_up, int64_t m, int64_t n, int64_t per,
+                        int64_t rows, MxOut along, MxOut across) {
+  // The waves of a workgroup take consecutive rows of the same columns, so that the
+  // 16 bytes that each writes to a row of the transpose's codes meet in one line of
+  // one L2 (with the waves side by side instead, a line was written from eight XCDs:
+  // 204 us for the transposes alone of 16384 x 6144, 174 so). The wave's index is
+  // made uniform so that rows are addressed from scalar registers.
+  const int64_t group = block_of_grid();
+  const int64_t r0 = (group / per * kGatedWaves +
+                      __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6))) * 32;
+  const int64_t tile = group % per;
+  if (r0 >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t c0 = tile * 128;
+  const int64_t c = c0 + 2 * lane;
+  const int64_t first = r0 < m ? r0 : m - 1;
+  constexpr int SIZE = DTYPE == kBF16 ? 2 : 4;
+  auto run = [&](auto whole) {
+    GatedTile<DTYPE, decltype(whole)::value, PAIRS || decltype(whole)::value> t;
+    t.src[0] = static_cast<const uint8_t*>(dh) + first * n * SIZE;
+    t.src[1] = static_cast<const uint8_t*>(z_gate) + first * n * SIZE;
+    t.src[2] = static_cast<const uint8_t*>(z_up) + first * n * SIZE;
+    t.stride = n * SIZE;
+    t.left = static_cast<int>(m - first < 32 ? m - first : 32);
+    if (r0 >= m) t.left = 0;
+    // columns past the end read the last ones
+    const int64_t a = PAIRS ? (c < n ? c : n - 2) : (c < n ? c : n - 1);
+    t.at[0] = static_cast<uint32_t>(a * SIZE);
+    t.at[1] = static_cast<uint32_t>((c + 1 < n ? c + 1 : n - 1) * SIZE);
+    if constexpr (DTYPE == kBF16) {
+      t.in_column[0] = (c < n ? 0xFFFFu : 0u) | (c + 1 < n ? 0xFFFF0000u : 0u);
+    } else {
+      t.in_column[0] = c < n ? ~0u : 0u;
+      t.in_column[1] = c + 1 < n ? ~0u : 0u;
+    }
+    t.run(along, across, r0, c, n, lane);
+  };
+  if (PAIRS && r0 + 32 <= m && c0 + 128 <= n)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
   // rows of scales past the last of the stack
-  if (tile % per == 0 && 2 * n + lane < across.scale_rows)
+  if (across.codes != nullptr && tile == 0 && 2 * n + lane < across.scale_rows)
     *mx_scale_at(across, 2 * n + lane, r0 / kMxBlock) = 0;
 }
 
@@ -565,16 +647,17 @@ hipError_t launch_mx_gated_backward(const void* dh, const void* z_gate, const vo
                                     hipStream_t stream) {
   const int64_t per =
       along.codes != nullptr ? mx_slices(n) * (kMxSlice / 128) : ceil_div(n, 128);
-  const int64_t tiles =
-      per * (across.codes != nullptr ? mx_slices(m) * kMxSliceBlocks : ceil_div(m, kMxBlock));
-  if (tiles == 0) return hipSuccess;
-  const dim3 grid = grid_of(ceil_div(tiles, kThreads / 64));
-  if (dtype == kBF16)
-    hipLaunchKernelGGL(k_mx_gated_backward<kBF16>, grid, dim3(kThreads), 0, stream, dh, z_gate,
-                       z_up, m, n, per, tiles, along, across);
-  else
-    hipLaunchKernelGGL(k_mx_gated_backward<kF32>, grid, dim3(kThreads), 0, stream, dh, z_gate, z_up,
-                       m, n, per, tiles, along, across);
+  // rows that something is written for
+  const int64_t rows =
+      across.codes != nullptr ? mx_slices(m) * kMxSlice : mx_pad_rows(m);
+  const int64_t groups = per * ceil_div(rows, 32 * kGatedWaves);
+  if (groups == 0) return hipSuccess;
+  auto* kernel = dtype == kBF16 ? (n % 2 == 0 ? k_mx_gated_backward<kBF16, true>
+                                              : k_mx_gated_backward<kBF16, false>)
+                                : (n % 2 == 0 ? k_mx_gated_backward<kF32, true>
+                                              : k_mx_gated_backward<kF32, false>);
+  hipLaunchKernelGGL(kernel, grid_of(groups), dim3(kGatedThreads), 0, stream, dh, z_gate, z_up, m,
+                     n, per, rows, along, across);
   return hipGetLastError();
 }
 

@@ -104,6 +104,8 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
   constexpr int SCALE_SEGS = (BM + BN + 127) / 128;
   static_assert(SCALE_SEGS <= NW, "a wave loads one segment of scales");
   constexpr int LPW = CODE_LPW + 1;
+  constexpr int EARLY = (LPW + 1) / 2;  // of a refill, issued in step 3; the others in step 0
+  constexpr int LATE = LPW - EARLY;
   static_assert(NS >= 2 && LPW * (NS - 1) < 64, "vmcnt range");
   constexpr int SCALES = (BM + BN) * kMxSliceBytes;
   constexpr int STAGE = SCALES + SCALE_SEGS * 1024;
@@ -202,8 +204,9 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) dma_one(smem + s * STAGE, s < ns ? s : ns - 1, i);
-  wait_sync<(NS - 1) * LPW>();
+    for (int i = 0; i < (s == NS - 1 ? EARLY : LPW); ++i)
+      dma_one(smem + s * STAGE, s < ns ? s : ns - 1, i);
+  wait_sync<(NS - 2) * LPW + EARLY>();
 #pragma unroll
   for (int j = 0; j < NFR; ++j) frag_one(smem, 0, j, fx);
 #pragma unroll
@@ -227,13 +230,19 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
     const int next = stage + 1 == NS ? 0 : stage + 1;
     uint8_t* st = smem + stage * STAGE;
     const uint8_t* nst = smem + next * STAGE;
-    RPX_MX_STEP(0, fx, RPX_MX_READS(st, 1, fy))
+    const int64_t late = t + NS - 1 < ns ? t + NS - 1 : ns - 1;
+    uint8_t* last = smem + (stage == 0 ? NS - 1 : stage - 1) * STAGE;
+    RPX_MX_STEP(0, fx, {
+      RPX_MX_READS(st, 1, fy)
+      _Pragma("unroll") for (int d = EARLY + i * LATE / NMF; d < EARLY + (i + 1) * LATE / NMF; ++d)
+          dma_one(last, late, d);
+    })
     RPX_MX_STEP(1, fy, RPX_MX_READS(st, 2, fx))
     RPX_MX_STEP(2, fx, RPX_MX_READS(st, 3, fy))
     wait_sync<(NS - 2) * LPW>();
     const int64_t refill = t + NS < ns ? t + NS : ns - 1;
     RPX_MX_STEP(3, fy, {
-      _Pragma("unroll") for (int d = i * LPW / NMF; d < (i + 1) * LPW / NMF; ++d)
+      _Pragma("unroll") for (int d = i * EARLY / NMF; d < (i + 1) * EARLY / NMF; ++d)
           dma_one(st, refill, d);
       RPX_MX_READS(nst, 0, fx)
       _Pragma("unroll") for (int j = read_from(i); j < read_from(i + 1); ++j)

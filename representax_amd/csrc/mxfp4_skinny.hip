@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_skinny(MxSkinny p) {
   store_rows<DTYPE, GATED>(p, token, n0 + 4 * q, sum);
 }
 
-// The same for up to TILES x 16 rows of x that are encoded already: a lane reads its
-// blocks' codes and scales as it reads the weight's.
+// The same for rows of x that are encoded already, TILES x 16 of them a workgroup: a
+// lane reads its blocks' codes and scales as it reads the weight's.
 template <int DTYPE, int TILES, bool GATED>
 __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
   constexpr int G = GATED ? 2 : 1;
@@ -212,15 +212,18 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int waves = blockDim.x >> 6;
   const int q = lane >> 4;
-  const int64_t n0 = block_of_grid() * kTokens;
-  if (n0 >= p.n) return;  // the whole workgroup
+  // workgroups of one group of rows of x after those of another
+  const int64_t per = ceil_div(p.n, kTokens);
+  const int64_t n0 = block_of_grid() % per * kTokens;
+  const int64_t m0 = block_of_grid() / per * (TILES * kTokens);
+  if (m0 >= p.m) return;  // the whole workgroup
   const int64_t r = n0 + (lane & 15) < p.n ? n0 + (lane & 15) : p.n - 1;
   const int64_t pad = mx_pad_rows(p.n);
   const int64_t x_pad = mx_pad_rows(p.m);
   int64_t token[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
-    token[t] = t * kTokens + (lane & 15);
+    token[t] = m0 + t * kTokens + (lane & 15);
     token[t] = token[t] < p.m ? token[t] : p.m - 1;
   }
   f32x4_t acc[TILES][G];
@@ -274,8 +277,8 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
       for (int g = 0; g < G; ++g)
         sum[g] += *reinterpret_cast<const f32x4_t*>(
             partial + (((v * TILES + t) * G + g) * 64 + lane) * 4);
-    if (t * kTokens + (lane & 15) < p.m)
-      store_rows<DTYPE, GATED>(p, t * kTokens + (lane & 15), n0 + 4 * q, sum);
+    if (m0 + t * kTokens + (lane & 15) < p.m)
+      store_rows<DTYPE, GATED>(p, m0 + t * kTokens + (lane & 15), n0 + 4 * q, sum);
   }
 }
 
@@ -296,7 +299,8 @@ hipError_t launch_thin(const MxSkinny& p, hipStream_t stream) {
   constexpr int kWaves = 64 / (TILES * G) < kMaxWaves ? 64 / (TILES * G) : kMaxWaves;
   const int waves = static_cast<int>(p.slices < kWaves ? p.slices : kWaves);
   const size_t lds = static_cast<size_t>(waves) * TILES * G * 64 * 4 * sizeof(float);
-  hipLaunchKernelGGL((k_mx_thin<DTYPE, TILES, GATED>), grid_of(ceil_div(p.n, kTokens)),
+  const int64_t groups = ceil_div(p.m, TILES * kTokens);
+  hipLaunchKernelGGL((k_mx_thin<DTYPE, TILES, GATED>), grid_of(groups * ceil_div(p.n, kTokens)),
                      dim3(64 * waves), lds, stream, p);
   return hipGetLastError();
 }
