@@ -464,20 +464,41 @@ Plan plan_for(int id, int64_t m, int64_t n, int64_t slices, bool gated) {
   return p;
 }
 
+// The tile: large where it fills the card, for fewer reads from LDS and the L2 a
+// product; smaller where that leaves CUs idle. Measured (us, bf16 outputs,
+// M x N <- K; tiles by id):
+//   16384 x 2048 <- 6144   2: 102, 4: 118        8192 x 8192 <- 8192   2: 250, 4: 305
+//   8192 x 3072 <- 768     2: 23.2, 4: 21.6      gated 16384 x 3072 <- 768   2: 74, 4: 81
+//   8192 x 768 <- 3072     2: 21.9, 4: 16.9, 6: 19.3
+//   333 x 6144 <- 2048     4: 7.9, 6: 8.4, 7: 8.0
+//   1024 x 2048 <- 2048    4: 7.8, 6: 6.7, 7: 7.3
+//   3072 x 768 <- 8192     4: 24.3, 5: 20.4, 6: 22.7 (144 tiles of 4 and 5: one a CU,
+//                          where 5's four stages take the place of a second workgroup)
+//   3500 x 768 <- 3072     4: 10.1, 5: 10.7
+// A product of few tiles over a long sum is split; the partial tiles and their sum
+// cost 7 to 10 us (768 x 768 <- 8192, tile 7: 13.3 us whole, 14.6 in two, 15.0 in four).
 Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {
+  auto tiles_of = [&](int id) {
+    const Plan p = plan_for(id, m, n, slices, gated);
+    return p.tiles_m * p.tiles_n;
+  };
   int id = tune(kTuneMxTile);
   if (id == 0) {
-    id = 1;
-    for (int c : {1, 4, 6}) {
-      id = c;
-      const Plan p = plan_for(c, m, n, slices, gated);
-      if (p.tiles_m * p.tiles_n >= 192) break;
-    }
+    const int64_t large = tiles_of(2), medium = tiles_of(4);
+    if (large >= 192 && (slices >= 6 || large >= 1024))
+      id = 2;
+    else if (medium >= 140)
+      id = medium <= 256 && slices >= 24 ? 5 : 4;
+    else
+      id = tiles_of(6) >= 192 ? 6 : 7;
   }
   Plan p = plan_for(id, m, n, slices, gated);
   const int64_t tiles = p.tiles_m * p.tiles_n;
   int64_t splits = tune(kTuneMxSplits);
-  if (splits == 0) splits = tiles >= 128 ? 1 : 256 / (tiles > 0 ? tiles : 1);
+  if (splits == 0) {
+    splits = slices < 48 || tiles == 0 ? 1 : 512 / tiles;
+    if (splits > slices / 16) splits = slices / 16;
+  }
   if (gated) splits = 1;
   if (splits > slices / 4) splits = slices / 4;
   if (splits > 1) {

@@ -1,4 +1,5 @@
-/* CPython binding of the per-token (small-M) INT4 + LoRA forward entry points.
+/* CPython binding of the per-token (small-M) forward entry points: INT4 + LoRA and
+ * kept MXFP4 weights.
  *
  * An eager small-M forward spends more time on the host than on the GPU, and
  * ctypes' per-argument conversion is a large share of it. These functions
@@ -185,6 +186,55 @@ static PyObject* fast_get_tuning(PyObject* self, PyObject* const* args, Py_ssize
   return PyLong_FromLong(rpx_get_tuning(knob));
 }
 
+/* mxfp4_linear(x, dtype, m, k, row_stride, codes, scales, n, y, workspace,
+ *              workspace_bytes, stream) -> status */
+static PyObject* fast_mxfp4_linear(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void *x, *codes, *scales, *y, *ws, *stream;
+  int dtype;
+  int64_t m, k, stride, n, ws_bytes;
+  if (!check_nargs("mxfp4_linear", nargs, 12)) return NULL;
+  if (!get_ptr(args[0], &x) || !get_int(args[1], &dtype) || !get_i64(args[2], &m) ||
+      !get_i64(args[3], &k) || !get_i64(args[4], &stride) || !get_ptr(args[5], &codes) ||
+      !get_ptr(args[6], &scales) || !get_i64(args[7], &n) || !get_ptr(args[8], &y) ||
+      !get_ptr(args[9], &ws) || !get_i64(args[10], &ws_bytes) || !get_ptr(args[11], &stream))
+    return NULL;
+  return PyLong_FromLong(rpx_mxfp4_linear(x, dtype, m, k, stride, codes, scales, n, y, ws,
+                                          (size_t)ws_bytes, stream));
+}
+
+/* mxfp4_gated(x, dtype, m, k, row_stride, gate_codes, gate_scales, up_codes,
+ *             up_scales, n, h, workspace, workspace_bytes, stream) -> status */
+static PyObject* fast_mxfp4_gated(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void *x, *gate, *gate_scales, *up, *up_scales, *h, *ws, *stream;
+  int dtype;
+  int64_t m, k, stride, n, ws_bytes;
+  if (!check_nargs("mxfp4_gated", nargs, 14)) return NULL;
+  if (!get_ptr(args[0], &x) || !get_int(args[1], &dtype) || !get_i64(args[2], &m) ||
+      !get_i64(args[3], &k) || !get_i64(args[4], &stride) || !get_ptr(args[5], &gate) ||
+      !get_ptr(args[6], &gate_scales) || !get_ptr(args[7], &up) ||
+      !get_ptr(args[8], &up_scales) || !get_i64(args[9], &n) || !get_ptr(args[10], &h) ||
+      !get_ptr(args[11], &ws) || !get_i64(args[12], &ws_bytes) || !get_ptr(args[13], &stream))
+    return NULL;
+  return PyLong_FromLong(rpx_mxfp4_gated(x, dtype, m, k, stride, gate, gate_scales, up, up_scales,
+                                         n, h, ws, (size_t)ws_bytes, stream));
+}
+
+/* mxfp4_serve_workspace(m, n, k, gated) -> bytes of either call */
+static PyObject* fast_mxfp4_serve_workspace(PyObject* self, PyObject* const* args,
+                                            Py_ssize_t nargs) {
+  (void)self;
+  int64_t m, n, k;
+  int gated;
+  if (!check_nargs("mxfp4_serve_workspace", nargs, 4)) return NULL;
+  if (!get_i64(args[0], &m) || !get_i64(args[1], &n) || !get_i64(args[2], &k) ||
+      !get_int(args[3], &gated))
+    return NULL;
+  return PyLong_FromSize_t(gated ? rpx_mxfp4_gated_workspace(m, n, k)
+                                 : rpx_mxfp4_linear_workspace(m, n, k));
+}
+
 static PyMethodDef methods[] = {
     {"get_tuning", (PyCFunction)(void (*)(void))fast_get_tuning, METH_FASTCALL, "rpx_get_tuning"},
     {"int4lora_forward", (PyCFunction)(void (*)(void))fast_int4lora_forward, METH_FASTCALL,
@@ -196,6 +246,12 @@ static PyMethodDef methods[] = {
     {"int4lora_forward_multi_workspace",
      (PyCFunction)(void (*)(void))fast_int4lora_forward_multi_workspace, METH_FASTCALL,
      "rpx_int4lora_forward_multi_workspace"},
+    {"mxfp4_linear", (PyCFunction)(void (*)(void))fast_mxfp4_linear, METH_FASTCALL,
+     "rpx_mxfp4_linear"},
+    {"mxfp4_gated", (PyCFunction)(void (*)(void))fast_mxfp4_gated, METH_FASTCALL,
+     "rpx_mxfp4_gated"},
+    {"mxfp4_serve_workspace", (PyCFunction)(void (*)(void))fast_mxfp4_serve_workspace,
+     METH_FASTCALL, "rpx_mxfp4_linear_workspace, rpx_mxfp4_gated_workspace"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rpxfast",

@@ -27,6 +27,8 @@ and a sum over nothing is zero.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -83,19 +85,23 @@ class MXFP4Matrix:
     def empty(cls, rows: int, columns: int, device: torch.device) -> "MXFP4Matrix":
         """Room for an encoded matrix, contents undefined."""
 
-        return cls(torch.empty((rows, _slices(columns) * (SLICE // 2)), dtype=torch.uint8,
-                               device=device),
-                   torch.empty(_scales_shape(rows, columns), dtype=torch.uint8, device=device),
-                   columns)
+        made = cls.__new__(cls)  # of the right layout: without the checks
+        slices = _slices(columns)
+        made.codes = torch.empty((rows, slices * (SLICE // 2)), dtype=torch.uint8, device=device)
+        made.scales = torch.empty((slices, _pad_rows(rows), 8), dtype=torch.uint8, device=device)
+        made.columns = columns
+        return made
 
     def dequantize(self, dtype: torch.dtype = BF16) -> torch.Tensor:
         """The values that the codes stand for (exact in bf16 and float32)."""
 
-        device = _on_device(self.codes, self.scales)
-        out = torch.empty(self.shape, dtype=dtype, device=device)
+        codes, scales = self.codes, self.scales
+        device = _on_device(codes, scales)
+        rows, columns = codes.shape[0], self.columns
+        out = torch.empty((rows, columns), dtype=dtype, device=device)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_dequantize", _ptr(self.codes), _ptr(self.scales), *self.shape,
-                     _ptr(out), _dtype_code(dtype), _stream(device))
+            nat.call("rpx_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), rows, columns,
+                     out.data_ptr(), _dtype_code(dtype), _stream(device))
         return out
 
     def __repr__(self) -> str:
@@ -142,17 +148,16 @@ def _part(t, along: MXFP4Matrix | None, across: MXFP4Matrix | None):
     """One matrix to encode, as the library takes it (``across``: its transpose)."""
 
     rows, columns = t.shape
-    return nat.Mxfp4Part(_ptr(t), rows, columns, max(t.stride(0), columns),
-                         _ptr(along.codes) if along else None,
-                         _ptr(along.scales) if along else None, 0,
-                         _ptr(across.codes) if across else None,
-                         _ptr(across.scales) if across else None, 0, _dtype_code(t.dtype))
+    return nat.Mxfp4Part(t.data_ptr(), rows, columns, max(t.stride(0), columns),
+                         along.codes.data_ptr() if along else None,
+                         along.scales.data_ptr() if along else None, 0,
+                         across.codes.data_ptr() if across else None,
+                         across.scales.data_ptr() if across else None, 0, _dtype_code(t.dtype))
 
 
-def _encode(parts, device: torch.device) -> None:
-    count = len(parts)
+def _encode(part, device: torch.device) -> None:
     with _launches_on(device):
-        nat.call("rpx_mxfp4_quantize", (nat.Mxfp4Part * count)(*parts), count, _stream(device))
+        nat.call("rpx_mxfp4_quantize", ctypes.byref(part), 1, _stream(device))
 
 
 def mxfp4_quantize(t: torch.Tensor) -> MXFP4Matrix:
@@ -162,11 +167,11 @@ def mxfp4_quantize(t: torch.Tensor) -> MXFP4Matrix:
     if t.stride(0) == 1 and t.stride(1) > 1:  # a transpose: encode along its own rows
         base = _dense_rows(t.t())
         out = MXFP4Matrix.empty(*t.shape, device)
-        _encode([_part(base, None, out)], device)
+        _encode(_part(base, None, out), device)
         return out
     t = _dense_rows(t)
     out = MXFP4Matrix.empty(*t.shape, device)
-    _encode([_part(t, out, None)], device)
+    _encode(_part(t, out, None), device)
     return out
 
 
@@ -182,7 +187,7 @@ def mxfp4_quantize_both(t: torch.Tensor) -> tuple[MXFP4Matrix, MXFP4Matrix]:
     t = _dense_rows(t)
     along = MXFP4Matrix.empty(*t.shape, device)
     across = MXFP4Matrix.empty(t.shape[1], t.shape[0], device)
-    _encode([_part(t, along, across)], device)
+    _encode(_part(t, along, across), device)
     return along, across
 
 
@@ -209,48 +214,60 @@ def mxfp4_matmul(a: MXFP4Matrix, b: MXFP4Matrix, out_dtype: torch.dtype = BF16) 
         return _gemm(a, b, out_dtype, device)
 
 
-def _check_serving(x2d: torch.Tensor, *weights: MXFP4Matrix):
+def _serve(x2d: torch.Tensor, weight: MXFP4Matrix, up: MXFP4Matrix | None) -> torch.Tensor:
+    """``mxfp4_linear``, or ``mxfp4_gated`` with ``up``. (Written for host time, which is
+    most of a single token's call: each torch attribute is read once.)"""
+
     _matrix_input(x2d, "x")
-    for w in weights:
-        if w.columns != x2d.shape[1]:
-            raise ValueError(f"x has {x2d.shape[1]} columns, the MXFP4 weight {w.columns}")
-        if w.rows != weights[0].rows:
-            raise ValueError(f"gate and up must have the same rows, got {weights[0].rows} and "
-                             f"{w.rows}")
-    device = _on_device(x2d, *[t for w in weights for t in (w.codes, w.scales)])
-    return device, _dense_rows(x2d)
+    m, k = x2d.shape
+    codes, scales = weight.codes, weight.scales
+    n = codes.shape[0]
+    if weight.columns != k or (up is not None and up.columns != k):
+        raise ValueError(f"x has {k} columns, the MXFP4 weight "
+                         f"{weight.columns if weight.columns != k else up.columns}")
+    if up is None:
+        device = _on_device(x2d, codes, scales)
+    else:
+        if up.codes.shape[0] != n:
+            raise ValueError(f"gate and up must have the same rows, got {n} and {up.rows}")
+        device = _on_device(x2d, codes, scales, up.codes, up.scales)
+    x2d = _dense_rows(x2d)
+    y = torch.empty((m, n), dtype=x2d.dtype, device=device)
+    stream = _stream(device)
+    fast = nat.fast()
+    gated = up is not None
+    if fast is not None:
+        need = fast.mxfp4_serve_workspace(m, n, k, gated)
+    else:
+        need = nat.query("rpx_mxfp4_gated_workspace" if gated else "rpx_mxfp4_linear_workspace",
+                         m, n, k)
+    # the call's scratch; none for a few rows
+    ws = _workspace(need, device, stream) if need else None
+    args = [x2d.data_ptr(), _dtype_code(x2d.dtype), m, k, max(x2d.stride(0), k), codes.data_ptr(),
+            scales.data_ptr()]
+    if gated:
+        args += (up.codes.data_ptr(), up.scales.data_ptr())
+    args += (n, y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), stream)
+    with _launches_on(device):
+        if fast is not None:
+            nat.check((fast.mxfp4_gated if gated else fast.mxfp4_linear)(*args))
+        else:
+            nat.call("rpx_mxfp4_gated" if gated else "rpx_mxfp4_linear", *args)
+    return y
 
 
 def mxfp4_linear(x2d: torch.Tensor, weight: MXFP4Matrix) -> torch.Tensor:
     """``x [M, K] W^T`` in x's dtype, ``weight`` the encoded ``W [N, K]``; x is encoded
     within the call. Inference: no gradients."""
 
-    device, x2d = _check_serving(x2d, weight)
-    m, k = x2d.shape
-    n = weight.rows
-    y = torch.empty((m, n), dtype=x2d.dtype, device=device)
-    ws = _workspace(nat.query("rpx_mxfp4_linear_workspace", m, n, k), device)
-    with _launches_on(device):
-        nat.call("rpx_mxfp4_linear", _ptr(x2d), _dtype_code(x2d.dtype), m, k,
-                 max(x2d.stride(0), k), _ptr(weight.codes), _ptr(weight.scales), n, _ptr(y),
-                 _ptr(ws), ws.numel(), _stream(device))
-    return y
+    return _serve(x2d, weight, None)
 
 
 def mxfp4_gated(x2d: torch.Tensor, gate: MXFP4Matrix, up: MXFP4Matrix) -> torch.Tensor:
     """``silu(x G^T) * (x U^T)`` in x's dtype over two kept weights, in one pass over x;
     both products are rounded to x's dtype before the activation. Inference."""
 
-    device, x2d = _check_serving(x2d, gate, up)
-    m, k = x2d.shape
-    n = gate.rows
-    h = torch.empty((m, n), dtype=x2d.dtype, device=device)
-    ws = _workspace(nat.query("rpx_mxfp4_gated_workspace", m, n, k), device)
-    with _launches_on(device):
-        nat.call("rpx_mxfp4_gated", _ptr(x2d), _dtype_code(x2d.dtype), m, k,
-                 max(x2d.stride(0), k), _ptr(gate.codes), _ptr(gate.scales), _ptr(up.codes),
-                 _ptr(up.scales), n, _ptr(h), _ptr(ws), ws.numel(), _stream(device))
-    return h
+    return _serve(x2d, gate, up)
 
 
 # ---------------------------------------------------------------------------
