@@ -95,6 +95,8 @@ int rpx_abi_version(void);
  *   RPX_TUNE_MX_TILE     MXFP4 GEMM tile: 0 planner, 1..7
  *   RPX_TUNE_MX_SPLITS   MXFP4 GEMM split count over the contracted columns:
  *                        0 planner, 1..64 (at least four slices each)
+ *   RPX_TUNE_MX_PAIR     an MXFP4 backward's two products in one launch: -1
+ *                        planner, 0 two launches
  * ------------------------------------------------------------------------- */
 #define RPX_TUNE_INT4_TILE 0
 #define RPX_TUNE_BF16_TILE 1
@@ -111,6 +113,7 @@ int rpx_abi_version(void);
 #define RPX_TUNE_FP8_PAIR 12
 #define RPX_TUNE_MX_TILE 13
 #define RPX_TUNE_MX_SPLITS 14
+#define RPX_TUNE_MX_PAIR 15
 
 /* RPX_ERR_INVALID for an unknown knob or value. */
 int rpx_set_tuning(int knob, int value);

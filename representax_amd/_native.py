@@ -48,6 +48,7 @@ TUNE_FP8_SPLITS = 11
 TUNE_FP8_PAIR = 12
 TUNE_MX_TILE = 13
 TUNE_MX_SPLITS = 14
+TUNE_MX_PAIR = 15
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64

@@ -195,6 +195,7 @@ bool knob_value_ok(int knob, int v) {
     case kTuneFp8Pair: return v == -1 || v == 0;
     case kTuneMxTile: return v >= 0 && v <= mx_tile_count();
     case kTuneMxSplits: return v >= 0 && v <= 64;
+    case kTuneMxPair: return v == -1 || v == 0;
     default: return false;
   }
 }
@@ -207,7 +208,7 @@ int env_int(const char* name, int fallback) {
 struct Knobs {
   std::atomic<int> v[kTuneCount];
   Knobs() {
-    const int defaults[kTuneCount] = {0, 0, 0, 0, -1, -1, 0, 0, -1, 0, 0, 0, -1, 0, 0};
+    const int defaults[kTuneCount] = {0, 0, 0, 0, -1, -1, 0, 0, -1, 0, 0, 0, -1, 0, 0, -1};
     for (int i = 0; i < kTuneCount; ++i) v[i].store(defaults[i], std::memory_order_relaxed);
     // RPX_GEMM_TILE names a tile of either GEMM (the id sets are disjoint)
     const int gemm = env_int("RPX_GEMM_TILE", 0);

@@ -73,6 +73,23 @@ int product(const char* who, const Encoded& a, const Encoded& b, void* out, int 
   return kOk;
 }
 
+// Two such products.
+int products(const char* who, const Encoded& a0, const Encoded& b0, void* out0, int dtype0,
+             const Encoded& a1, const Encoded& b1, void* out1, int dtype1, float* partials,
+             hipStream_t st) {
+  if (out0 == nullptr || out1 == nullptr || a0.columns == 0 || a1.columns == 0) {
+    if (out0 != nullptr) RPX_TRY(product(who, a0, b0, out0, dtype0, partials, st));
+    if (out1 != nullptr) RPX_TRY(product(who, a1, b1, out1, dtype1, partials, st));
+    return kOk;
+  }
+  const MxGemm g0{a0.codes, a0.scales, b0.codes, b0.scales, nullptr, nullptr, a0.rows, b0.rows,
+                  mx_slices(a0.columns), out0, nullptr, nullptr, dtype0};
+  const MxGemm g1{a1.codes, a1.scales, b1.codes, b1.scales, nullptr, nullptr, a1.rows, b1.rows,
+                  mx_slices(a1.columns), out1, nullptr, nullptr, dtype1};
+  RPX_HIP(launch_mx_gemm_pair(g0, g1, partials, st), who);
+  return kOk;
+}
+
 int64_t product_floats(int64_t m, int64_t n, int64_t k) {
   return m <= 0 || n <= 0 || k <= 0 ? 0 : mx_gemm_workspace_floats(m, n, mx_slices(k));
 }
@@ -440,9 +457,7 @@ int rpx_mxfp4_linear_backward(const void* grad, int grad_dtype, int64_t m, int64
     parts.part[0] = MxPart{grad, grad_dtype, m, n, m > 1 ? grad_stride : n, gq.out(), gt.out(), 0};
     RPX_HIP(launch_mx_quantize(parts, 1, st), who);
   }
-  if (d_right != nullptr) RPX_TRY(product(who, gt, xt, d_right, right_dtype, partials, st));
-  if (d_left != nullptr) RPX_TRY(product(who, gq, wt, d_left, left_dtype, partials, st));
-  return kOk;
+  return products(who, gt, xt, d_right, right_dtype, gq, wt, d_left, left_dtype, partials, st);
 }
 
 // --- the gated block's training step --------------------------------------------
@@ -562,9 +577,8 @@ int rpx_mxfp4_gated_backward_products(const void* dh, const void* z_gate, const 
   hipStream_t st = static_cast<hipStream_t>(stream);
   RPX_TRY(rpx_mxfp4_gated_backward(dh, z_gate, z_up, dtype, m, n, dz.codes, dz.scales, dzt.codes,
                                    dzt.scales, stream));
-  if (d_weights != nullptr) RPX_TRY(product(who, dzt, xt, d_weights, weights_dtype, partials, st));
-  if (d_left != nullptr) RPX_TRY(product(who, dz, both, d_left, left_dtype, partials, st));
-  return kOk;
+  return products(who, dzt, xt, d_weights, weights_dtype, dz, both, d_left, left_dtype, partials,
+                  st);
 }
 
 }  // extern "C"

@@ -367,6 +367,9 @@ struct MxGemm {
 int mx_tile_count();
 int64_t mx_gemm_workspace_floats(int64_t m, int64_t n, int64_t slices);
 hipError_t launch_mx_gemm(const MxGemm& p, float* partials, hipStream_t stream);
+// Two products (no gated ones), in one launch where that pays.
+hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials,
+                               hipStream_t stream);
 
 // The same for few rows over kept weights (codes2: the up projection's, or null):
 // from x itself, m <= 16 rows of k columns of `dtype`, or (x_scales given) from its

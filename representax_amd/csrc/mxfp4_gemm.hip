@@ -17,8 +17,12 @@ namespace {
 
 // Writes a wave's sub-tile of ROWS x COLS bf16 values, staged in LDS with a row
 // pitch of 2 COLS + 16 bytes, as 16-byte pieces of whole row segments. m0, n0:
-// its first row and column in the output.
-template <int ROWS, int COLS>
+// its first row and column in the output. PAST: past the L2, for what is not read
+// soon (the projections that a training step keeps: 308 -> 286 us for the gated block
+// of 16384 x 2048 -> 2 x 6144, 1013 -> 992 for its step. Outputs that the next kernel
+// reads gain as much and lose it there: 16384 x 6144 <- 2048 and its encoding 176 us
+// either way).
+template <int ROWS, int COLS, bool PAST>
 __device__ __forceinline__ void store_staged(const uint8_t* reg, uint16_t* out, int64_t m0,
                                              int64_t n0, int64_t M, int64_t N, int lane) {
   constexpr int P = COLS * 2 + 16;
@@ -35,10 +39,16 @@ __device__ __forceinline__ void store_staged(const uint8_t* reg, uint16_t* out, 
         const int idx = (i0 + i) * 64 + lane;
         v[i] = *reinterpret_cast<const u32x4_t*>(reg + (idx / CPR) * P + (idx % CPR) * 16);
       }
-#pragma unroll
-      for (int i = 0; i < UN; ++i) {
+      auto at = [&](int i) {
         const int idx = (i0 + i) * 64 + lane;
-        *reinterpret_cast<u32x4_t*>(out + (m0 + idx / CPR) * N + n0 + 8 * (idx % CPR)) = v[i];
+        return reinterpret_cast<u32x4_t*>(out + (m0 + idx / CPR) * N + n0 + 8 * (idx % CPR));
+      };
+      if constexpr (PAST) {
+#pragma unroll
+        for (int i = 0; i < UN; ++i) __builtin_nontemporal_store(v[i], at(i));
+      } else {
+#pragma unroll
+        for (int i = 0; i < UN; ++i) *at(i) = v[i];
       }
     }
     return;
@@ -338,7 +348,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
           }
           stage_block(fm, fn, g, pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3]));
         }
-    store_staged<TM, OUT_N / WN>(reg, static_cast<uint16_t*>(p.out), mw, nw, p.m, p.n, lane);
+    store_staged<TM, OUT_N / WN, false>(reg, static_cast<uint16_t*>(p.out), mw, nw, p.m, p.n, lane);
     if (p.z_gate == nullptr) return;
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
@@ -352,8 +362,8 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
             stage_block(fm, fn, g, pack_bf16x2(a[4 * g], a[4 * g + 1]),
                         pack_bf16x2(a[4 * g + 2], a[4 * g + 3]));
           }
-      store_staged<TM, OUT_N / WN>(reg, static_cast<uint16_t*>(z == 0 ? p.z_gate : p.z_up), mw, nw,
-                                   p.m, p.n, lane);
+      store_staged<TM, OUT_N / WN, true>(reg, static_cast<uint16_t*>(z == 0 ? p.z_gate : p.z_up),
+                                         mw, nw, p.m, p.n, lane);
     }
   } else {
 #pragma unroll
@@ -366,7 +376,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
           stage_block(fm, fn, g, pack_bf16x2(a[4 * g], a[4 * g + 1]),
                       pack_bf16x2(a[4 * g + 2], a[4 * g + 3]));
         }
-    store_staged<TM, TN>(reg, static_cast<uint16_t*>(p.out), mw, nw, p.m, p.n, lane);
+    store_staged<TM, TN, false>(reg, static_cast<uint16_t*>(p.out), mw, nw, p.m, p.n, lane);
   }
 }
 
@@ -383,6 +393,20 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   band_tile(b % tiles, tiles_m, tiles_n, band, tile_m, tile_n);
   mx_gemm_tile<BM, BN, WM, WN, NS, GATED>(p, b / tiles, slices_per_split, tile_m, tile_n, tiles,
                                           tile_m * tiles_n + tile_n, partials);
+}
+
+// Two products in one launch: the first blocks run p's tiles, the others q's.
+template <int BM, int BN, int WM, int WN, int NS, int WPE>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
+    k_mx_gemm_pair(MxGemm p, MxGemm q, int p_tiles_n, int p_tiles, int q_tiles_n, int band) {
+  const bool first = static_cast<int>(blockIdx.x) < p_tiles;
+  const MxGemm g = first ? p : q;
+  const int block = first ? blockIdx.x : blockIdx.x - p_tiles;
+  const int tiles = first ? p_tiles : gridDim.x - p_tiles;
+  const int tiles_n = first ? p_tiles_n : q_tiles_n;
+  int tile_m, tile_n;
+  band_tile(xcd_block(block, tiles), tiles / tiles_n, tiles_n, band, tile_m, tile_n);
+  mx_gemm_tile<BM, BN, WM, WN, NS, false>(g, 0, g.slices, tile_m, tile_n, tiles, 0, nullptr);
 }
 
 // Sums the partial tiles of a split product in split order. One thread per
@@ -477,21 +501,22 @@ Plan plan_for(int id, int64_t m, int64_t n, int64_t slices, bool gated) {
 //   3500 x 768 <- 3072     4: 10.1, 5: 10.7
 // A product of few tiles over a long sum is split; the partial tiles and their sum
 // cost 7 to 10 us (768 x 768 <- 8192, tile 7: 13.3 us whole, 14.6 in two, 15.0 in four).
+template <class TilesOf>
+int tile_for(TilesOf tiles_of, int64_t slices) {
+  if (tune(kTuneMxTile) != 0) return tune(kTuneMxTile);
+  const int64_t large = tiles_of(2), medium = tiles_of(4);
+  if (large >= 192 && (slices >= 6 || large >= 1024)) return 2;
+  if (medium >= 140) return medium <= 256 && slices >= 24 ? 5 : 4;
+  return tiles_of(6) >= 192 ? 6 : 7;
+}
+
 Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {
-  auto tiles_of = [&](int id) {
-    const Plan p = plan_for(id, m, n, slices, gated);
-    return p.tiles_m * p.tiles_n;
-  };
-  int id = tune(kTuneMxTile);
-  if (id == 0) {
-    const int64_t large = tiles_of(2), medium = tiles_of(4);
-    if (large >= 192 && (slices >= 6 || large >= 1024))
-      id = 2;
-    else if (medium >= 140)
-      id = medium <= 256 && slices >= 24 ? 5 : 4;
-    else
-      id = tiles_of(6) >= 192 ? 6 : 7;
-  }
+  const int id = tile_for(
+      [&](int c) {
+        const Plan p = plan_for(c, m, n, slices, gated);
+        return p.tiles_m * p.tiles_n;
+      },
+      slices);
   Plan p = plan_for(id, m, n, slices, gated);
   const int64_t tiles = p.tiles_m * p.tiles_n;
   int64_t splits = tune(kTuneMxSplits);
@@ -508,22 +533,44 @@ Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {
   return p;
 }
 
+template <int BM, int BN, int WM, int WN, bool GATED>
+constexpr int lds_bytes(int stages) {
+  constexpr int SCALE_SEGS = (BM + BN + 127) / 128;
+  constexpr int STAGE = (BM + BN) * kMxSliceBytes + SCALE_SEGS * 1024;
+  constexpr int OUT = WM * WN * (BM / WM) * ((GATED ? BN / 2 : BN) / WN * 2 + 16);
+  return stages * STAGE > OUT ? stages * STAGE : OUT;
+}
+
+int band_of() { return tune(kTuneBand) > 0 ? tune(kTuneBand) : 4; }
+
+template <int BM, int BN, int WM, int WN, int NS, int WPE>
+hipError_t launch_pair_config(const MxGemm& p, const MxGemm& q, const Plan& pp, const Plan& qp,
+                              hipStream_t stream) {
+  constexpr int LDS = lds_bytes<BM, BN, WM, WN, false>(NS);
+  const void* kernel = reinterpret_cast<const void*>(k_mx_gemm_pair<BM, BN, WM, WN, NS, WPE>);
+  static std::atomic<unsigned> done{0};
+  if (hipError_t e = ensure_lds_limit(kernel, LDS, done); e != hipSuccess) return e;
+  const int64_t tiles = pp.tiles_m * pp.tiles_n + qp.tiles_m * qp.tiles_n;
+  if (tiles > (int64_t{1} << 30)) return hipErrorInvalidValue;
+  k_mx_gemm_pair<BM, BN, WM, WN, NS, WPE>
+      <<<dim3(static_cast<unsigned>(tiles)), dim3(64 * WM * WN), LDS, stream>>>(
+          p, q, static_cast<int>(pp.tiles_n), static_cast<int>(pp.tiles_m * pp.tiles_n),
+          static_cast<int>(qp.tiles_n), band_of());
+  return hipGetLastError();
+}
+
 template <int BM, int BN, int WM, int WN, int NS, int WPE, bool GATED>
 hipError_t launch_config(const MxGemm& g, const Plan& p, float* partials, hipStream_t stream) {
-  constexpr int SCALE_SEGS = (BM + BN + 127) / 128;
-  constexpr int STAGES = NS * ((BM + BN) * kMxSliceBytes + SCALE_SEGS * 1024);
-  constexpr int OUT = WM * WN * (BM / WM) * ((GATED ? BN / 2 : BN) / WN * 2 + 16);
-  constexpr int LDS = STAGES > OUT ? STAGES : OUT;
+  constexpr int LDS = lds_bytes<BM, BN, WM, WN, GATED>(NS);
   static_assert(LDS <= 160 * 1024, "LDS");
   const void* kernel = reinterpret_cast<const void*>(k_mx_gemm<BM, BN, WM, WN, NS, WPE, GATED>);
   static std::atomic<unsigned> done{0};
   if (hipError_t e = ensure_lds_limit(kernel, LDS, done); e != hipSuccess) return e;
   const int64_t tiles = p.tiles_m * p.tiles_n;
   if (tiles * p.splits > (int64_t{1} << 30)) return hipErrorInvalidValue;
-  const int band = tune(kTuneBand) > 0 ? tune(kTuneBand) : 4;
   k_mx_gemm<BM, BN, WM, WN, NS, WPE, GATED>
       <<<dim3(static_cast<unsigned>(tiles * p.splits)), dim3(64 * WM * WN), LDS, stream>>>(
-          g, p.per_split, static_cast<int>(p.tiles_m), static_cast<int>(p.tiles_n), band,
+          g, p.per_split, static_cast<int>(p.tiles_m), static_cast<int>(p.tiles_n), band_of(),
           p.splits > 1 ? partials : nullptr);
   if (p.splits > 1) {
     const int64_t chunks = tiles * (BM * BN / 4);
@@ -557,6 +604,44 @@ hipError_t launch_mx_gemm(const MxGemm& g, float* partials, hipStream_t stream) 
   case ID:                                                                        \
     return gated ? launch_config<BM, BN, WM, WN, NS, WPE, true>(g, p, partials, stream) \
                  : launch_config<BM, BN, WM, WN, NS, WPE, false>(g, p, partials, stream);
+    RPX_MX_CONFIGS(X)
+#undef X
+  }
+  return hipErrorInvalidValue;
+}
+
+// A backward's two products in one launch, in the tile that suits them together,
+// the longer sums first: a product's last round of tiles leaves CUs idle, which the
+// other's then fill, and there is one launch. A whole step in graph replays, one
+// launch against two: the linear of 1001 x 500 -> 1300 29.9 / 35.2 us, of 3500 x 3072
+// -> 768 61 / 69, of 5003 x 2048 -> 6144 171 / 182, its gated block 331 / 376; of
+// 16384 x 2048 -> 2048 233 / 234.
+// A product that is split runs on its own, so that an output has the same bits
+// whether or not the other one is wanted.
+hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials,
+                               hipStream_t stream) {
+  const bool alone = a.m == 0 || a.n == 0 || b.m == 0 || b.n == 0 || tune(kTuneMxPair) == 0 ||
+                     choose(a.m, a.n, a.slices, false).splits > 1 ||
+                     choose(b.m, b.n, b.slices, false).splits > 1;
+  if (alone) {
+    if (hipError_t e = launch_mx_gemm(a, partials, stream); e != hipSuccess) return e;
+    return launch_mx_gemm(b, partials, stream);
+  }
+  const MxGemm& p = a.slices >= b.slices ? a : b;
+  const MxGemm& q = a.slices >= b.slices ? b : a;
+  const int64_t slices = q.slices;
+  auto tiles_of = [&](int id) {
+    const Plan x = plan_for(id, p.m, p.n, p.slices, false);
+    const Plan y = plan_for(id, q.m, q.n, q.slices, false);
+    return x.tiles_m * x.tiles_n + y.tiles_m * y.tiles_n;
+  };
+  const int id = tile_for(tiles_of, slices);
+  const Plan pp = plan_for(id, p.m, p.n, p.slices, false);
+  const Plan qp = plan_for(id, q.m, q.n, q.slices, false);
+  switch (id) {
+#define X(ID, BM, BN, WM, WN, NS, WPE) \
+  case ID:                             \
+    return launch_pair_config<BM, BN, WM, WN, NS, WPE>(p, q, pp, qp, stream);
     RPX_MX_CONFIGS(X)
 #undef X
   }

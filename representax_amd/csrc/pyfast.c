@@ -1,7 +1,7 @@
-/* CPython binding of the per-token (small-M) forward entry points: INT4 + LoRA and
- * kept MXFP4 weights.
+/* CPython binding of the per-token (small-M) INT4 + LoRA forward and of the MXFP4
+ * entry points.
  *
- * An eager small-M forward spends more time on the host than on the GPU, and
+ * Such an eager call spends more time on the host than on the GPU, and
  * ctypes' per-argument conversion is a large share of it. These functions
  * take the same arguments as the C ABI (device pointers as Python ints, NULL
  * as None) through METH_FASTCALL and forward them unchanged; each returns the
@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <stdint.h>
+#include <string.h>
 
 #include "../../include/representax_amd.h"
 
@@ -186,53 +187,105 @@ static PyObject* fast_get_tuning(PyObject* self, PyObject* const* args, Py_ssize
   return PyLong_FromLong(rpx_get_tuning(knob));
 }
 
-/* mxfp4_linear(x, dtype, m, k, row_stride, codes, scales, n, y, workspace,
- *              workspace_bytes, stream) -> status */
+typedef union {
+  void* p;
+  int64_t l;
+  int i;
+} Value;
+
+/* Arguments by a format: p pointer, l int64, i int. */
+static int parse(const char* name, const char* format, PyObject* const* args, Py_ssize_t nargs,
+                 Value* v) {
+  if (!check_nargs(name, nargs, (Py_ssize_t)strlen(format))) return 0;
+  for (Py_ssize_t j = 0; j < nargs; ++j) {
+    const int ok = format[j] == 'p'   ? get_ptr(args[j], &v[j].p)
+                   : format[j] == 'l' ? get_i64(args[j], &v[j].l)
+                                      : get_int(args[j], &v[j].i);
+    if (!ok) return 0;
+  }
+  return 1;
+}
+
+/* The MXFP4 calls take the C functions' arguments, without the stream's cast. */
 static PyObject* fast_mxfp4_linear(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  void *x, *codes, *scales, *y, *ws, *stream;
-  int dtype;
-  int64_t m, k, stride, n, ws_bytes;
-  if (!check_nargs("mxfp4_linear", nargs, 12)) return NULL;
-  if (!get_ptr(args[0], &x) || !get_int(args[1], &dtype) || !get_i64(args[2], &m) ||
-      !get_i64(args[3], &k) || !get_i64(args[4], &stride) || !get_ptr(args[5], &codes) ||
-      !get_ptr(args[6], &scales) || !get_i64(args[7], &n) || !get_ptr(args[8], &y) ||
-      !get_ptr(args[9], &ws) || !get_i64(args[10], &ws_bytes) || !get_ptr(args[11], &stream))
-    return NULL;
-  return PyLong_FromLong(rpx_mxfp4_linear(x, dtype, m, k, stride, codes, scales, n, y, ws,
-                                          (size_t)ws_bytes, stream));
+  Value v[12];
+  if (!parse("mxfp4_linear", "pilllpplpplp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(rpx_mxfp4_linear(v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].p,
+                                          v[7].l, v[8].p, v[9].p, (size_t)v[10].l, v[11].p));
 }
 
-/* mxfp4_gated(x, dtype, m, k, row_stride, gate_codes, gate_scales, up_codes,
- *             up_scales, n, h, workspace, workspace_bytes, stream) -> status */
 static PyObject* fast_mxfp4_gated(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  void *x, *gate, *gate_scales, *up, *up_scales, *h, *ws, *stream;
-  int dtype;
-  int64_t m, k, stride, n, ws_bytes;
-  if (!check_nargs("mxfp4_gated", nargs, 14)) return NULL;
-  if (!get_ptr(args[0], &x) || !get_int(args[1], &dtype) || !get_i64(args[2], &m) ||
-      !get_i64(args[3], &k) || !get_i64(args[4], &stride) || !get_ptr(args[5], &gate) ||
-      !get_ptr(args[6], &gate_scales) || !get_ptr(args[7], &up) ||
-      !get_ptr(args[8], &up_scales) || !get_i64(args[9], &n) || !get_ptr(args[10], &h) ||
-      !get_ptr(args[11], &ws) || !get_i64(args[12], &ws_bytes) || !get_ptr(args[13], &stream))
-    return NULL;
-  return PyLong_FromLong(rpx_mxfp4_gated(x, dtype, m, k, stride, gate, gate_scales, up, up_scales,
-                                         n, h, ws, (size_t)ws_bytes, stream));
+  Value v[14];
+  if (!parse("mxfp4_gated", "pilllpppplpplp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(rpx_mxfp4_gated(v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].p,
+                                         v[7].p, v[8].p, v[9].l, v[10].p, v[11].p,
+                                         (size_t)v[12].l, v[13].p));
 }
 
-/* mxfp4_serve_workspace(m, n, k, gated) -> bytes of either call */
-static PyObject* fast_mxfp4_serve_workspace(PyObject* self, PyObject* const* args,
+static PyObject* fast_mxfp4_linear_forward(PyObject* self, PyObject* const* args,
+                                           Py_ssize_t nargs) {
+  (void)self;
+  Value v[19];
+  if (!parse("mxfp4_linear_forward", "pilllpilllpipliiplp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(rpx_mxfp4_linear_forward(
+      v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].i, v[7].l, v[8].l, v[9].l, v[10].p,
+      v[11].i, v[12].p, (size_t)v[13].l, v[14].i, v[15].i, v[16].p, (size_t)v[17].l, v[18].p));
+}
+
+static PyObject* fast_mxfp4_linear_backward(PyObject* self, PyObject* const* args,
                                             Py_ssize_t nargs) {
   (void)self;
-  int64_t m, n, k;
-  int gated;
-  if (!check_nargs("mxfp4_serve_workspace", nargs, 4)) return NULL;
-  if (!get_i64(args[0], &m) || !get_i64(args[1], &n) || !get_i64(args[2], &k) ||
-      !get_int(args[3], &gated))
-    return NULL;
-  return PyLong_FromSize_t(gated ? rpx_mxfp4_gated_workspace(m, n, k)
-                                 : rpx_mxfp4_linear_workspace(m, n, k));
+  Value v[17];
+  if (!parse("mxfp4_linear_backward", "pilllplliipipiplp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(rpx_mxfp4_linear_backward(
+      v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, (size_t)v[6].l, v[7].l, v[8].i, v[9].i,
+      v[10].p, v[11].i, v[12].p, v[13].i, v[14].p, (size_t)v[15].l, v[16].p));
+}
+
+static PyObject* fast_mxfp4_gated_forward(PyObject* self, PyObject* const* args,
+                                          Py_ssize_t nargs) {
+  (void)self;
+  Value v[25];
+  if (!parse("mxfp4_gated_forward", "pilllpillpilllpppipliiplp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(rpx_mxfp4_gated_forward(
+      v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].i, v[7].l, v[8].l, v[9].p, v[10].i,
+      v[11].l, v[12].l, v[13].l, v[14].p, v[15].p, v[16].p, v[17].i, v[18].p, (size_t)v[19].l,
+      v[20].i, v[21].i, v[22].p, (size_t)v[23].l, v[24].p));
+}
+
+static PyObject* fast_mxfp4_gated_backward(PyObject* self, PyObject* const* args,
+                                           Py_ssize_t nargs) {
+  (void)self;
+  Value v[18];
+  if (!parse("mxfp4_gated_backward_products", "pppillplliipipiplp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(rpx_mxfp4_gated_backward_products(
+      v[0].p, v[1].p, v[2].p, v[3].i, v[4].l, v[5].l, v[6].p, (size_t)v[7].l, v[8].l, v[9].i,
+      v[10].i, v[11].p, v[12].i, v[13].p, v[14].i, v[15].p, (size_t)v[16].l, v[17].p));
+}
+
+/* mxfp4_bytes(what, m, n, k, need_left, need_right) -> bytes; what: 0 linear, 1
+ * gated (serving workspaces), 2 and 3 their saved buffers, 4 and 5 their forward,
+ * 6 and 7 their backward workspaces */
+static PyObject* fast_mxfp4_bytes(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[6];
+  if (!parse("mxfp4_bytes", "illlii", args, nargs, v)) return NULL;
+  const int64_t m = v[1].l, n = v[2].l, k = v[3].l;
+  const int left = v[4].i, right = v[5].i;
+  switch (v[0].i) {
+    case 0: return PyLong_FromSize_t(rpx_mxfp4_linear_workspace(m, n, k));
+    case 1: return PyLong_FromSize_t(rpx_mxfp4_gated_workspace(m, n, k));
+    case 2: return PyLong_FromSize_t(rpx_mxfp4_linear_saved_bytes(m, n, k, left, right));
+    case 3: return PyLong_FromSize_t(rpx_mxfp4_gated_saved_bytes(m, n, k, left, right));
+    case 4: return PyLong_FromSize_t(rpx_mxfp4_linear_forward_workspace(m, n, k));
+    case 5: return PyLong_FromSize_t(rpx_mxfp4_gated_forward_workspace(m, n, k));
+    case 6: return PyLong_FromSize_t(rpx_mxfp4_linear_backward_workspace(m, n, k, left, right));
+    case 7: return PyLong_FromSize_t(rpx_mxfp4_gated_backward_workspace(m, n, k, left, right));
+  }
+  PyErr_SetString(PyExc_ValueError, "mxfp4_bytes: unknown size");
+  return NULL;
 }
 
 static PyMethodDef methods[] = {
@@ -250,8 +303,16 @@ static PyMethodDef methods[] = {
      "rpx_mxfp4_linear"},
     {"mxfp4_gated", (PyCFunction)(void (*)(void))fast_mxfp4_gated, METH_FASTCALL,
      "rpx_mxfp4_gated"},
-    {"mxfp4_serve_workspace", (PyCFunction)(void (*)(void))fast_mxfp4_serve_workspace,
-     METH_FASTCALL, "rpx_mxfp4_linear_workspace, rpx_mxfp4_gated_workspace"},
+    {"mxfp4_linear_forward", (PyCFunction)(void (*)(void))fast_mxfp4_linear_forward,
+     METH_FASTCALL, "rpx_mxfp4_linear_forward"},
+    {"mxfp4_linear_backward", (PyCFunction)(void (*)(void))fast_mxfp4_linear_backward,
+     METH_FASTCALL, "rpx_mxfp4_linear_backward"},
+    {"mxfp4_gated_forward", (PyCFunction)(void (*)(void))fast_mxfp4_gated_forward, METH_FASTCALL,
+     "rpx_mxfp4_gated_forward"},
+    {"mxfp4_gated_backward_products", (PyCFunction)(void (*)(void))fast_mxfp4_gated_backward,
+     METH_FASTCALL, "rpx_mxfp4_gated_backward_products"},
+    {"mxfp4_bytes", (PyCFunction)(void (*)(void))fast_mxfp4_bytes, METH_FASTCALL,
+     "the MXFP4 calls' buffer sizes"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rpxfast",

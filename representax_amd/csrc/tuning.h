@@ -28,7 +28,8 @@ enum TuneKnob : int {
   kTuneFp8Pair = 12,    // fp8 backward's two products in one launch: -1 planner, 0 never  RPX_FP8_PAIR
   kTuneMxTile = 13,     // MXFP4 GEMM tile (0: planner)
   kTuneMxSplits = 14,   // MXFP4 GEMM split count (0: planner)
-  kTuneCount = 15
+  kTuneMxPair = 15,     // MXFP4 backward's two products in one launch: -1 planner, 0 never
+  kTuneCount = 16
 };
 
 // Current value of a knob.

@@ -51,6 +51,35 @@ def _scales_shape(rows: int, columns: int) -> tuple[int, int, int]:
     return (_slices(columns), _pad_rows(rows), 8)
 
 
+# what ``_bytes`` is asked for: a linear's, the gated block's is one more
+_SERVE, _SAVED, _FORWARD, _BACKWARD = 0, 2, 4, 6
+_BYTES = ("rpx_mxfp4_linear_workspace", "rpx_mxfp4_gated_workspace",
+          "rpx_mxfp4_linear_saved_bytes", "rpx_mxfp4_gated_saved_bytes",
+          "rpx_mxfp4_linear_forward_workspace", "rpx_mxfp4_gated_forward_workspace",
+          "rpx_mxfp4_linear_backward_workspace", "rpx_mxfp4_gated_backward_workspace")
+
+
+def _bytes(what: int, m: int, n: int, k: int, need_left: bool, need_right: bool) -> int:
+    """The size of a call's buffer."""
+
+    fast = nat.fast()
+    if fast is not None:
+        return fast.mxfp4_bytes(what, m, n, k, need_left, need_right)
+    needs = (need_left, need_right) if what in (2, 3, 6, 7) else ()
+    return nat.query(_BYTES[what], m, n, k, *needs)
+
+
+def _call(name: str, *args) -> None:
+    """``rpx_mxfp4_<name>`` through the fast binding where it is loaded: an eager step of
+    a linear is three calls whose host time would be a third ctypes' conversions."""
+
+    fast = nat.fast()
+    if fast is not None:
+        nat.check(getattr(fast, "mxfp4_" + name)(*args))
+    else:
+        nat.call("rpx_mxfp4_" + name, *args)
+
+
 class MXFP4Matrix:
     """An encoded matrix ``[rows, columns]``: ``codes`` uint8 ``[rows, C / 2]`` and
     ``scales`` uint8 ``[C / 256, R, 8]`` (C and R the columns and rows rounded up to
@@ -234,25 +263,16 @@ def _serve(x2d: torch.Tensor, weight: MXFP4Matrix, up: MXFP4Matrix | None) -> to
     x2d = _dense_rows(x2d)
     y = torch.empty((m, n), dtype=x2d.dtype, device=device)
     stream = _stream(device)
-    fast = nat.fast()
     gated = up is not None
-    if fast is not None:
-        need = fast.mxfp4_serve_workspace(m, n, k, gated)
-    else:
-        need = nat.query("rpx_mxfp4_gated_workspace" if gated else "rpx_mxfp4_linear_workspace",
-                         m, n, k)
-    # the call's scratch; none for a few rows
-    ws = _workspace(need, device, stream) if need else None
+    need = _bytes(_SERVE + gated, m, n, k, False, False)
+    ws = _workspace(need, device, stream) if need else None  # none for a few rows
     args = [x2d.data_ptr(), _dtype_code(x2d.dtype), m, k, max(x2d.stride(0), k), codes.data_ptr(),
             scales.data_ptr()]
     if gated:
         args += (up.codes.data_ptr(), up.scales.data_ptr())
-    args += (n, y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), stream)
     with _launches_on(device):
-        if fast is not None:
-            nat.check((fast.mxfp4_gated if gated else fast.mxfp4_linear)(*args))
-        else:
-            nat.call("rpx_mxfp4_gated" if gated else "rpx_mxfp4_linear", *args)
+        _call("gated" if gated else "linear", *args, n, y.data_ptr(), _ptr(ws),
+              0 if ws is None else ws.numel(), stream)
     return y
 
 
@@ -292,12 +312,12 @@ def _right(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-def _saved(name: str, m: int, n: int, k: int, need_left: bool, need_right: bool, device):
+def _saved(what: int, m: int, n: int, k: int, need_left: bool, need_right: bool, device):
     """The buffer that a forward keeps for its backward, or None."""
 
     if not (need_left or need_right):
         return None
-    return torch.empty(nat.query(name, m, n, k, need_left, need_right), dtype=torch.uint8,
+    return torch.empty(_bytes(what, m, n, k, need_left, need_right), dtype=torch.uint8,
                        device=device)
 
 
@@ -314,11 +334,11 @@ class MXFP4LinearFn(torch.autograd.Function):
         need_left, need_right = ctx.needs_input_grad[:2]
         x, w = _dense_rows(left), _right(right)
         y = torch.empty((m, n), dtype=out_dtype, device=device)
-        saved = _saved("rpx_mxfp4_linear_saved_bytes", m, n, k, need_left, need_right, device)
+        saved = _saved(_SAVED, m, n, k, need_left, need_right, device)
         stream = _stream(device)
-        ws = _workspace(nat.query("rpx_mxfp4_linear_forward_workspace", m, n, k), device, stream)
+        ws = _workspace(_bytes(_FORWARD, m, n, k, False, False), device, stream)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_linear_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
+            _call("linear_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
                      x.stride(0), w.data_ptr(), _dtype_code(w.dtype), n, *w.stride(),
                      y.data_ptr(), _dtype_code(out_dtype), _ptr(saved),
                      0 if saved is None else saved.numel(), need_left, need_right, ws.data_ptr(),
@@ -339,10 +359,9 @@ class MXFP4LinearFn(torch.autograd.Function):
         d_left = torch.empty((m, k), dtype=left_dtype, device=device) if need_left else None
         d_right = torch.empty((n, k), dtype=right_dtype, device=device) if need_right else None
         stream = _stream(device)
-        ws = _workspace(nat.query("rpx_mxfp4_linear_backward_workspace", m, n, k, need_left,
-                                  need_right), device, stream)
+        ws = _workspace(_bytes(_BACKWARD, m, n, k, need_left, need_right), device, stream)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_linear_backward", g.data_ptr(), _dtype_code(g.dtype), m, n,
+            _call("linear_backward", g.data_ptr(), _dtype_code(g.dtype), m, n,
                      g.stride(0), saved.data_ptr(), saved.numel(), k, saved_left, saved_right,
                      _ptr(d_left), _dtype_code(left_dtype), _ptr(d_right),
                      _dtype_code(right_dtype), ws.data_ptr(), ws.numel(), stream)
@@ -373,11 +392,11 @@ class MXFP4GatedFn(torch.autograd.Function):
         z_gate = z_up = None
         if need_left or need_w:
             z_gate, z_up = (torch.empty((m, n), dtype=out_dtype, device=device) for _ in range(2))
-        saved = _saved("rpx_mxfp4_gated_saved_bytes", m, n, k, need_left, need_w, device)
+        saved = _saved(_SAVED + 1, m, n, k, need_left, need_w, device)
         stream = _stream(device)
-        ws = _workspace(nat.query("rpx_mxfp4_gated_forward_workspace", m, n, k), device, stream)
+        ws = _workspace(_bytes(_FORWARD + 1, m, n, k, False, False), device, stream)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_gated_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
+            _call("gated_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
                      x.stride(0), wg.data_ptr(), _dtype_code(wg.dtype), *wg.stride(),
                      wu.data_ptr(), _dtype_code(wu.dtype), *wu.stride(), n, h.data_ptr(),
                      _ptr(z_gate), _ptr(z_up), _dtype_code(out_dtype), _ptr(saved),
@@ -401,10 +420,9 @@ class MXFP4GatedFn(torch.autograd.Function):
         d_x = torch.empty((m, k), dtype=left_dtype, device=device) if need_left else None
         d_w = torch.empty((2 * n, k), dtype=wide, device=device) if need_w else None
         stream = _stream(device)
-        ws = _workspace(nat.query("rpx_mxfp4_gated_backward_workspace", m, n, k, need_left,
-                                  need_w), device, stream)
+        ws = _workspace(_bytes(_BACKWARD + 1, m, n, k, need_left, need_w), device, stream)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_gated_backward_products", dh.data_ptr(), z_gate.data_ptr(),
+            _call("gated_backward_products", dh.data_ptr(), z_gate.data_ptr(),
                      z_up.data_ptr(), _dtype_code(dh.dtype), m, n, saved.data_ptr(),
                      saved.numel(), k, saved_left, saved_w, _ptr(d_x), _dtype_code(left_dtype),
                      _ptr(d_w), _dtype_code(wide), ws.data_ptr(), ws.numel(), stream)

@@ -244,6 +244,7 @@ TUNING_KNOBS = {
     "fp8_pair": nat.TUNE_FP8_PAIR,
     "mx_tile": nat.TUNE_MX_TILE,
     "mx_splits": nat.TUNE_MX_SPLITS,
+    "mx_pair": nat.TUNE_MX_PAIR,
 }
 
 

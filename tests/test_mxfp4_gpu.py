@@ -383,6 +383,24 @@ def test_linear_gradients_are_the_three_products(m, k, n):
     assert torch.equal(torch.autograd.grad(y3, xd, to_dev_bf16(dy))[0], xd.grad)
 
 
+@pytest.mark.parametrize("tile", [0, *TILES])
+def test_gradients_of_one_launch_equal_two(tile):
+    g = rng(30 + tile)
+    for m, k, n in ((300, 520, 130), (1100, 256, 700), (64, 33, 900)):
+        x, w, u = _data(g, m, k), _data(g, n, k, 0.05), _data(g, n, k, 0.05)
+        dy = to_dev_bf16(_data(g, m, n, 1e-3))
+        leaves = [to_dev_bf16(t).requires_grad_() for t in (x, w, u)]
+        grads = []
+        for pair in (-1, 0):
+            with ops.tuning(mx_tile=tile, mx_pair=pair), rx.precision_context(POLICY):
+                y = rx.linear_matmul(leaves[0], leaves[1].t())
+                h = rx.gated_matmul(leaves[0], leaves[1].t(), leaves[2].t())
+                grads.append(torch.autograd.grad(y, leaves[:2], dy) +
+                             torch.autograd.grad(h, leaves, dy))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+        _check_product(grads[0][1], from_dev(dy).T, x.T, BF16)
+
+
 def test_linear_gradients_against_differences():
     """Operands that MXFP4 holds exactly along both axes make the product linear: moving
     one of them from 4 to 6 moves the loss by exactly the gradient times 2."""
