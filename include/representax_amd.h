@@ -92,7 +92,8 @@ int rpx_abi_version(void);
  *   RPX_TUNE_FP8_PAIR    fp8 linear backward's input and weight gradients in
  *                        one launch: -1 planner (where both products' tiles
  *                        allow it), 0 two launches (env RPX_FP8_PAIR)
- *   RPX_TUNE_MX_TILE     MXFP4 GEMM tile: 0 planner, 1..7
+ *   RPX_TUNE_MX_TILE     MXFP4 GEMM tile: 0 planner, 1 256x256, 2 128x128,
+ *                        3 128x128 with four stages, 4 64x128, 5 64x64
  *   RPX_TUNE_MX_SPLITS   MXFP4 GEMM split count over the contracted columns:
  *                        0 planner, 1..64 (at least four slices each)
  *   RPX_TUNE_MX_PAIR     an MXFP4 backward's two products in one launch: -1

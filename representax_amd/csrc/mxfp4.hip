@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
   const int64_t first = r0 < m ? r0 : m - 1;
   constexpr int SIZE = DTYPE == kBF16 ? 2 : 4;
   auto run = [&](auto whole) {
-    GatedTile<DTYPE, decltype(whole)::value, PAIRS || decltype(whole)::value> t;
+    GatedTile<DTYPE, decltype(whole)::value, PAIRS> t;
     t.src[0] = static_cast<const uint8_t*>(dh) + first * n * SIZE;
     t.src[1] = static_cast<const uint8_t*>(z_gate) + first * n * SIZE;
     t.src[2] = static_cast<const uint8_t*>(z_up) + first * n * SIZE;
@@ -513,10 +513,14 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
     }
     t.run(along, across, r0, c, n, lane);
   };
-  if (PAIRS && r0 + 32 <= m && c0 + 128 <= n)
-    run(std::true_type{});
-  else
+  if constexpr (PAIRS) {
+    if (r0 + 32 <= m && c0 + 128 <= n)
+      run(std::true_type{});
+    else
+      run(std::false_type{});
+  } else {
     run(std::false_type{});
+  }
   // rows of scales past the last of the stack
   if (across.codes != nullptr && tile == 0 && 2 * n + lane < across.scale_rows)
     *mx_scale_at(across, 2 * n + lane, r0 / kMxBlock) = 0;

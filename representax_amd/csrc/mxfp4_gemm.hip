@@ -452,15 +452,15 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Tiles: id, rows of A, rows of B, waves along each, stages, waves per SIMD.
+// Tiles: id, rows of A, rows of B, waves along each, stages, waves per SIMD. (A 256 x
+// 256 tile of four waves, which reads less of LDS but has one wave a SIMD, measured as
+// the first: 257 against 253 us at 8192 x 8192 <- 8192; 256 x 128 with three stages 290.)
 #define RPX_MX_CONFIGS(X)     \
-  X(1, 256, 256, 2, 2, 2, 1)  \
-  X(2, 256, 256, 4, 2, 2, 2)  \
-  X(3, 256, 128, 2, 2, 3, 1)  \
-  X(4, 128, 128, 2, 2, 2, 2)  \
-  X(5, 128, 128, 2, 2, 4, 1)  \
-  X(6, 64, 128, 2, 2, 2, 2)   \
-  X(7, 64, 64, 2, 1, 2, 2)
+  X(1, 256, 256, 4, 2, 2, 2)  \
+  X(2, 128, 128, 2, 2, 2, 2)  \
+  X(3, 128, 128, 2, 2, 4, 1)  \
+  X(4, 64, 128, 2, 2, 2, 2)   \
+  X(5, 64, 64, 2, 1, 2, 2)
 
 struct Plan {
   int id, bm, bn;
@@ -491,23 +491,23 @@ Plan plan_for(int id, int64_t m, int64_t n, int64_t slices, bool gated) {
 // The tile: large where it fills the card, for fewer reads from LDS and the L2 a
 // product; smaller where that leaves CUs idle. Measured (us, bf16 outputs,
 // M x N <- K; tiles by id):
-//   16384 x 2048 <- 6144   2: 102, 4: 118        8192 x 8192 <- 8192   2: 250, 4: 305
-//   8192 x 3072 <- 768     2: 23.2, 4: 21.6      gated 16384 x 3072 <- 768   2: 74, 4: 81
-//   8192 x 768 <- 3072     2: 21.9, 4: 16.9, 6: 19.3
-//   333 x 6144 <- 2048     4: 7.9, 6: 8.4, 7: 8.0
-//   1024 x 2048 <- 2048    4: 7.8, 6: 6.7, 7: 7.3
-//   3072 x 768 <- 8192     4: 24.3, 5: 20.4, 6: 22.7 (144 tiles of 4 and 5: one a CU,
-//                          where 5's four stages take the place of a second workgroup)
-//   3500 x 768 <- 3072     4: 10.1, 5: 10.7
+//   16384 x 2048 <- 6144   1: 102, 2: 118        8192 x 8192 <- 8192   1: 250, 2: 305
+//   8192 x 3072 <- 768     1: 23.2, 2: 21.6      gated 16384 x 3072 <- 768   1: 74, 2: 81
+//   8192 x 768 <- 3072     1: 21.9, 2: 16.9, 4: 19.3
+//   333 x 6144 <- 2048     2: 7.9, 4: 8.4, 5: 8.0
+//   1024 x 2048 <- 2048    2: 7.8, 4: 6.7, 5: 7.3
+//   3072 x 768 <- 8192     2: 24.3, 3: 20.4, 4: 22.7 (144 tiles of 2 and 3: one a CU,
+//                          where 3's four stages take the place of a second workgroup)
+//   3500 x 768 <- 3072     2: 10.1, 3: 10.7
 // A product of few tiles over a long sum is split; the partial tiles and their sum
-// cost 7 to 10 us (768 x 768 <- 8192, tile 7: 13.3 us whole, 14.6 in two, 15.0 in four).
+// cost 7 to 10 us (768 x 768 <- 8192, tile 5: 13.3 us whole, 14.6 in two, 15.0 in four).
 template <class TilesOf>
 int tile_for(TilesOf tiles_of, int64_t slices) {
   if (tune(kTuneMxTile) != 0) return tune(kTuneMxTile);
-  const int64_t large = tiles_of(2), medium = tiles_of(4);
-  if (large >= 192 && (slices >= 6 || large >= 1024)) return 2;
-  if (medium >= 140) return medium <= 256 && slices >= 24 ? 5 : 4;
-  return tiles_of(6) >= 192 ? 6 : 7;
+  const int64_t large = tiles_of(1), medium = tiles_of(2);
+  if (large >= 192 && (slices >= 6 || large >= 1024)) return 1;
+  if (medium >= 140) return medium <= 256 && slices >= 24 ? 3 : 2;
+  return tiles_of(4) >= 192 ? 4 : 5;
 }
 
 Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {

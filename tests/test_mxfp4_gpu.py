@@ -160,7 +160,7 @@ def test_products_over_long_sums(m, n, k):
     _check_product(got, a, b, F32)
 
 
-TILES = range(1, 8)
+TILES = range(1, 6)
 
 
 @pytest.mark.parametrize("tile", TILES)
