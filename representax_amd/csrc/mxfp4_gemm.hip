@@ -331,8 +331,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm& p, int split, int64_t
         u32x2_t{lo, hi};
   };
   if constexpr (GATED) {
-    // pass 0 leaves the rounded projections in acc's low words, pass 1 and 2 (if
-    // asked for) store them
+    // first h, of the rounded projections; then, if asked for, the projections
 #pragma unroll
     for (int fn = 0; fn < FO; ++fn)
 #pragma unroll

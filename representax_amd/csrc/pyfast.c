@@ -206,7 +206,7 @@ static int parse(const char* name, const char* format, PyObject* const* args, Py
   return 1;
 }
 
-/* The MXFP4 calls take the C functions' arguments, without the stream's cast. */
+/* The MXFP4 calls take the C functions' arguments (mxfp4_quantize: of its one part). */
 static PyObject* fast_mxfp4_linear(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   Value v[12];
@@ -222,6 +222,25 @@ static PyObject* fast_mxfp4_gated(PyObject* self, PyObject* const* args, Py_ssiz
   return PyLong_FromLong(rpx_mxfp4_gated(v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].p,
                                          v[7].p, v[8].p, v[9].l, v[10].p, v[11].p,
                                          (size_t)v[12].l, v[13].p));
+}
+
+/* mxfp4_quantize(t, rows, columns, row_stride, codes, scales, codes_t, scales_t, dtype,
+ * stream): one matrix, its codes dense. */
+static PyObject* fast_mxfp4_quantize(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[10];
+  if (!parse("mxfp4_quantize", "plllppppip", args, nargs, v)) return NULL;
+  const rpx_mxfp4_part part = {v[0].p, v[1].l, v[2].l, v[3].l, v[4].p, v[5].p,
+                               0,      v[6].p, v[7].p, 0,      v[8].i};
+  return PyLong_FromLong(rpx_mxfp4_quantize(&part, 1, v[9].p));
+}
+
+static PyObject* fast_mxfp4_dequantize(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[7];
+  if (!parse("mxfp4_dequantize", "ppllpip", args, nargs, v)) return NULL;
+  return PyLong_FromLong(
+      rpx_mxfp4_dequantize(v[0].p, v[1].p, v[2].l, v[3].l, v[4].p, v[5].i, v[6].p));
 }
 
 static PyObject* fast_mxfp4_linear_forward(PyObject* self, PyObject* const* args,
@@ -303,6 +322,10 @@ static PyMethodDef methods[] = {
      "rpx_mxfp4_linear"},
     {"mxfp4_gated", (PyCFunction)(void (*)(void))fast_mxfp4_gated, METH_FASTCALL,
      "rpx_mxfp4_gated"},
+    {"mxfp4_quantize", (PyCFunction)(void (*)(void))fast_mxfp4_quantize, METH_FASTCALL,
+     "rpx_mxfp4_quantize of one matrix"},
+    {"mxfp4_dequantize", (PyCFunction)(void (*)(void))fast_mxfp4_dequantize, METH_FASTCALL,
+     "rpx_mxfp4_dequantize"},
     {"mxfp4_linear_forward", (PyCFunction)(void (*)(void))fast_mxfp4_linear_forward,
      METH_FASTCALL, "rpx_mxfp4_linear_forward"},
     {"mxfp4_linear_backward", (PyCFunction)(void (*)(void))fast_mxfp4_linear_backward,

@@ -129,8 +129,8 @@ class MXFP4Matrix:
         rows, columns = codes.shape[0], self.columns
         out = torch.empty((rows, columns), dtype=dtype, device=device)
         with _launches_on(device):
-            nat.call("rpx_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), rows, columns,
-                     out.data_ptr(), _dtype_code(dtype), _stream(device))
+            _call("dequantize", codes.data_ptr(), scales.data_ptr(), rows, columns,
+                  out.data_ptr(), _dtype_code(dtype), _stream(device))
         return out
 
     def __repr__(self) -> str:
@@ -173,20 +173,23 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-def _part(t, along: MXFP4Matrix | None, across: MXFP4Matrix | None):
-    """One matrix to encode, as the library takes it (``across``: its transpose)."""
+def _encode(t: torch.Tensor, along: MXFP4Matrix | None, across: MXFP4Matrix | None,
+            device: torch.device) -> None:
+    """``t`` (dense columns) encoded into ``along``, its transpose into ``across``."""
 
     rows, columns = t.shape
-    return nat.Mxfp4Part(t.data_ptr(), rows, columns, max(t.stride(0), columns),
-                         along.codes.data_ptr() if along else None,
-                         along.scales.data_ptr() if along else None, 0,
-                         across.codes.data_ptr() if across else None,
-                         across.scales.data_ptr() if across else None, 0, _dtype_code(t.dtype))
-
-
-def _encode(part, device: torch.device) -> None:
+    outs = []
+    for out in (along, across):
+        outs += (None, None) if out is None else (out.codes.data_ptr(), out.scales.data_ptr())
+    source = (t.data_ptr(), rows, columns, max(t.stride(0), columns))
     with _launches_on(device):
-        nat.call("rpx_mxfp4_quantize", ctypes.byref(part), 1, _stream(device))
+        stream = _stream(device)
+        fast = nat.fast()
+        if fast is not None:
+            nat.check(fast.mxfp4_quantize(*source, *outs, _dtype_code(t.dtype), stream))
+        else:
+            part = nat.Mxfp4Part(*source, *outs[:2], 0, *outs[2:], 0, _dtype_code(t.dtype))
+            nat.call("rpx_mxfp4_quantize", ctypes.byref(part), 1, stream)
 
 
 def mxfp4_quantize(t: torch.Tensor) -> MXFP4Matrix:
@@ -196,11 +199,11 @@ def mxfp4_quantize(t: torch.Tensor) -> MXFP4Matrix:
     if t.stride(0) == 1 and t.stride(1) > 1:  # a transpose: encode along its own rows
         base = _dense_rows(t.t())
         out = MXFP4Matrix.empty(*t.shape, device)
-        _encode(_part(base, None, out), device)
+        _encode(base, None, out, device)
         return out
     t = _dense_rows(t)
     out = MXFP4Matrix.empty(*t.shape, device)
-    _encode(_part(t, out, None), device)
+    _encode(t, out, None, device)
     return out
 
 
@@ -216,7 +219,7 @@ def mxfp4_quantize_both(t: torch.Tensor) -> tuple[MXFP4Matrix, MXFP4Matrix]:
     t = _dense_rows(t)
     along = MXFP4Matrix.empty(*t.shape, device)
     across = MXFP4Matrix.empty(t.shape[1], t.shape[0], device)
-    _encode(_part(t, along, across), device)
+    _encode(t, along, across, device)
     return along, across
 
 
@@ -339,10 +342,10 @@ class MXFP4LinearFn(torch.autograd.Function):
         ws = _workspace(_bytes(_FORWARD, m, n, k, False, False), device, stream)
         with _launches_on(device):
             _call("linear_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
-                     x.stride(0), w.data_ptr(), _dtype_code(w.dtype), n, *w.stride(),
-                     y.data_ptr(), _dtype_code(out_dtype), _ptr(saved),
-                     0 if saved is None else saved.numel(), need_left, need_right, ws.data_ptr(),
-                     ws.numel(), stream)
+                  x.stride(0), w.data_ptr(), _dtype_code(w.dtype), n, *w.stride(),
+                  y.data_ptr(), _dtype_code(out_dtype), _ptr(saved),
+                  0 if saved is None else saved.numel(), need_left, need_right, ws.data_ptr(),
+                  ws.numel(), stream)
         if saved is not None:
             ctx.save_for_backward(saved)
             ctx.cfg = (m, k, n, left.dtype, right.dtype, need_left, need_right)
@@ -362,9 +365,9 @@ class MXFP4LinearFn(torch.autograd.Function):
         ws = _workspace(_bytes(_BACKWARD, m, n, k, need_left, need_right), device, stream)
         with _launches_on(device):
             _call("linear_backward", g.data_ptr(), _dtype_code(g.dtype), m, n,
-                     g.stride(0), saved.data_ptr(), saved.numel(), k, saved_left, saved_right,
-                     _ptr(d_left), _dtype_code(left_dtype), _ptr(d_right),
-                     _dtype_code(right_dtype), ws.data_ptr(), ws.numel(), stream)
+                  g.stride(0), saved.data_ptr(), saved.numel(), k, saved_left, saved_right,
+                  _ptr(d_left), _dtype_code(left_dtype), _ptr(d_right),
+                  _dtype_code(right_dtype), ws.data_ptr(), ws.numel(), stream)
         return d_left, None if d_right is None else d_right.t(), None
 
 
@@ -397,11 +400,11 @@ class MXFP4GatedFn(torch.autograd.Function):
         ws = _workspace(_bytes(_FORWARD + 1, m, n, k, False, False), device, stream)
         with _launches_on(device):
             _call("gated_forward", x.data_ptr(), _dtype_code(x.dtype), m, k,
-                     x.stride(0), wg.data_ptr(), _dtype_code(wg.dtype), *wg.stride(),
-                     wu.data_ptr(), _dtype_code(wu.dtype), *wu.stride(), n, h.data_ptr(),
-                     _ptr(z_gate), _ptr(z_up), _dtype_code(out_dtype), _ptr(saved),
-                     0 if saved is None else saved.numel(), need_left, need_w, ws.data_ptr(),
-                     ws.numel(), stream)
+                  x.stride(0), wg.data_ptr(), _dtype_code(wg.dtype), *wg.stride(),
+                  wu.data_ptr(), _dtype_code(wu.dtype), *wu.stride(), n, h.data_ptr(),
+                  _ptr(z_gate), _ptr(z_up), _dtype_code(out_dtype), _ptr(saved),
+                  0 if saved is None else saved.numel(), need_left, need_w, ws.data_ptr(),
+                  ws.numel(), stream)
         if saved is not None:
             ctx.save_for_backward(z_gate, z_up, saved)
             ctx.cfg = (m, k, n, left.dtype, gate.dtype, up.dtype, need_left, need_w)
@@ -423,9 +426,9 @@ class MXFP4GatedFn(torch.autograd.Function):
         ws = _workspace(_bytes(_BACKWARD + 1, m, n, k, need_left, need_w), device, stream)
         with _launches_on(device):
             _call("gated_backward_products", dh.data_ptr(), z_gate.data_ptr(),
-                     z_up.data_ptr(), _dtype_code(dh.dtype), m, n, saved.data_ptr(),
-                     saved.numel(), k, saved_left, saved_w, _ptr(d_x), _dtype_code(left_dtype),
-                     _ptr(d_w), _dtype_code(wide), ws.data_ptr(), ws.numel(), stream)
+                  z_up.data_ptr(), _dtype_code(dh.dtype), m, n, saved.data_ptr(),
+                  saved.numel(), k, saved_left, saved_w, _ptr(d_x), _dtype_code(left_dtype),
+                  _ptr(d_w), _dtype_code(wide), ws.data_ptr(), ws.numel(), stream)
         return (d_x, _as(d_w[:n], gate_dtype).t() if need_g else None,
                 _as(d_w[n:], up_dtype).t() if need_u else None, None)
 

@@ -642,3 +642,31 @@ def test_refusals():
         rx.mxfp4_linear(x.cpu(), wq)
     with pytest.raises(ValueError, match="bias"):
         rx.MXFP4Linear(wq, torch.zeros(9, device=DEVICE))
+
+
+def test_both_bindings_give_the_same_bytes(monkeypatch):
+    """The CPython fast-call binding and the ctypes one reach the same kernels."""
+
+    g = rng(77)
+    m, k, n = 65, 300, 96
+    x = to_dev_bf16(_data(g, m, k)).requires_grad_()
+    w, u = (to_dev_bf16(_data(g, n, k, 0.1)).requires_grad_() for _ in range(2))
+    dy = to_dev_bf16(_data(g, m, n))
+
+    def everything():
+        out = []
+        with rx.precision_context(POLICY):
+            y, h = rx.linear_matmul(x, w.t()), rx.gated_matmul(x, w.t(), u.t())
+        out += [y, h, *torch.autograd.grad(y, (x, w), dy), *torch.autograd.grad(h, (x, w, u), dy)]
+        q, t = rx.mxfp4_quantize_both(x.detach())
+        a, b = rx.mxfp4_quantize(w.detach()), rx.mxfp4_quantize(u.detach())
+        out += [q.codes, q.scales, t.codes, t.scales, t.dequantize(), a.dequantize(F32)]
+        for rows in (1, 20, m):
+            out += [rx.mxfp4_linear(x.detach()[:rows], a), rx.mxfp4_gated(x.detach()[:rows], a, b)]
+        return out
+
+    assert nat.fast() is not None
+    fast = everything()
+    monkeypatch.setattr(nat, "fast", lambda: None)
+    for a, b in zip(fast, everything(), strict=True):
+        assert torch.equal(a, b)

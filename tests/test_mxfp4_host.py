@@ -173,3 +173,36 @@ def test_training_entries_refuse_before_any_launch():
     with pytest.raises(ValueError, match="null"):
         nat.call("rpx_mxfp4_gated_backward_products", None, P, P, BF16, 40, 48, P, big, 64, 1, 1, P,
                  BF16, P, BF16, P, big, None)
+
+
+@pytest.mark.parametrize("shape", [(1, 2048, 6144), (13, 6144, 2048), (65, 300, 777),
+                                   (768, 768, 16384), (1001, 500, 1300), (0, 64, 64), (64, 0, 64)])
+def test_fast_binding_sizes_and_validates_as_the_library_does(shape):
+    fast, lib = nat.fast(), nat.load()
+    assert fast is not None
+    for what, name in enumerate(rx.mxfp4._BYTES):
+        for left in (False, True):
+            for right in (False, True):
+                needs = (int(left), int(right)) if what in (2, 3, 6, 7) else ()
+                assert fast.mxfp4_bytes(what, *shape, left, right) == getattr(lib, name)(*shape, *needs)
+    with pytest.raises(ValueError):
+        fast.mxfp4_bytes(len(rx.mxfp4._BYTES), *shape, 1, 1)
+
+
+def test_fast_binding_refuses():
+    fast = nat.fast()
+    p = 16  # never dereferenced: validation fails first
+    with pytest.raises(ValueError, match="overlap"):
+        nat.check(fast.mxfp4_quantize(p, 4, 64, 32, p, p, None, None, nat.DTYPE_BF16, None))
+    with pytest.raises(ValueError, match="no output"):
+        nat.check(fast.mxfp4_quantize(p, 4, 64, 64, None, None, None, None, nat.DTYPE_BF16, None))
+    with pytest.raises(ValueError, match="aligned"):
+        nat.check(fast.mxfp4_quantize(p, 4, 64, 64, 8, p, None, None, nat.DTYPE_BF16, None))
+    with pytest.raises(ValueError, match="null"):
+        nat.check(fast.mxfp4_dequantize(None, p, 4, 64, p, nat.DTYPE_BF16, None))
+    with pytest.raises(ValueError, match="workspace"):
+        nat.check(fast.mxfp4_linear(p, nat.DTYPE_BF16, 65, 64, 64, p, p, 64, p, None, 0, None))
+    for name in ("quantize", "dequantize", "linear", "gated", "linear_forward", "linear_backward",
+                 "gated_forward", "gated_backward_products"):
+        with pytest.raises(TypeError):
+            getattr(fast, "mxfp4_" + name)(p)
