@@ -670,3 +670,72 @@ def test_both_bindings_give_the_same_bytes(monkeypatch):
     monkeypatch.setattr(nat, "fast", lambda: None)
     for a, b in zip(fast, everything(), strict=True):
         assert torch.equal(a, b)
+
+
+# launches of more tiles than the card holds at once: a workgroup goes from one to the next
+MANY = [(1, 4100, 4099), (2, 1500, 6001)]
+
+
+def _normal(seed, rows, columns, scale=1.0):
+    g = torch.Generator(device=DEVICE).manual_seed(seed)
+    return (torch.randn((rows, columns), generator=g, device=DEVICE) * scale).to(BF16)
+
+
+@pytest.mark.parametrize("k", [40, 256, 300, 700, 1100])
+@pytest.mark.parametrize("tile,m,n", MANY)
+def test_workgroups_of_many_tiles(tile, m, n, k):
+    """The bits of the small tile, whose workgroups take one each, and some rows against
+    the oracle: sums of one slice, two, and more; ragged edges."""
+
+    a, b = _normal(k, m, k), _normal(k + 1, n, k)
+    aq, bq = rx.mxfp4_quantize(a), rx.mxfp4_quantize(b)
+    rows = torch.tensor([0, 1, m // 2, m - 2, m - 1], device=DEVICE)
+    for out in (BF16, F32):
+        with ops.tuning(mx_tile=5):
+            want = rx.mxfp4_matmul(aq, bq, out)
+        with ops.tuning(mx_tile=tile):
+            got = rx.mxfp4_matmul(aq, bq, out)
+        assert torch.equal(got, want)
+        _check_product(got[rows], from_dev(a[rows]), from_dev(b), out)
+
+
+@pytest.mark.parametrize("k", [200, 512, 1000])
+@pytest.mark.parametrize("tile,m,n", [(1, 4100, 2051), (2, 1500, 3004)])
+def test_gated_workgroups_of_many_tiles(tile, m, n, k):
+    x, g, u = _normal(k, m, k).requires_grad_(), _normal(k + 1, n, k), _normal(k + 2, n, k)
+    for out in (BF16, F32):
+        got = []
+        for t in (5, tile):
+            with ops.tuning(mx_tile=t):
+                h = mxfp4.gated_product(x, g.t(), u.t(), out)
+                with torch.no_grad():
+                    got.append((h.detach(), *h.grad_fn.saved_tensors[:2],
+                                mxfp4.gated_product(x, g.t(), u.t(), out)))
+        assert all(torch.equal(a, b) for a, b in zip(*got, strict=True))
+
+
+@pytest.mark.parametrize("tile,m,k,n", [(1, 4000, 1300, 4200), (1, 5000, 3300, 200),
+                                        (2, 3000, 2100, 700), (2, 200, 5000, 3300)])
+def test_two_products_of_many_tiles(tile, m, k, n):
+    """Both products of a backward in one launch, sums of different lengths."""
+
+    x, w = _normal(m, m, k).requires_grad_(), _normal(n, n, k, 0.05).requires_grad_()
+    dy = _normal(k, m, n, 1e-3)
+    grads = []
+    for t, pair in ((5, 0), (tile, 0), (tile, -1)):
+        with ops.tuning(mx_tile=t, mx_pair=pair, mx_splits=1), rx.precision_context(POLICY):
+            grads.append(torch.autograd.grad(rx.linear_matmul(x, w.t()), (x, w), dy))
+    for other in grads[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(grads[0], other, strict=True))
+
+
+def test_split_sums_of_many_tiles():
+    a, b = _normal(1, 2500, 5200), _normal(2, 2500, 5200, 0.05)
+    aq, bq = rx.mxfp4_quantize(a), rx.mxfp4_quantize(b)
+    rows = torch.tensor([0, 1300, 2499], device=DEVICE)
+    with ops.tuning(mx_tile=1, mx_splits=5):
+        got = rx.mxfp4_matmul(aq, bq, F32)
+        with ops.tuning(mx_tile=5):
+            want = rx.mxfp4_matmul(aq, bq, F32)
+    assert torch.equal(got, want)
+    _check_product(got[rows], from_dev(a[rows]), from_dev(b), F32)
