@@ -112,12 +112,15 @@ int weight_part(const char* who, const void* right, int dtype, int64_t k, int64_
 }
 
 // Whether a serving call encodes x within its product's launch: up to 16 rows,
-// which every workgroup (16 rows of the weight) reads, 16 MB of such reads in all.
-// One launch against two, bf16 and float32 (graph replays, cold weights): 4 rows of
-// 2048 to 6144, 6 MB, 5.8 / 7.4 us; 16 rows of 2048 to 2048, 8 MB, 5.3 / 6.7; 13 of
-// 2048 to 6144, 20 MB, 7.4 / 7.4; 13 of 6144 to 2048, 20 MB, 9.2 / 8.4; 13 float32
-// rows of 2048 to 6144, 41 MB, 9.7 / 7.5.
-constexpr int64_t kMxSkinnyReads = int64_t{16} << 20;
+// which every workgroup (16 rows of the weight) reads, 24 MB of such reads in all.
+// One launch against two, us (cold weights, graph replays; then eager calls, of which
+// a launch is 4): bf16, 13 rows of 2048 to 2048, 6 MB, 4.7 / 6.3, 9.2 / 12.6; 13 of
+// 2048 to 6144, 20 MB, 7.0 / 7.3, 9.1 / 12.9; 13 of 6144 to 2048, 20 MB, 8.8 / 8.2, 9.0 /
+// 12.9; 16 of 6144 to 2048, 24 MB, 9.7 / 8.4, 9.4 / 14.3; float32, 8 rows of 2048 to
+// 6144, 24 MB, 8.1 / 7.1, 9.1 / 14.0; 16 of 1024 to 8192, 32 MB, 6.9 / 6.6, 9.1 / 14.0; 13
+// of 2048 to 6144, 39 MB, 9.3 / 7.3, 9.8 / 14.7; 16 of 6144 to 2048, 48 MB, 14.5 / 8.4, 14.5
+// / 14.3.
+constexpr int64_t kMxSkinnyReads = int64_t{24} << 20;
 bool encodes_on_the_way(int64_t m, int64_t n, int64_t k, int dtype) {
   return m <= kMxSkinnyRows &&
          m * k * static_cast<int64_t>(elem_size(dtype)) <= kMxSkinnyReads / ceil_div(n, 16);
