@@ -333,6 +333,16 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
 // so the bookkeeping is kept small: one exponential a pair, a maximum that takes two
 // new values an operation, no test for infinities and NaN but one of the whole tile
 // (the tile is then encoded again, with the tests).
+constexpr int kGatedWaves = 4;
+constexpr int kGatedThreads = 64 * kGatedWaves;
+
+// What a workgroup's waves have of 128 columns of both transposes: 64 bytes of a row of
+// codes, padded by 16 for the banks, and four of its scales.
+struct __align__(16) GatedAcross {
+  uint8_t codes[2][128][kGatedWaves * 16 + 16];
+  uint8_t scales[2][128][kGatedWaves];
+};
+
 template <int DTYPE, bool WHOLE, bool PAIRS>
 struct GatedTile {
   static constexpr int WORDS = DTYPE == kBF16 ? 1 : 2;
@@ -427,8 +437,8 @@ struct GatedTile {
     return seen;
   }
 
-  __device__ __forceinline__ void run(const MxOut& along, const MxOut& across, int64_t r0,
-                                      int64_t c, int64_t n, int lane) {
+  __device__ __forceinline__ void run(const MxOut& along, bool to_across, int64_t r0, int64_t c,
+                                      int lane, int wave, GatedAcross& staged) {
     uint32_t kept[2] = {0, 0};  // this lane's share of the scales of sixteen rows
     uint32_t seen = 0;
     const bool to_along = along.codes != nullptr && left > 0;
@@ -446,7 +456,7 @@ struct GatedTile {
       __builtin_amdgcn_sched_barrier(0);
     }
     if (to_along && __any(seen >= 0x7F800000u)) encode_along<32, true>(along, r0, c, lane, 0, kept);
-    if (across.codes == nullptr) return;
+    if (!to_across) return;
 #pragma unroll
     for (int z = 0; z < 2; ++z)
 #pragma unroll
@@ -460,34 +470,30 @@ struct GatedTile {
         u32x4_t code = {mx_encode8(v, scale), mx_encode8(v + 8, scale), mx_encode8(v + 16, scale),
                         mx_encode8(v + 24, scale)};
         if (byte == 255u) code = u32x4_t{0, 0, 0, 0};
-        if (WHOLE || c + e < n) {
-          const int64_t row = z * n + c + e;
-          *reinterpret_cast<u32x4_t*>(across.codes + row * across.row_bytes + r0 / 2) = code;
-          *mx_scale_at(across, row, r0 / kMxBlock) = static_cast<uint8_t>(byte);
-        }
+        *reinterpret_cast<u32x4_t*>(staged.codes[z][2 * lane + e] + 16 * wave) = code;
+        staged.scales[z][2 * lane + e][wave] = static_cast<uint8_t>(byte);
         __builtin_amdgcn_sched_barrier(0);
       }
   }
 };
-
-constexpr int kGatedWaves = 4;
-constexpr int kGatedThreads = 64 * kGatedWaves;
 
 template <int DTYPE, bool PAIRS>
 __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per_eu(2)))
     k_mx_gated_backward(const void* __restrict__ dh, const void* __restrict__ z_gate,
                         const void* __restrict__ z_up, int64_t m, int64_t n, int64_t per,
                         int64_t rows, MxOut along, MxOut across) {
-  // The waves of a workgroup take consecutive rows of the same columns, so that the
-  // 16 bytes that each writes to a row of the transpose's codes meet in one line of
-  // one L2 (with the waves side by side instead, a line was written from eight XCDs:
-  // 204 us for the transposes alone of 16384 x 6144, 174 so). The wave's index is
-  // made uniform so that rows are addressed from scalar registers.
+  // The waves of a workgroup take consecutive rows of the same columns, and what they
+  // have of the transposes meets in LDS, to be stored 64 bytes of a row of codes at a
+  // time: 189 us for 16384 x 6144, 205 with each wave's own stores of 16 bytes (160 and
+  // 175 for the transposes alone, 148 for the rows' alone). The wave's index is made uniform so that rows are addressed from scalar
+  // registers.
+  __shared__ GatedAcross staged;
   const int64_t group = block_of_grid();
-  const int64_t r0 = (group / per * kGatedWaves +
-                      __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6))) * 32;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t first_row = group / per * (kGatedWaves * 32);
+  const int64_t r0 = first_row + wave * 32;
   const int64_t tile = group % per;
-  if (r0 >= rows) return;
+  if (r0 >= rows) return;  // with transposes the whole workgroup: `rows` is padded to 256
   const int lane = threadIdx.x & 63;
   const int64_t c0 = tile * 128;
   const int64_t c = c0 + 2 * lane;
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
       t.in_column[0] = c < n ? ~0u : 0u;
       t.in_column[1] = c + 1 < n ? ~0u : 0u;
     }
-    t.run(along, across, r0, c, n, lane);
+    t.run(along, across.codes != nullptr, r0, c, lane, wave, staged);
   };
   if constexpr (PAIRS) {
     if (r0 + 32 <= m && c0 + 128 <= n)
@@ -521,8 +527,28 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
   } else {
     run(std::false_type{});
   }
+  if (across.codes == nullptr) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2 * 128 * 4 / kGatedThreads; ++i) {
+    const int row = (i * kGatedThreads + static_cast<int>(threadIdx.x)) / 4;  // of 2 x 128
+    const int piece = threadIdx.x % 4;
+    const int64_t column = c0 + row % 128;
+    if (column < n)
+      *reinterpret_cast<u32x4_t*>(across.codes + (row / 128 * n + column) * across.row_bytes +
+                                  first_row / 2 + 16 * piece) =
+          *reinterpret_cast<const u32x4_t*>(staged.codes[row / 128][row % 128] + 16 * piece);
+  }
+  {
+    const int row = threadIdx.x;
+    const int64_t column = c0 + row % 128;
+    if (column < n)
+      *reinterpret_cast<uint32_t*>(mx_scale_at(across, row / 128 * n + column,
+                                               first_row / kMxBlock)) =
+          *reinterpret_cast<const uint32_t*>(staged.scales[row / 128][row % 128]);
+  }
   // rows of scales past the last of the stack
-  if (across.codes != nullptr && tile == 0 && 2 * n + lane < across.scale_rows)
+  if (tile == 0 && 2 * n + lane < across.scale_rows)
     *mx_scale_at(across, 2 * n + lane, r0 / kMxBlock) = 0;
 }
 
