@@ -14,9 +14,9 @@ namespace {
 constexpr int kThreads = 256;
 // Waves of the fused form (32 KB read each) from which both encodings come from one
 // read; below, each from its own. Measured, fused against apart: 12.3 / 8.1 us at
-// 8192 x 768 bf16 (384 waves), 15.5 / 14.7 at 6144 x 2048 (768), 23.2 / 34.3 at
+// 8192 x 768 bf16 (384 waves), 13.4 / 14.7 at 6144 x 2048 (768), 23.0 / 34.3 at
 // 16384 x 2048 (2048); 11.5 / 12.2 at 5003 x 1000 float32 (640), 12.2 / 13.3 at
-// 8192 x 768 (768), 12.9 / 16.7 at 2048 x 4096 (1024).
+// 8192 x 768 (768), 12.4 / 16.7 at 2048 x 4096 (1024).
 constexpr int64_t kMxFusedWaves = 768;
 
 // Maximum over the LANES neighbouring lanes that share a block.
@@ -145,6 +145,19 @@ struct Column {
   }
 };
 
+// The work of block b of `total`: runs of `run` consecutive pieces go to one XCD (blocks
+// go round the eight), whose L2 then has whole lines of what they write; the rest at the
+// end as they come.
+__device__ __forceinline__ int64_t of_xcd(int64_t b, int64_t total, int64_t run) {
+  const int64_t round = 8 * run;
+  return b < total / round * round ? b / round * round + b % 8 * run + b % round / 8 : b;
+}
+
+// A pass over a large matrix by 64 blocks an XCD against one, us: bf16 40.0 / 44.2 for 16384
+// x 6144, 15.8 / 17.2 for 16384 x 2048, 7.2 / 7.1 for 6144 x 2048; float32 93 / 91, 26.4 /
+// 26.5, 11.7 / 11.8.
+constexpr int64_t kRowsRun = 64;
+
 // Along the columns only: a thread takes 16 bytes of a row, neighbouring lanes a
 // block. A pass over memory (serving: the input of a product).
 template <int DTYPE>
@@ -173,8 +186,10 @@ __device__ __forceinline__ void quantize_rows(const MxPart& part, int64_t i) {
 }
 
 __global__ void __launch_bounds__(kThreads) k_mx_quantize_rows(MxParts parts) {
-  const int64_t blk = block_of_grid();
-  if (blk >= parts.first[kMxParts]) return;
+  int64_t blk = block_of_grid();
+  const int64_t total = parts.first[kMxParts];
+  if (blk >= total) return;
+  blk = of_xcd(blk, total, kRowsRun);
   int p = 0;
   while (blk >= parts.first[p + 1]) ++p;
   const int64_t i = (blk - parts.first[p]) * kThreads + threadIdx.x;
@@ -182,6 +197,13 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_rows(MxParts parts) {
     quantize_rows<kBF16>(parts.part[p], i);
   else
     quantize_rows<kF32>(parts.part[p], i);
+}
+
+// Waves of `cols` columns that cover a part's.
+__host__ __device__ __forceinline__ int64_t mx_tiles_of_row(const MxPart& part, int cols) {
+  return ceil_div(part.along.codes != nullptr ? mx_slices(part.columns) * kMxSlice
+                                              : part.across.scale_rows,
+                  cols);
 }
 
 // Along both axes from one read. A thread owns 32 rows of its W words: whole
@@ -193,9 +215,7 @@ template <int DTYPE, int W>
 __device__ __forceinline__ void quantize_both(const MxPart& part, int64_t tile, int lane) {
   using P = Piece<DTYPE, W>;
   constexpr int COLS = 16 * P::COLS;
-  const int64_t per = ceil_div(part.along.codes != nullptr ? mx_slices(part.columns) * kMxSlice
-                                                           : part.across.scale_rows,
-                               COLS);
+  const int64_t per = mx_tiles_of_row(part, COLS);
   const int64_t r0 = (tile / per) * 128 + (lane >> 4) * 32;
   const int64_t c = (tile % per) * COLS + (lane & 15) * P::COLS;
   const Column<DTYPE, W> col(part, c);
@@ -281,9 +301,20 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_both(MxParts parts) {
   if (blk >= parts.first[kMxParts]) return;
   int p = 0;
   while (blk >= parts.first[p + 1]) ++p;
-  const int64_t wave = (blk - parts.first[p]) * (kThreads / 64) + (threadIdx.x >> 6);
-  if (wave >= parts.part[p].tiles) return;
-  quantize_both<DTYPE, 4>(parts.part[p], wave, threadIdx.x & 63);
+  // In a launch of a workgroup a CU, two rows of tiles, 256 rows of the matrix, run on one
+  // XCD, whose L2 then has whole lines of the transpose's codes: 13.4 / 15.4 us for 6144 x
+  // 2048 bf16, 13.3 / 14.3 for 2048 x 6144, 12.3 / 14.0 for 8192 x 1024 float32; longer
+  // launches lose by it: 23.9 / 22.9 for 16384 x 2048 bf16, 119 / 112 for 16384 x 6144
+  // float32.
+  const MxPart& part = parts.part[p];
+  int64_t block = blk - parts.first[p];
+  if (parts.first[kMxParts] <= 256) {
+    const int64_t run = mx_tiles_of_row(part, 16 * Piece<DTYPE, 4>::COLS) * 2 / (kThreads / 64);
+    block = of_xcd(block, parts.first[p + 1] - parts.first[p], run > 0 ? run : 1);
+  }
+  const int64_t wave = block * (kThreads / 64) + (threadIdx.x >> 6);
+  if (wave >= part.tiles) return;
+  quantize_both<DTYPE, 4>(part, wave, threadIdx.x & 63);
 }
 
 // The two encodings of a small matrix by different workgroups, each from its own
@@ -484,11 +515,13 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
                         int64_t rows, MxOut along, MxOut across) {
   // The waves of a workgroup take consecutive rows of the same columns, and what they
   // have of the transposes meets in LDS, to be stored 64 bytes of a row of codes at a
-  // time: 189 us for 16384 x 6144, 205 with each wave's own stores of 16 bytes (160 and
-  // 175 for the transposes alone, 148 for the rows' alone). The wave's index is made uniform so that rows are addressed from scalar
+  // time: 188 us for 16384 x 6144, 205 with each wave's own stores of 16 bytes (160 and
+  // 175 for the transposes alone). The wave's index is made uniform so that rows are addressed from scalar
   // registers.
   __shared__ GatedAcross staged;
-  const int64_t group = block_of_grid();
+  // The two groups of a slice of columns run on one XCD, whose L2 then has whole lines of
+  // their scales (178 us against 188).
+  const int64_t group = of_xcd(block_of_grid(), per * ceil_div(rows, 32 * kGatedWaves), 2);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int64_t first_row = group / per * (kGatedWaves * 32);
   const int64_t r0 = first_row + wave * 32;
@@ -614,9 +647,7 @@ hipError_t launch_mx_zero(void* out, int64_t bytes, hipStream_t stream) {
 hipError_t launch_mx_quantize(MxParts parts, int count, hipStream_t stream) {
   // waves of 128 rows of 16 pieces of `cols` columns
   auto tiles_of = [](const MxPart& part, int cols) {
-    const int64_t columns =
-        part.along.codes != nullptr ? mx_slices(part.columns) * kMxSlice : part.across.scale_rows;
-    return mx_slices(part.rows) * 2 * ceil_div(columns, 16 * cols);
+    return mx_slices(part.rows) * 2 * mx_tiles_of_row(part, 16 * cols);
   };
   int64_t waves = 0;
   for (int p = 0; p < count; ++p)
