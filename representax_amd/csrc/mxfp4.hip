@@ -516,8 +516,8 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
   // The waves of a workgroup take consecutive rows of the same columns, and what they
   // have of the transposes meets in LDS, to be stored 64 bytes of a row of codes at a
   // time: 188 us for 16384 x 6144, 205 with each wave's own stores of 16 bytes (160 and
-  // 175 for the transposes alone). The wave's index is made uniform so that rows are addressed from scalar
-  // registers.
+  // 175 for the transposes alone). The wave's index is made uniform so that rows are
+  // addressed from scalar registers.
   __shared__ GatedAcross staged;
   // The two groups of a slice of columns run on one XCD, whose L2 then has whole lines of
   // their scales (178 us against 188).
