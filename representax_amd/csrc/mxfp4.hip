@@ -159,7 +159,8 @@ __device__ __forceinline__ int64_t of_xcd(int64_t b, int64_t total, int64_t run)
 constexpr int64_t kRowsRun = 64;
 
 // Along the columns only: a thread takes 16 bytes of a row, neighbouring lanes a
-// block. A pass over memory (serving: the input of a product).
+// block. A pass over memory (serving: the input of a product): 50 us for 16384 x 6144 bf16
+// from HBM (5.1 TB/s).
 template <int DTYPE>
 __device__ __forceinline__ void quantize_rows(const MxPart& part, int64_t i) {
   using P = Piece<DTYPE, 4>;
@@ -210,7 +211,8 @@ __host__ __device__ __forceinline__ int64_t mx_tiles_of_row(const MxPart& part, 
 // blocks of the transpose, in registers, so nothing goes through LDS; a block
 // along the columns is shared by neighbouring lanes as above. A wave covers 128
 // rows of 16 pieces, so that its stores of the transpose are 64 contiguous bytes
-// of a row of codes.
+// of a row of codes. 23.0 us for 16384 x 2048 bf16 (4.5 TB/s); half the columns a thread,
+// twice the waves, 27.9.
 template <int DTYPE, int W>
 __device__ __forceinline__ void quantize_both(const MxPart& part, int64_t tile, int lane) {
   using P = Piece<DTYPE, W>;
@@ -585,7 +587,8 @@ __global__ void __launch_bounds__(kGatedThreads) __attribute__((amdgpu_waves_per
     *mx_scale_at(across, 2 * n + lane, r0 / kMxBlock) = 0;
 }
 
-// Eight columns of one row per thread.
+// Eight columns of one row per thread: a pass over memory, 6.6 us for 6144 x 2048 to bf16
+// (4.8 TB/s).
 template <int DTYPE>
 __global__ void __launch_bounds__(kThreads)
     k_mx_dequantize(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,

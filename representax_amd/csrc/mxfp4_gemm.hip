@@ -1,6 +1,12 @@
 // Products of MXFP4 matrices: out[i, j] = sum_c A[i, c] B[j, c], and the first
 // half of a gated feed-forward block, silu(A G^T) * (A U^T), from one pass over
 // A. mxfp4.h states the format and the order in which a slice's blocks meet.
+//
+// What bounds them: the fp4 MFMAs issue 7.3 PFLOP/s, which zeros nearly reach (8192 x 8192
+// <- 8192 6.3); on random codes the card's power holds that product at 4.5 (243 us), 16384
+// x 2048 <- 6144 at 4.3 (96 us). A tile of few slices adds what runs with no MFMA beside
+// it, the activation and the staging of its outputs: 3.5 for the gated block of 16384 x
+// 2048 -> 2 x 6144 (232 us), 3.2 with its projections kept (256 us, 604 MB of outputs).
 #include <atomic>
 #include <type_traits>
 
@@ -181,14 +187,18 @@ __device__ __forceinline__ void mx_store_tile(const MxJob& job,
       for (int fn = 0; fn < FO; ++fn)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          float h[4];
+          const f32x16_t& a = acc[fn][fm];
+          const f32x16_t& b = acc[FO + fn][fm];
+          uint32_t h[2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float zg = round_bf16(acc[fn][fm][4 * g + e]);
-            const float zu = round_bf16(acc[FO + fn][fm][4 * g + e]);
-            h[e] = act_apply<kActSiluMulFwd>(zu, zg, 0.0f, nullptr);
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t zg = pack_bf16x2(a[4 * g + 2 * e], a[4 * g + 2 * e + 1]);
+            const uint32_t zu = pack_bf16x2(b[4 * g + 2 * e], b[4 * g + 2 * e + 1]);
+            h[e] = pack_bf16x2(
+                act_apply<kActSiluMulFwd>(bf16lo_to_f32(zu), bf16lo_to_f32(zg), 0.0f, nullptr),
+                act_apply<kActSiluMulFwd>(bf16hi_to_f32(zu), bf16hi_to_f32(zg), 0.0f, nullptr));
           }
-          stage_block(fn, g, pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3]));
+          stage_block(fn, g, h[0], h[1]);
         }
       store_staged<32, COLS, false>(reg, static_cast<uint16_t*>(p.out), m, nw, p.m, p.n, lane);
       if (p.z_gate == nullptr) continue;
@@ -228,8 +238,8 @@ __device__ __forceinline__ void mx_store_tile(const MxJob& job,
 // a tile's last slice to the next tile's first, so that a tile begins with its first
 // slice in LDS and its first fragments in registers, while the outputs of the one before
 // are on their way; they are staged in the stage of its last slice, which is refilled
-// after that. Against a tile a workgroup: 226 / 242 us for the gated block of 16384 x
-// 2048 -> 2 x 6144 (twelve tiles a CU of eight slices), 260 / 285 with its projections
+// after that. Against a tile a workgroup: 232 / 243 us for the gated block of 16384 x
+// 2048 -> 2 x 6144 (twelve tiles a CU of eight slices), 256 / 278 with its projections
 // kept, 78 / 83 of 5003 rows; 219 / 246 for 16384 x 12288 <- 2048, 19.0 / 21.0 for 8192 x
 // 3072 <- 768, 245 / 251 for 8192 x 8192 <- 8192. Code that only these need costs the
 // others 1.5 us: 333 x 6144 <- 2048 9.4 / 7.9.

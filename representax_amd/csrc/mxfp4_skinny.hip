@@ -11,6 +11,10 @@
 // a block of x is encoded by the lane that needs it, with no exchange: 64 values
 // a slice, while the weight's loads are in flight. Every workgroup encodes x anew;
 // for a few tokens that is cheaper than a launch that would do it once.
+//
+// One row, weights from HBM, graph replays: 2048 -> 6144 4.8 us (6.7 MB, 1.4 TB/s: the
+// launch and two dependent trips to memory), two weights of it 5.9 (13.4 MB, 2.3 TB/s),
+// 6144 -> 2048 6.2. Sixteen rows 7.7, 8.3 and 9.7.
 #include <hip/hip_runtime.h>
 
 #include "act.h"
@@ -203,7 +207,8 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_skinny(MxSkinny p) {
 }
 
 // The same for rows of x that are encoded already, TILES x 16 of them a workgroup: a
-// lane reads its blocks' codes and scales as it reads the weight's.
+// lane reads its blocks' codes and scales as it reads the weight's. 32 rows of 2048 ->
+// 6144 with their encoding 8.8 us.
 template <int DTYPE, int TILES, bool GATED>
 __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
   constexpr int G = GATED ? 2 : 1;
