@@ -739,3 +739,48 @@ def test_split_sums_of_many_tiles():
             want = rx.mxfp4_matmul(aq, bq, F32)
     assert torch.equal(got, want)
     _check_product(got[rows], from_dev(a[rows]), from_dev(b), F32)
+
+
+def test_codes_beyond_32_bits():
+    """More than 2^32 bytes of codes, along a matrix's rows and in the rows of its
+    transpose: both encodings, a product over either axis, and the projections'
+    gradients give what the last rows alone give."""
+
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GB of device memory")
+    rows, columns, last = 1 << 22, 2304, 64
+    g = rng(15)
+    tail = _data(g, last, columns)
+    t = torch.zeros((rows, columns), dtype=BF16, device=DEVICE)
+    t[-last:] = to_dev_bf16(tail)
+    along, across = rx.mxfp4_quantize_both(t)
+    del t
+    assert along.codes.numel() > 1 << 32 and across.codes.numel() > 1 << 32
+    codes, scales = omx.stored(tail)
+    assert np.array_equal(along.codes[-last:].cpu().numpy(), codes)
+    assert np.array_equal(along.scales[:, -last:].cpu().numpy(), scales)
+    codes, scales = omx.stored(tail.T)
+    assert np.array_equal(across.codes[:, -last // 2:].cpu().numpy(), codes[:, :last // 2])
+    assert np.array_equal(across.scales[-1, :, -2:].cpu().numpy(), scales[0, :, :2])
+    assert not across.codes[:, :-last // 2].any() and not along.codes[:-last].any()
+    w = _data(g, 40, columns, 0.05)
+    y = rx.mxfp4_matmul(along, rx.mxfp4_quantize(to_dev_bf16(w)))
+    _check_product(y[-last:], tail, w, BF16)
+    assert not y[:-last].any()
+    dy = _normal(16, 40, rows, 1e-3)
+    got = rx.mxfp4_matmul(rx.mxfp4_quantize(dy), across, F32)
+    _check_product(got, from_dev(dy[:, -last:]), tail.T, F32)
+    del along, across, y, dy
+    rows = 1 << 20
+    parts = [_normal(17 + i, last, columns) for i in range(3)]
+    whole = []
+    for p in parts:
+        whole.append(torch.zeros((rows, columns), dtype=BF16, device=DEVICE))
+        whole[-1][-last:] = p
+    few, few_t, _ = _gated_backward(parts[0], parts[1:])
+    many, many_t, _ = _gated_backward(whole[0], whole[1:])
+    assert torch.equal(many.codes[-last:], few.codes)
+    assert torch.equal(many.scales[:, -last:], few.scales)
+    assert torch.equal(many_t.codes[:, -last // 2:], few_t.codes[:, :last // 2])
+    assert torch.equal(many_t.scales[-1, :, -2:], few_t.scales[0, :, :2])
+    assert not many.codes[:-last].any()
