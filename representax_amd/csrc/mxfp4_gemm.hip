@@ -357,14 +357,23 @@ __device__ __forceinline__ void mx_gemm_tiles(int first, int stride, int jobs,
   constexpr int RPM = NFR * 2 <= NMF ? 2 : NFR <= NMF ? 2 : NFR;
   u32x4_t fx[NFR], fy[NFR];       // fragments of two consecutive steps: A's, then B's
   uint32_t sc[NFR], sc_next[NFR];  // scale words of a slice
-  auto frag_row = [&](int j) {
-    return j < FM ? wm * TM + j * 32 + frow : BM + wn * TN + (j - FM) * 32 + frow;
-  };
+  // The wave's rows of A and of B are whole blocks of 32, over which the swizzle repeats:
+  // one offset of the lane a step, and the block's as the read's immediate.
+  uint32_t lane_at[4];
+#pragma unroll
+  for (int step = 0; step < 4; ++step)
+    lane_at[step] = frow * 128 + (((4 * half + step) ^ swz(frow)) << 4);
+  const int a_rows = wm * TM;
+  const int b_rows = BM + wn * TN;
   auto frag_one = [&](const uint8_t* st, int step, int j, u32x4_t* f) {
-    f[j] = lds_chunk(st, frag_row(j), 4 * half + step);
+    f[j] = *reinterpret_cast<const u32x4_t*>(st + (j < FM ? a_rows : b_rows) * 128 +
+                                             lane_at[step] + (j < FM ? j : j - FM) * (32 * 128));
   };
+  const uint32_t scale_at = SCALES + frow * kMxSliceBlocks + 4 * half;
   auto scale_one = [&](const uint8_t* st, int j, uint32_t* s) {
-    s[j] = *reinterpret_cast<const uint32_t*>(st + SCALES + frag_row(j) * kMxSliceBlocks + 4 * half);
+    s[j] = *reinterpret_cast<const uint32_t*>(st + (j < FM ? a_rows : b_rows) * kMxSliceBlocks +
+                                              scale_at +
+                                              (j < FM ? j : j - FM) * (32 * kMxSliceBlocks));
   };
 
   load_from(job_at(first));
