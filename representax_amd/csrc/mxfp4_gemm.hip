@@ -3,10 +3,11 @@
 // A. mxfp4.h states the format and the order in which a slice's blocks meet.
 //
 // What bounds them: the fp4 MFMAs issue 7.3 PFLOP/s, which zeros nearly reach (8192 x 8192
-// <- 8192 6.3); on random codes the card's power holds that product at 4.5 (243 us), 16384
-// x 2048 <- 6144 at 4.3 (96 us). A tile of few slices adds what runs with no MFMA beside
-// it, the activation and the staging of its outputs: 3.5 for the gated block of 16384 x
-// 2048 -> 2 x 6144 (232 us), 3.2 with its projections kept (256 us, 604 MB of outputs).
+// <- 8192 6.6, 166 us); on random codes the card's power holds that product at 4.7 (235
+// us), 16384 x 2048 <- 6144 at 4.4 (94 us), so an operation saved in the loop counts also
+// where it is hidden. A tile of few slices adds what runs with no MFMA beside it, the
+// activation and the staging of its outputs: 3.85 for the gated block of 16384 x 2048 -> 2 x
+// 6144 (214 us), 3.4 with its projections kept (244 us, 604 MB of outputs).
 #include <atomic>
 #include <type_traits>
 
@@ -25,8 +26,8 @@ namespace {
 // Writes a wave's sub-tile of ROWS x COLS bf16 values, staged in LDS with a row
 // pitch of 2 COLS + 16 bytes, as 16-byte pieces of whole row segments. m0, n0:
 // its first row and column in the output. PAST: past the L2, for what is not read
-// soon (the projections that a training step keeps: 278 -> 256 us for the gated block
-// of 16384 x 2048 -> 2 x 6144, 968 -> 940 for its step. Outputs that the next kernel
+// soon (the projections that a training step keeps: 267 -> 244 us for the gated block
+// of 16384 x 2048 -> 2 x 6144, 917 -> 872 for its step. Outputs that the next kernel
 // reads gain as much and lose it there: 16384 x 6144 <- 2048 and its encoding, 176 us
 // either way when the product took 138).
 template <int ROWS, int COLS, bool PAST>
@@ -238,11 +239,11 @@ __device__ __forceinline__ void mx_store_tile(const MxJob& job,
 // a tile's last slice to the next tile's first, so that a tile begins with its first
 // slice in LDS and its first fragments in registers, while the outputs of the one before
 // are on their way; they are staged in the stage of its last slice, which is refilled
-// after that. Against a tile a workgroup: 232 / 243 us for the gated block of 16384 x
-// 2048 -> 2 x 6144 (twelve tiles a CU of eight slices), 256 / 278 with its projections
-// kept, 78 / 83 of 5003 rows; 219 / 246 for 16384 x 12288 <- 2048, 19.0 / 21.0 for 8192 x
-// 3072 <- 768, 245 / 251 for 8192 x 8192 <- 8192. Code that only these need costs the
-// others 1.5 us: 333 x 6144 <- 2048 9.4 / 7.9.
+// after that. Against a tile a workgroup: 214 / 234 us for the gated block of 16384 x
+// 2048 -> 2 x 6144 (twelve tiles a CU of eight slices), 244 / 258 with its projections
+// kept, 73 / 79 of 5003 rows; 108 / 121 for 16384 x 6144 <- 2048, 18.9 / 20.9 for 8192 x
+// 3072 <- 768, 235 / 243 for 8192 x 8192 <- 8192. Code that only these need costs the
+// others 1.5 us: 333 x 6144 <- 2048 9.4 / 7.9 when it was theirs too.
 //
 // GATED: B's BN rows are, for each wave, half gate and half up projections of the
 // same output columns, so that both meet in the wave's registers.
@@ -358,7 +359,9 @@ __device__ __forceinline__ void mx_gemm_tiles(int first, int stride, int jobs,
   u32x4_t fx[NFR], fy[NFR];       // fragments of two consecutive steps: A's, then B's
   uint32_t sc[NFR], sc_next[NFR];  // scale words of a slice
   // The wave's rows of A and of B are whole blocks of 32, over which the swizzle repeats:
-  // one offset of the lane a step, and the block's as the read's immediate.
+  // one offset of the lane a step, and the block's as the read's immediate (27 VALU
+  // operations a slice for 32 MFMAs, 53 with an address a read: 235 / 240 us for 8192 x
+  // 8192 <- 8192, 215 / 226 for the gated block of 16384 x 2048 -> 2 x 6144).
   uint32_t lane_at[4];
 #pragma unroll
   for (int step = 0; step < 4; ++step)
@@ -617,16 +620,16 @@ Plan plan_for(int id, int64_t m, int64_t n, int64_t slices, bool gated) {
 // The tile: large where it fills the card, for fewer reads from LDS and the L2 a
 // product; smaller where that leaves CUs idle. Measured (us, bf16 outputs,
 // M x N <- K; tiles by id):
-//   16384 x 2048 <- 6144   1: 96, 2: 115, 4: 160     8192 x 8192 <- 8192   1: 243, 2: 298
-//   8192 x 3072 <- 768     1: 21.3, 2: 20.2      gated 16384 x 3072 <- 768   1: 63, 2: 73
-//   8192 x 768 <- 3072     1: 21.6, 2: 17.4, 4: 20.7
-//   333 x 6144 <- 2048     2: 7.8, 4: 8.1, 5: 7.8
-//   1024 x 2048 <- 2048    2: 7.8, 4: 6.8, 5: 7.1
-//   3072 x 768 <- 8192     2: 24.9, 3: 18.9, 4: 23.0 (144 tiles of 2 and 3: one a CU,
+//   16384 x 2048 <- 6144   1: 94, 2: 114, 4: 158     8192 x 8192 <- 8192   1: 235, 2: 297
+//   8192 x 3072 <- 768     1: 20.0, 2: 19.0      gated 16384 x 3072 <- 768   1: 59, 2: 71
+//   8192 x 768 <- 3072     1: 20.6, 2: 16.1, 4: 20.1
+//   333 x 6144 <- 2048     2: 7.5, 4: 8.0, 5: 7.7
+//   1024 x 2048 <- 2048    2: 7.5, 4: 6.7, 5: 7.0
+//   3072 x 768 <- 8192     2: 23.9, 3: 17.2, 4: 22.3 (144 tiles of 2 and 3: one a CU,
 //                          where 3's four stages take the place of a second workgroup)
-//   3500 x 768 <- 3072     2: 10.3, 3: 10.3
+//   3500 x 768 <- 3072     2: 9.7, 3: 9.8
 // A product of few tiles over a long sum is split; the partial tiles and their sum
-// cost 7 to 10 us (768 x 768 <- 8192, tile 5: 13.3 us whole, 14.6 in two, 14.9 in four).
+// cost 7 to 10 us (768 x 768 <- 8192, tile 5: 13.0 us whole, 13.8 in two, 14.9 in four).
 template <class TilesOf>
 int tile_for(TilesOf tiles_of, int64_t slices) {
   if (tune(kTuneMxTile) != 0) return tune(kTuneMxTile);
@@ -765,9 +768,9 @@ hipError_t launch_mx_gemm(const MxGemm& g, float* partials, hipStream_t stream) 
 // A backward's two products in one launch, in the tile that suits them together,
 // the longer sums first: a product's last round of tiles leaves CUs idle, which the
 // other's then fill, and there is one launch. A whole step in graph replays, one
-// launch against two: the linear of 1001 x 500 -> 1300 29.9 / 35.2 us, of 3500 x 3072
-// -> 768 61 / 69, of 5003 x 2048 -> 6144 171 / 182, its gated block 331 / 376; of
-// 16384 x 2048 -> 2048 233 / 234.
+// launch against two: the linear of 1001 x 500 -> 1300 29.7 / 34.8 us, of 3500 x 3072
+// -> 768 59.7 / 67.6, of 5003 x 2048 -> 6144 162 / 173, its gated block 315 / 354; of
+// 16384 x 2048 -> 2048 220 / 220.
 // A product that is split runs on its own, so that an output has the same bits
 // whether or not the other one is wanted.
 hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials,
