@@ -14,7 +14,8 @@ blocks are composed from the separate projections.
 
 ``swiglu_mlp`` over native ``Linear`` projections under the MXFP4 policy, or over
 kept ``MXFP4Linear`` weights, runs both input projections, the activation and the
-product in one kernel (``gated_matmul``, ``mxfp4_gated``).
+product in one kernel (``gated_matmul``, ``mxfp4_gated``). Subclasses of either,
+modules with a replaced ``forward`` and modules with hooks are called instead.
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ from . import ops
 from .adapters import QuantizedLoRALinear
 from .components import Linear, MXFP4Linear
 from .mxfp4 import mxfp4_gated
+from .norms import _unhooked
 from .precision import (activation_inputs, active_compute_dtype, active_policy,
                         compute_operands, compute_parameter, compute_parameter_dtype, gated_matmul)
 
@@ -66,11 +68,12 @@ def gelu_mlp(value: torch.Tensor, up: torch.nn.Module, down: torch.nn.Module) ->
 
 def _gated(value: torch.Tensor, gate: torch.nn.Module, up: torch.nn.Module):
     """``silu(gate(value)) * up(value)`` in one kernel where gate and up are MXFP4
-    projections without biases; None otherwise."""
+    projections without biases; None otherwise, and where calling them is more than
+    their class's forward (a subclass, a replaced forward, hooks)."""
 
-    kept = isinstance(gate, MXFP4Linear) and isinstance(up, MXFP4Linear)
-    native = (isinstance(gate, Linear) and isinstance(up, Linear) and gate.weight.ndim == 2
-              and up.weight.ndim == 2)
+    kept = _unhooked(gate, MXFP4Linear) and _unhooked(up, MXFP4Linear)
+    native = not kept and (_unhooked(gate, Linear) and _unhooked(up, Linear)
+                           and gate.weight.ndim == 2 and up.weight.ndim == 2)
     if not (kept or native) or gate.bias is not None or up.bias is not None:
         return None
     if kept:
