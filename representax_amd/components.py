@@ -96,11 +96,7 @@ class MXFP4Linear(torch.nn.Module):
     def inputs(self, value: torch.Tensor) -> torch.Tensor:
         """``value`` as rows in the activation dtype."""
 
-        value = activation_inputs(value)
-        if torch.is_grad_enabled() and value.requires_grad:
-            raise RuntimeError("MXFP4Linear gives no gradients (its weight is kept for "
-                               "inference); train a Linear under PrecisionConfig.mxfp4_mixed()")
-        return value.reshape(-1, self.input_size)
+        return activation_inputs(value).reshape(-1, self.input_size)
 
     def forward(self, value: torch.Tensor) -> torch.Tensor:
         y = mxfp4_linear(self.inputs(value), self.weight)

@@ -251,6 +251,9 @@ def _serve(x2d: torch.Tensor, weight: MXFP4Matrix, up: MXFP4Matrix | None) -> to
     most of a single token's call: each torch attribute is read once.)"""
 
     _matrix_input(x2d, "x")
+    if x2d.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("a product over kept MXFP4 weights gives no gradients; train a Linear "
+                           "under PrecisionConfig.mxfp4_mixed(), or detach x")
     m, k = x2d.shape
     codes, scales = weight.codes, weight.scales
     n = codes.shape[0]
@@ -281,14 +284,15 @@ def _serve(x2d: torch.Tensor, weight: MXFP4Matrix, up: MXFP4Matrix | None) -> to
 
 def mxfp4_linear(x2d: torch.Tensor, weight: MXFP4Matrix) -> torch.Tensor:
     """``x [M, K] W^T`` in x's dtype, ``weight`` the encoded ``W [N, K]``; x is encoded
-    within the call. Inference: no gradients."""
+    within the call. Inference: an x that requires a gradient is refused."""
 
     return _serve(x2d, weight, None)
 
 
 def mxfp4_gated(x2d: torch.Tensor, gate: MXFP4Matrix, up: MXFP4Matrix) -> torch.Tensor:
     """``silu(x G^T) * (x U^T)`` in x's dtype over two kept weights, in one pass over x;
-    both products are rounded to x's dtype before the activation. Inference."""
+    both products are rounded to x's dtype before the activation. Inference: an x that
+    requires a gradient is refused."""
 
     return _serve(x2d, gate, up)
 

@@ -1,5 +1,5 @@
 """MXFP4 modules on the host: which projections ``swiglu_mlp`` calls and which it runs
-in one kernel (CPU only, nothing launched)."""
+in one kernel, and which calls refuse gradients (CPU only, nothing launched)."""
 
 from __future__ import annotations
 
@@ -86,3 +86,23 @@ def test_projections_without_hooks_stay_in_one_kernel(monkeypatch):
     for pair in (_linears(rx.Linear, (6, 8), (6, 8)), [_kept(6, 8), _kept(6, 8)]):
         with rx.precision_context(POLICY), pytest.raises(RuntimeError, match="ROCm"):
             rx.swiglu_mlp(x, *pair, torch.nn.Identity())
+
+
+def test_kept_weights_refuse_a_gradient():
+    """Their results would be cut off from the graph without a word."""
+
+    x = torch.randn(5, 8).to(torch.bfloat16).requires_grad_()
+    module = _kept(6, 8)
+    calls = [lambda v: rx.mxfp4_linear(v, module.weight),
+             lambda v: rx.mxfp4_gated(v, module.weight, module.weight), module,
+             lambda v: rx.swiglu_mlp(v, module, module, torch.nn.Identity())]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(x)
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(x * 2)  # no leaf
+        # no gradient is wanted: refused only for the device
+        with pytest.raises(RuntimeError, match="ROCm"):
+            call(x.detach())
+        with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm"):
+            call(x)
