@@ -252,11 +252,17 @@ class DeviceError(NativeError):
     """A kernel reported a problem through the device error word."""
 
 
-_LIB: ctypes.CDLL | None = None
+_LIB: ctypes.PyDLL | None = None
+# These wait for the device, so other threads run meanwhile; they use no shared scratch.
+_WAITING = ("rpx_check_device_errors",)
 
 
-def load() -> ctypes.CDLL:
-    """Load the library, or raise: there is no fallback implementation."""
+def load() -> ctypes.PyDLL:
+    """Load the library, or raise: there is no fallback implementation.
+
+    Its functions hold the interpreter's lock (as the fast-call binding's do): a call
+    may enqueue several kernels over its stream's cached scratch, and no other thread's
+    call may enqueue between them. None of them waits, but for ``_WAITING``."""
 
     global _LIB
     if _LIB is not None:
@@ -267,11 +273,12 @@ def load() -> ctypes.CDLL:
             f"{path} is missing; build it with `python -m representax_amd.build` "
             "(the quantized-linear path has no non-HIP implementation)"
         )
-    lib = ctypes.CDLL(str(path))
+    lib, released = ctypes.PyDLL(str(path)), ctypes.CDLL(str(path))  # one loaded library
     for name, (restype, argtypes) in SIGNATURES.items():
-        fn = getattr(lib, name)
+        fn = getattr(released if name in _WAITING else lib, name)
         fn.restype = restype
         fn.argtypes = argtypes
+        setattr(lib, name, fn)
     _LIB = lib
     return lib
 
