@@ -193,15 +193,19 @@ typedef union {
   int i;
 } Value;
 
-/* Arguments by a format: p pointer, l int64, i int. */
+/* Arguments by a format: p pointer, l int64, s size (not negative), i int. */
 static int parse(const char* name, const char* format, PyObject* const* args, Py_ssize_t nargs,
                  Value* v) {
   if (!check_nargs(name, nargs, (Py_ssize_t)strlen(format))) return 0;
   for (Py_ssize_t j = 0; j < nargs; ++j) {
     const int ok = format[j] == 'p'   ? get_ptr(args[j], &v[j].p)
-                   : format[j] == 'l' ? get_i64(args[j], &v[j].l)
-                                      : get_int(args[j], &v[j].i);
+                   : format[j] == 'i' ? get_int(args[j], &v[j].i)
+                                      : get_i64(args[j], &v[j].l);
     if (!ok) return 0;
+    if (format[j] == 's' && v[j].l < 0) {
+      PyErr_Format(PyExc_ValueError, "%s: buffer sizes must be non-negative", name);
+      return 0;
+    }
   }
   return 1;
 }
@@ -210,7 +214,7 @@ static int parse(const char* name, const char* format, PyObject* const* args, Py
 static PyObject* fast_mxfp4_linear(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   Value v[12];
-  if (!parse("mxfp4_linear", "pilllpplpplp", args, nargs, v)) return NULL;
+  if (!parse("mxfp4_linear", "pilllpplppsp", args, nargs, v)) return NULL;
   return PyLong_FromLong(rpx_mxfp4_linear(v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].p,
                                           v[7].l, v[8].p, v[9].p, (size_t)v[10].l, v[11].p));
 }
@@ -218,7 +222,7 @@ static PyObject* fast_mxfp4_linear(PyObject* self, PyObject* const* args, Py_ssi
 static PyObject* fast_mxfp4_gated(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   Value v[14];
-  if (!parse("mxfp4_gated", "pilllpppplpplp", args, nargs, v)) return NULL;
+  if (!parse("mxfp4_gated", "pilllpppplppsp", args, nargs, v)) return NULL;
   return PyLong_FromLong(rpx_mxfp4_gated(v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].p,
                                          v[7].p, v[8].p, v[9].l, v[10].p, v[11].p,
                                          (size_t)v[12].l, v[13].p));
@@ -247,7 +251,7 @@ static PyObject* fast_mxfp4_linear_forward(PyObject* self, PyObject* const* args
                                            Py_ssize_t nargs) {
   (void)self;
   Value v[19];
-  if (!parse("mxfp4_linear_forward", "pilllpilllpipliiplp", args, nargs, v)) return NULL;
+  if (!parse("mxfp4_linear_forward", "pilllpilllpipsiipsp", args, nargs, v)) return NULL;
   return PyLong_FromLong(rpx_mxfp4_linear_forward(
       v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].i, v[7].l, v[8].l, v[9].l, v[10].p,
       v[11].i, v[12].p, (size_t)v[13].l, v[14].i, v[15].i, v[16].p, (size_t)v[17].l, v[18].p));
@@ -257,7 +261,7 @@ static PyObject* fast_mxfp4_linear_backward(PyObject* self, PyObject* const* arg
                                             Py_ssize_t nargs) {
   (void)self;
   Value v[17];
-  if (!parse("mxfp4_linear_backward", "pilllplliipipiplp", args, nargs, v)) return NULL;
+  if (!parse("mxfp4_linear_backward", "pilllpsliipipipsp", args, nargs, v)) return NULL;
   return PyLong_FromLong(rpx_mxfp4_linear_backward(
       v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, (size_t)v[6].l, v[7].l, v[8].i, v[9].i,
       v[10].p, v[11].i, v[12].p, v[13].i, v[14].p, (size_t)v[15].l, v[16].p));
@@ -267,7 +271,7 @@ static PyObject* fast_mxfp4_gated_forward(PyObject* self, PyObject* const* args,
                                           Py_ssize_t nargs) {
   (void)self;
   Value v[25];
-  if (!parse("mxfp4_gated_forward", "pilllpillpilllpppipliiplp", args, nargs, v)) return NULL;
+  if (!parse("mxfp4_gated_forward", "pilllpillpilllpppipsiipsp", args, nargs, v)) return NULL;
   return PyLong_FromLong(rpx_mxfp4_gated_forward(
       v[0].p, v[1].i, v[2].l, v[3].l, v[4].l, v[5].p, v[6].i, v[7].l, v[8].l, v[9].p, v[10].i,
       v[11].l, v[12].l, v[13].l, v[14].p, v[15].p, v[16].p, v[17].i, v[18].p, (size_t)v[19].l,
@@ -278,7 +282,7 @@ static PyObject* fast_mxfp4_gated_backward(PyObject* self, PyObject* const* args
                                            Py_ssize_t nargs) {
   (void)self;
   Value v[18];
-  if (!parse("mxfp4_gated_backward_products", "pppillplliipipiplp", args, nargs, v)) return NULL;
+  if (!parse("mxfp4_gated_backward_products", "pppillpsliipipipsp", args, nargs, v)) return NULL;
   return PyLong_FromLong(rpx_mxfp4_gated_backward_products(
       v[0].p, v[1].p, v[2].p, v[3].i, v[4].l, v[5].l, v[6].p, (size_t)v[7].l, v[8].l, v[9].i,
       v[10].i, v[11].p, v[12].i, v[13].p, v[14].i, v[15].p, (size_t)v[16].l, v[17].p));
