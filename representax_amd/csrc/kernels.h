@@ -372,10 +372,10 @@ hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials
                                hipStream_t stream);
 
 // The same for few rows over kept weights (codes2: the up projection's, or null):
-// from x itself, m <= 16 rows of k columns of `dtype`, or (x_scales given) from its
-// codes (any m; meant for kMxThinRows).
+// from x itself, up to kMxSkinnyRows rows of k columns of `dtype`, or (x_scales given)
+// from its codes, up to kMxThinRows.
 constexpr int64_t kMxSkinnyRows = 16;
-constexpr int64_t kMxThinRows = 64;
+constexpr int64_t kMxThinRows = 64;  // 16 a tile, up to four tiles
 struct MxSkinny {
   const void* x;
   const uint8_t* x_scales;

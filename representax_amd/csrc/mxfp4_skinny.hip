@@ -206,9 +206,9 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_skinny(MxSkinny p) {
   store_rows<DTYPE, GATED>(p, token, n0 + 4 * q, sum);
 }
 
-// The same for rows of x that are encoded already, TILES x 16 of them a workgroup: a
-// lane reads its blocks' codes and scales as it reads the weight's. 32 rows of 2048 ->
-// 6144 with their encoding 8.8 us.
+// The same for up to TILES x 16 rows of x that are encoded already: a lane reads its
+// blocks' codes and scales as it reads the weight's. 32 rows of 2048 -> 6144 with their
+// encoding 8.8 us.
 template <int DTYPE, int TILES, bool GATED>
 __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
   constexpr int G = GATED ? 2 : 1;
@@ -217,18 +217,15 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int waves = blockDim.x >> 6;
   const int q = lane >> 4;
-  // workgroups of one group of rows of x after those of another
-  const int64_t per = ceil_div(p.n, kTokens);
-  const int64_t n0 = block_of_grid() % per * kTokens;
-  const int64_t m0 = block_of_grid() / per * (TILES * kTokens);
-  if (m0 >= p.m) return;  // the whole workgroup
+  const int64_t n0 = block_of_grid() * kTokens;
+  if (n0 >= p.n) return;  // the whole workgroup
   const int64_t r = n0 + (lane & 15) < p.n ? n0 + (lane & 15) : p.n - 1;
   const int64_t pad = mx_pad_rows(p.n);
   const int64_t x_pad = mx_pad_rows(p.m);
   int64_t token[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
-    token[t] = m0 + t * kTokens + (lane & 15);
+    token[t] = t * kTokens + (lane & 15);
     token[t] = token[t] < p.m ? token[t] : p.m - 1;
   }
   f32x4_t acc[TILES][G];
@@ -282,8 +279,8 @@ __global__ void __launch_bounds__(64 * kMaxWaves) k_mx_thin(MxSkinny p) {
       for (int g = 0; g < G; ++g)
         sum[g] += *reinterpret_cast<const f32x4_t*>(
             partial + (((v * TILES + t) * G + g) * 64 + lane) * 4);
-    if (m0 + t * kTokens + (lane & 15) < p.m)
-      store_rows<DTYPE, GATED>(p, m0 + t * kTokens + (lane & 15), n0 + 4 * q, sum);
+    if (t * kTokens + (lane & 15) < p.m)
+      store_rows<DTYPE, GATED>(p, t * kTokens + (lane & 15), n0 + 4 * q, sum);
   }
 }
 
@@ -304,8 +301,7 @@ hipError_t launch_thin(const MxSkinny& p, hipStream_t stream) {
   constexpr int kWaves = 64 / (TILES * G) < kMaxWaves ? 64 / (TILES * G) : kMaxWaves;
   const int waves = static_cast<int>(p.slices < kWaves ? p.slices : kWaves);
   const size_t lds = static_cast<size_t>(waves) * TILES * G * 64 * 4 * sizeof(float);
-  const int64_t groups = ceil_div(p.m, TILES * kTokens);
-  hipLaunchKernelGGL((k_mx_thin<DTYPE, TILES, GATED>), grid_of(groups * ceil_div(p.n, kTokens)),
+  hipLaunchKernelGGL((k_mx_thin<DTYPE, TILES, GATED>), grid_of(ceil_div(p.n, kTokens)),
                      dim3(64 * waves), lds, stream, p);
   return hipGetLastError();
 }
@@ -316,8 +312,9 @@ hipError_t launch_thin_tiles(const MxSkinny& p, hipStream_t stream) {
     case 1: return launch_thin<DTYPE, 1, GATED>(p, stream);
     case 2: return launch_thin<DTYPE, 2, GATED>(p, stream);
     case 3: return launch_thin<DTYPE, 3, GATED>(p, stream);
-    default: return launch_thin<DTYPE, 4, GATED>(p, stream);
+    case 4: return launch_thin<DTYPE, 4, GATED>(p, stream);
   }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
@@ -325,6 +322,7 @@ hipError_t launch_thin_tiles(const MxSkinny& p, hipStream_t stream) {
 // A wave takes one slice while there are waves for it. Beyond, two of bf16's fit
 // its registers where there is one weight.
 hipError_t launch_mx_skinny(const MxSkinny& p, int dtype, hipStream_t stream) {
+  if (p.m > (p.x_scales != nullptr ? kMxThinRows : kMxSkinnyRows)) return hipErrorInvalidValue;
   const bool gated = p.codes2 != nullptr;
   if (p.x_scales != nullptr) {
     if (dtype == kBF16)
