@@ -666,6 +666,7 @@ constexpr int lds_bytes(int bm, int bn, int stages) {
   return stages * ((bm + bn) * static_cast<int>(kMxSliceBytes) + (bm + bn + 127) / 128 * 1024);
 }
 
+constexpr int64_t kCus = 256;
 constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1024;  // of an operand
 constexpr int64_t kMaxJobs = int64_t{1} << 30;
 
@@ -674,7 +675,7 @@ constexpr int64_t kMaxJobs = int64_t{1} << 30;
 // small ones, which tile_for takes for products of few tiles.
 constexpr int64_t resident(int bm, int bn, int stages) {
   return stages == 2 && bm * bn >= 128 * 128
-             ? int64_t{256} * (160 * 1024 / lds_bytes(bm, bn, stages))
+             ? kCus * (160 * 1024 / lds_bytes(bm, bn, stages))
              : kMaxJobs;
 }
 
@@ -773,16 +774,26 @@ hipError_t launch_mx_gemm(const MxGemm& g, float* partials, hipStream_t stream) 
 // 16384 x 2048 -> 2048 220 / 220.
 // A product that is split runs on its own, so that an output has the same bits
 // whether or not the other one is wanted.
+// The 256 x 256 tile is for launches whose longest tile ends with the others: one of few
+// tiles over a long sum runs on by itself, where a launch of its own takes a smaller tile.
+// Slices of the longest sum beyond an even share of all, and a backward with its encoding
+// in graph replays, one launch / two, us (m x k -> n): none, 5003 x 2048 -> 6144 91 / 101,
+// 16384 x 2048 -> 6144 269 / 276; 8, 4096 x 2048 -> 2048 38.0 / 40.5; 12, 6144 x 2048 ->
+// 2048 54.3 / 51.9; 16, 8192 x 2048 -> 2048 64 / 60; 46, 16384 x 768 -> 3072 118 / 89; 64,
+// 32768 x 2048 -> 2048 276 / 204. The 128 x 128 tile has two workgroups a CU: 28, 16384 x
+// 3072 -> 768 73 / 77; 35, 20480 x 3072 -> 768 88 / 92.
+constexpr int64_t kMxPairExcess = 10;
 hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials,
                                hipStream_t stream) {
   const bool alone = a.m == 0 || a.n == 0 || b.m == 0 || b.n == 0 || tune(kTuneMxPair) == 0 ||
                      choose(a.m, a.n, a.slices, false).splits > 1 ||
                      choose(b.m, b.n, b.slices, false).splits > 1 ||
                      a.m > kMaxRows || a.n > kMaxRows || b.m > kMaxRows || b.n > kMaxRows;
-  if (alone) {
-    if (hipError_t e = launch_mx_gemm(a, partials, stream); e != hipSuccess) return e;
-    return launch_mx_gemm(b, partials, stream);
-  }
+  auto apart = [&] {
+    const hipError_t e = launch_mx_gemm(a, partials, stream);
+    return e != hipSuccess ? e : launch_mx_gemm(b, partials, stream);
+  };
+  if (alone) return apart();
   const MxGemm& p = a.slices >= b.slices ? a : b;
   const MxGemm& q = a.slices >= b.slices ? b : a;
   const int64_t slices = q.slices;
@@ -794,6 +805,9 @@ hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials
   const int id = tile_for(tiles_of, slices);
   const Plan pp = plan_for(id, p.m, p.n, p.slices, false);
   const Plan qp = plan_for(id, q.m, q.n, q.slices, false);
+  const int64_t share =
+      ceil_div(pp.tiles_m * pp.tiles_n * p.slices + qp.tiles_m * qp.tiles_n * q.slices, kCus);
+  if (id == 1 && tune(kTuneMxTile) == 0 && p.slices - share > kMxPairExcess) return apart();
   switch (id) {
 #define X(ID, BM, BN, WM, WN, NS, WPE) \
   case ID:                             \

@@ -1,0 +1,32 @@
+"""Which launches an MXFP4 backward is made of (GPU)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import representax_amd as rx
+from representax_amd import ops
+from tests.helpers import DEVICE, kernel_names
+
+pytestmark = pytest.mark.gpu
+
+POLICY = rx.resolve_precision_policy(rx.PrecisionConfig.mxfp4_mixed())
+
+
+# (11776, 768, 3072): the smaller tile, two workgroups a CU
+@pytest.mark.parametrize("m,k,n,joint", [(5003, 2048, 6144, True), (4096, 2048, 2048, True),
+                                         (11776, 768, 3072, True), (8192, 2048, 2048, False),
+                                         (11008, 2048, 2048, False), (10240, 1024, 4096, False)])
+def test_products_share_a_launch_where_the_longest_tile_ends_with_the_others(m, k, n, joint):
+    g = torch.Generator(device=DEVICE).manual_seed(m + k)
+    x, w, dy = (torch.randn(s, generator=g, device=DEVICE).to(torch.bfloat16)
+                for s in ((m, k), (n, k), (m, n)))
+    x.requires_grad_(), w.requires_grad_()
+    with rx.precision_context(POLICY):
+        y = rx.linear_matmul(x, w.t())
+    grads, names = kernel_names(lambda: torch.autograd.grad(y, (x, w), dy, retain_graph=True))
+    assert any("k_mx_gemm_pair" in name for name in names) == joint, names
+    with ops.tuning(mx_pair=0):
+        apart = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(a, b) for a, b in zip(grads, apart))
