@@ -778,11 +778,11 @@ hipError_t launch_mx_gemm(const MxGemm& g, float* partials, hipStream_t stream) 
 // tiles over a long sum runs on by itself, where a launch of its own takes a smaller tile.
 // Slices of the longest sum beyond an even share of all, and a backward with its encoding
 // in graph replays, one launch / two, us (m x k -> n): none, 5003 x 2048 -> 6144 91 / 101,
-// 16384 x 2048 -> 6144 269 / 276; 8, 4096 x 2048 -> 2048 38.0 / 40.5; 12, 6144 x 2048 ->
-// 2048 54.3 / 51.9; 16, 8192 x 2048 -> 2048 64 / 60; 46, 16384 x 768 -> 3072 118 / 89; 64,
-// 32768 x 2048 -> 2048 276 / 204. The 128 x 128 tile has two workgroups a CU: 28, 16384 x
-// 3072 -> 768 73 / 77; 35, 20480 x 3072 -> 768 88 / 92.
-constexpr int64_t kMxPairExcess = 10;
+// 16384 x 2048 -> 6144 269 / 276; 8, 4096 x 2048 -> 2048 38.0 / 40.5; 16, 8192 x 2048 ->
+// 2048 64 / 60 on one card and 68.5 / 69 on another; 24, 12288 x 2048 -> 2048 90 / 83; 46,
+// 16384 x 768 -> 3072 118 / 89; 64, 32768 x 2048 -> 2048 276 / 204. The 128 x 128 tile has
+// two workgroups a CU: 28, 16384 x 3072 -> 768 73 / 77; 35, 20480 x 3072 -> 768 88 / 92.
+constexpr int64_t kMxPairExcess = 16;
 hipError_t launch_mx_gemm_pair(const MxGemm& a, const MxGemm& b, float* partials,
                                hipStream_t stream) {
   const bool alone = a.m == 0 || a.n == 0 || b.m == 0 || b.n == 0 || tune(kTuneMxPair) == 0 ||
