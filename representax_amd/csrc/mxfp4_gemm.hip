@@ -628,8 +628,6 @@ Plan plan_for(int id, int64_t m, int64_t n, int64_t slices, bool gated) {
 //   3072 x 768 <- 8192     2: 23.9, 3: 17.2, 4: 22.3 (144 tiles of 2 and 3: one a CU,
 //                          where 3's four stages take the place of a second workgroup)
 //   3500 x 768 <- 3072     2: 9.7, 3: 9.8
-// A product of few tiles over a long sum is split; the partial tiles and their sum
-// cost 7 to 10 us (768 x 768 <- 8192, tile 5: 13.0 us whole, 13.8 in two, 14.9 in four).
 template <class TilesOf>
 int tile_for(TilesOf tiles_of, int64_t slices) {
   if (tune(kTuneMxTile) != 0) return tune(kTuneMxTile);
@@ -637,6 +635,30 @@ int tile_for(TilesOf tiles_of, int64_t slices) {
   if (large >= 192 && (slices >= 6 || large >= 1024)) return 1;
   if (medium >= 140) return medium <= 256 && slices >= 24 ? 3 : 2;
   return tiles_of(4) >= 192 ? 4 : 5;
+}
+
+// Parts of a sum, for a product whose tiles leave CUs idle; the partial tiles and
+// their sum cost 3 to 15 us by their size. Whole / split, us, operands from memory:
+//   tiles 4 and 5, 48 slices and more:
+//     256 x 256 <- 12288 (16 tiles) 27.6 / 13.9, 768 x 768 <- 12288 (144) 27.5 / 18.0,
+//     <- 16384 35.1 / 19.5, 512 x 3072 <- 12288 (192) 40.2 / 31.2, 1024 x 2048 <- 12288
+//     (256) 30.5 / 29.5
+//   the same, 32 to 40 slices: 256 x 256 <- 8192 19.3 / 13.5, 768 x 768 <- 8192 19.4 /
+//     15.4, but 1024 x 2048 <- 8192 22.1 / 22.0, 512 x 3072 <- 10240 26.0 / 26.9; and a
+//     backward's other product is then not in the same launch (8192 x 1024 -> 1024, the
+//     step 64.8 / 65.4)
+//   tile 3 in three parts: 768 x 3072 <- 16384 40.0 / 46.4, <- 32768 74 / 72; in a
+//     backward, 28672 x 3072 -> 768 147 / 159, 32768 168 / 172, 32768 x 768 -> 3072 201 /
+//     192, 36864 x 3072 -> 768 203 / 195, 65536 x 768 -> 3072 387 / 358
+//   tile 3 in two parts, and the larger tiles: 2048 x 2048 <- 16384 42.7 / 57.2, <- 65536
+//     156 / 167; the backward of 16384 x 2048 -> 6144 276 / 312, of 16384 x 6144 -> 2048
+//     240 / 285
+int64_t splits_for(int id, int64_t tiles, int64_t slices) {
+  if (tiles == 0) return 1;
+  if (id == 3) return slices >= 128 && tiles <= 512 / 3 ? 512 / tiles : 1;
+  if (id < 4 || slices < 48) return 1;
+  const int64_t splits = 512 / tiles;
+  return splits < slices / 16 ? splits : slices / 16;
 }
 
 Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {
@@ -649,10 +671,7 @@ Plan choose(int64_t m, int64_t n, int64_t slices, bool gated) {
   Plan p = plan_for(id, m, n, slices, gated);
   const int64_t tiles = p.tiles_m * p.tiles_n;
   int64_t splits = tune(kTuneMxSplits);
-  if (splits == 0) {
-    splits = slices < 48 || tiles == 0 ? 1 : 512 / tiles;
-    if (splits > slices / 16) splits = slices / 16;
-  }
+  if (splits == 0) splits = splits_for(id, tiles, slices);
   if (gated) splits = 1;
   if (splits > slices / 4) splits = slices / 4;
   if (splits > 1) {

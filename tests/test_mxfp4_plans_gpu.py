@@ -14,9 +14,12 @@ pytestmark = pytest.mark.gpu
 POLICY = rx.resolve_precision_policy(rx.PrecisionConfig.mxfp4_mixed())
 
 
-# (11776, 768, 3072): the smaller tile, two workgroups a CU
+# (11776, 768, 3072) and (16384, 3072, 768): the smaller tile, two workgroups a CU; (16384,
+# 2048, 6144): a long sum of many tiles
 @pytest.mark.parametrize("m,k,n,joint", [(5003, 2048, 6144, True), (4096, 2048, 2048, True),
-                                         (11776, 768, 3072, True), (8192, 2048, 2048, True),
+                                         (11776, 768, 3072, True), (16384, 3072, 768, True),
+                                         (16384, 2048, 6144, True), (8192, 2048, 2048, True),
+                                         (16384, 768, 3072, False),
                                          (11008, 2048, 2048, False), (10240, 1024, 4096, False)])
 def test_products_share_a_launch_where_the_longest_tile_ends_with_the_others(m, k, n, joint):
     g = torch.Generator(device=DEVICE).manual_seed(m + k)
