@@ -13,11 +13,21 @@ namespace {
 
 constexpr int kThreads = 256;
 // Waves of the fused form (32 KB read each) from which both encodings come from one
-// read; below, each from its own. Measured, fused against apart: 12.3 / 8.1 us at
-// 8192 x 768 bf16 (384 waves), 13.4 / 14.7 at 6144 x 2048 (768), 23.0 / 34.3 at
-// 16384 x 2048 (2048); 11.5 / 12.2 at 5003 x 1000 float32 (640), 12.2 / 13.3 at
-// 8192 x 768 (768), 12.4 / 16.7 at 2048 x 4096 (1024).
-constexpr int64_t kMxFusedWaves = 768;
+// read; below, each from its own. The two meet earlier where the matrix lies in the caches,
+// later where it comes from memory; the limit is where their mean does. Fused against
+// apart, us, from the caches and from memory:
+//   bf16     8192 x 768 (384 waves)   11.6 / 8.0, 15.4 / 9.9
+//            5632 x 2048 (704)        13.7 / 13.8, 18.2 / 16.1
+//            6144 x 2048 (768)        14.0 / 14.7, 18.6 / 17.5
+//            7168 x 2048 (896)        15.2 / 16.6, 19.9 / 19.6
+//            8192 x 2048 (1024)       15.9 / 18.6, 20.8 / 22.2
+//   float32  3072 x 1024 (384)        11.1 / 6.4, 13.4 / 9.2
+//            6144 x 768 (576)         11.1 / 10.8, 14.2 / 12.6
+//            5120 x 1024 (640)        11.2 / 11.6, 14.5 / 13.5
+//            5003 x 1000 (640)        10.9 / 12.4, 14.3 / 14.0
+//            8192 x 768 (768)         11.6 / 13.5, 15.2 / 16.0
+constexpr int64_t kMxFusedWavesBF16 = 800;
+constexpr int64_t kMxFusedWavesF32 = 640;
 
 // Maximum over the LANES neighbouring lanes that share a block.
 template <int LANES>
@@ -652,11 +662,18 @@ hipError_t launch_mx_quantize(MxParts parts, int count, hipStream_t stream) {
   auto tiles_of = [](const MxPart& part, int cols) {
     return mx_slices(part.rows) * 2 * mx_tiles_of_row(part, 16 * cols);
   };
-  int64_t waves = 0;
-  for (int p = 0; p < count; ++p)
-    if (parts.part[p].across.codes != nullptr)
-      waves += tiles_of(parts.part[p], parts.part[p].dtype == kBF16 ? 8 : 4);
-  const bool fused = waves >= kMxFusedWaves;
+  int64_t bf16_waves = 0, f32_waves = 0;
+  for (int p = 0; p < count; ++p) {
+    const MxPart& part = parts.part[p];
+    if (part.across.codes == nullptr) continue;
+    if (part.dtype == kBF16)
+      bf16_waves += tiles_of(part, 8);
+    else
+      f32_waves += tiles_of(part, 4);
+  }
+  const bool both_axes = bf16_waves + f32_waves > 0;
+  const bool fused = bf16_waves * kMxFusedWavesF32 + f32_waves * kMxFusedWavesBF16 >=
+                     kMxFusedWavesBF16 * kMxFusedWavesF32;
   enum { kRows, kFusedF32, kFusedBF16, kApart, kKinds };
   MxParts some[kKinds] = {};
   int jobs[kKinds] = {};
@@ -677,7 +694,7 @@ hipError_t launch_mx_quantize(MxParts parts, int count, hipStream_t stream) {
     const bool bf16 = part.dtype == kBF16;
     if (part.across.codes == nullptr) {
       // beside encodings along both axes it costs no launch of its own
-      add(waves > 0 && !fused ? kApart : kRows, part, row_blocks(part));
+      add(both_axes && !fused ? kApart : kRows, part, row_blocks(part));
     } else if (fused && part.along.codes != nullptr) {
       part.tiles = tiles_of(part, bf16 ? 8 : 4);
       add(bf16 ? kFusedBF16 : kFusedF32, part, ceil_div(part.tiles, kThreads / 64));

@@ -1,4 +1,4 @@
-"""Which launches an MXFP4 backward is made of (GPU)."""
+"""Which launches MXFP4 encodings and backwards are made of (GPU)."""
 
 from __future__ import annotations
 
@@ -33,3 +33,16 @@ def test_products_share_a_launch_where_the_longest_tile_ends_with_the_others(m, 
     with ops.tuning(mx_pair=0):
         apart = torch.autograd.grad(y, (x, w), dy)
     assert all(torch.equal(a, b) for a, b in zip(grads, apart))
+
+
+# 704 and 896 waves of the form that reads once, of 800; 576 and 640, of 640
+@pytest.mark.parametrize("rows,columns,dtype,once", [
+    (5632, 2048, torch.bfloat16, False), (7168, 2048, torch.bfloat16, True),
+    (6144, 768, torch.float32, False), (5003, 1000, torch.float32, True)])
+def test_large_matrices_are_read_once_for_both_axes(rows, columns, dtype, once):
+    t = torch.ones((rows, columns), device=DEVICE, dtype=dtype)
+    (along, across), names = kernel_names(lambda: rx.mxfp4_quantize_both(t))
+    assert any("k_mx_quantize_both" in n for n in names) == once, names
+    assert any("k_mx_quantize_apart" in n for n in names) != once, names
+    for q in (along, across):
+        assert torch.equal(q.dequantize(dtype), torch.ones(q.shape, device=DEVICE, dtype=dtype))
