@@ -8,7 +8,8 @@
  *     is enqueued on it; no entry point allocates device memory, and none
  *     synchronizes except the diagnostic rpx_check_device_errors. Scratch
  *     comes from the caller's `workspace`, sized by the matching
- *     *_workspace() query.
+ *     *_workspace() query; calls that threads enqueue on one stream at the
+ *     same time need one each, as a call may be several launches over it.
  *   - bf16 tensors are passed as their 16-bit patterns; fp8 tensors as uint8
  *     codes in the OCP e4m3fn / e5m2 encodings.
  *   - Matrices are row-major and dense unless strides are given.
@@ -622,8 +623,10 @@ typedef struct rpx_mxfp4_part {
   int dtype;
 } rpx_mxfp4_part;
 
-/* Up to four matrices in one launch (a linear's input and weight). `parts` is
- * a host array, read before the call returns. */
+/* Up to four matrices in one call (a linear's input and weight): one launch for
+ * each form among them (along columns only, or, for large ones, both axes from
+ * one read, by type; small ones share a launch). `parts` is a host array, read
+ * before the call returns. */
 int rpx_mxfp4_quantize(const rpx_mxfp4_part* parts, int64_t count, void* stream);
 
 /* out [rows, columns] = the values that the codes stand for. */

@@ -314,10 +314,10 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_both(MxParts parts) {
   int p = 0;
   while (blk >= parts.first[p + 1]) ++p;
   // In a launch of a workgroup a CU, two rows of tiles, 256 rows of the matrix, run on one
-  // XCD, whose L2 then has whole lines of the transpose's codes: 13.4 / 15.4 us for 6144 x
-  // 2048 bf16, 13.3 / 14.3 for 2048 x 6144, 12.3 / 14.0 for 8192 x 1024 float32; longer
-  // launches lose by it: 23.9 / 22.9 for 16384 x 2048 bf16, 119 / 112 for 16384 x 6144
-  // float32.
+  // XCD, whose L2 then has whole lines of the transpose's codes: 12.3 / 14.0 us for 8192 x
+  // 1024 float32 and, forced into this form, 13.4 / 15.4 for 6144 x 2048 bf16, 13.3 / 14.3
+  // for 2048 x 6144; longer launches lose by it: 23.9 / 22.9 for 16384 x 2048 bf16, 119 /
+  // 112 for 16384 x 6144 float32.
   const MxPart& part = parts.part[p];
   int64_t block = blk - parts.first[p];
   if (parts.first[kMxParts] <= 256) {

@@ -4,8 +4,9 @@
 //
 // What bounds them: the fp4 MFMAs issue 7.3 PFLOP/s, which zeros nearly reach (8192 x 8192
 // <- 8192 6.6, 166 us); on random codes the card's power holds that product at 4.7 (235
-// us), 16384 x 2048 <- 6144 at 4.4 (94 us), so an operation saved in the loop counts also
-// where it is hidden. A tile of few slices adds what runs with no MFMA beside it, the
+// us; the same instructions and the same 65% of cycles with an MFMA under way, at 1.69 GHz
+// against 2.26), 16384 x 2048 <- 6144 at 4.4 (94 us), so an operation saved in the loop
+// counts also where it is hidden. A tile of few slices adds what runs with no MFMA beside it, the
 // activation and the staging of its outputs: 3.85 for the gated block of 16384 x 2048 -> 2 x
 // 6144 (214 us), 3.4 with its projections kept (244 us, 604 MB of outputs).
 #include <atomic>
