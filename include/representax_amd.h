@@ -729,6 +729,80 @@ int rpx_mxfp4_gated(const void* x, int dtype, int64_t m, int64_t k, int64_t row_
                     const uint8_t* up_codes, const uint8_t* up_scales, int64_t n, void* h,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Dropout from a counter, with no stored mask, and the boundary between two
+ * blocks of a transformer. No reference counterparts (its encoders run without
+ * dropout and with norms, sums and gates as separate operations).
+ *
+ * A dropout's bits: element i of a tensor, in its dense order, takes the 16
+ * bits number i % 8 of Philox4x32-10 (Salmon et al., 2011) for the counter
+ * (i / 8 modulo 2^32, i / 8 >> 32, site, step) and the key `seed`, and is kept
+ * where they are below `threshold` (65536 (1 - rate), 1 to 65536), times
+ * 65536 / threshold; else it is zero. key is a device pointer to {seed, step}
+ * (int64); threshold 65536 is no dropout, and key may be NULL then.
+ * ------------------------------------------------------------------------- */
+
+/* out = dropout(x), count dense elements, both 16-byte aligned; out may be x.
+ * The gradient is the same call on the gradient. */
+int rpx_dropout(const void* x, int dtype, int64_t count, const int64_t* key, int64_t site,
+                int64_t threshold, void* out, void* stream);
+
+/* t = x + scale * dropout(gate * post(u)) rounded to dtype, h = norm(t), over
+ * rows [rows, size] of x and u, size at most 8192. post and norm are a
+ * LayerNorm or an RMSNorm (kind RPX_NORM_*), or none where their weight is
+ * NULL; their weights and biases are f32 or bf16, and a LayerNorm takes them
+ * rounded to dtype. gate [rows / rows_per_gate, size] or NULL. x, u, t, h and
+ * the gradients of `rpx_block_backward` are dense and aligned to their type.
+ * Element (row, column) of the dropout is element row * size + column. */
+typedef struct rpx_block_norm {
+  const void* weight;
+  const void* bias;
+  int dtype;
+  int kind;
+  float eps;
+} rpx_block_norm;
+
+typedef struct rpx_block {
+  const void* x;
+  const void* u;
+  const void* gate;
+  int64_t rows_per_gate;
+  rpx_block_norm post;
+  rpx_block_norm norm;
+  const int64_t* key;
+  int64_t site;
+  int64_t threshold;
+  int64_t rows;
+  int64_t size;
+  void* t;
+  void* h;
+  int dtype;
+  int gate_dtype;
+  float scale;
+} rpx_block;
+
+int rpx_block_forward(const rpx_block* block, void* stream);
+
+/* The gradients for those of t and h (dt, dh; NULL: none), from the forward's
+ * t and u (x and h are not read). Each output may be NULL: dx and du [rows,
+ * size], d_gate in the gate's shape and type, the others [size] in the weights'
+ * types. */
+typedef struct rpx_block_gradients {
+  const void* dt;
+  const void* dh;
+  void* dx;
+  void* du;
+  void* d_gate;
+  void* d_weight;
+  void* d_bias;
+  void* d_post_weight;
+  void* d_post_bias;
+} rpx_block_gradients;
+
+size_t rpx_block_backward_workspace(const rpx_block* block, const rpx_block_gradients* gradients);
+int rpx_block_backward(const rpx_block* block, const rpx_block_gradients* gradients,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

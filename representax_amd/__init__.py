@@ -18,6 +18,7 @@ from .adapters import (
 )
 from .components import Linear, MXFP4Linear
 from .config import PrecisionConfig, QuantizedLoRAConfig
+from .dropout import DropoutKeys, dropout
 from .mlp import gelu_mlp, shared_input_projections, swiglu_mlp
 from .mxfp4 import (
     MXFP4Matrix,
@@ -27,6 +28,7 @@ from .mxfp4 import (
     mxfp4_quantize,
     mxfp4_quantize_both,
 )
+from .norms import LayerNorm, RMSNorm, add_norm, block_norm
 from .precision import (
     FP32_POLICY,
     DelayedScaling,
@@ -45,7 +47,9 @@ from .sharding import activation_out_sharding, constrain_activation, replicate
 
 __all__ = [
     "DelayedScaling",
+    "DropoutKeys",
     "FP32_POLICY",
+    "LayerNorm",
     "Linear",
     "MXFP4Linear",
     "MXFP4Matrix",
@@ -53,10 +57,12 @@ __all__ = [
     "PrecisionPolicy",
     "QuantizedLoRAConfig",
     "QuantizedLoRALinear",
+    "RMSNorm",
     "activation_inputs",
     "activation_out_sharding",
     "active_compute_dtype",
     "active_model_for_compute",
+    "add_norm",
     "apply_quantized_lora",
     "compute_parameter",
     "constrain_activation",

@@ -195,6 +195,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rpx_mxfp4_gated": (
         _int, [_p, _int, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p, _size, _p]
     ),
+    "rpx_dropout": (_int, [_p, _int, _i64, _p, _i64, _i64, _p, _p]),
+    "rpx_block_forward": (_int, [_p, _p]),
+    "rpx_block_backward_workspace": (_size, [_p, _p]),
+    "rpx_block_backward": (_int, [_p, _p, _p, _size, _p]),
     "rpx_head_norm": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _int, _p]),
 }
 
@@ -206,6 +210,32 @@ class HeadPart(ctypes.Structure):
     _fields_ += [(name, ctypes.c_int64)
                  for name in ("stride_b", "stride_s", "stride_h", "heads", "repeat")]
     _fields_ += [("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
+class BlockNorm(ctypes.Structure):
+    """``rpx_block_norm`` of include/representax_amd.h."""
+
+    _fields_ = [("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("kind", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
+class Block(ctypes.Structure):
+    """``rpx_block`` of include/representax_amd.h."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("u", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("rows_per_gate", ctypes.c_int64), ("post", BlockNorm), ("norm", BlockNorm),
+                ("key", ctypes.c_void_p), ("site", ctypes.c_int64), ("threshold", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("size", ctypes.c_int64), ("t", ctypes.c_void_p),
+                ("h", ctypes.c_void_p), ("dtype", ctypes.c_int), ("gate_dtype", ctypes.c_int),
+                ("scale", ctypes.c_float)]
+
+
+class BlockGradients(ctypes.Structure):
+    """``rpx_block_gradients`` of include/representax_amd.h."""
+
+    _fields_ = [(name, ctypes.c_void_p)
+                for name in ("dt", "dh", "dx", "du", "d_gate", "d_weight", "d_bias",
+                             "d_post_weight", "d_post_bias")]
 
 
 class Mxfp4Part(ctypes.Structure):

@@ -1,0 +1,594 @@
+// The boundary between two blocks of a transformer, for rows of x (the stream)
+// and u (the update that the first block computed):
+//   p = post(u)            a norm after the block, or u itself
+//   t = x + c drop(g p)    its gate, dropout and residual scale; rounded to the
+//                          stream's type, as it is stored
+//   h = norm(t)            the norm before the next block, of that t
+// and its gradients, with those of the norms' weights and of the gate. A norm is
+// a LayerNorm or an RMSNorm; statistics, sums and everything between the loads
+// and the stores are f32.
+//
+// A pass over memory: a row lives in the registers of L lanes, eight consecutive
+// values a lane and chunk; x and u are read once, t and h written once. The
+// backward reads dt, dh, t and u, recomputes the statistics, the normalised rows
+// and the dropout's bits, and writes dx and du.
+//
+// The sums over rows (weights, biases, gate) are kept by the lanes that own the
+// columns, over the rows that a worker (L lanes) takes one after another, and
+// joined by a second launch in a fixed order: no atomics, so a call gives the
+// same bits every time. A worker's rows lie in one group of rows that share a
+// gate, or are whole groups.
+#include "kernels.h"
+#include "vector8.h"
+
+namespace rpx {
+
+namespace {
+
+// Sums of K values over the L lanes of a row, the same in each lane, in a fixed
+// order. Rows of more than one wave meet in LDS; two buffers in turn need one
+// barrier a sum.
+template <int L, int K>
+struct RowSum {
+  float (*lds)[K][L / 64 > 0 ? L / 64 : 1];
+  int parity = 0;
+  __device__ __forceinline__ void operator()(float (&v)[K]) {
+    constexpr int W = L < 64 ? L : 64;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int off = W / 2; off > 0; off >>= 1) v[k] += __shfl_xor(v[k], off, 64);
+    if constexpr (L > 64) {
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) lds[parity][k][wave] = v[k];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < L / 64; ++w) s += lds[parity][k][w];
+        v[k] = s;
+      }
+      parity ^= 1;
+    }
+  }
+};
+
+constexpr int threads_of(int lanes) { return lanes > 256 ? lanes : 256; }
+
+// Eight weights from column e on; `round` rounds a float32 master to the values'
+// type first (a LayerNorm takes its weights in that type).
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void load_weight8(const void* w, int dtype, bool round, int64_t e,
+                                             int count, float* v) {
+  if (dtype == kBF16) {
+    load_row8<WHOLE>(static_cast<const Bf16*>(w) + e, count, v);
+    return;
+  }
+  load_row8<WHOLE>(static_cast<const float*>(w) + e, count, v);
+  if (round) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = rounded(static_cast<const T*>(nullptr), v[i]);
+  }
+}
+
+template <typename T, int L, int C, bool WHOLE>
+__global__ void __launch_bounds__(threads_of(L)) k_block_fwd(BlockArgs a) {
+  constexpr int kRows = threads_of(L) / L;
+  __shared__ float lds[2][2][L / 64 > 0 ? L / 64 : 1];
+  RowSum<L, 2> row_sum{lds};
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t row = block_of_grid() * kRows + threadIdx.x / L;
+  if (row >= a.rows) return;  // a row of several waves is the whole workgroup
+  const int size = a.size;
+  const float inv = 1.0f / static_cast<float>(size);
+  const int64_t base = row * size;
+  const T* x = static_cast<const T*>(a.x) + base;
+  const T* u = static_cast<const T*>(a.u) + base;
+  float v[C][8], r[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int e = (c * L + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[c][i] = r[c][i] = 0.0f;
+    if (e >= size) continue;
+    load_row8<WHOLE>(u + e, size - e, v[c]);
+    load_row8<WHOLE>(x + e, size - e, r[c]);
+  }
+  // mean and 1 / deviation of the row in v, whose entries past the end are zero
+  auto statistics = [&](int kind, float eps, float& mean, float& rstd) {
+    float s[2] = {0.0f, 0.0f};
+    mean = 0.0f;
+    if (kind == kNormLayer) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[0] += v[c][i];
+      row_sum(s);
+      mean = s[0] * inv;
+    }
+    s[0] = s[1] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int n = size - (c * L + lane) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = v[c][i] - mean;
+        if (i < n) s[0] = __builtin_fmaf(d, d, s[0]);
+      }
+    }
+    row_sum(s);
+    rstd = rsqrtf(s[0] * inv + eps);
+  };
+  float mean, rstd;
+  if (a.post.weight != nullptr) {
+    statistics(a.post.kind, a.post.eps, mean, rstd);
+    const bool layer = a.post.kind == kNormLayer;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+      if (e >= size) continue;
+      float w[8], b[8];
+      load_weight8<WHOLE, T>(a.post.weight, a.post.dtype, layer, e, size - e, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+      if (layer) load_weight8<WHOLE, T>(a.post.bias, a.post.dtype, true, e, size - e, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, w[i], b[i]);
+    }
+  }
+  if (a.gate != nullptr) {
+    const int64_t at = (row / a.rows_per_gate) * size;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+      if (e >= size) continue;
+      float g[8];
+      load_weight8<WHOLE, T>(a.gate, a.gate_dtype, false, at + e, size - e, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] *= g[i];
+    }
+  }
+  if (a.drop.threshold < 65536u) {
+    const PhiloxCall call = philox_call(a.drop);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+      if (e < size) dropout8<WHOLE>(call, a.drop, base + e, v[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int e = (c * L + lane) * 8;
+    if (e >= size) continue;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[c][i] = rounded(static_cast<const T*>(nullptr),
+                        i < size - e ? __builtin_fmaf(a.scale, v[c][i], r[c][i]) : 0.0f);
+    store_row8<WHOLE>(static_cast<T*>(a.t) + base + e, size - e, v[c]);
+  }
+  if (a.norm.weight == nullptr) return;
+  statistics(a.norm.kind, a.norm.eps, mean, rstd);
+  const bool layer = a.norm.kind == kNormLayer;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int e = (c * L + lane) * 8;
+    if (e >= size) continue;
+    float w[8], b[8];
+    load_weight8<WHOLE, T>(a.norm.weight, a.norm.dtype, layer, e, size - e, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+    if (layer) load_weight8<WHOLE, T>(a.norm.bias, a.norm.dtype, true, e, size - e, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, w[i], b[i]);
+    store_row8<WHOLE>(static_cast<T*>(a.h) + base + e, size - e, v[c]);
+  }
+}
+
+// What a lane sums over a worker's rows: the columns of its chunks.
+enum Column : int { kWeight = 0, kBias = 1, kPostWeight = 2, kPostBias = 3, kGate = 4, kColumns = 5 };
+
+template <typename T, int L, int C, bool WHOLE>
+__global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
+  constexpr int kThreads = threads_of(L);
+  constexpr int kWorkers = kThreads / L;
+  __shared__ float sums[2][4][L / 64 > 0 ? L / 64 : 1];
+  // the columns of this workgroup's workers, where there are several
+  __shared__ float meet[kWorkers > 1 ? kWorkers * L * C * 8 : 1];
+  RowSum<L, 4> row_sum{sums};
+  const BlockArgs& f = a.forward;
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t worker = block_of_grid() * kWorkers + threadIdx.x / L;
+  const int size = f.size;
+  const float inv = 1.0f / static_cast<float>(size);
+  const bool has_norm = f.norm.weight != nullptr && a.dh != nullptr;
+  const bool has_post = f.post.weight != nullptr;
+  const bool norm_mean = has_norm && f.norm.kind == kNormLayer;
+  const bool post_mean = has_post && f.post.kind == kNormLayer;
+  const bool read_u = has_post || f.gate != nullptr;
+  float acc[kColumns][C][8];
+#pragma unroll
+  for (int k = 0; k < kColumns; ++k)
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[k][c][i] = 0.0f;
+  // the worker's rows: slice worker % slices of a group, or whole groups
+  int64_t row, end;
+  if (a.slices > 0) {
+    const int64_t group = worker / a.slices;
+    row = group * a.group_rows + (worker % a.slices) * a.worker_rows;
+    end = row + a.worker_rows;
+    const int64_t last = (group + 1) * a.group_rows;
+    end = end < last ? end : last;
+  } else {
+    row = worker * a.worker_rows;
+    end = row + a.worker_rows;
+  }
+  end = end < f.rows ? end : f.rows;
+  if (worker >= a.workers) row = end = 0;
+  PhiloxCall call{};
+  const bool drop = f.drop.threshold < 65536u;
+  if (drop) call = philox_call(f.drop);
+  int64_t group_left = a.slices > 0 ? end - row : a.group_rows;  // rows to the group's end
+  for (; row < end; ++row) {
+    const int64_t base = row * size;
+    float t[C][8], u[C][8], g[C][8], d[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[c][i] = u[c][i] = g[c][i] = d[c][i] = 0.0f;
+      if (e >= size) continue;
+      if (has_norm) {
+        load_row8<WHOLE>(static_cast<const T*>(f.t) + base + e, size - e, t[c]);
+        load_row8<WHOLE>(static_cast<const T*>(a.dh) + base + e, size - e, g[c]);
+      }
+      if (a.dt != nullptr) load_row8<WHOLE>(static_cast<const T*>(a.dt) + base + e, size - e, d[c]);
+      if (read_u) load_row8<WHOLE>(static_cast<const T*>(f.u) + base + e, size - e, u[c]);
+    }
+    float mean = 0.0f, u_mean = 0.0f;
+    if (norm_mean || post_mean) {
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s[0] += t[c][i];
+          s[1] += u[c][i];
+        }
+      row_sum(s);
+      mean = norm_mean ? s[0] * inv : 0.0f;
+      u_mean = post_mean ? s[1] * inv : 0.0f;
+    }
+    // the statistics, and what the norm's gradient takes out of its row:
+    // sum (t - mean)^2, sum (u - mean)^2, sum w dh, sum w dh (t - mean)
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+      if (e >= size) continue;
+      float w[8];
+      if (has_norm)
+        load_weight8<WHOLE, T>(f.norm.weight, f.norm.dtype, norm_mean, e, size - e, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!WHOLE && i >= size - e) continue;
+        t[c][i] -= mean;
+        s[0] = __builtin_fmaf(t[c][i], t[c][i], s[0]);
+        const float du = u[c][i] - u_mean;
+        s[1] = __builtin_fmaf(du, du, s[1]);
+        const float gw = has_norm ? g[c][i] * w[i] : 0.0f;
+        s[2] += gw;
+        s[3] = __builtin_fmaf(gw, t[c][i], s[3]);
+      }
+    }
+    if (has_norm || has_post) row_sum(s);
+    const float u_rstd = rsqrtf(s[1] * inv + f.post.eps);
+    if (has_norm) {
+      const float rstd = rsqrtf(s[0] * inv + f.norm.eps);
+      const float mg = norm_mean ? s[2] * inv : 0.0f;
+      const float mgt = s[3] * rstd * inv;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = (c * L + lane) * 8;
+        if (e >= size) continue;
+        float w[8];
+        load_weight8<WHOLE, T>(f.norm.weight, f.norm.dtype, norm_mean, e, size - e, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float n = t[c][i] * rstd;
+          acc[kWeight][c][i] = __builtin_fmaf(g[c][i], n, acc[kWeight][c][i]);
+          acc[kBias][c][i] += g[c][i];
+          d[c][i] = __builtin_fmaf(rstd, g[c][i] * w[i] - mg - n * mgt, d[c][i]);
+        }
+      }
+    }
+    // d is the gradient of t, and of x; from here on d becomes that of p, with
+    // u the normalised row
+    const int64_t gate_at = f.gate == nullptr ? 0 : (row / f.rows_per_gate) * size;
+    float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+      if (e >= size) continue;
+      if (a.dx != nullptr) store_row8<WHOLE>(static_cast<T*>(a.dx) + base + e, size - e, d[c]);
+      if (drop) dropout8<WHOLE>(call, f.drop, base + e, d[c]);
+      float w[8], b[8], k[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = k[i] = 1.0f;
+        b[i] = 0.0f;
+      }
+      if (has_post) {
+        load_weight8<WHOLE, T>(f.post.weight, f.post.dtype, post_mean, e, size - e, w);
+        if (post_mean) load_weight8<WHOLE, T>(f.post.bias, f.post.dtype, true, e, size - e, b);
+      }
+      if (f.gate != nullptr)
+        load_weight8<WHOLE, T>(f.gate, f.gate_dtype, false, gate_at + e, size - e, k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!WHOLE && i >= size - e) continue;
+        if (has_post) u[c][i] = (u[c][i] - u_mean) * u_rstd;
+        d[c][i] *= f.scale;
+        acc[kGate][c][i] = __builtin_fmaf(d[c][i], __builtin_fmaf(u[c][i], w[i], b[i]),
+                                          acc[kGate][c][i]);
+        d[c][i] *= k[i];
+        acc[kPostWeight][c][i] = __builtin_fmaf(d[c][i], u[c][i], acc[kPostWeight][c][i]);
+        acc[kPostBias][c][i] += d[c][i];
+        d[c][i] *= w[i];
+        q[0] += d[c][i];
+        q[1] = __builtin_fmaf(d[c][i], u[c][i], q[1]);
+      }
+    }
+    float md = 0.0f, mdu = 0.0f, factor = 1.0f;
+    if (has_post) {
+      row_sum(q);
+      md = post_mean ? q[0] * inv : 0.0f;
+      mdu = q[1] * inv;
+      factor = u_rstd;
+    }
+    if (a.du != nullptr) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = (c * L + lane) * 8;
+        if (e >= size) continue;
+        if (has_post) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[c][i] = factor * (d[c][i] - md - u[c][i] * mdu);
+        }
+        store_row8<WHOLE>(static_cast<T*>(a.du) + base + e, size - e, d[c]);
+      }
+    }
+    if (a.dgate != nullptr && --group_left == 0) {
+      // whole groups: the gate's gradient as it is; a slice: for the joining launch
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = (c * L + lane) * 8;
+        if (e < size) {
+          if (a.gate_partials != nullptr)
+            store_row8<WHOLE>(a.gate_partials + worker * size + e, size - e, acc[kGate][c]);
+          else if (f.gate_dtype == kBF16)
+            store_row8<WHOLE>(static_cast<Bf16*>(a.dgate) + gate_at + e, size - e, acc[kGate][c]);
+          else
+            store_row8<WHOLE>(static_cast<float*>(a.dgate) + gate_at + e, size - e, acc[kGate][c]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[kGate][c][i] = 0.0f;
+      }
+      group_left = a.group_rows;
+    }
+  }
+  if (a.partials == nullptr) return;
+  // one row of partials a workgroup: [workgroup][column][size]
+#pragma unroll
+  for (int k = 0; k < kGate; ++k) {
+    if (a.columns[k] == nullptr) continue;
+    float* out = a.partials + (block_of_grid() * kGate + k) * size;
+    if constexpr (kWorkers > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          meet[(threadIdx.x / L) * (L * C * 8) + (c * L + lane) * 8 + i] = acc[k][c][i];
+      __syncthreads();
+      for (int e = threadIdx.x; e < size; e += kThreads) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWorkers; ++w) s += meet[w * (L * C * 8) + e];
+        out[e] = s;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = (c * L + lane) * 8;
+        if (e < size) store_row8<WHOLE>(out + e, size - e, acc[k][c]);
+      }
+    }
+  }
+}
+
+// Joins the partials of one column and of 64 of its entries: 16 lanes of 4
+// entries by 16 rows of partials, then over LDS in row order.
+struct BlockJoin {
+  const float* partials;
+  int64_t count, stride;  // partials and floats from one to the next
+  void* out;
+  int dtype;
+};
+
+__device__ __forceinline__ void join(const BlockJoin& j, int size, int64_t e0) {
+  __shared__ float lds[16][64];
+  const int64_t e = e0 + (threadIdx.x & 63);
+  const int part = threadIdx.x >> 6;
+  float s = 0.0f;
+  if (e < size) {
+    int64_t p = part;
+    for (; p + 48 < j.count; p += 64) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = j.partials[(p + 16 * i) * j.stride + e];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += v[i];
+    }
+    for (; p < j.count; p += 16) s += j.partials[p * j.stride + e];
+  }
+  lds[part][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (part == 0 && e < size) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += lds[i][threadIdx.x & 63];
+    if (j.dtype == kBF16)
+      store1(static_cast<Bf16*>(j.out) + e, s);
+    else
+      store1(static_cast<float*>(j.out) + e, s);
+  }
+}
+
+__global__ void __launch_bounds__(1024) k_block_join(BlockGradients a, int64_t workgroups,
+                                                     int columns, int64_t gates) {
+  const int size = a.forward.size;
+  const int64_t blocks = ceil_div(size, 64);
+  const int64_t job = block_of_grid() / blocks;
+  const int64_t e0 = (block_of_grid() % blocks) * 64;
+  if (job < columns) {
+    int k = 0;
+    for (int64_t left = job; k < kGate; ++k)
+      if (a.columns[k] != nullptr && left-- == 0) break;
+    const int dtype = k < kPostWeight ? a.forward.norm.dtype : a.forward.post.dtype;
+    join(BlockJoin{a.partials + k * size, workgroups, static_cast<int64_t>(kGate) * size,
+                   a.columns[k], dtype},
+         size, e0);
+  } else if (job - columns < gates) {
+    const int64_t g = job - columns;
+    const size_t bytes = a.forward.gate_dtype == kBF16 ? 2 : 4;
+    join(BlockJoin{a.gate_partials + g * a.slices * size, a.slices, size,
+                   static_cast<uint8_t*>(a.dgate) + g * size * bytes, a.forward.gate_dtype},
+         size, e0);
+  }
+}
+
+struct Shape {
+  int lanes, workers;  // lanes a row, rows a workgroup
+};
+
+Shape shape_of(int size) {
+  if (size <= 128) return {16, 16};
+  if (size <= 1024) return {64, 4};
+  if (size <= 4096) return {256, 1};
+  return {512, 1};
+}
+
+#define RPX_BLOCK_SIZES(CALL)            \
+  if (size <= 128) CALL(16, 1);          \
+  else if (size <= 512) CALL(64, 1);     \
+  else if (size <= 1024) CALL(64, 2);    \
+  else if (size <= 2048) CALL(256, 1);   \
+  else if (size <= 4096) CALL(256, 2);   \
+  else CALL(512, 2);
+
+template <typename T, bool WHOLE>
+void forward(const BlockArgs& a, hipStream_t stream) {
+  const int size = a.size;
+#define RPX_FWD(L, C)                                                                      \
+  hipLaunchKernelGGL((k_block_fwd<T, L, C, WHOLE>),                                        \
+                     grid_of(ceil_div(a.rows, threads_of(L) / L)), dim3(threads_of(L)), 0, \
+                     stream, a)
+  RPX_BLOCK_SIZES(RPX_FWD)
+#undef RPX_FWD
+}
+
+template <typename T, bool WHOLE>
+void backward(const BlockGradients& a, int64_t workgroups, hipStream_t stream) {
+  const int size = a.forward.size;
+#define RPX_BWD(L, C)                                                                           \
+  hipLaunchKernelGGL((k_block_bwd<T, L, C, WHOLE>), grid_of(workgroups), dim3(threads_of(L)), 0, \
+                     stream, a)
+  RPX_BLOCK_SIZES(RPX_BWD)
+#undef RPX_BWD
+}
+
+// The split of the rows over workers. Each has at least kMinRows rows, so that the
+// columns' partials stay a small part of what is read, and at most about kWorkgroups
+// workgroups' worth are made (four workgroups of four waves on each of 256 CUs run
+// at a time).
+constexpr int64_t kMinRows = 4;
+constexpr int64_t kWorkgroups = 1024;
+
+struct Split {
+  int64_t slices, worker_rows, workers, workgroups, gates;
+};
+
+Split split_of(int64_t rows, int size, int64_t group_rows) {
+  const Shape shape = shape_of(size);
+  int64_t want = ceil_div(rows, kWorkgroups * shape.workers);
+  want = want < kMinRows ? kMinRows : want;
+  Split s{};
+  const int64_t groups = group_rows > 0 ? ceil_div(rows, group_rows) : 0;
+  if (groups == 0) return s;
+  if (group_rows > want) {
+    s.slices = ceil_div(group_rows, want);
+    s.worker_rows = ceil_div(group_rows, s.slices);
+    s.slices = ceil_div(group_rows, s.worker_rows);
+    s.workers = groups * s.slices;
+  } else {
+    s.worker_rows = (want / group_rows) * group_rows;
+    s.workers = ceil_div(rows, s.worker_rows);
+  }
+  s.workgroups = ceil_div(s.workers, shape.workers);
+  s.gates = s.slices > 1 ? groups : 0;
+  return s;
+}
+
+}  // namespace
+
+int64_t block_gradients_floats(int64_t rows, int size, int64_t group_rows, bool columns, bool gate) {
+  const Split s = split_of(rows, size, group_rows);
+  return (columns ? s.workgroups * kGate * size : 0) +
+         (gate && s.gates > 0 ? s.workers * size : 0);
+}
+
+hipError_t launch_block_forward(const BlockArgs& a, hipStream_t stream) {
+  if (a.rows <= 0) return hipSuccess;
+  const bool whole = a.size % 8 == 0;
+  if (a.dtype == kBF16)
+    whole ? forward<Bf16, true>(a, stream) : forward<Bf16, false>(a, stream);
+  else
+    whole ? forward<float, true>(a, stream) : forward<float, false>(a, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_block_backward(BlockGradients a, float* scratch, hipStream_t stream) {
+  const BlockArgs& f = a.forward;
+  if (f.rows <= 0) return hipSuccess;
+  a.group_rows = a.dgate != nullptr ? f.rows_per_gate : f.rows;
+  const Split s = split_of(f.rows, f.size, a.group_rows);
+  a.slices = s.slices;
+  a.worker_rows = s.worker_rows;
+  a.workers = s.workers;
+  int columns = 0;
+  for (int k = 0; k < kGate; ++k) columns += a.columns[k] != nullptr;
+  a.partials = columns > 0 ? scratch : nullptr;
+  const bool gates = a.dgate != nullptr && s.gates > 0;
+  a.gate_partials = gates ? scratch + (columns > 0 ? s.workgroups * kGate * f.size : 0) : nullptr;
+  const bool whole = f.size % 8 == 0;
+  if (f.dtype == kBF16)
+    whole ? backward<Bf16, true>(a, s.workgroups, stream)
+          : backward<Bf16, false>(a, s.workgroups, stream);
+  else
+    whole ? backward<float, true>(a, s.workgroups, stream)
+          : backward<float, false>(a, s.workgroups, stream);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || (columns == 0 && !gates)) return e;
+  const int64_t jobs = columns + (gates ? s.gates : 0);
+  hipLaunchKernelGGL(k_block_join, grid_of(jobs * ceil_div(f.size, 64)), dim3(1024), 0, stream, a,
+                     s.workgroups, columns, gates ? s.gates : 0);
+  return hipGetLastError();
+}
+
+}  // namespace rpx

@@ -3,6 +3,7 @@
 
 #include "common.h"
 #include "mxfp4.h"
+#include "philox.h"
 
 namespace rpx {
 
@@ -323,6 +324,47 @@ struct HeadNormArgs {
 
 hipError_t launch_norm(const NormArgs& args, int kind, bool backward, hipStream_t stream);
 hipError_t launch_head_norm(HeadNormArgs args, int parts, bool backward, hipStream_t stream);
+
+// Dropout (dropout.hip): out = x * scale where kept, else zero; `count` dense
+// elements of 16-byte aligned x and out (which may be the same).
+hipError_t launch_dropout(const void* x, int dtype, int64_t count, const Dropout& d, void* out,
+                          hipStream_t stream);
+
+// The boundary between two blocks (block.hip).
+constexpr int64_t kBlockMaxSize = 8192;
+struct BlockNorm {
+  const void* weight;  // nullptr: no norm
+  const void* bias;    // LayerNorm only
+  int dtype, kind;
+  float eps;
+};
+struct BlockArgs {
+  const void *x, *u;  // [rows, size] of `dtype`
+  const void* gate;   // [rows / rows_per_gate, size] or nullptr
+  int gate_dtype;
+  int64_t rows_per_gate;
+  BlockNorm post, norm;
+  float scale;
+  Dropout drop;
+  int dtype;
+  int64_t rows;
+  int size;
+  void *t, *h;  // h: nullptr without a norm
+};
+struct BlockGradients {
+  BlockArgs forward;  // x and h are not read
+  const void *dt, *dh;  // nullptr: none
+  void *dx, *du, *dgate;  // nullptr: not wanted
+  void* columns[4];  // d weight, d bias, d post weight, d post bias, or nullptr
+  // set by the launcher
+  int64_t group_rows, slices, worker_rows, workers;
+  float *partials, *gate_partials;
+};
+hipError_t launch_block_forward(const BlockArgs& a, hipStream_t stream);
+// Scratch floats of a backward: group_rows is rows_per_gate where the gate's gradient
+// is wanted, else rows; columns: whether any of the weights' are.
+int64_t block_gradients_floats(int64_t rows, int size, int64_t group_rows, bool columns, bool gate);
+hipError_t launch_block_backward(BlockGradients a, float* scratch, hipStream_t stream);
 
 // Conversions of up to kCastMany f32 tensors to bf16 in one launch (cast.hip);
 // 16-byte aligned pointers. `first` is filled by the launcher.

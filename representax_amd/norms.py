@@ -13,12 +13,16 @@ the backward as they are, so they do not change between a call and its backward.
 
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
 import torch.nn.functional as F
 
 from . import _native as nat
-from .ops import (BF16, F32, _aligned, _dtype_code, _on_device, _ptr, _stream, eager_calls,
-                  on_current_device, plain_tensor)
+from .dropout import check_key, dropout_threshold, dropped
+from .ops import (BF16, F32, _aligned, _dtype_code, _on_device, _ptr, _stream, _workspace,
+                  eager_calls, on_current_device, plain_tensor)
 
 _MAX_SIZE = 4096  # elements of a row that the kernels keep in registers
 
@@ -334,4 +338,211 @@ def attention_heads(query_norm: torch.nn.Module, key_norm: torch.nn.Module, q: t
     return q, k, v
 
 
-__all__ = ["LayerNorm", "RMSNorm", "add_norm", "attention_heads"]
+# ---------------------------------------------------------------------------
+# the boundary between two blocks
+# ---------------------------------------------------------------------------
+_BLOCK_MAX_SIZE = 8192  # elements of a row that the lanes of a workgroup keep
+
+
+def _expression_norm(kind: int, v, weight, bias, eps, dtype):
+    """The norm of wide values, its weights taken as the module takes them for
+    values of ``dtype``."""
+
+    if kind == nat.NORM_RMS:
+        return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * weight.to(v.dtype)
+    return F.layer_norm(v, v.shape[-1:], weight.to(dtype).to(v.dtype), bias.to(dtype).to(v.dtype),
+                        eps)
+
+
+def _block_expression(x, u, gate, weight, bias, post_weight, post_bias, key, cfg):
+    """The torch expression of ``block_norm``: what the kernels compute, in
+    float32 (float64 for float64 values) with t and h rounded to the values' type."""
+
+    wide = torch.promote_types(x.dtype, F32)
+    p = u.to(wide)
+    if post_weight is not None:
+        p = _expression_norm(cfg["post_kind"], p, post_weight, post_bias, cfg["post_eps"], x.dtype)
+    if gate is not None:
+        p = gate.to(wide) * p
+    if cfg["threshold"] < 65536:
+        p = dropped(p, key, cfg["threshold"], cfg["site"])
+    t = (x.to(wide) + cfg["scale"] * p).to(x.dtype)
+    if weight is None:
+        return t, None
+    h = _expression_norm(cfg["kind"], t.to(wide), weight, bias, cfg["eps"], x.dtype)
+    return t, h.to(x.dtype)
+
+
+def _norm_struct(weight, bias, kind, eps):
+    if weight is None:
+        return nat.BlockNorm()
+    return nat.BlockNorm(weight.data_ptr(), _ptr(bias), _dtype_code(weight.dtype), kind, eps)
+
+
+def _block_struct(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, shape, dtype, t, h):
+    size = shape[-1]
+    rows = math.prod(shape[:-1])
+    return nat.Block(
+        _ptr(x), _ptr(u), _ptr(gate), cfg["rows_per_gate"],
+        _norm_struct(post_weight, post_bias, cfg["post_kind"], cfg["post_eps"]),
+        _norm_struct(weight, bias, cfg["kind"], cfg["eps"]),
+        _ptr(key) if cfg["threshold"] < 65536 else None, cfg["site"], cfg["threshold"], rows, size,
+        _ptr(t), _ptr(h), _dtype_code(dtype), _dtype_code(dtype if gate is None else gate.dtype),
+        cfg["scale"])
+
+
+def _block_forward(x, u, gate, weight, bias, post_weight, post_bias, key, cfg):
+    device = _on_device(x, u, gate, weight, bias, post_weight, post_bias)
+    t = torch.empty(x.shape, dtype=x.dtype, device=device)
+    h = None if weight is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    block = _block_struct(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, x.shape,
+                          x.dtype, t, h)
+    nat.call("rpx_block_forward", ctypes.byref(block), _stream(device))
+    return t, h
+
+
+class BlockNormFn(torch.autograd.Function):
+    """``(t, h)`` of ``block_norm`` (``(t, None)`` without a norm), with the
+    gradients of everything. The backward reads t and u."""
+
+    @staticmethod
+    def forward(ctx, x, u, gate, weight, bias, post_weight, post_bias, key, cfg):
+        ctx.set_materialize_grads(False)
+        t, h = _block_forward(x, u, gate, weight, bias, post_weight, post_bias, key, cfg)
+        ctx.cfg = cfg
+        # x is read only where the expressions are differentiated instead
+        ctx.save_for_backward(x, u, gate, weight, bias, post_weight, post_bias, key, t)
+        return t, h
+
+    @staticmethod
+    def backward(ctx, dt, dh):
+        *inputs, key, t = ctx.saved_tensors
+        x, u, gate, weight, bias, post_weight, post_bias = inputs
+        wanted = ctx.needs_input_grad[:7]
+        none = (None, None)
+        if dt is None and dh is None:
+            return (None,) * 9
+        if not _kernel_gradients(dt, dh):
+            again = torch.is_grad_enabled()
+            with torch.enable_grad():
+                outs = _block_expression(*inputs, key, ctx.cfg)
+            pairs = [(o, g) for o, g in zip(outs, (dt, dh)) if g is not None]
+            leaves = [v for v, need in zip(inputs, wanted) if need]
+            grads = iter(torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs],
+                                             create_graph=again, allow_unused=True))
+            return (*(next(grads) if need else None for need in wanted), *none)
+        device = _on_device(dt, dh, u)
+        dt = None if dt is None else dt.contiguous()
+        dh = None if dh is None else dh.contiguous()
+        outs = [torch.empty(v.shape, dtype=v.dtype, device=device) if need else None
+                for v, need in zip(inputs, wanted)]
+        block = _block_struct(None, u, gate, weight, bias, post_weight, post_bias, key, ctx.cfg,
+                              u.shape, u.dtype, t, None)
+        grads = nat.BlockGradients(_ptr(dt), _ptr(dh), *(_ptr(o) for o in outs))
+        refs = ctypes.byref(block), ctypes.byref(grads)
+        need = nat.query("rpx_block_backward_workspace", *refs)
+        ws = _workspace(need, device) if need else None
+        nat.call("rpx_block_backward", *refs, _ptr(ws), 0 if ws is None else ws.numel(),
+                 _stream(device))
+        return (*outs, *none)
+
+
+def _rows_per_gate(gate: torch.Tensor, shape) -> int | None:
+    """How many consecutive rows share a row of the gate; None where it does not
+    go by leading axes."""
+
+    lead = shape[:-1]
+    g = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
+    if g[-1] != shape[-1]:
+        return None
+    i = 0
+    while i < len(lead) and g[i] == lead[i]:
+        i += 1
+    return math.prod(lead[i:]) if all(n == 1 for n in g[i:-1]) else None
+
+
+def _parts(norm: torch.nn.Module | None):
+    """(kind, weight, bias, eps) of a norm that the kernels know; None otherwise."""
+
+    if norm is None:
+        return nat.NORM_RMS, None, None, 0.0
+    kind = {LayerNorm: nat.NORM_LAYER, RMSNorm: nat.NORM_RMS}.get(type(norm))
+    if kind is None or not _unhooked(norm, type(norm)):
+        return None
+    return kind, norm.weight, norm.bias if kind == nat.NORM_LAYER else None, norm.eps
+
+
+def _block_kernel(value, update, gate, weights, key) -> bool:
+    size = value.shape[-1]
+    tensors = [value, update, *(w for w in weights if w is not None)]
+    return (value.dtype in (BF16, F32) and update.dtype == value.dtype
+            and 1 <= size <= _BLOCK_MAX_SIZE and value.numel() > 0
+            and all(plain_tensor(t) and t.device == value.device and t.dtype in (BF16, F32)
+                    for t in tensors)
+            and all(w is None or w.shape == (size,) for w in weights)
+            and all(b is None or b.dtype == w.dtype for w, b in (weights[:2], weights[2:]))
+            and (gate is None or (plain_tensor(gate) and gate.device == value.device
+                                  and gate.dtype in (BF16, F32)
+                                  and _rows_per_gate(gate, value.shape) is not None))
+            and (key is None or plain_tensor(key)) and on_current_device(value)
+            and not torch.is_autocast_enabled("cuda"))
+
+
+def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.Tensor, *,
+               post: torch.nn.Module | None = None, gate: torch.Tensor | None = None,
+               scale: float = 1.0, rate: float = 0.0, key: torch.Tensor | None = None,
+               site: int = 0):
+    """The boundary between two blocks: ``t = value + scale * dropout(gate *
+    post(update))``, rounded to the values' type, and ``norm(t)``: ``(t, norm(t))``.
+
+    ``post`` (the norm after the block), ``gate`` and the dropout (``rate`` with a
+    ``key`` and ``site``) may be left out, and ``norm`` may be None (``(t, None)``).
+    ``gate`` broadcasts over ``value [..., D]``: ``[D]``, a row for each of its
+    leading axes (``[B, 1, D]`` over ``[B, S, D]``), or a value for each of its
+    elements. Gradients reach value, update, gate and the norms' weights.
+
+    One pass forward and one backward (with a small second launch where weights or
+    the gate train) for bf16 and float32 rows of up to 8192 values of one type; the
+    backward reads t and update, which must not change in place. Everything else
+    runs the same steps by torch operations."""
+
+    if update.shape != value.shape or value.dim() < 1:
+        raise ValueError(f"update {tuple(update.shape)} must have the shape of value "
+                         f"{tuple(value.shape)}")
+    if gate is not None and torch.broadcast_shapes(gate.shape, value.shape) != value.shape:
+        raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over {tuple(value.shape)}")
+    threshold = dropout_threshold(rate)
+    if threshold < 65536:
+        check_key(key, site, value.device)
+    else:
+        key = None
+    eager = eager_calls()
+    before, after = _parts(norm), _parts(post)
+    if before is None or after is None:
+        # norms that are not ours to fuse: called as they are
+        p = update if post is None else post(update)
+        p = p if gate is None else gate * p
+        wide = torch.promote_types(value.dtype, F32)
+        p = dropped(p.to(wide), key, threshold, int(site))
+        t = (value.to(wide) + scale * p).to(value.dtype)
+        return t, None if norm is None else norm(t)
+    kind, weight, bias, eps = before
+    post_kind, post_weight, post_bias, post_eps = after
+    cfg = {"kind": kind, "eps": eps, "post_kind": post_kind, "post_eps": post_eps,
+           "scale": float(scale), "threshold": threshold, "site": int(site), "rows_per_gate": 1}
+    weights = (weight, bias, post_weight, post_bias)
+    if not (eager and _block_kernel(value, update, gate, weights, key)):
+        return _block_expression(value, update, gate, *weights, key, cfg)
+    value, update = value.contiguous(), update.contiguous()
+    weights = [None if w is None else w.contiguous() for w in weights]
+    if gate is not None:
+        cfg["rows_per_gate"] = _rows_per_gate(gate, value.shape)
+        gate = gate.contiguous()
+    key = None if key is None else key.contiguous()
+    operands = (value, update, gate, *weights, key, cfg)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands[:7]):
+        return BlockNormFn.apply(*operands)
+    return _block_forward(*operands)
+
+
+__all__ = ["LayerNorm", "RMSNorm", "add_norm", "attention_heads", "block_norm"]
