@@ -803,6 +803,61 @@ size_t rpx_block_backward_workspace(const rpx_block* block, const rpx_block_grad
 int rpx_block_backward(const rpx_block* block, const rpx_block_gradients* gradients,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside one INT4 projection: row i of x
+ * takes the adapter e = index[i] of a bank of `adapters`, or none where it is -1:
+ *   y[i] = x[i] W_b^T + bias + s_e (dropout(x[i]) A_e^T) B_e^T
+ * in bf16 with f32 sums (QuantizedLoRALinear.__call__, adapters.py:158-182, for
+ * each row with its own adapter; one rounding of y instead of the reference's
+ * three). h = dropout(x) A_e^T and its gradient are rounded to bf16, also where
+ * they are f32 sums within a call.
+ * ------------------------------------------------------------------------- */
+
+/* The rows of a batch sorted by adapter, for every projection that the batch
+ * goes through: index int32 or int64 [m] (index_bytes 4 or 8). An entry that is
+ * neither -1 nor an adapter's number counts as -1, and rpx_check_device_errors
+ * reports it. At most 2^25 rows and 1024 adapters; plan is 16-byte aligned. */
+size_t rpx_adapter_plan_bytes(int64_t m, int64_t adapters);
+int rpx_adapter_plan(const void* index, int index_bytes, int64_t m, int64_t adapters, void* plan,
+                     size_t plan_bytes, void* stream);
+
+/* x bf16 [m, k]; packed, scale_bits, group_size, bias_bits as in
+ * rpx_int4lora_forward; lora_a bf16 [adapters, rank, k], lora_b bf16 [adapters,
+ * n, rank], scalings f32 [adapters]; rank at most 64, n and k below 2^23; plan
+ * one of m rows and `adapters`. key, site and threshold are the dropout's
+ * (element (i, c) of x is element i * k + c). x, packed, scale_bits, lora_a,
+ * lora_b, y, h and the gradients are dense and 16-byte aligned. */
+typedef struct rpx_bank {
+  const void* x;
+  int64_t m, k;
+  const uint8_t* packed;
+  const uint16_t* scale_bits;
+  int64_t n, group_size;
+  const uint16_t* bias_bits;
+  const void* lora_a;
+  const void* lora_b;
+  const float* scalings;
+  int64_t adapters, rank;
+  const void* plan;
+  size_t plan_bytes;
+  const int64_t* key;
+  int64_t site, threshold;
+} rpx_bank;
+
+/* y bf16 [m, n]; h bf16 [m, rank rounded up to 8] (what the backward reads) or
+ * NULL. Rows of h without an adapter are left as they are. */
+size_t rpx_bank_forward_workspace(const rpx_bank* bank, int h_given);
+int rpx_bank_forward(const rpx_bank* bank, void* y, void* h, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* dx bf16 [m, k], d_a and d_b in the adapters' shapes, f32 or bf16 (each may be
+ * NULL), for the gradient grad bf16 [m, n] of y, from the forward's h. Adapters
+ * without rows get zeros. bias_bits is not read. */
+size_t rpx_bank_backward_workspace(const rpx_bank* bank, int need_x, int need_a, int need_b);
+int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, void* dx, void* d_a,
+                      int a_dtype, void* d_b, int b_dtype, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,14 @@ from .adapters import (
     matched_linear_paths,
     merge_quantized_lora,
 )
+from .bank import (
+    AdapterPlan,
+    QuantizedLoRABank,
+    adapter_plan,
+    adapter_rows,
+    bank_linear,
+    bank_quantized_lora,
+)
 from .components import Linear, MXFP4Linear
 from .config import PrecisionConfig, QuantizedLoRAConfig
 from .dropout import DropoutKeys, dropout
@@ -46,6 +54,7 @@ from .precision import (
 from .sharding import activation_out_sharding, constrain_activation, replicate
 
 __all__ = [
+    "AdapterPlan",
     "DelayedScaling",
     "DropoutKeys",
     "FP32_POLICY",
@@ -55,6 +64,7 @@ __all__ = [
     "MXFP4Matrix",
     "PrecisionConfig",
     "PrecisionPolicy",
+    "QuantizedLoRABank",
     "QuantizedLoRAConfig",
     "QuantizedLoRALinear",
     "RMSNorm",
@@ -62,6 +72,8 @@ __all__ = [
     "activation_out_sharding",
     "active_compute_dtype",
     "active_model_for_compute",
+    "adapter_plan",
+    "adapter_rows",
     "add_norm",
     "apply_quantized_lora",
     "compute_parameter",

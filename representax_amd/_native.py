@@ -195,6 +195,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rpx_mxfp4_gated": (
         _int, [_p, _int, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p, _size, _p]
     ),
+    "rpx_adapter_plan_bytes": (_size, [_i64, _i64]),
+    "rpx_adapter_plan": (_int, [_p, _int, _i64, _i64, _p, _size, _p]),
+    "rpx_bank_forward_workspace": (_size, [_p, _int]),
+    "rpx_bank_forward": (_int, [_p, _p, _p, _p, _size, _p]),
+    "rpx_bank_backward_workspace": (_size, [_p, _int, _int, _int]),
+    "rpx_bank_backward": (_int, [_p, _p, _p, _p, _p, _int, _p, _int, _p, _size, _p]),
     "rpx_dropout": (_int, [_p, _int, _i64, _p, _i64, _i64, _p, _p]),
     "rpx_block_forward": (_int, [_p, _p]),
     "rpx_block_backward_workspace": (_size, [_p, _p]),
@@ -236,6 +242,19 @@ class BlockGradients(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p)
                 for name in ("dt", "dh", "dx", "du", "d_gate", "d_weight", "d_bias",
                              "d_post_weight", "d_post_bias")]
+
+
+class Bank(ctypes.Structure):
+    """``rpx_bank`` of include/representax_amd.h."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("m", ctypes.c_int64), ("k", ctypes.c_int64),
+                ("packed", ctypes.c_void_p), ("scale_bits", ctypes.c_void_p),
+                ("n", ctypes.c_int64), ("group_size", ctypes.c_int64),
+                ("bias_bits", ctypes.c_void_p), ("lora_a", ctypes.c_void_p),
+                ("lora_b", ctypes.c_void_p), ("scalings", ctypes.c_void_p),
+                ("adapters", ctypes.c_int64), ("rank", ctypes.c_int64), ("plan", ctypes.c_void_p),
+                ("plan_bytes", ctypes.c_size_t), ("key", ctypes.c_void_p),
+                ("site", ctypes.c_int64), ("threshold", ctypes.c_int64)]
 
 
 class Mxfp4Part(ctypes.Structure):

@@ -329,9 +329,13 @@ int rpx_check_device_errors(void* stream, uint32_t* flags_out) {
   RPX_HIP(hipStreamSynchronize(s), "rpx_check_device_errors: sync");
   if (bits == 0) return kOk;
   if (flags_out != nullptr) *flags_out = bits;
-  std::string msg = "a kernel's bounded wait expired (its outputs hold NaN):";
+  std::string msg;
+  if (bits & (kDevErrSkinnyWait | kDevErrSkinnyOneWait))
+    msg += "a kernel's bounded wait expired (its outputs hold NaN):";
   if (bits & kDevErrSkinnyWait) msg += " skinny-M forward (one launch, M <= 64): adapter arrivals;";
   if (bits & kDevErrSkinnyOneWait) msg += " skinny-M forward (one launch, M <= 4): adapter partials;";
+  if (bits & kDevErrBankIndex)
+    msg += " adapter plan: an index outside the bank (its row runs without an adapter);";
   set_error(msg);
   return kErrDevice;
 }

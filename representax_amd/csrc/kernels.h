@@ -12,6 +12,7 @@ namespace rpx {
 // wait expired; read and cleared by rpx_check_device_errors.
 constexpr unsigned int kDevErrSkinnyWait = 1u;     // k_skinny: adapter arrivals
 constexpr unsigned int kDevErrSkinnyOneWait = 2u;  // k_skinny_one: adapter partials
+constexpr unsigned int kDevErrBankIndex = 4u;      // k_bank_plan: no adapter of that number
 // This device's word (nullptr if its address could not be resolved).
 unsigned int* device_error_word();
 

@@ -33,6 +33,7 @@ their norm are not finite (``optax.tree.where(finite, proposed, state)``).
 from __future__ import annotations
 
 import math
+from contextlib import ExitStack
 from dataclasses import dataclass
 
 import torch
@@ -41,6 +42,7 @@ from torch.utils.checkpoint import checkpoint
 
 from . import ops
 from .adapters import apply_quantized_lora, lora_parameters
+from .bank import active_adapter_rows, adapter_rows
 from .components import Linear
 from .config import PrecisionConfig
 from .mlp import gelu_mlp, shared_input_projections, swiglu_mlp
@@ -93,15 +95,20 @@ def run_layer(layer: torch.nn.Module, remat: str, *args):
 
     if remat == "full" and torch.is_grad_enabled():
         # the recompute runs inside backward(), outside the caller's precision
-        # context: it re-enters the policy (and compute views) the forward
-        # saw, as jax.checkpoint replays the function traced under them
+        # context: it re-enters the policy (and compute views, and a batch's
+        # adapters) the forward saw, as jax.checkpoint replays the function
+        # traced under them
         policy = active_policy()
         views = active_compute_views()
+        rows = active_adapter_rows()
 
         def layer_under_policy(*inputs):
-            if policy is None:
-                return layer(*inputs)
-            with precision_context(policy), compute_views(views):
+            with ExitStack() as stack:
+                if rows is not None:
+                    stack.enter_context(adapter_rows(*rows))
+                if policy is not None:
+                    stack.enter_context(precision_context(policy))
+                    stack.enter_context(compute_views(views))
                 return layer(*inputs)
 
         return checkpoint(layer_under_policy, *args, use_reentrant=False,
