@@ -19,6 +19,7 @@ enum ActMode : int {
   kActGeluBwd = 3,     // out = v * gelu'(z)
   kActSiluMulBwd = 4,  // out = v * silu(gate) (d up), out2 = v * up * silu'(gate) (d gate)
   kActAddBwd = 5,      // out = v + z: an input gradient added to the one accumulated so far
+  kActBank = 6,        // no transform: the low-rank term is that of each row's own adapter
 };
 
 constexpr float kInvSqrt2 = 0.70710678118654752440f;

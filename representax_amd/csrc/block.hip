@@ -57,7 +57,7 @@ struct RowSum {
   }
 };
 
-constexpr int threads_of(int lanes) { return lanes > 256 ? lanes : 256; }
+constexpr int threads_of(int lanes) { return lanes > 64 ? lanes : 256; }
 
 // Eight weights from column e on; `round` rounds a float32 master to the values'
 // type first (a LayerNorm takes its weights in that type).
@@ -75,126 +75,149 @@ __device__ __forceinline__ void load_weight8(const void* w, int dtype, bool roun
   }
 }
 
+// A workgroup's rows are those it reaches in steps of the grid; the next ones' loads
+// run under these ones' arithmetic, and with one chunk a lane the weights stay in
+// registers.
 template <typename T, int L, int C, bool WHOLE>
 __global__ void __launch_bounds__(threads_of(L)) k_block_fwd(BlockArgs a) {
   constexpr int kRows = threads_of(L) / L;
+  constexpr bool KEEP = C == 1;
   __shared__ float lds[2][2][L / 64 > 0 ? L / 64 : 1];
   RowSum<L, 2> row_sum{lds};
   const int lane = threadIdx.x & (L - 1);
-  const int64_t row = block_of_grid() * kRows + threadIdx.x / L;
-  if (row >= a.rows) return;  // a row of several waves is the whole workgroup
   const int size = a.size;
   const float inv = 1.0f / static_cast<float>(size);
-  const int64_t base = row * size;
-  const T* x = static_cast<const T*>(a.x) + base;
-  const T* u = static_cast<const T*>(a.u) + base;
-  float v[C][8], r[C][8];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / L;
+  const bool has_post = a.post.weight != nullptr, post_layer = a.post.kind == kNormLayer;
+  const bool has_norm = a.norm.weight != nullptr, norm_layer = a.norm.kind == kNormLayer;
+  auto weights = [&](const BlockNorm& n, bool there, bool layer, int c, float* w, float* b) {
     const int e = (c * L + lane) * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[c][i] = r[c][i] = 0.0f;
-    if (e >= size) continue;
-    load_row8<WHOLE>(u + e, size - e, v[c]);
-    load_row8<WHOLE>(x + e, size - e, r[c]);
-  }
-  // mean and 1 / deviation of the row in v, whose entries past the end are zero
-  auto statistics = [&](int kind, float eps, float& mean, float& rstd) {
-    float s[2] = {0.0f, 0.0f};
-    mean = 0.0f;
-    if (kind == kNormLayer) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[0] += v[c][i];
-      row_sum(s);
-      mean = s[0] * inv;
-    }
-    s[0] = s[1] = 0.0f;
+    for (int i = 0; i < 8; ++i) w[i] = b[i] = 0.0f;
+    if (!there || e >= size) return;
+    load_weight8<WHOLE, T>(n.weight, n.dtype, layer, e, size - e, w);
+    if (layer) load_weight8<WHOLE, T>(n.bias, n.dtype, true, e, size - e, b);
+  };
+  Raw8<T> rx[C], ru[C];
+  auto load = [&](int64_t at) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int n = size - (c * L + lane) * 8;
+      const int e = (c * L + lane) * 8;
+      rx[c].zero();
+      ru[c].zero();
+      if (e >= size) continue;
+      load_raw8<WHOLE>(static_cast<const T*>(a.u) + at * size + e, size - e, ru[c]);
+      load_raw8<WHOLE>(static_cast<const T*>(a.x) + at * size + e, size - e, rx[c]);
+    }
+  };
+  if (row < a.rows) load(row);
+  float pw[8], pb[8], nw[8], nb[8], gw[8];
+  if constexpr (KEEP) {
+    weights(a.post, has_post, post_layer, 0, pw, pb);
+    weights(a.norm, has_norm, norm_layer, 0, nw, nb);
+  }
+  auto gate = [&](int64_t at, int c, float* g) {
+    const int e = (c * L + lane) * 8;
+    if (e < size)
+      load_weight8<WHOLE, T>(a.gate, a.gate_dtype, false, (at / a.rows_per_gate) * size + e,
+                             size - e, g);
+  };
+  PhiloxCall call{};
+  const bool drop = a.drop.threshold < 65536u;
+  if (drop) call = philox_call(a.drop);
+  for (; row < a.rows; row += step) {
+    const int64_t base = row * size;
+    if (KEEP && a.gate != nullptr) gate(row, 0, gw);
+    float v[C][8], r[C][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[c][i] - mean;
-        if (i < n) s[0] = __builtin_fmaf(d, d, s[0]);
+    for (int c = 0; c < C; ++c) {
+      ru[c].get(v[c]);
+      rx[c].get(r[c]);
+    }
+    if (row + step < a.rows) load(row + step);
+    // mean and 1 / deviation of the row in v, whose entries past the end are zero
+    auto statistics = [&](bool layer, float eps, float& mean, float& rstd) {
+      float s[2] = {0.0f, 0.0f};
+      mean = 0.0f;
+      if (layer) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[0] += v[c][i];
+        row_sum(s);
+        mean = s[0] * inv;
+      }
+      s[0] = s[1] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int n = size - (c * L + lane) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = v[c][i] - mean;
+          if (WHOLE ? n > 0 : i < n) s[0] = __builtin_fmaf(d, d, s[0]);
+        }
+      }
+      row_sum(s);
+      rstd = rsqrtf(s[0] * inv + eps);
+    };
+    float mean, rstd;
+    if (has_post) {
+      statistics(post_layer, a.post.eps, mean, rstd);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if constexpr (!KEEP) weights(a.post, true, post_layer, c, pw, pb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, pw[i], pb[i]);
       }
     }
-    row_sum(s);
-    rstd = rsqrtf(s[0] * inv + eps);
-  };
-  float mean, rstd;
-  if (a.post.weight != nullptr) {
-    statistics(a.post.kind, a.post.eps, mean, rstd);
-    const bool layer = a.post.kind == kNormLayer;
+    if (a.gate != nullptr) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if constexpr (!KEEP) gate(row, c, gw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] *= gw[i];
+      }
+    }
+    if (drop) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = (c * L + lane) * 8;
+        if (e < size) dropout8<WHOLE>(call, a.drop, base + e, v[c]);
+      }
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int e = (c * L + lane) * 8;
-      if (e >= size) continue;
-      float w[8], b[8];
-      load_weight8<WHOLE, T>(a.post.weight, a.post.dtype, layer, e, size - e, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = 0.0f;
-      if (layer) load_weight8<WHOLE, T>(a.post.bias, a.post.dtype, true, e, size - e, b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, w[i], b[i]);
+      for (int i = 0; i < 8; ++i)
+        v[c][i] = rounded(static_cast<const T*>(nullptr),
+                          i < size - e ? __builtin_fmaf(a.scale, v[c][i], r[c][i]) : 0.0f);
+      if (e < size) store_row8<WHOLE>(static_cast<T*>(a.t) + base + e, size - e, v[c]);
     }
-  }
-  if (a.gate != nullptr) {
-    const int64_t at = (row / a.rows_per_gate) * size;
+    if (!has_norm) continue;
+    statistics(norm_layer, a.norm.eps, mean, rstd);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int e = (c * L + lane) * 8;
-      if (e >= size) continue;
-      float g[8];
-      load_weight8<WHOLE, T>(a.gate, a.gate_dtype, false, at + e, size - e, g);
+      if constexpr (!KEEP) weights(a.norm, true, norm_layer, c, nw, nb);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[c][i] *= g[i];
+      for (int i = 0; i < 8; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, nw[i], nb[i]);
+      if (e < size) store_row8<WHOLE>(static_cast<T*>(a.h) + base + e, size - e, v[c]);
     }
-  }
-  if (a.drop.threshold < 65536u) {
-    const PhiloxCall call = philox_call(a.drop);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int e = (c * L + lane) * 8;
-      if (e < size) dropout8<WHOLE>(call, a.drop, base + e, v[c]);
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int e = (c * L + lane) * 8;
-    if (e >= size) continue;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[c][i] = rounded(static_cast<const T*>(nullptr),
-                        i < size - e ? __builtin_fmaf(a.scale, v[c][i], r[c][i]) : 0.0f);
-    store_row8<WHOLE>(static_cast<T*>(a.t) + base + e, size - e, v[c]);
-  }
-  if (a.norm.weight == nullptr) return;
-  statistics(a.norm.kind, a.norm.eps, mean, rstd);
-  const bool layer = a.norm.kind == kNormLayer;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int e = (c * L + lane) * 8;
-    if (e >= size) continue;
-    float w[8], b[8];
-    load_weight8<WHOLE, T>(a.norm.weight, a.norm.dtype, layer, e, size - e, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = 0.0f;
-    if (layer) load_weight8<WHOLE, T>(a.norm.bias, a.norm.dtype, true, e, size - e, b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, w[i], b[i]);
-    store_row8<WHOLE>(static_cast<T*>(a.h) + base + e, size - e, v[c]);
   }
 }
 
 // What a lane sums over a worker's rows: the columns of its chunks.
 enum Column : int { kWeight = 0, kBias = 1, kPostWeight = 2, kPostBias = 3, kGate = 4, kColumns = 5 };
 
-template <typename T, int L, int C, bool WHOLE>
+// MEAN: one of the norms is a LayerNorm. The next row's loads run under this one's
+// arithmetic; with one chunk a lane its weights stay in registers too.
+template <typename T, int L, int C, bool WHOLE, bool MEAN>
 __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
   constexpr int kThreads = threads_of(L);
   constexpr int kWorkers = kThreads / L;
+  constexpr bool KEEP = C == 1;
   __shared__ float sums[2][4][L / 64 > 0 ? L / 64 : 1];
   // the columns of this workgroup's workers, where there are several
   __shared__ float meet[kWorkers > 1 ? kWorkers * L * C * 8 : 1];
@@ -206,9 +229,10 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
   const float inv = 1.0f / static_cast<float>(size);
   const bool has_norm = f.norm.weight != nullptr && a.dh != nullptr;
   const bool has_post = f.post.weight != nullptr;
-  const bool norm_mean = has_norm && f.norm.kind == kNormLayer;
-  const bool post_mean = has_post && f.post.kind == kNormLayer;
-  const bool read_u = has_post || f.gate != nullptr;
+  const bool has_gate = f.gate != nullptr;
+  const bool norm_mean = MEAN && has_norm && f.norm.kind == kNormLayer;
+  const bool post_mean = MEAN && has_post && f.post.kind == kNormLayer;
+  const bool read_u = has_post || has_gate;
   float acc[kColumns][C][8];
 #pragma unroll
   for (int k = 0; k < kColumns; ++k)
@@ -234,24 +258,76 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
   const bool drop = f.drop.threshold < 65536u;
   if (drop) call = philox_call(f.drop);
   int64_t group_left = a.slices > 0 ? end - row : a.group_rows;  // rows to the group's end
+
+  auto norm_weight = [&](int c, float* w) {
+    const int e = (c * L + lane) * 8;
+    load_weight8<WHOLE, T>(f.norm.weight, f.norm.dtype, norm_mean, e, size - e, w);
+  };
+  auto post_weight = [&](int c, float* w, float* b) {
+    const int e = (c * L + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = 1.0f;
+      b[i] = 0.0f;
+    }
+    if (!has_post) return;
+    load_weight8<WHOLE, T>(f.post.weight, f.post.dtype, post_mean, e, size - e, w);
+    if (post_mean) load_weight8<WHOLE, T>(f.post.bias, f.post.dtype, true, e, size - e, b);
+  };
+  auto gate_weight = [&](int c, int64_t at, float* k) {
+    const int e = (c * L + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = 1.0f;
+    if (has_gate) load_weight8<WHOLE, T>(f.gate, f.gate_dtype, false, at + e, size - e, k);
+  };
+  float nw[8], pw[8], pb[8], gw[8];
+  int64_t gate_row = -1;
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nw[i] = 0.0f;
+    if (lane * 8 < size) {
+      if (has_norm) norm_weight(0, nw);
+      post_weight(0, pw, pb);
+    }
+  }
+  Raw8<T> rt[C], ru[C], rg[C], rd[C];
+  auto load = [&](int64_t at) {
+    const int64_t base = at * size;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int e = (c * L + lane) * 8;
+      rt[c].zero();
+      ru[c].zero();
+      rg[c].zero();
+      rd[c].zero();
+      if (e >= size) continue;
+      if (has_norm) {
+        load_raw8<WHOLE>(static_cast<const T*>(f.t) + base + e, size - e, rt[c]);
+        load_raw8<WHOLE>(static_cast<const T*>(a.dh) + base + e, size - e, rg[c]);
+      }
+      if (a.dt != nullptr) load_raw8<WHOLE>(static_cast<const T*>(a.dt) + base + e, size - e, rd[c]);
+      if (read_u) load_raw8<WHOLE>(static_cast<const T*>(f.u) + base + e, size - e, ru[c]);
+    }
+  };
+  if (row < end) load(row);
   for (; row < end; ++row) {
     const int64_t base = row * size;
     float t[C][8], u[C][8], g[C][8], d[C][8];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int e = (c * L + lane) * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[c][i] = u[c][i] = g[c][i] = d[c][i] = 0.0f;
-      if (e >= size) continue;
-      if (has_norm) {
-        load_row8<WHOLE>(static_cast<const T*>(f.t) + base + e, size - e, t[c]);
-        load_row8<WHOLE>(static_cast<const T*>(a.dh) + base + e, size - e, g[c]);
-      }
-      if (a.dt != nullptr) load_row8<WHOLE>(static_cast<const T*>(a.dt) + base + e, size - e, d[c]);
-      if (read_u) load_row8<WHOLE>(static_cast<const T*>(f.u) + base + e, size - e, u[c]);
+      rt[c].get(t[c]);
+      ru[c].get(u[c]);
+      rg[c].get(g[c]);
+      rd[c].get(d[c]);
+    }
+    if (row + 1 < end) load(row + 1);
+    const int64_t gate_at = has_gate ? (row / f.rows_per_gate) * size : 0;
+    if constexpr (KEEP) {
+      if (gate_at != gate_row && lane * 8 < size) gate_weight(0, gate_at, gw);
+      gate_row = gate_at;
     }
     float mean = 0.0f, u_mean = 0.0f;
-    if (norm_mean || post_mean) {
+    if constexpr (MEAN) {
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -271,23 +347,25 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
     for (int c = 0; c < C; ++c) {
       const int e = (c * L + lane) * 8;
       if (e >= size) continue;
-      float w[8];
-      if (has_norm)
-        load_weight8<WHOLE, T>(f.norm.weight, f.norm.dtype, norm_mean, e, size - e, w);
+      if constexpr (!KEEP) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) nw[i] = 0.0f;
+        if (has_norm) norm_weight(c, nw);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (!WHOLE && i >= size - e) continue;
         t[c][i] -= mean;
         s[0] = __builtin_fmaf(t[c][i], t[c][i], s[0]);
-        const float du = u[c][i] - u_mean;
-        s[1] = __builtin_fmaf(du, du, s[1]);
-        const float gw = has_norm ? g[c][i] * w[i] : 0.0f;
-        s[2] += gw;
-        s[3] = __builtin_fmaf(gw, t[c][i], s[3]);
+        u[c][i] -= u_mean;
+        s[1] = __builtin_fmaf(u[c][i], u[c][i], s[1]);
+        const float v = g[c][i] * nw[i];
+        s[2] += v;
+        s[3] = __builtin_fmaf(v, t[c][i], s[3]);
       }
     }
-    if (has_norm || has_post) row_sum(s);
-    const float u_rstd = rsqrtf(s[1] * inv + f.post.eps);
+    row_sum(s);
+    const float u_rstd = has_post ? rsqrtf(s[1] * inv + f.post.eps) : 1.0f;
     if (has_norm) {
       const float rstd = rsqrtf(s[0] * inv + f.norm.eps);
       const float mg = norm_mean ? s[2] * inv : 0.0f;
@@ -296,20 +374,18 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
       for (int c = 0; c < C; ++c) {
         const int e = (c * L + lane) * 8;
         if (e >= size) continue;
-        float w[8];
-        load_weight8<WHOLE, T>(f.norm.weight, f.norm.dtype, norm_mean, e, size - e, w);
+        if constexpr (!KEEP) norm_weight(c, nw);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float n = t[c][i] * rstd;
           acc[kWeight][c][i] = __builtin_fmaf(g[c][i], n, acc[kWeight][c][i]);
-          acc[kBias][c][i] += g[c][i];
-          d[c][i] = __builtin_fmaf(rstd, g[c][i] * w[i] - mg - n * mgt, d[c][i]);
+          if constexpr (MEAN) acc[kBias][c][i] += g[c][i];
+          d[c][i] = __builtin_fmaf(rstd, g[c][i] * nw[i] - mg - n * mgt, d[c][i]);
         }
       }
     }
     // d is the gradient of t, and of x; from here on d becomes that of p, with
     // u the normalised row
-    const int64_t gate_at = f.gate == nullptr ? 0 : (row / f.rows_per_gate) * size;
     float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -317,39 +393,30 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
       if (e >= size) continue;
       if (a.dx != nullptr) store_row8<WHOLE>(static_cast<T*>(a.dx) + base + e, size - e, d[c]);
       if (drop) dropout8<WHOLE>(call, f.drop, base + e, d[c]);
-      float w[8], b[8], k[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = k[i] = 1.0f;
-        b[i] = 0.0f;
+      if constexpr (!KEEP) {
+        post_weight(c, pw, pb);
+        gate_weight(c, gate_at, gw);
       }
-      if (has_post) {
-        load_weight8<WHOLE, T>(f.post.weight, f.post.dtype, post_mean, e, size - e, w);
-        if (post_mean) load_weight8<WHOLE, T>(f.post.bias, f.post.dtype, true, e, size - e, b);
-      }
-      if (f.gate != nullptr)
-        load_weight8<WHOLE, T>(f.gate, f.gate_dtype, false, gate_at + e, size - e, k);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (!WHOLE && i >= size - e) continue;
-        if (has_post) u[c][i] = (u[c][i] - u_mean) * u_rstd;
+        u[c][i] *= u_rstd;
         d[c][i] *= f.scale;
-        acc[kGate][c][i] = __builtin_fmaf(d[c][i], __builtin_fmaf(u[c][i], w[i], b[i]),
-                                          acc[kGate][c][i]);
-        d[c][i] *= k[i];
+        const float p = MEAN ? __builtin_fmaf(u[c][i], pw[i], pb[i]) : u[c][i] * pw[i];
+        acc[kGate][c][i] = __builtin_fmaf(d[c][i], p, acc[kGate][c][i]);
+        d[c][i] *= gw[i];
         acc[kPostWeight][c][i] = __builtin_fmaf(d[c][i], u[c][i], acc[kPostWeight][c][i]);
-        acc[kPostBias][c][i] += d[c][i];
-        d[c][i] *= w[i];
+        if constexpr (MEAN) acc[kPostBias][c][i] += d[c][i];
+        d[c][i] *= pw[i];
         q[0] += d[c][i];
         q[1] = __builtin_fmaf(d[c][i], u[c][i], q[1]);
       }
     }
-    float md = 0.0f, mdu = 0.0f, factor = 1.0f;
+    float md = 0.0f, mdu = 0.0f;
     if (has_post) {
       row_sum(q);
       md = post_mean ? q[0] * inv : 0.0f;
       mdu = q[1] * inv;
-      factor = u_rstd;
     }
     if (a.du != nullptr) {
 #pragma unroll
@@ -358,7 +425,7 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
         if (e >= size) continue;
         if (has_post) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[c][i] = factor * (d[c][i] - md - u[c][i] * mdu);
+          for (int i = 0; i < 8; ++i) d[c][i] = u_rstd * (d[c][i] - md - u[c][i] * mdu);
         }
         store_row8<WHOLE>(static_cast<T*>(a.du) + base + e, size - e, d[c]);
       }
@@ -412,8 +479,9 @@ __global__ void __launch_bounds__(threads_of(L)) k_block_bwd(BlockGradients a) {
   }
 }
 
-// Joins the partials of one column and of 64 of its entries: 16 lanes of 4
-// entries by 16 rows of partials, then over LDS in row order.
+// Joins the partials of one column for 16 of its entries: 64 lanes an entry, each
+// over every 64th partial, then over LDS, in a fixed order.
+constexpr int kJoin = 16;
 struct BlockJoin {
   const float* partials;
   int64_t count, stride;  // partials and floats from one to the next
@@ -422,27 +490,35 @@ struct BlockJoin {
 };
 
 __device__ __forceinline__ void join(const BlockJoin& j, int size, int64_t e0) {
-  __shared__ float lds[16][64];
-  const int64_t e = e0 + (threadIdx.x & 63);
-  const int part = threadIdx.x >> 6;
+  __shared__ float lds[64][17], half[16][17];
+  const int c = threadIdx.x & 15;
+  const int part = threadIdx.x >> 4;
+  const int64_t e = e0 + c;
   float s = 0.0f;
   if (e < size) {
     int64_t p = part;
-    for (; p + 48 < j.count; p += 64) {
-      float v[4];
+    for (; p + 64 * 7 < j.count; p += 64 * 8) {
+      float v[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = j.partials[(p + 16 * i) * j.stride + e];
+      for (int i = 0; i < 8; ++i) v[i] = j.partials[(p + 64 * i) * j.stride + e];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s += v[i];
+      for (int i = 0; i < 8; ++i) s += v[i];
     }
-    for (; p < j.count; p += 16) s += j.partials[p * j.stride + e];
+    for (; p < j.count; p += 64) s += j.partials[p * j.stride + e];
   }
-  lds[part][threadIdx.x & 63] = s;
+  lds[part][c] = s;
+  __syncthreads();
+  if (part < 16) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += lds[4 * part + i][c];
+    half[part][c] = s;
+  }
   __syncthreads();
   if (part == 0 && e < size) {
     s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += lds[i][threadIdx.x & 63];
+    for (int i = 0; i < 16; ++i) s += half[i][c];
     if (j.dtype == kBF16)
       store1(static_cast<Bf16*>(j.out) + e, s);
     else
@@ -450,55 +526,101 @@ __device__ __forceinline__ void join(const BlockJoin& j, int size, int64_t e0) {
   }
 }
 
+// The same for a group's slices, of which there are few: a thread an entry.
+__device__ __forceinline__ void join_few(const BlockJoin& j, int size, int64_t e) {
+  if (e >= size) return;
+  float s = 0.0f;
+  int64_t p = 0;
+  for (; p + 7 < j.count; p += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = j.partials[(p + i) * j.stride + e];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i];
+  }
+  for (; p < j.count; ++p) s += j.partials[p * j.stride + e];
+  if (j.dtype == kBF16)
+    store1(static_cast<Bf16*>(j.out) + e, s);
+  else
+    store1(static_cast<float*>(j.out) + e, s);
+}
+
+// Gates of more slices than this join as the columns do (one gate for all rows).
+constexpr int64_t kFewSlices = 64;
+
+__host__ __device__ inline int64_t join_blocks(int size, bool few) {
+  return few ? ceil_div(size, 1024) : ceil_div(size, kJoin);
+}
+
 __global__ void __launch_bounds__(1024) k_block_join(BlockGradients a, int64_t workgroups,
                                                      int columns, int64_t gates) {
   const int size = a.forward.size;
-  const int64_t blocks = ceil_div(size, 64);
-  const int64_t job = block_of_grid() / blocks;
-  const int64_t e0 = (block_of_grid() % blocks) * 64;
-  if (job < columns) {
+  const int64_t blocks = join_blocks(size, false);
+  int64_t block = block_of_grid();
+  if (block < columns * blocks) {
+    const int64_t job = block / blocks;
     int k = 0;
     for (int64_t left = job; k < kGate; ++k)
       if (a.columns[k] != nullptr && left-- == 0) break;
     const int dtype = k < kPostWeight ? a.forward.norm.dtype : a.forward.post.dtype;
     join(BlockJoin{a.partials + k * size, workgroups, static_cast<int64_t>(kGate) * size,
                    a.columns[k], dtype},
-         size, e0);
-  } else if (job - columns < gates) {
-    const int64_t g = job - columns;
-    const size_t bytes = a.forward.gate_dtype == kBF16 ? 2 : 4;
-    join(BlockJoin{a.gate_partials + g * a.slices * size, a.slices, size,
-                   static_cast<uint8_t*>(a.dgate) + g * size * bytes, a.forward.gate_dtype},
-         size, e0);
+         size, (block % blocks) * kJoin);
+    return;
   }
+  block -= columns * blocks;
+  const bool few = a.slices <= kFewSlices;
+  const int64_t gate_blocks = join_blocks(size, few);
+  const int64_t g = block / gate_blocks;
+  if (g >= gates) return;
+  const size_t bytes = a.forward.gate_dtype == kBF16 ? 2 : 4;
+  const BlockJoin j{a.gate_partials + g * a.slices * size, a.slices, size,
+                    static_cast<uint8_t*>(a.dgate) + g * size * bytes, a.forward.gate_dtype};
+  if (few)
+    join_few(j, size, (block % gate_blocks) * 1024 + threadIdx.x);
+  else
+    join(j, size, (block % gate_blocks) * kJoin);
 }
 
-struct Shape {
-  int lanes, workers;  // lanes a row, rows a workgroup
-};
+// Lanes a row and chunks a lane: a wave while one chunk a lane holds the row, then more
+// waves, so that rows, weights and the backward's five sums a column stay in registers.
+#define RPX_BLOCK_SIZES(CALL) \
+  if (size <= 128) {          \
+    CALL(16, 1);              \
+  } else if (size <= 512) {   \
+    CALL(64, 1);              \
+  } else if (size <= 1024) {  \
+    CALL(128, 1);             \
+  } else if (size <= 2048) {  \
+    CALL(256, 1);             \
+  } else if (size <= 4096) {  \
+    CALL(512, 1);             \
+  } else {                    \
+    CALL(512, 2);             \
+  }
 
-Shape shape_of(int size) {
-  if (size <= 128) return {16, 16};
-  if (size <= 1024) return {64, 4};
-  if (size <= 4096) return {256, 1};
-  return {512, 1};
+// The split of the rows over workers: as many waves as run at a time (registers allow
+// two a SIMD with a LayerNorm's sums, three without), one round of them.
+constexpr int64_t kMeanWaves = 256 * 8, kWaves = 256 * 12;
+
+bool has_mean(const BlockArgs& f) {
+  return (f.norm.weight != nullptr && f.norm.kind == kNormLayer) ||
+         (f.post.weight != nullptr && f.post.kind == kNormLayer);
 }
 
-#define RPX_BLOCK_SIZES(CALL)            \
-  if (size <= 128) CALL(16, 1);          \
-  else if (size <= 512) CALL(64, 1);     \
-  else if (size <= 1024) CALL(64, 2);    \
-  else if (size <= 2048) CALL(256, 1);   \
-  else if (size <= 4096) CALL(256, 2);   \
-  else CALL(512, 2);
+constexpr int64_t kForwardWaves = 256 * 20;  // that run at a time
 
 template <typename T, bool WHOLE>
 void forward(const BlockArgs& a, hipStream_t stream) {
   const int size = a.size;
 #define RPX_FWD(L, C)                                                                      \
-  hipLaunchKernelGGL((k_block_fwd<T, L, C, WHOLE>),                                        \
-                     grid_of(ceil_div(a.rows, threads_of(L) / L)), dim3(threads_of(L)), 0, \
-                     stream, a)
+  {                                                                                        \
+    const int64_t all = ceil_div(a.rows, threads_of(L) / L);                               \
+    const int64_t most = kForwardWaves * 64 / threads_of(L);                               \
+    hipLaunchKernelGGL((k_block_fwd<T, L, C, WHOLE>),                                      \
+                       dim3(static_cast<unsigned>(all < most ? all : most)),               \
+                       dim3(threads_of(L)), 0, stream, a);                                 \
+  }
   RPX_BLOCK_SIZES(RPX_FWD)
 #undef RPX_FWD
 }
@@ -506,28 +628,26 @@ void forward(const BlockArgs& a, hipStream_t stream) {
 template <typename T, bool WHOLE>
 void backward(const BlockGradients& a, int64_t workgroups, hipStream_t stream) {
   const int size = a.forward.size;
-#define RPX_BWD(L, C)                                                                           \
-  hipLaunchKernelGGL((k_block_bwd<T, L, C, WHOLE>), grid_of(workgroups), dim3(threads_of(L)), 0, \
-                     stream, a)
+  const bool mean = has_mean(a.forward);
+#define RPX_BWD(L, C)                                                                         \
+  if (mean)                                                                                   \
+    hipLaunchKernelGGL((k_block_bwd<T, L, C, WHOLE, true>), grid_of(workgroups),              \
+                       dim3(threads_of(L)), 0, stream, a);                                    \
+  else                                                                                        \
+    hipLaunchKernelGGL((k_block_bwd<T, L, C, WHOLE, false>), grid_of(workgroups),             \
+                       dim3(threads_of(L)), 0, stream, a)
   RPX_BLOCK_SIZES(RPX_BWD)
 #undef RPX_BWD
 }
-
-// The split of the rows over workers. Each has at least kMinRows rows, so that the
-// columns' partials stay a small part of what is read, and at most about kWorkgroups
-// workgroups' worth are made (four workgroups of four waves on each of 256 CUs run
-// at a time).
-constexpr int64_t kMinRows = 4;
-constexpr int64_t kWorkgroups = 1024;
 
 struct Split {
   int64_t slices, worker_rows, workers, workgroups, gates;
 };
 
-Split split_of(int64_t rows, int size, int64_t group_rows) {
-  const Shape shape = shape_of(size);
-  int64_t want = ceil_div(rows, kWorkgroups * shape.workers);
-  want = want < kMinRows ? kMinRows : want;
+Split split_of(int64_t rows, int size, int64_t group_rows, bool mean) {
+  const int at_once = size <= 128 ? 16 : (size <= 512 ? 4 : 1);  // rows of a workgroup
+  const int waves = size <= 512 ? 4 : (size <= 1024 ? 2 : (size <= 2048 ? 4 : 8));
+  const int64_t want = ceil_div(rows, (mean ? kMeanWaves : kWaves) / waves * at_once);
   Split s{};
   const int64_t groups = group_rows > 0 ? ceil_div(rows, group_rows) : 0;
   if (groups == 0) return s;
@@ -540,15 +660,16 @@ Split split_of(int64_t rows, int size, int64_t group_rows) {
     s.worker_rows = (want / group_rows) * group_rows;
     s.workers = ceil_div(rows, s.worker_rows);
   }
-  s.workgroups = ceil_div(s.workers, shape.workers);
+  s.workgroups = ceil_div(s.workers, at_once);
   s.gates = s.slices > 1 ? groups : 0;
   return s;
 }
 
 }  // namespace
 
-int64_t block_gradients_floats(int64_t rows, int size, int64_t group_rows, bool columns, bool gate) {
-  const Split s = split_of(rows, size, group_rows);
+int64_t block_gradients_floats(const BlockArgs& f, bool columns, bool gate) {
+  const int size = f.size;
+  const Split s = split_of(f.rows, size, gate ? f.rows_per_gate : f.rows, has_mean(f));
   return (columns ? s.workgroups * kGate * size : 0) +
          (gate && s.gates > 0 ? s.workers * size : 0);
 }
@@ -567,7 +688,7 @@ hipError_t launch_block_backward(BlockGradients a, float* scratch, hipStream_t s
   const BlockArgs& f = a.forward;
   if (f.rows <= 0) return hipSuccess;
   a.group_rows = a.dgate != nullptr ? f.rows_per_gate : f.rows;
-  const Split s = split_of(f.rows, f.size, a.group_rows);
+  const Split s = split_of(f.rows, f.size, a.group_rows, has_mean(f));
   a.slices = s.slices;
   a.worker_rows = s.worker_rows;
   a.workers = s.workers;
@@ -585,9 +706,11 @@ hipError_t launch_block_backward(BlockGradients a, float* scratch, hipStream_t s
           : backward<float, false>(a, s.workgroups, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || (columns == 0 && !gates)) return e;
-  const int64_t jobs = columns + (gates ? s.gates : 0);
-  hipLaunchKernelGGL(k_block_join, grid_of(jobs * ceil_div(f.size, 64)), dim3(1024), 0, stream, a,
-                     s.workgroups, columns, gates ? s.gates : 0);
+  const int64_t gate_count = gates ? s.gates : 0;
+  const int64_t blocks = columns * join_blocks(f.size, false) +
+                         gate_count * join_blocks(f.size, s.slices <= kFewSlices);
+  hipLaunchKernelGGL(k_block_join, grid_of(blocks), dim3(1024), 0, stream, a, s.workgroups, columns,
+                     gate_count);
   return hipGetLastError();
 }
 

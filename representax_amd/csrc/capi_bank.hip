@@ -3,6 +3,7 @@
 #include <type_traits>
 
 #include "../../include/representax_amd.h"
+#include "act.h"
 #include "bank.h"
 #include "capi.h"
 #include "tuning.h"
@@ -94,8 +95,26 @@ BankSkinny skinny_of(const Bank& b, uint16_t* y, uint16_t* h) {
 
 bool skinny(const Bank& b) { return bank_skinny_ok(b.m, b.k, b.w.n_groups, b.w.group); }
 
+// The adapters' term of a product over `columns` columns, added in its epilogue.
+LowRankEpilogue bank_epilogue(const Bank& b, const uint16_t* h, const uint16_t* rows,
+                              int64_t columns) {
+  LowRankEpilogue epi;
+  epi.rows = rows;
+  epi.rows_sn = b.rank;
+  epi.rows_sj = 1;
+  epi.cols = h;
+  epi.cols_sm = bank_rank_stride(b.rank);
+  epi.cols_sj = 1;
+  epi.rank = b.rank;
+  epi.act = kActBank;
+  epi.adapter_rows = b.plan.rows;
+  epi.adapter_scales = b.scalings;
+  epi.adapter_stride = columns * b.rank;
+  return epi;
+}
+
 int wide_tile(const Bank& b) {
-  return wide_plan(b.m, b.n, b.k, tune(kTuneInt4Tile), 0, true);
+  return wide_plan(b.m, b.n, b.k, tune(kTuneInt4Tile), kActBank, true);
 }
 
 struct ForwardScratch {
@@ -229,18 +248,25 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
   RPX_HIP(launch_bank_shrink(b.x, b.k, b.a, b.rank, b.plan, b.drop, h, nullptr, 1, st),
           "rpx_bank_forward: down-projections");
   if (fast(b)) {
-    LowRankEpilogue epi;
-    epi.bias = b.bias;
+    // Ranks that the wide tiles' epilogue does not take (above 32, or no multiple of 8)
+    // follow the base product in a pass of their own there.
+    LowRankEpilogue epi = bank_epilogue(b, h, b.b, b.n), base;
+    epi.bias = base.bias = b.bias;
     const int tile = wide_tile(b);
-    if (tile != 0 && wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi)) {
+    const bool fused = wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi);
+    if (tile != 0 &&
+        (fused || wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, base))) {
       RPX_HIP(launch_int4_dequant(b.w.packed, b.w.scales, s.weight, b.n, b.k, b.w.packed_cols,
                                   b.w.n_groups, b.w.group, st),
               "rpx_bank_forward: weight");
-      RPX_HIP(launch_gemm_wide(tile, b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi, st),
-              "rpx_bank_forward: base product");
+      RPX_HIP(launch_gemm_wide(tile, b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n,
+                               fused ? epi : base, st),
+              "rpx_bank_forward: product");
+      if (fused) return kOk;
     } else {
       RPX_HIP(launch_gemm_int4(b.x, b.k, b.w, b.m, b.n, b.k, y, b.n, epi, st),
-              "rpx_bank_forward: base product");
+              "rpx_bank_forward: product");
+      return kOk;
     }
   } else {
     RPX_HIP(launch_generic_gemm(b.x, kBF16, b.k, 1, nullptr, kBF16, 0, 0, &b.w, false, b.m, b.n, b.k,
@@ -290,6 +316,7 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
             "rpx_bank_backward: dh");
   }
   if (b.m > 0 && dx_wanted) {
+    bool expand = true;
     if (fast(b)) {
       const int64_t n64 = ceil_div(b.n, 64) * 64;
       const uint16_t* ga = g;
@@ -303,16 +330,22 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
       RPX_HIP(launch_int4_dequant_t(b.w.packed, b.w.scales, s.wt, b.n, b.k, b.w.packed_cols,
                                     b.w.n_groups, b.w.group, n64, st),
               "rpx_bank_backward: weight");
-      RPX_HIP(launch_gemm_bf16(ga, n64, s.wt, n64, b.m, b.k, n64, dx, b.k, LowRankEpilogue{}, st),
+      // the dropout's mask lies on the adapters' part alone: a pass after the product
+      const bool fused = b.drop.threshold >= 65536u;
+      const LowRankEpilogue epi =
+          fused ? bank_epilogue(b, s.dh, s.at, b.k) : LowRankEpilogue{};
+      RPX_HIP(launch_gemm_bf16(ga, n64, s.wt, n64, b.m, b.k, n64, dx, b.k, epi, st),
               "rpx_bank_backward: dx");
+      expand = !fused;
     } else {
       RPX_HIP(launch_generic_gemm(g, kBF16, b.n, 1, nullptr, kBF16, 0, 0, &b.w, true, b.m, b.k, b.n,
                                   s.base, st),
               "rpx_bank_backward: dx");
       RPX_HIP(launch_bank_store(s.base, nullptr, b.m, b.k, dx, st), "rpx_bank_backward: dx");
     }
-    RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, dx, st),
-            "rpx_bank_backward: dx of the adapters");
+    if (expand)
+      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, dx, st),
+              "rpx_bank_backward: dx of the adapters");
   }
   if (da || db) {
     const BankAdapterGradients p{b.x, g, static_cast<const uint16_t*>(h), s.dh, b.k, b.n, b.rank,

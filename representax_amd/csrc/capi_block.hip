@@ -87,9 +87,7 @@ bool any_column(const rpx_block_gradients& g) {
 
 size_t block_backward_bytes(const BlockArgs& a, const rpx_block_gradients& g) {
   return sizeof(float) *
-         static_cast<size_t>(block_gradients_floats(
-             a.rows, a.size, g.d_gate != nullptr ? a.rows_per_gate : a.rows, any_column(g),
-             g.d_gate != nullptr));
+         static_cast<size_t>(block_gradients_floats(a, any_column(g), g.d_gate != nullptr));
 }
 
 }  // namespace

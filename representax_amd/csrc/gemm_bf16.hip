@@ -517,19 +517,21 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   // idx = it * NT + tid of the tile) before the last K slice so that their
   // latency overlaps it; that slice runs outside the loop so the loop itself
   // does not carry their registers.
-  constexpr bool AUX_OPS = ACT != kActNone && ACT != kActGeluFwd;
+  constexpr bool BANK = ACT == kActBank;
+  constexpr bool PLAIN = ACT == kActNone || BANK;  // the rounded outputs are the results
+  constexpr bool AUX_OPS = !PLAIN && ACT != kActGeluFwd;
   constexpr bool TWO_OPS = ACT == kActSiluMulBwd;
   constexpr bool PREFETCH = AUX_OPS && !INT4 && !I4L;
   constexpr int SEG_ROW = BN / 8;  // 8-column segments per tile row
   constexpr int SEG_ITS = BM * SEG_ROW / NT;
-  static_assert(ACT == kActNone || (BM * SEG_ROW) % NT == 0,
+  static_assert(PLAIN || (BM * SEG_ROW) % NT == 0,
                 "tile segments must split evenly over the threads");
   const uintptr_t act_ptrs = reinterpret_cast<uintptr_t>(out) |
                              reinterpret_cast<uintptr_t>(epi.aux) |
                              reinterpret_cast<uintptr_t>(epi.aux2) |
                              reinterpret_cast<uintptr_t>(epi.pre_out) |
                              reinterpret_cast<uintptr_t>(epi.out2);
-  const bool act_vec = ACT != kActNone && m0 + BM <= M && n0 + BN <= N && (ldc & 7) == 0 &&
+  const bool act_vec = !PLAIN && m0 + BM <= M && n0 + BN <= N && (ldc & 7) == 0 &&
                        (act_ptrs & 15) == 0;
   u32x4_t av[AUX_OPS ? SEG_ITS : 1], a2v[TWO_OPS ? SEG_ITS : 1];
   auto load_aux = [&]() {
@@ -927,7 +929,59 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       ((reinterpret_cast<uintptr_t>(epi.rows) | reinterpret_cast<uintptr_t>(epi.cols)) & 15) == 0;
   bf16x8_t cf[kMaxJB][FM];
   bf16x8_t rf[kMaxJB][FN];
-  if (jblocks > 0) {
+  if constexpr (BANK) {
+    // Lane's row frow of each 32-row block has its own adapter: for each adapter of a
+    // block's rows in turn, t = C R_e^T for all of them, added (scaled, in f32) where the
+    // row is its: by a branch, so that no value of another adapter reaches a row. R_e's
+    // fragments stay while the adapter does; the rows of a request are consecutive, so
+    // most blocks have one.
+    int cur = -1;
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      const int64_t m = mw + fm * 32 + frow;
+      const int mine = m < M ? epi.adapter_rows[m] : -1;
+#pragma unroll
+      for (int jb = 0; jb < kMaxJB; ++jb) {
+        const int64_t jl = jb * 16 + half * 8;
+        cf[jb][fm] = load8_j(epi.cols + (mine >= 0 ? m * epi.cols_sm + jl : 0), 1,
+                             mine >= 0 ? valid8(epi.rank, jl) : 0);
+      }
+      uint32_t left = static_cast<uint32_t>(__ballot(mine >= 0));
+      while (left != 0) {
+        const int e = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+        if (e != cur) {
+          cur = e;
+          const uint16_t* rows = epi.rows + e * epi.adapter_stride;
+#pragma unroll
+          for (int jb = 0; jb < kMaxJB; ++jb) {
+            const int64_t jl = jb * 16 + half * 8;
+#pragma unroll
+            for (int fn = 0; fn < FN; ++fn) {
+              const int64_t n = nw + fn * 32 + frow;
+              rf[jb][fn] = load8_j(rows + (n < N ? n * epi.rows_sn + jl : 0), 1,
+                                   n < N ? valid8(epi.rank, jl) : 0);
+            }
+          }
+        }
+        const float scale = epi.adapter_scales[e];
+#pragma unroll
+        for (int fn = 0; fn < FN; ++fn) {
+          f32x16_t t;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) t[v] = 0.0f;
+#pragma unroll
+          for (int jb = 0; jb < kMaxJB; ++jb)
+            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[jb][fn], cf[jb][fm], t, 0, 0, 0);
+          if (mine == e) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+              acc[fn][fm][v] = __builtin_fmaf(scale, t[v], acc[fn][fm][v]);
+          }
+        }
+        left &= ~static_cast<uint32_t>(__ballot(mine == e));
+      }
+    }
+  } else if (jblocks > 0) {
 #pragma unroll
     for (int jb = 0; jb < kMaxJB; ++jb) {
       if (jb >= jblocks) break;
@@ -986,14 +1040,14 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       for (int v = 0; v < 16; ++v) t[v] = 0.0f;
 #pragma unroll
       for (int jb = 0; jb < kMaxJB; ++jb) {
-        if (jb >= jblocks) break;
+        if (BANK || jb >= jblocks) break;
         t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[jb][fn], cf[jb][fm], t, 0, 0, 0);
       }
 #pragma unroll
       for (int v = 0; v < 16; v += 2) {
         float a0 = acc[fn][fm][v];
         float a1 = acc[fn][fm][v + 1];
-        if (jblocks > 0) {
+        if (!BANK && jblocks > 0) {
           round2(a0, a1);
           float t0 = t[v];
           float t1 = t[v + 1];
@@ -1005,7 +1059,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
           a1 += t1;
         }
         if (has_bias) {
-          round2(a0, a1);
+          if constexpr (!BANK) round2(a0, a1);
           a0 += bias4[fn][v / 4][v % 4];
           a1 += bias4[fn][v / 4][v % 4 + 1];
         }
@@ -1015,7 +1069,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   }
 
   constexpr int P = BN * 2 + 16;  // LDS row pitch of the staged tile
-  if constexpr (ACT == kActNone) {
+  if constexpr (PLAIN) {
     const bool vec_out = (ldc & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     if constexpr (BM * P <= LDS_ALL) {
       wait_sync<0>();  // every wave is done reading the pipeline stages
@@ -1269,6 +1323,9 @@ hipError_t run_gemm_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
   run_gemm_act<BM, BN, WM, WN, NS, WPE, BK, JB, ACT>(a, lda, b, ldb, w, m, n, k, out, ldc, epi, stream)
   if (epi.act == kActNone) return RPX_RUN_ACT(kActNone);
   if constexpr (JB > 0 && !(BM == 256 && BN == 256)) {
+    if constexpr (BK != kBInt4T) {
+      if (epi.act == kActBank) return RPX_RUN_ACT(kActBank);
+    }
     if constexpr (BK == kBInt4 || BK == kBInt4L) {
       if (epi.act == kActGeluFwd) return RPX_RUN_ACT(kActGeluFwd);
       if (epi.act == kActSiluMulFwd) return RPX_RUN_ACT(kActSiluMulFwd);

@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   // bf16(t) * scale is already a bf16 value when scale = 2^k, k >= 0
   const bool scale_exact = (sbits & 0x807FFFFFu) == 0 && sbits >= 0x3F800000u && sbits < 0x7F800000u;
   // (the backward epilogues carry no bias)
-  const bool has_bias = (ACT == kActNone || ACT == kActGeluFwd || ACT == kActSiluMulFwd) && epi.bias != nullptr;
+  constexpr bool BANK = ACT == kActBank;
+  const bool has_bias = (ACT == kActNone || BANK || ACT == kActGeluFwd || ACT == kActSiluMulFwd) && epi.bias != nullptr;
   const bool bias_vec = (reinterpret_cast<uintptr_t>(epi.bias) & 7) == 0;
   constexpr int kJB = JB > 0 ? JB : 1;
 
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     band_tile(t, tiles_m, tiles_n, band, tm, tn);
     const int mw = tm * BM + wm * TM;
     const int nw = tn * BN + wn * TN;
-    constexpr bool AUX = ACT != kActNone && ACT != kActGeluFwd;
+    constexpr bool AUX = ACT != kActNone && ACT != kActGeluFwd && !BANK;
     constexpr bool TWO = ACT == kActSiluMulBwd;
     constexpr bool FWD = ACT == kActGeluFwd || ACT == kActSiluMulFwd;
     // The epilogue's operands: the LoRA fragments of the wave's columns and
@@ -259,14 +260,49 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
       }
     };
+    // BANK: the rows' adapters, and the adapter whose fragments rf holds, at first that
+    // of the sub-tile's first row
+    int mine[BANK ? FM : 1];
+    int cur = 0;
+    if constexpr (BANK) {
+      cur = epi.adapter_rows[mw < M ? mw : M - 1];
+      cur = cur < 0 ? 0 : cur;
+    }
     auto load_cols = [&](int fm) {
       int r = mw + fm * 32 + (el & 31);
       r = r < M ? r : M - 1;
       const uint32_t at = static_cast<uint32_t>(r) * static_cast<uint32_t>(2 * epi.cols_sm) + (el >> 5) * 16;
+      if constexpr (BANK) {
+        // ranks of 8 and 24 end in the middle of a 16-rank block
+#pragma unroll
+        for (int jb = 0; jb < kJB; ++jb) {
+          const bool in = jb * 16 + (el >> 5) * 8 < epi.rank;
+          const u32x4_t v = *reinterpret_cast<const u32x4_t*>(
+              reinterpret_cast<const uint8_t*>(epi.cols) + at + (in ? jb * 32 : -(el >> 5) * 16));
+          cf[fm & 1][jb] = as_bf16x8(in ? v : u32x4_t{0u, 0u, 0u, 0u});
+        }
+        return;
+      }
 #pragma unroll
       for (int jb = 0; jb < kJB; ++jb)
         cf[fm & 1][jb] = *reinterpret_cast<const bf16x8_t*>(
             reinterpret_cast<const uint8_t*>(epi.cols) + at + jb * 32);
+    };
+    auto load_rows = [&](int e) {
+      const uint8_t* rows = reinterpret_cast<const uint8_t*>(epi.rows + e * epi.adapter_stride);
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) {
+        int n = nw + fn * 32 + (el & 31);
+        n = n < N ? n : N - 1;
+        const uint32_t at = static_cast<uint32_t>(n) * static_cast<uint32_t>(2 * epi.rows_sn);
+#pragma unroll
+        for (int jb = 0; jb < kJB; ++jb) {
+          const int j = jb * 16 + (el >> 5) * 8;
+          const u32x4_t v =
+              *reinterpret_cast<const u32x4_t*>(rows + at + (j < epi.rank ? 2 * j : 0));
+          rf[jb][fn] = as_bf16x8(j < epi.rank ? v : u32x4_t{0u, 0u, 0u, 0u});
+        }
+      }
     };
     constexpr bool kBiasEarly = BN == 192;  // 256 columns leave no registers for it
     u32x2_t bias2[FN][4];  // bf16 pairs of columns 32 fn + 8 vg + 4 half + [0, 4)
@@ -287,7 +323,16 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto load_epilogue = [&]() {
       asm volatile("" : "+v"(el));
       if (kBiasEarly && has_bias) load_bias();
-      if constexpr (JB > 0) {
+      if constexpr (BANK) {
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm) {
+          const int r = mw + fm * 32 + (el & 31);
+          mine[fm] = epi.adapter_rows[r < M ? r : M - 1];
+          if (r >= M) mine[fm] = -1;
+        }
+        load_rows(cur);
+        load_cols(0);
+      } else if constexpr (JB > 0) {
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn) {
           int n = nw + fn * 32 + (el & 31);
@@ -358,13 +403,42 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       if constexpr (JB > 0) {
         if (fm + 1 < FM) load_cols(fm + 1);
       }
+      if constexpr (BANK) {
+        // each adapter of the block's rows in turn: its term for all of them, kept where
+        // the row is its, by a branch (no value of another adapter reaches a row)
+        uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
+        while (left != 0) {
+          const int e = __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left));
+          if (e != cur) {
+            cur = e;
+            load_rows(e);
+          }
+          const float scale = epi.adapter_scales[e];
+#pragma unroll
+          for (int fn = 0; fn < FN; ++fn) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16_t lr;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) lr[v] = 0.0f;
+#pragma unroll
+            for (int jb = 0; jb < kJB; ++jb)
+              lr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[jb][fn], cf[fm & 1][jb], lr, 0, 0, 0);
+            if (mine[fm] == e) {
+#pragma unroll
+              for (int v = 0; v < 16; ++v)
+                acc[fn][fm][v] = __builtin_fmaf(scale, lr[v], acc[fn][fm][v]);
+            }
+          }
+          left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e));
+        }
+      }
 #pragma unroll
       for (int fn = 0; fn < FN; ++fn) {
         __builtin_amdgcn_sched_barrier(0);
         f32x16_t lr;
 #pragma unroll
         for (int v = 0; v < 16; ++v) lr[v] = 0.0f;
-        if constexpr (JB > 0) {
+        if constexpr (JB > 0 && !BANK) {
 #pragma unroll
           for (int jb = 0; jb < kJB; ++jb)
             lr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[jb][fn], cf[fm & 1][jb], lr, 0, 0, 0);
@@ -384,7 +458,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
               const int v = 4 * vg + 2 * p;
               float a0 = acc[fn][fm][v];
               float a1 = acc[fn][fm][v + 1];
-              if constexpr (JB > 0) {
+              if constexpr (JB > 0 && !BANK) {
                 round2(a0, a1);
                 float t0 = lr[v];
                 float t1 = lr[v + 1];
@@ -396,7 +470,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
                 a1 += t1;
               }
               if constexpr (BIAS) {
-                round2(a0, a1);
+                if constexpr (!BANK) round2(a0, a1);
                 a0 += bf16lo_to_f32(bias2[fn][vg][p]);
                 a1 += bf16hi_to_f32(bias2[fn][vg][p]);
               }
@@ -431,7 +505,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + r * (TN * 2) +
                                                             (stage_chunk<CPR>(r, c) << 4));
         u32x4_t o = v, o2{0u, 0u, 0u, 0u};
-        if constexpr (ACT != kActNone) {
+        if constexpr (ACT != kActNone && !BANK) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float x0 = 0.0f, x1 = 0.0f, y0 = 0.0f, y1 = 0.0f, s0 = 0.0f, s1 = 0.0f;
@@ -533,6 +607,7 @@ hipError_t run_wide_act(const uint16_t* a, int64_t lda, const uint16_t* b, int64
     case kActGeluBwd: return RPX_WIDE(kActGeluBwd);
     case kActSiluMulBwd: return RPX_WIDE(kActSiluMulBwd);
     case kActAddBwd: return RPX_WIDE(kActAddBwd);
+    case kActBank: return RPX_WIDE(kActBank);
     default: return hipErrorInvalidValue;
   }
 #undef RPX_WIDE
@@ -544,7 +619,7 @@ hipError_t run_wide_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
                        const LowRankEpilogue& epi, hipStream_t stream) {
   if (epi.rank == 0 && epi.act == kActNone)
     return run_wide<BN, WM, WN, 0, kActNone>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
-  if (epi.rank == 16)
+  if (epi.rank <= 16)
     return run_wide_act<BN, WM, WN, 1>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
   return run_wide_act<BN, WM, WN, 2>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
 }
@@ -575,7 +650,7 @@ int wide_plan(int64_t m, int64_t n, int64_t k, int knob, int act, bool dequant) 
   const double t192 = first + ceil_div(tm * ceil_div(n, 192), 256) * (1.30 * s + 5.0);
   const double other =
       10.0 + 2.0 * static_cast<double>(m) * n * k / 0.93e9 * (1.0 + 200.0 / static_cast<double>(k));
-  const double margin = act == kActNone || act == kActAddBwd ? 0.95 : 0.90;
+  const double margin = act == kActNone || act == kActAddBwd || act == kActBank ? 0.95 : 0.90;
   const double t = t256 <= t192 ? t256 : t192;
   if (t >= margin * other) return 0;
   return t256 <= t192 ? kTileWide_256x256 : kTileWide_256x192;
@@ -599,7 +674,8 @@ bool wide_gemm_ok(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb
          ldc % 8 == 0 && (ptrs & 15) == 0 && m * lda * 2 < lim && n * ldb * 2 < lim &&
          m < (int64_t{1} << 31) - 256 && n < (int64_t{1} << 31) - 256 &&
          ceil_div(m, 256) * ceil_div(n, 192) < (int64_t{1} << 30) &&
-         (epi.rank == 16 || epi.rank == 32 || (epi.rank == 0 && epi.act == kActNone)) &&
+         (epi.rank == 16 || epi.rank == 32 || (epi.rank == 0 && epi.act == kActNone) ||
+          (epi.act == kActBank && (epi.rank == 8 || epi.rank == 24) && epi.adapter_stride % 8 == 0)) &&
          (epi.rank == 0 || (epi.rows_sj == 1 && epi.cols_sj == 1 && epi.rows_sn % 8 == 0 &&
                             epi.cols_sm % 8 == 0 && m * epi.cols_sm * 2 < lim &&
                             n * epi.rows_sn * 2 < lim)) &&

@@ -52,6 +52,12 @@ struct LowRankEpilogue {
   const uint16_t* aux2 = nullptr;  // up (SiLU-mul backward)
   uint16_t* pre_out = nullptr;     // v itself (forward modes)
   uint16_t* out2 = nullptr;        // d gate (SiLU-mul backward)
+  // kActBank: row m's R is rows + adapter_rows[m] * adapter_stride (none where it is
+  // negative) and its scale adapter_scales[adapter_rows[m]], and the sum of product,
+  // term and bias is rounded once. C's columns past the rank are not read.
+  const int32_t* adapter_rows = nullptr;
+  const float* adapter_scales = nullptr;
+  int64_t adapter_stride = 0;
 };
 
 // Packed INT4 operand [N, K] (row n holds ceil(K/2) bytes).
@@ -362,9 +368,9 @@ struct BlockGradients {
   float *partials, *gate_partials;
 };
 hipError_t launch_block_forward(const BlockArgs& a, hipStream_t stream);
-// Scratch floats of a backward: group_rows is rows_per_gate where the gate's gradient
-// is wanted, else rows; columns: whether any of the weights' are.
-int64_t block_gradients_floats(int64_t rows, int size, int64_t group_rows, bool columns, bool gate);
+// Scratch floats of a backward that wants any of the weights' gradients (columns) or the
+// gate's.
+int64_t block_gradients_floats(const BlockArgs& f, bool columns, bool gate);
 hipError_t launch_block_backward(BlockGradients a, float* scratch, hipStream_t stream);
 
 // Conversions of up to kCastMany f32 tensors to bf16 in one launch (cast.hip);
