@@ -26,7 +26,7 @@ from .bank import (
 )
 from .components import Linear, MXFP4Linear
 from .config import PrecisionConfig, QuantizedLoRAConfig
-from .dropout import DropoutKeys, dropout
+from .philox import DropoutKeys, dropout
 from .mlp import gelu_mlp, shared_input_projections, swiglu_mlp
 from .mxfp4 import (
     MXFP4Matrix,

@@ -374,3 +374,49 @@ def call(name: str, *args) -> None:
 
 def query(name: str, *args) -> int:
     return int(getattr(load(), name)(*args))
+
+
+def block_of(fields: tuple) -> Block:
+    """The fields of an ``rpx_block`` as the fast binding takes them (its norms' five in
+    their places), as the structure."""
+
+    return Block(*fields[:4], BlockNorm(*fields[4:9]), BlockNorm(*fields[9:14]), *fields[14:])
+
+
+def block_forward(fields: tuple, stream) -> None:
+    binding = fast()
+    if binding is not None:
+        check(binding.block_forward(*fields, stream))
+    else:
+        call("rpx_block_forward", ctypes.byref(block_of(fields)), stream)
+
+
+def block_backward_workspace(fields: tuple, gradients: tuple) -> int:
+    binding = fast()
+    if binding is not None:
+        return binding.block_backward_workspace(*fields, *gradients)
+    return query("rpx_block_backward_workspace", ctypes.byref(block_of(fields)),
+                 ctypes.byref(BlockGradients(*gradients)))
+
+
+def block_backward(fields: tuple, gradients: tuple, workspace, nbytes: int, stream) -> None:
+    binding = fast()
+    if binding is not None:
+        check(binding.block_backward(*fields, *gradients, workspace, nbytes, stream))
+    else:
+        call("rpx_block_backward", ctypes.byref(block_of(fields)),
+             ctypes.byref(BlockGradients(*gradients)), workspace, nbytes, stream)
+
+
+def bank_call(name: str, fields: tuple, *args) -> int:
+    """``rpx_bank_<name>`` of a bank's fields: a size, or a checked status."""
+
+    binding = fast()
+    if binding is not None:
+        out = getattr(binding, "bank_" + name)(*fields, *args)
+    else:
+        out = getattr(load(), "rpx_bank_" + name)(ctypes.byref(Bank(*fields)), *args)
+    if name.endswith("_workspace"):
+        return int(out)
+    check(out)
+    return 0

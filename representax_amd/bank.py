@@ -30,7 +30,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from .adapters import QuantizedLoRALinear, _set_module
-from .dropout import check_key, dropout_threshold
+from .philox import check_key, dropout_threshold
 from .ops import (BF16, F32, _aligned, _as, _check_extent, _dtype_code, _on_device, _ptr, _stream,
                   _u16, _workspace, cast_many, group_arg, on_current_device)
 from .precision import active_compute_dtype, activation_inputs, compute_operands
@@ -41,10 +41,13 @@ MAX_RANK = 64
 MAX_ROWS = 1 << 25
 
 
+_HERE = nullcontext()
+
+
 def _on(device: torch.device, t: torch.Tensor):
     """Launches go to the current device: make it the tensors'."""
 
-    return nullcontext() if on_current_device(t) else torch.cuda.device(device)
+    return _HERE if on_current_device(t) else torch.cuda.device(device)
 
 
 class AdapterPlan:
@@ -92,27 +95,29 @@ def adapter_plan(index, adapters: int, device=None) -> AdapterPlan:
     return AdapterPlan(buffer, rows, adapters)
 
 
-def _bank_struct(x2d, packed, scale_bits, bias, a, b, scalings, plan, key, cfg):
+def _bank_fields(x2d, packed, scale_bits, bias, a, b, scalings, plan, key, cfg):
+    """The fields of an ``rpx_bank``."""
+
     m, k = x2d.shape
     e, r, _ = a.shape
-    return nat.Bank(_ptr(x2d), m, k, _ptr(packed), _ptr(scale_bits), packed.shape[0], cfg["group"],
-                    _ptr(bias), _ptr(a), _ptr(b), _ptr(scalings), e, r, _ptr(plan), plan.numel(),
-                    _ptr(key), cfg["site"], cfg["threshold"])
+    return (x2d.data_ptr(), m, k, packed.data_ptr(), scale_bits.data_ptr(), packed.shape[0],
+            cfg["group"], _ptr(bias), a.data_ptr(), b.data_ptr(), scalings.data_ptr(), e, r,
+            plan.data_ptr(), plan.numel(), _ptr(key), cfg["site"], cfg["threshold"])
 
 
 def _forward(x2d, a, b, packed, scale_bits, bias, scalings, plan, key, cfg, need_h):
     device = _on_device(x2d, a, b, packed, scale_bits, bias, scalings, plan, key)
-    bank = _bank_struct(x2d, packed, scale_bits, bias, a, b, scalings, plan, key, cfg)
-    y = torch.empty((x2d.shape[0], packed.shape[0]), dtype=BF16, device=device)
+    fields = _bank_fields(x2d, packed, scale_bits, bias, a, b, scalings, plan, key, cfg)
+    m = x2d.shape[0]
+    y = torch.empty((m, packed.shape[0]), dtype=BF16, device=device)
     h = None
     if need_h:
-        h = torch.empty((x2d.shape[0], -(-a.shape[1] // 8) * 8), dtype=BF16, device=device)
+        h = torch.empty((m, -(-a.shape[1] // 8) * 8), dtype=BF16, device=device)
     with _on(device, x2d):
-        ref = ctypes.byref(bank)
-        nbytes = nat.query("rpx_bank_forward_workspace", ref, int(need_h))
-        ws = _workspace(nbytes, device) if nbytes else None
-        nat.call("rpx_bank_forward", ref, _ptr(y), _ptr(h), _ptr(ws),
-                 0 if ws is None else ws.numel(), _stream(device))
+        stream = _stream(device)
+        nbytes = nat.bank_call("forward_workspace", fields, int(need_h))
+        ws = _workspace(nbytes, device, stream) if nbytes else None
+        nat.bank_call("forward", fields, y.data_ptr(), _ptr(h), _ptr(ws), nbytes, stream)
     return y, h
 
 
@@ -135,17 +140,17 @@ class BankLinearFn(torch.autograd.Function):
         need_x, need_a, need_b = ctx.needs_input_grad[:3]
         grad = _aligned(_as(grad, BF16))
         device = _on_device(grad, x2d)
-        bank = _bank_struct(x2d, packed, scale_bits, None, a, b, scalings, plan, key, ctx.cfg)
+        fields = _bank_fields(x2d, packed, scale_bits, None, a, b, scalings, plan, key, ctx.cfg)
         dx = torch.empty_like(x2d) if need_x else None
         d_a = torch.empty(a.shape, dtype=ctx.dtypes[0], device=device) if need_a else None
         d_b = torch.empty(b.shape, dtype=ctx.dtypes[1], device=device) if need_b else None
         with _on(device, x2d):
-            ref = ctypes.byref(bank)
-            nbytes = nat.query("rpx_bank_backward_workspace", ref, need_x, need_a, need_b)
-            ws = _workspace(nbytes, device) if nbytes else None
-            nat.call("rpx_bank_backward", ref, _ptr(grad), _ptr(h), _ptr(dx), _ptr(d_a),
-                     _dtype_code(ctx.dtypes[0]), _ptr(d_b), _dtype_code(ctx.dtypes[1]), _ptr(ws),
-                     0 if ws is None else ws.numel(), _stream(device))
+            stream = _stream(device)
+            nbytes = nat.bank_call("backward_workspace", fields, need_x, need_a, need_b)
+            ws = _workspace(nbytes, device, stream) if nbytes else None
+            nat.bank_call("backward", fields, grad.data_ptr(), h.data_ptr(), _ptr(dx), _ptr(d_a),
+                          _dtype_code(ctx.dtypes[0]), _ptr(d_b), _dtype_code(ctx.dtypes[1]),
+                          _ptr(ws), nbytes, stream)
         return dx, d_a, d_b, None, None, None, None, None, None, None
 
 

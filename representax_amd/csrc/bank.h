@@ -10,7 +10,7 @@ namespace rpx {
 
 constexpr int64_t kBankMaxAdapters = 1024;
 constexpr int64_t kBankMaxRank = 64;
-constexpr int64_t kBankSkinnyRows = 64;
+constexpr int64_t kBankSkinnyRows = 256;
 
 // Rows of one adapter: positions [pos, end) of the plan's order.
 struct BankTile {
@@ -40,12 +40,10 @@ hipError_t launch_bank_plan(const void* index, int index_bytes, const BankPlan& 
 constexpr int64_t bank_rank_stride(int64_t rank) { return (rank + 7) / 8 * 8; }
 
 // h[m, j] = sum_k drop(x[m, k]) w[adapter(m), j, k] for the rows that have an
-// adapter; w [adapters, rank, k]. With splits > 1 f32 partial sums go to
-// partials [splits][m][stride] instead of bf16 to h [m, stride].
-int bank_shrink_splits(int64_t m, int64_t k);
+// adapter, bf16 [m, stride]; w [adapters, rank, k].
 hipError_t launch_bank_shrink(const uint16_t* x, int64_t k, const uint16_t* w, int64_t rank,
                               const BankPlan& plan, const Dropout& drop, uint16_t* h,
-                              float* partials, int splits, hipStream_t stream);
+                              hipStream_t stream);
 // out[m, n] += s[adapter(m)] drop(sum_j h[m, j] w[adapter(m), n, j]); w [adapters, n, rank].
 hipError_t launch_bank_expand(const uint16_t* h, const uint16_t* w, int64_t rank, int64_t n,
                               const float* scalings, const BankPlan& plan, const Dropout& drop,
@@ -94,9 +92,9 @@ struct BankSkinny {
   uint16_t* y;
   uint16_t* h;  // [m, stride] or nullptr
 };
-bool bank_skinny_ok(int64_t m, int64_t k, int64_t n_groups, int64_t group);
-// Whether the call needs no partial sums of h ([bank_shrink_splits][m][stride] f32).
-bool bank_skinny_fused(const BankSkinny& p, const Dropout& drop);
+bool bank_skinny_ok(int64_t m, int64_t n, int64_t k, int64_t n_groups, int64_t group);
+// f32 partial sums of a call.
+int64_t bank_skinny_floats(const BankSkinny& p, const Dropout& drop);
 hipError_t launch_bank_skinny(const BankSkinny& p, const Dropout& drop, float* partials,
                               hipStream_t stream);
 

@@ -203,8 +203,7 @@ __global__ void __launch_bounds__(kPlanThreads)
 
 // ---------------------------------------------------------------------------
 // h = drop(x) A_e^T, and dh = g B_e with B_e^T in A_e's place: one workgroup per
-// tile of 16 G rows of an adapter (and per slice of K), whose four waves take
-// interleaved 32-deep steps of K and meet in LDS.
+// 16 G rows of an adapter, whose four waves take a quarter of K each and meet in LDS.
 // ---------------------------------------------------------------------------
 struct ShrinkArgs {
   const uint16_t* x;
@@ -214,19 +213,19 @@ struct ShrinkArgs {
   int stride;  // columns of the output
   const BankTile* tiles;
   const int32_t* order;
-  int64_t m;
   Dropout drop;
   uint16_t* h;
-  float* partials;
-  int64_t slice;  // of K, a multiple of 128
+  int parts;      // workgroups a tile
 };
 
 // DROP: 0 none, 1 dropout. WHOLE: K is a multiple of eight.
 template <int RB, int G, int U, bool DROP, bool WHOLE>
 __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
   __shared__ float red[3][G][RB][4][64];
-  const BankTile tile = a.tiles[blockIdx.x];
-  if (tile.adapter < 0) return;
+  BankTile tile = a.tiles[blockIdx.x / a.parts];
+  tile.pos += 16 * G * (blockIdx.x % a.parts);
+  if (tile.pos >= tile.end) return;  // an unused record has no rows
+  tile.end = tile.pos + 16 * G < tile.end ? tile.pos + 16 * G : tile.end;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int koff = (lane >> 4) * 8;
@@ -238,8 +237,6 @@ __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
     row[gi] = a.order[p < tile.end ? p : tile.pos];
   }
   const uint16_t* w = a.w + static_cast<int64_t>(tile.adapter) * a.rank * a.k;
-  const int64_t k0 = blockIdx.y * a.slice;
-  const int64_t k1 = k0 + a.slice < a.k ? k0 + a.slice : a.k;
   PhiloxCall call{};
   if constexpr (DROP) call = philox_call(a.drop);
   f32x4_t acc[G][RB];
@@ -247,13 +244,19 @@ __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
   for (int gi = 0; gi < G; ++gi)
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) acc[gi][rb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int64_t kb = k0 + wave * 32; kb < k1; kb += 128 * U) {
+  // a wave takes a quarter of K, whole lines at a time: interleaved steps of the waves
+  // put all workgroups on the same columns of rows a multiple of 4 KB apart, and so on
+  // few memory channels (16384 rows of 6144: 63 us interleaved, 57 so)
+  const int64_t span = ceil_div(a.k, 4 * 64) * 64;
+  const int64_t w0 = wave * span;
+  const int64_t w1 = w0 + span < a.k ? w0 + span : a.k;
+  for (int64_t kb = w0; kb < w1; kb += 32 * U) {
     u32x4_t xv[U][G], wv[U][RB];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t kc = kb + 128 * u + koff;
-      const int kv = clamp8(k1 - kc);
-      const int64_t at = kv > 0 ? kc : k0;  // nothing is read past a row's end
+      const int64_t kc = kb + 32 * u + koff;
+      const int kv = clamp8(w1 - kc);
+      const int64_t at = kv > 0 ? kc : 0;  // nothing is read past a row's end
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) xv[u][gi] = bits8<WHOLE>(a.x + row[gi] * a.k + at, kv);
 #pragma unroll
@@ -268,7 +271,8 @@ __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
       for (int gi = 0; gi < G; ++gi) {
         u32x4_t v = xv[u][gi];
         if constexpr (DROP)
-          v = masked8<WHOLE>(v, call, a.drop.threshold, row[gi] * a.k + kb + 128 * u + koff);
+          v = masked8<WHOLE>(v, call, a.drop.threshold,
+                             row[gi] * a.k + kb + 32 * u + koff);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
           acc[gi][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(v), as_bf16x8(wv[u][rb]),
@@ -302,10 +306,7 @@ __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
         const float s = jj < a.rank ? scale * (acc[gi][rb][v] + red[0][gi][rb][v][lane] +
                                                red[1][gi][rb][v][lane] + red[2][gi][rb][v][lane])
                                     : 0.0f;
-        if (a.partials != nullptr)
-          a.partials[(blockIdx.y * a.m + out_row) * a.stride + jj] = s;
-        else
-          a.h[out_row * a.stride + jj] = f32_to_bf16(s);
+        a.h[out_row * a.stride + jj] = f32_to_bf16(s);
       }
     }
 }
@@ -396,12 +397,13 @@ __global__ void __launch_bounds__(256) k_bank_expand(ExpandArgs a) {
 
 // ---------------------------------------------------------------------------
 // The adapters' gradients: a workgroup takes a chunk of one adapter's rows and
-// 128 columns of x (or g), [128 rows x 128 columns] at a time into LDS, from where
+// 128 columns of x (or g), [64 rows x 128 columns] at a time into LDS, from where
 // transposing reads feed the matrix cores; the chunks' f32 sums are joined in
 // order by a second launch, which also scales and rounds them.
 // ---------------------------------------------------------------------------
-constexpr int kGradRows = 128;
+constexpr int kGradRows = 64;
 constexpr int kGradColumns = 128;
+constexpr int kMaxChunk = 256;
 
 struct GradArgs {
   const uint16_t* x;  // [m, p]
@@ -444,6 +446,7 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
   constexpr int PH = 16 * RB + 8;
   __shared__ __align__(16) uint16_t sx[kGradRows * PX];
   __shared__ __align__(16) uint16_t sh[kGradRows * PH];
+  __shared__ int32_t rows[kMaxChunk];
   const BankTile chunk = a.chunks[blockIdx.y];
   if (chunk.adapter < 0) return;
   const int which = static_cast<int>(blockIdx.x) < a.part[0].blocks ? 0 : 1;
@@ -456,6 +459,10 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
   constexpr int HV = (kGradRows * (2 * RB) + 255) / 256;
   PhiloxCall call{};
   if constexpr (DROP) call = philox_call(a.drop);
+  // the chunk's rows, once: what is loaded per step does not wait for its addresses
+  const int count = chunk.end - chunk.pos;
+  for (int i = tid; i < count; i += 256) rows[i] = a.order[chunk.pos + i];
+  __syncthreads();
   u32x4_t xr[XV], hr[HV];
   auto load = [&](int base) {
 #pragma unroll
@@ -463,8 +470,8 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
       const int v = tid + 256 * u;
       const int pos = base + v / 16;
       const int64_t c = p0 + (v % 16) * 8;
-      const bool in = pos < chunk.end;
-      const int64_t row = a.order[in ? pos : chunk.pos];
+      const bool in = pos < count;
+      const int64_t row = rows[in ? pos : 0];
       const int valid = in ? clamp8(g.p - c) : 0;
       xr[u] = bits8<WHOLE>(g.x + row * g.p + (valid > 0 ? c : 0), valid);
       if constexpr (DROP) {
@@ -476,8 +483,8 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
       const int v = tid + 256 * u;
       const int pos = base + v / (2 * RB);
       const int c = (v % (2 * RB)) * 8;
-      const bool in = v < kGradRows * 2 * RB && pos < chunk.end;
-      const int64_t row = a.order[in ? pos : chunk.pos];
+      const bool in = v < kGradRows * 2 * RB && pos < count;
+      const int64_t row = rows[in ? pos : 0];
       const int valid = in ? clamp8(a.stride - c) : 0;
       hr[u] = bits8<true>(g.h + row * a.stride + (valid > 0 ? c : 0), valid);
     }
@@ -487,8 +494,8 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) acc[i][rb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  load(chunk.pos);
-  for (int base = chunk.pos; base < chunk.end; base += kGradRows) {
+  load(0);
+  for (int base = 0; base < count; base += kGradRows) {
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < XV; ++u) {
@@ -502,8 +509,8 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
         *reinterpret_cast<u32x4_t*>(&sh[(v / (2 * RB)) * PH + (v % (2 * RB)) * 8]) = hr[u];
     }
     __syncthreads();
-    if (base + kGradRows < chunk.end) load(base + kGradRows);
-    const int left = chunk.end - base;
+    if (base + kGradRows < count) load(base + kGradRows);
+    const int left = count - base;
     const int steps = left >= kGradRows ? kGradRows / 32 : (left + 31) / 32;
     for (int st = 0; st < steps; ++st) {
       bf16x8_t hf[RB];
@@ -656,10 +663,12 @@ BankPlan bank_plan(void* buffer, int64_t m, int64_t adapters) {
   p.adapters = adapters;
   // Rows of a tile: 64 share the fragments of an adapter's weights between four
   // groups of 16 rows; few rows take tiles of 16, for more workgroups. A chunk of
-  // the gradients' sums is a sixteenth of the rows, between 128 and 1024.
+  // the gradients' sums is a sixteenth of the rows, 64 to 256 of them (16384 rows of
+  // 2048 and 6144, with the joining launch: 72 us with chunks of 256, 79 with 512, 95
+  // with 1024).
   p.tile = m >= 4096 ? 64 : 16;
   int64_t chunk = ceil_div(ceil_div(m, 16), kGradRows) * kGradRows;
-  p.chunk = static_cast<int>(chunk < kGradRows ? kGradRows : (chunk > 1024 ? 1024 : chunk));
+  p.chunk = static_cast<int>(chunk < kGradRows ? kGradRows : (chunk > kMaxChunk ? kMaxChunk : chunk));
   const int64_t used = adapters < m ? adapters : m;
   p.tile_count = m / p.tile + used;
   p.chunk_count = m / p.chunk + used;
@@ -698,26 +707,21 @@ hipError_t launch_bank_plan(const void* index, int index_bytes, const BankPlan& 
   return hipGetLastError();
 }
 
-int bank_shrink_splits(int64_t m, int64_t k) {
-  // few rows: slices of K fill the chip; their partial sums are added by what reads h
-  if (m > kBankSkinnyRows) return 1;
-  const int64_t s = k / 512;
-  return static_cast<int>(s < 1 ? 1 : (s > 8 ? 8 : s));
-}
-
 hipError_t launch_bank_shrink(const uint16_t* x, int64_t k, const uint16_t* w, int64_t rank,
                               const BankPlan& plan, const Dropout& dropout, uint16_t* h,
-                              float* partials, int splits, hipStream_t stream) {
+                              hipStream_t stream) {
   if (plan.m <= 0) return hipSuccess;
   ShrinkArgs a{x, k, w, static_cast<int>(rank), static_cast<int>(bank_rank_stride(rank)),
-               plan.tiles, plan.order, plan.m, dropout, h, partials,
-               ceil_div(ceil_div(k, splits), 128) * 128};
-  const dim3 grid(static_cast<unsigned>(plan.tile_count),
-                  static_cast<unsigned>(ceil_div(k, a.slice)));
+               plan.tiles, plan.order, dropout, h, 1};
   const bool drop = drops(dropout), whole = k % 8 == 0;
   const int rb = rank_blocks(rank);
+  // tiles of 64 rows: ranks to 16 in halves, twice the workgroups (16384 rows of 6144:
+  // 56 us against 57, of 2048 with dropout 25 against 32); rank 32 whole, for half the
+  // reads of A (64 us against 73)
+  if (plan.tile == 64 && rb == 1) a.parts = 2;
+  const dim3 grid(static_cast<unsigned>(plan.tile_count * a.parts));
   if (plan.tile == 64) {
-    if (rb == 1) RPX_BANK_LAUNCH(k_bank_shrink, 1, 4, 4);
+    if (rb == 1) RPX_BANK_LAUNCH(k_bank_shrink, 1, 2, 4);
     else if (rb == 2) RPX_BANK_LAUNCH(k_bank_shrink, 2, 4, 2);
     else RPX_BANK_LAUNCH(k_bank_shrink, 4, 4, 2);
   } else {

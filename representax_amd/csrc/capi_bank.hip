@@ -93,7 +93,7 @@ BankSkinny skinny_of(const Bank& b, uint16_t* y, uint16_t* h) {
   return BankSkinny{b.x, b.m, b.k, b.w, b.n, b.bias, b.a, b.b, b.rank, b.scalings, b.plan, y, h};
 }
 
-bool skinny(const Bank& b) { return bank_skinny_ok(b.m, b.k, b.w.n_groups, b.w.group); }
+bool skinny(const Bank& b) { return bank_skinny_ok(b.m, b.n, b.k, b.w.n_groups, b.w.group); }
 
 // The adapters' term of a product over `columns` columns, added in its epilogue.
 LowRankEpilogue bank_epilogue(const Bank& b, const uint16_t* h, const uint16_t* rows,
@@ -139,8 +139,8 @@ void forward_scratch(A& arena, const Bank& b, bool h_given, ForwardScratch* s) {
   };
   const int64_t stride = bank_rank_stride(b.rank);
   if (skinny(b)) {
-    if (!bank_skinny_fused(skinny_of(b, nullptr, nullptr), b.drop))
-      s->sums = floats(bank_shrink_splits(b.m, b.k) * b.m * stride);
+    const int64_t n = bank_skinny_floats(skinny_of(b, nullptr, nullptr), b.drop);
+    if (n > 0) s->sums = floats(n);
     return;
   }
   if (!h_given) s->h = halves(b.m * stride);
@@ -245,15 +245,17 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
     return kOk;
   }
   if (h == nullptr) h = s.h;
-  RPX_HIP(launch_bank_shrink(b.x, b.k, b.a, b.rank, b.plan, b.drop, h, nullptr, 1, st),
+  RPX_HIP(launch_bank_shrink(b.x, b.k, b.a, b.rank, b.plan, b.drop, h, st),
           "rpx_bank_forward: down-projections");
   if (fast(b)) {
-    // Ranks that the wide tiles' epilogue does not take (above 32, or no multiple of 8)
-    // follow the base product in a pass of their own there.
-    LowRankEpilogue epi = bank_epilogue(b, h, b.b, b.n), base;
+    // Ranks above 32, and in the wide tiles those that are no multiple of 8, follow the
+    // base product in a pass of their own.
+    const bool narrow = b.rank <= 32;
+    LowRankEpilogue epi = narrow ? bank_epilogue(b, h, b.b, b.n) : LowRankEpilogue{}, base;
     epi.bias = base.bias = b.bias;
     const int tile = wide_tile(b);
-    const bool fused = wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi);
+    const bool fused =
+        narrow && wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi);
     if (tile != 0 &&
         (fused || wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, base))) {
       RPX_HIP(launch_int4_dequant(b.w.packed, b.w.scales, s.weight, b.n, b.k, b.w.packed_cols,
@@ -266,7 +268,7 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
     } else {
       RPX_HIP(launch_gemm_int4(b.x, b.k, b.w, b.m, b.n, b.k, y, b.n, epi, st),
               "rpx_bank_forward: product");
-      return kOk;
+      if (narrow) return kOk;
     }
   } else {
     RPX_HIP(launch_generic_gemm(b.x, kBF16, b.k, 1, nullptr, kBF16, 0, 0, &b.w, false, b.m, b.n, b.k,
@@ -312,7 +314,7 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
     const BankTranspose ta{dx_wanted ? b.a : nullptr, s.at, b.rank, b.k};
     const BankTranspose tb{b.b, s.bt, b.n, b.rank};
     RPX_HIP(launch_bank_transpose(tb, ta, b.adapters, st), "rpx_bank_backward: transposes");
-    RPX_HIP(launch_bank_shrink(g, b.n, s.bt, b.rank, b.plan, kNoDropout, s.dh, nullptr, 1, st),
+    RPX_HIP(launch_bank_shrink(g, b.n, s.bt, b.rank, b.plan, kNoDropout, s.dh, st),
             "rpx_bank_backward: dh");
   }
   if (b.m > 0 && dx_wanted) {
@@ -330,8 +332,8 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
       RPX_HIP(launch_int4_dequant_t(b.w.packed, b.w.scales, s.wt, b.n, b.k, b.w.packed_cols,
                                     b.w.n_groups, b.w.group, n64, st),
               "rpx_bank_backward: weight");
-      // the dropout's mask lies on the adapters' part alone: a pass after the product
-      const bool fused = b.drop.threshold >= 65536u;
+      // a dropout's mask lies on the adapters' part alone: a pass after the product
+      const bool fused = b.drop.threshold >= 65536u && b.rank <= 32;
       const LowRankEpilogue epi =
           fused ? bank_epilogue(b, s.dh, s.at, b.k) : LowRankEpilogue{};
       RPX_HIP(launch_gemm_bf16(ga, n64, s.wt, n64, b.m, b.k, n64, dx, b.k, epi, st),

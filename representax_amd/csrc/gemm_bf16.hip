@@ -930,55 +930,74 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   bf16x8_t cf[kMaxJB][FM];
   bf16x8_t rf[kMaxJB][FN];
   if constexpr (BANK) {
-    // Lane's row frow of each 32-row block has its own adapter: for each adapter of a
+    // Lane's row frow of each 32-row block has its own adapter: for the adapters of a
     // block's rows in turn, t = C R_e^T for all of them, added (scaled, in f32) where the
-    // row is its: by a branch, so that no value of another adapter reaches a row. R_e's
-    // fragments stay while the adapter does; the rows of a request are consecutive, so
-    // most blocks have one.
-    int cur = -1;
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm) {
-      const int64_t m = mw + fm * 32 + frow;
-      const int mine = m < M ? epi.adapter_rows[m] : -1;
+    // row is its: by a branch, so that no value of another adapter reaches a row. The
+    // fragments of one adapter stay while blocks have no other (the rows of a request
+    // are consecutive); of several, those of GA are loaded together.
+    constexpr int GA = kMaxJB * FN > 2 ? 2 : 4;
+    bf16x8_t ga[GA][kMaxJB][FN];
+    auto load_adapter = [&](int g, int e) {
+      const uint16_t* rows = epi.rows + e * epi.adapter_stride;
 #pragma unroll
       for (int jb = 0; jb < kMaxJB; ++jb) {
         const int64_t jl = jb * 16 + half * 8;
-        cf[jb][fm] = load8_j(epi.cols + (mine >= 0 ? m * epi.cols_sm + jl : 0), 1,
-                             mine >= 0 ? valid8(epi.rank, jl) : 0);
-      }
-      uint32_t left = static_cast<uint32_t>(__ballot(mine >= 0));
-      while (left != 0) {
-        const int e = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
-        if (e != cur) {
-          cur = e;
-          const uint16_t* rows = epi.rows + e * epi.adapter_stride;
-#pragma unroll
-          for (int jb = 0; jb < kMaxJB; ++jb) {
-            const int64_t jl = jb * 16 + half * 8;
-#pragma unroll
-            for (int fn = 0; fn < FN; ++fn) {
-              const int64_t n = nw + fn * 32 + frow;
-              rf[jb][fn] = load8_j(rows + (n < N ? n * epi.rows_sn + jl : 0), 1,
-                                   n < N ? valid8(epi.rank, jl) : 0);
-            }
-          }
-        }
-        const float scale = epi.adapter_scales[e];
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn) {
-          f32x16_t t;
-#pragma unroll
-          for (int v = 0; v < 16; ++v) t[v] = 0.0f;
-#pragma unroll
-          for (int jb = 0; jb < kMaxJB; ++jb)
-            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[jb][fn], cf[jb][fm], t, 0, 0, 0);
-          if (mine == e) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v)
-              acc[fn][fm][v] = __builtin_fmaf(scale, t[v], acc[fn][fm][v]);
-          }
+          const int64_t n = nw + fn * 32 + frow;
+          ga[g][jb][fn] =
+              load8_j(rows + (n < N ? n * epi.rows_sn + jl : 0), 1, n < N ? valid8(epi.rank, jl) : 0);
         }
-        left &= ~static_cast<uint32_t>(__ballot(mine == e));
+      }
+    };
+    auto add_adapter = [&](int g, int fm, bool own, float scale) {
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn) {
+        f32x16_t t;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) t[v] = 0.0f;
+#pragma unroll
+        for (int jb = 0; jb < kMaxJB; ++jb)
+          t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga[g][jb][fn], cf[jb][fm], t, 0, 0, 0);
+        if (own) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            acc[fn][fm][v] = __builtin_fmaf(scale, t[v], acc[fn][fm][v]);
+        }
+      }
+    };
+    int mine[FM];
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      const int64_t m = mw + fm * 32 + frow;
+      mine[fm] = m < M ? epi.adapter_rows[m] : -1;
+    }
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      const int64_t m = mw + fm * 32 + frow;
+#pragma unroll
+      for (int jb = 0; jb < kMaxJB; ++jb) {
+        const int64_t jl = jb * 16 + half * 8;
+        cf[jb][fm] = load8_j(epi.cols + (mine[fm] >= 0 ? m * epi.cols_sm + jl : 0), 1,
+                             mine[fm] >= 0 ? valid8(epi.rank, jl) : 0);
+      }
+    }
+    int cur = -1;  // the adapter whose fragments ga[0] holds
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
+      while (left != 0) {
+        int e[GA];
+#pragma unroll
+        for (int g = 0; g < GA; ++g) {
+          e[g] = left != 0 ? __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left)) : -1;
+          left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e[g]));
+          if (e[g] >= 0 && !(g == 0 && e[0] == cur)) load_adapter(g, e[g]);
+        }
+        cur = e[0];
+#pragma unroll
+        for (int g = 0; g < GA; ++g)
+          if (e[g] >= 0) add_adapter(g, fm, mine[fm] == e[g], epi.adapter_scales[e[g]]);
       }
     }
   } else if (jblocks > 0) {
@@ -1323,7 +1342,7 @@ hipError_t run_gemm_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
   run_gemm_act<BM, BN, WM, WN, NS, WPE, BK, JB, ACT>(a, lda, b, ldb, w, m, n, k, out, ldc, epi, stream)
   if (epi.act == kActNone) return RPX_RUN_ACT(kActNone);
   if constexpr (JB > 0 && !(BM == 256 && BN == 256)) {
-    if constexpr (BK != kBInt4T) {
+    if constexpr (BK != kBInt4T && JB <= 2) {
       if (epi.act == kActBank) return RPX_RUN_ACT(kActBank);
     }
     if constexpr (BK == kBInt4 || BK == kBInt4L) {

@@ -288,7 +288,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         cf[fm & 1][jb] = *reinterpret_cast<const bf16x8_t*>(
             reinterpret_cast<const uint8_t*>(epi.cols) + at + jb * 32);
     };
-    auto load_rows = [&](int e) {
+    // the fragments of up to GA adapters, ga[0] those of `cur`
+    constexpr int GA = JB > 1 ? 2 : 4;
+    bf16x8_t ga[BANK ? GA : 1][kJB][FN];
+    auto load_rows = [&](int g, int e) {
       const uint8_t* rows = reinterpret_cast<const uint8_t*>(epi.rows + e * epi.adapter_stride);
 #pragma unroll
       for (int fn = 0; fn < FN; ++fn) {
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           const int j = jb * 16 + (el >> 5) * 8;
           const u32x4_t v =
               *reinterpret_cast<const u32x4_t*>(rows + at + (j < epi.rank ? 2 * j : 0));
-          rf[jb][fn] = as_bf16x8(j < epi.rank ? v : u32x4_t{0u, 0u, 0u, 0u});
+          ga[g][jb][fn] = as_bf16x8(j < epi.rank ? v : u32x4_t{0u, 0u, 0u, 0u});
         }
       }
     };
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           mine[fm] = epi.adapter_rows[r < M ? r : M - 1];
           if (r >= M) mine[fm] = -1;
         }
-        load_rows(cur);
+        load_rows(0, cur);
         load_cols(0);
       } else if constexpr (JB > 0) {
 #pragma unroll
@@ -404,32 +407,40 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         if (fm + 1 < FM) load_cols(fm + 1);
       }
       if constexpr (BANK) {
-        // each adapter of the block's rows in turn: its term for all of them, kept where
-        // the row is its, by a branch (no value of another adapter reaches a row)
+        // the adapters of the block's rows, GA at a time: their terms for all rows, kept
+        // where the row is its, by a branch (no value of another adapter reaches a row)
         uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
         while (left != 0) {
-          const int e = __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left));
-          if (e != cur) {
-            cur = e;
-            load_rows(e);
+          int e[GA];
+#pragma unroll
+          for (int g = 0; g < GA; ++g) {
+            e[g] = left != 0 ? __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left)) : -1;
+            left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e[g]));
+            if (e[g] >= 0 && !(g == 0 && e[0] == cur)) load_rows(g, e[g]);
           }
-          const float scale = epi.adapter_scales[e];
+          cur = e[0];
 #pragma unroll
-          for (int fn = 0; fn < FN; ++fn) {
-            __builtin_amdgcn_sched_barrier(0);
-            f32x16_t lr;
+          for (int g = 0; g < GA; ++g) {
+            if (e[g] < 0) continue;
+            const float scale = epi.adapter_scales[e[g]];
+            const bool own = mine[fm] == e[g];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) lr[v] = 0.0f;
+            for (int fn = 0; fn < FN; ++fn) {
+              __builtin_amdgcn_sched_barrier(0);
+              f32x16_t lr;
 #pragma unroll
-            for (int jb = 0; jb < kJB; ++jb)
-              lr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[jb][fn], cf[fm & 1][jb], lr, 0, 0, 0);
-            if (mine[fm] == e) {
+              for (int v = 0; v < 16; ++v) lr[v] = 0.0f;
 #pragma unroll
-              for (int v = 0; v < 16; ++v)
-                acc[fn][fm][v] = __builtin_fmaf(scale, lr[v], acc[fn][fm][v]);
+              for (int jb = 0; jb < kJB; ++jb)
+                lr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga[g][jb][fn], cf[fm & 1][jb], lr, 0,
+                                                             0, 0);
+              if (own) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                  acc[fn][fm][v] = __builtin_fmaf(scale, lr[v], acc[fn][fm][v]);
+              }
             }
           }
-          left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e));
         }
       }
 #pragma unroll

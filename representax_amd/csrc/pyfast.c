@@ -1,5 +1,5 @@
-/* CPython binding of the per-token (small-M) INT4 + LoRA forward and of the MXFP4
- * entry points.
+/* CPython binding of the per-token (small-M) INT4 + LoRA forward and of the MXFP4,
+ * adapter bank, dropout and block boundary entry points.
  *
  * Such an eager call spends more time on the host than on the GPU, and
  * ctypes' per-argument conversion is a large share of it. These functions
@@ -191,15 +191,17 @@ typedef union {
   void* p;
   int64_t l;
   int i;
+  float f;
 } Value;
 
-/* Arguments by a format: p pointer, l int64, s size (not negative), i int. */
+/* Arguments by a format: p pointer, l int64, s size (not negative), i int, f float. */
 static int parse(const char* name, const char* format, PyObject* const* args, Py_ssize_t nargs,
                  Value* v) {
   if (!check_nargs(name, nargs, (Py_ssize_t)strlen(format))) return 0;
   for (Py_ssize_t j = 0; j < nargs; ++j) {
     const int ok = format[j] == 'p'   ? get_ptr(args[j], &v[j].p)
                    : format[j] == 'i' ? get_int(args[j], &v[j].i)
+                   : format[j] == 'f' ? get_f32(args[j], &v[j].f)
                                       : get_i64(args[j], &v[j].l);
     if (!ok) return 0;
     if (format[j] == 's' && v[j].l < 0) {
@@ -311,7 +313,130 @@ static PyObject* fast_mxfp4_bytes(PyObject* self, PyObject* const* args, Py_ssiz
   return NULL;
 }
 
+static PyObject* fast_dropout(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[8];
+  if (!parse("dropout", "pilpllpp", args, nargs, v)) return NULL;
+  return PyLong_FromLong(
+      rpx_dropout(v[0].p, v[1].i, v[2].l, v[3].p, v[4].l, v[5].l, v[6].p, v[7].p));
+}
+
+/* The fields of an rpx_block, its norms' in their places: x, u, gate, rows_per_gate, post
+ * (weight, bias, dtype, kind, eps), norm (the same), key, site, threshold, rows, size, t,
+ * h, dtype, gate_dtype, scale. */
+#define BLOCK "ppplppiifppiifpllllppiif"
+static rpx_block block_of(const Value* v) {
+  const rpx_block b = {v[0].p,
+                       v[1].p,
+                       v[2].p,
+                       v[3].l,
+                       {v[4].p, v[5].p, v[6].i, v[7].i, v[8].f},
+                       {v[9].p, v[10].p, v[11].i, v[12].i, v[13].f},
+                       v[14].p,
+                       v[15].l,
+                       v[16].l,
+                       v[17].l,
+                       v[18].l,
+                       v[19].p,
+                       v[20].p,
+                       v[21].i,
+                       v[22].i,
+                       v[23].f};
+  return b;
+}
+
+static PyObject* fast_block_forward(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[25];
+  if (!parse("block_forward", BLOCK "p", args, nargs, v)) return NULL;
+  const rpx_block b = block_of(v);
+  return PyLong_FromLong(rpx_block_forward(&b, v[24].p));
+}
+
+static rpx_block_gradients gradients_of(const Value* v) {
+  const rpx_block_gradients g = {v[0].p, v[1].p, v[2].p, v[3].p, v[4].p,
+                                 v[5].p, v[6].p, v[7].p, v[8].p};
+  return g;
+}
+
+/* block_backward_workspace(block fields, gradients) -> bytes */
+static PyObject* fast_block_backward_workspace(PyObject* self, PyObject* const* args,
+                                               Py_ssize_t nargs) {
+  (void)self;
+  Value v[33];
+  if (!parse("block_backward_workspace", BLOCK "ppppppppp", args, nargs, v)) return NULL;
+  const rpx_block b = block_of(v);
+  const rpx_block_gradients g = gradients_of(v + 24);
+  return PyLong_FromSize_t(rpx_block_backward_workspace(&b, &g));
+}
+
+static PyObject* fast_block_backward(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[36];
+  if (!parse("block_backward", BLOCK "ppppppppppsp", args, nargs, v)) return NULL;
+  const rpx_block b = block_of(v);
+  const rpx_block_gradients g = gradients_of(v + 24);
+  return PyLong_FromLong(rpx_block_backward(&b, &g, v[33].p, (size_t)v[34].l, v[35].p));
+}
+
+/* The fields of an rpx_bank in their order. */
+#define BANK "pllppllppppllpspll"
+static rpx_bank bank_of(const Value* v) {
+  const rpx_bank b = {v[0].p,  v[1].l,  v[2].l, v[3].p, v[4].p,  v[5].l,          v[6].l,
+                      v[7].p,  v[8].p,  v[9].p, v[10].p, v[11].l, v[12].l,         v[13].p,
+                      (size_t)v[14].l, v[15].p, v[16].l, v[17].l};
+  return b;
+}
+
+/* bank_forward_workspace(bank fields, h_given) -> bytes */
+static PyObject* fast_bank_forward_workspace(PyObject* self, PyObject* const* args,
+                                             Py_ssize_t nargs) {
+  (void)self;
+  Value v[19];
+  if (!parse("bank_forward_workspace", BANK "i", args, nargs, v)) return NULL;
+  const rpx_bank b = bank_of(v);
+  return PyLong_FromSize_t(rpx_bank_forward_workspace(&b, v[18].i));
+}
+
+static PyObject* fast_bank_forward(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[23];
+  if (!parse("bank_forward", BANK "pppsp", args, nargs, v)) return NULL;
+  const rpx_bank b = bank_of(v);
+  return PyLong_FromLong(
+      rpx_bank_forward(&b, v[18].p, v[19].p, v[20].p, (size_t)v[21].l, v[22].p));
+}
+
+/* bank_backward_workspace(bank fields, need_x, need_a, need_b) -> bytes */
+static PyObject* fast_bank_backward_workspace(PyObject* self, PyObject* const* args,
+                                              Py_ssize_t nargs) {
+  (void)self;
+  Value v[21];
+  if (!parse("bank_backward_workspace", BANK "iii", args, nargs, v)) return NULL;
+  const rpx_bank b = bank_of(v);
+  return PyLong_FromSize_t(rpx_bank_backward_workspace(&b, v[18].i, v[19].i, v[20].i));
+}
+
+static PyObject* fast_bank_backward(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  Value v[28];
+  if (!parse("bank_backward", BANK "ppppipipsp", args, nargs, v)) return NULL;
+  const rpx_bank b = bank_of(v);
+  return PyLong_FromLong(rpx_bank_backward(&b, v[18].p, v[19].p, v[20].p, v[21].p, v[22].i,
+                                           v[23].p, v[24].i, v[25].p, (size_t)v[26].l, v[27].p));
+}
+
+#define METHOD(name) {#name, (PyCFunction)(void (*)(void))fast_##name, METH_FASTCALL, "rpx_" #name}
+
 static PyMethodDef methods[] = {
+    METHOD(dropout),
+    METHOD(block_forward),
+    METHOD(block_backward_workspace),
+    METHOD(block_backward),
+    METHOD(bank_forward_workspace),
+    METHOD(bank_forward),
+    METHOD(bank_backward_workspace),
+    METHOD(bank_backward),
     {"get_tuning", (PyCFunction)(void (*)(void))fast_get_tuning, METH_FASTCALL, "rpx_get_tuning"},
     {"int4lora_forward", (PyCFunction)(void (*)(void))fast_int4lora_forward, METH_FASTCALL,
      "rpx_int4lora_forward"},

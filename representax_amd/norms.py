@@ -13,14 +13,13 @@ the backward as they are, so they do not change between a call and its backward.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 import torch.nn.functional as F
 
 from . import _native as nat
-from .dropout import check_key, dropout_threshold, dropped
+from .philox import check_key, dropout_threshold, dropped
 from .ops import (BF16, F32, _aligned, _dtype_code, _on_device, _ptr, _stream, _workspace,
                   eager_calls, on_current_device, plain_tensor)
 
@@ -373,31 +372,27 @@ def _block_expression(x, u, gate, weight, bias, post_weight, post_bias, key, cfg
     return t, h.to(x.dtype)
 
 
-def _norm_struct(weight, bias, kind, eps):
-    if weight is None:
-        return nat.BlockNorm()
-    return nat.BlockNorm(weight.data_ptr(), _ptr(bias), _dtype_code(weight.dtype), kind, eps)
+def _block_fields(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, like, t, h):
+    """The fields of an ``rpx_block`` whose rows are those of ``like``."""
 
-
-def _block_struct(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, shape, dtype, t, h):
-    size = shape[-1]
-    rows = math.prod(shape[:-1])
-    return nat.Block(
+    size = like.shape[-1]
+    dtype = _dtype_code(like.dtype)
+    return (
         _ptr(x), _ptr(u), _ptr(gate), cfg["rows_per_gate"],
-        _norm_struct(post_weight, post_bias, cfg["post_kind"], cfg["post_eps"]),
-        _norm_struct(weight, bias, cfg["kind"], cfg["eps"]),
-        _ptr(key) if cfg["threshold"] < 65536 else None, cfg["site"], cfg["threshold"], rows, size,
-        _ptr(t), _ptr(h), _dtype_code(dtype), _dtype_code(dtype if gate is None else gate.dtype),
-        cfg["scale"])
+        _ptr(post_weight), _ptr(post_bias),
+        0 if post_weight is None else _dtype_code(post_weight.dtype), cfg["post_kind"],
+        cfg["post_eps"],
+        _ptr(weight), _ptr(bias), 0 if weight is None else _dtype_code(weight.dtype), cfg["kind"],
+        cfg["eps"],
+        _ptr(key), cfg["site"], cfg["threshold"], like.numel() // size, size, _ptr(t), _ptr(h),
+        dtype, dtype if gate is None else _dtype_code(gate.dtype), cfg["scale"])
 
 
 def _block_forward(x, u, gate, weight, bias, post_weight, post_bias, key, cfg):
-    device = _on_device(x, u, gate, weight, bias, post_weight, post_bias)
-    t = torch.empty(x.shape, dtype=x.dtype, device=device)
-    h = None if weight is None else torch.empty(x.shape, dtype=x.dtype, device=device)
-    block = _block_struct(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, x.shape,
-                          x.dtype, t, h)
-    nat.call("rpx_block_forward", ctypes.byref(block), _stream(device))
+    t = torch.empty_like(x)
+    h = None if weight is None else torch.empty_like(x)
+    nat.block_forward(_block_fields(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, x,
+                                    t, h), _stream(x.device))
     return t, h
 
 
@@ -431,19 +426,17 @@ class BlockNormFn(torch.autograd.Function):
             grads = iter(torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs],
                                              create_graph=again, allow_unused=True))
             return (*(next(grads) if need else None for need in wanted), *none)
-        device = _on_device(dt, dh, u)
+        _on_device(dt, dh, u)
         dt = None if dt is None else dt.contiguous()
         dh = None if dh is None else dh.contiguous()
-        outs = [torch.empty(v.shape, dtype=v.dtype, device=device) if need else None
-                for v, need in zip(inputs, wanted)]
-        block = _block_struct(None, u, gate, weight, bias, post_weight, post_bias, key, ctx.cfg,
-                              u.shape, u.dtype, t, None)
-        grads = nat.BlockGradients(_ptr(dt), _ptr(dh), *(_ptr(o) for o in outs))
-        refs = ctypes.byref(block), ctypes.byref(grads)
-        need = nat.query("rpx_block_backward_workspace", *refs)
-        ws = _workspace(need, device) if need else None
-        nat.call("rpx_block_backward", *refs, _ptr(ws), 0 if ws is None else ws.numel(),
-                 _stream(device))
+        outs = [torch.empty_like(v) if need else None for v, need in zip(inputs, wanted)]
+        fields = _block_fields(None, u, gate, weight, bias, post_weight, post_bias, key, ctx.cfg,
+                               u, t, None)
+        grads = (_ptr(dt), _ptr(dh), *map(_ptr, outs))
+        stream = _stream(u.device)
+        need = nat.block_backward_workspace(fields, grads)
+        ws = _workspace(need, u.device, stream) if need else None
+        nat.block_backward(fields, grads, _ptr(ws), need, stream)
         return (*outs, *none)
 
 
@@ -473,19 +466,24 @@ def _parts(norm: torch.nn.Module | None):
 
 
 def _block_kernel(value, update, gate, weights, key) -> bool:
-    size = value.shape[-1]
-    tensors = [value, update, *(w for w in weights if w is not None)]
-    return (value.dtype in (BF16, F32) and update.dtype == value.dtype
-            and 1 <= size <= _BLOCK_MAX_SIZE and value.numel() > 0
-            and all(plain_tensor(t) and t.device == value.device and t.dtype in (BF16, F32)
-                    for t in tensors)
-            and all(w is None or w.shape == (size,) for w in weights)
-            and all(b is None or b.dtype == w.dtype for w, b in (weights[:2], weights[2:]))
-            and (gate is None or (plain_tensor(gate) and gate.device == value.device
+    shape = value.shape
+    size = shape[-1]
+    index = value.get_device()
+    if not (value.dtype in (BF16, F32) and update.dtype == value.dtype
+            and 1 <= size <= _BLOCK_MAX_SIZE and value.numel() > 0 and plain_tensor(value)
+            and plain_tensor(update) and update.get_device() == index and on_current_device(value)
+            and not torch.is_autocast_enabled("cuda")):
+        return False
+    for weight, bias in (weights[:2], weights[2:]):
+        for w in (weight, bias):
+            if w is not None and not (plain_tensor(w) and w.get_device() == index
+                                      and w.dtype == weight.dtype and w.dtype in (BF16, F32)
+                                      and w.dim() == 1 and w.shape[0] == size):
+                return False
+    return ((key is None or plain_tensor(key))
+            and (gate is None or (plain_tensor(gate) and gate.get_device() == index
                                   and gate.dtype in (BF16, F32)
-                                  and _rows_per_gate(gate, value.shape) is not None))
-            and (key is None or plain_tensor(key)) and on_current_device(value)
-            and not torch.is_autocast_enabled("cuda"))
+                                  and _rows_per_gate(gate, shape) is not None)))
 
 
 def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.Tensor, *,
@@ -506,10 +504,12 @@ def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.
     backward reads t and update, which must not change in place. Everything else
     runs the same steps by torch operations."""
 
-    if update.shape != value.shape or value.dim() < 1:
+    shape = value.shape
+    if update.shape != shape or not shape:
         raise ValueError(f"update {tuple(update.shape)} must have the shape of value "
                          f"{tuple(value.shape)}")
-    if gate is not None and torch.broadcast_shapes(gate.shape, value.shape) != value.shape:
+    if gate is not None and gate.shape != shape[-1:] and (
+            torch.broadcast_shapes(gate.shape, shape) != shape):
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over {tuple(value.shape)}")
     threshold = dropout_threshold(rate)
     if threshold < 65536:
@@ -534,14 +534,16 @@ def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.
     if not (eager and _block_kernel(value, update, gate, weights, key)):
         return _block_expression(value, update, gate, *weights, key, cfg)
     value, update = value.contiguous(), update.contiguous()
-    weights = [None if w is None else w.contiguous() for w in weights]
+    weight, bias, post_weight, post_bias = (None if w is None else w.contiguous() for w in weights)
     if gate is not None:
         cfg["rows_per_gate"] = _rows_per_gate(gate, value.shape)
         gate = gate.contiguous()
     key = None if key is None else key.contiguous()
-    operands = (value, update, gate, *weights, key, cfg)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands[:7]):
-        return BlockNormFn.apply(*operands)
+    operands = (value, update, gate, weight, bias, post_weight, post_bias, key, cfg)
+    if torch.is_grad_enabled():
+        for t in operands[:7]:
+            if t is not None and t.requires_grad:
+                return BlockNormFn.apply(*operands)
     return _block_forward(*operands)
 
 

@@ -15,13 +15,16 @@ gives a new one each step, and a step's calls differ in their ``site``.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _native as nat
-from .ops import (BF16, F32, _aligned, _dtype_code, _ptr, _stream, eager_calls, on_current_device,
+from .ops import (BF16, F32, _aligned, _dtype_code, _stream, eager_calls, on_current_device,
                   plain_tensor)
 
 _WORD = 0xFFFFFFFF
+_KEY_SHAPE = torch.Size((2,))
 
 
 class DropoutKeys(torch.nn.Module):
@@ -44,7 +47,11 @@ class DropoutKeys(torch.nn.Module):
 def dropout_threshold(rate: float) -> int:
     """T of the given rate: 65536ths that are kept (at least one)."""
 
-    rate = float(rate)
+    return _threshold(float(rate))
+
+
+@lru_cache(maxsize=256)
+def _threshold(rate: float) -> int:
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"dropout rate must be in [0, 1), got {rate}")
     return min(65536, max(1, round(65536 * (1.0 - rate))))
@@ -53,10 +60,10 @@ def dropout_threshold(rate: float) -> int:
 def check_key(key: torch.Tensor | None, site: int, device: torch.device) -> None:
     if key is None:
         raise ValueError("dropout needs a key (DropoutKeys.next)")
-    if key.dtype != torch.int64 or tuple(key.shape) != (2,) or key.device != device:
+    if key.dtype != torch.int64 or key.shape != _KEY_SHAPE or key.device != device:
         raise ValueError(f"dropout key must be int64 [2] on {device}, got {key.dtype} "
                          f"{tuple(key.shape)} on {key.device}")
-    if not 0 <= int(site) <= _WORD:
+    if not 0 <= site <= _WORD:
         raise ValueError(f"dropout site must be 0 to 2^32 - 1, got {site}")
 
 
@@ -92,20 +99,33 @@ def _wide(dtype: torch.dtype) -> torch.dtype:
     return torch.promote_types(dtype, F32)
 
 
+def _launch(x, key, threshold, site):
+    x = _aligned(x)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    args = (x.data_ptr(), _dtype_code(x.dtype), x.numel(), key.data_ptr(), site, threshold,
+            out.data_ptr(), _stream(x.device))
+    binding = nat.fast()
+    if binding is not None:
+        nat.check(binding.dropout(*args))
+    else:
+        nat.call("rpx_dropout", *args)
+    return out
+
+
 class DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, key, rate, threshold, site):
         ctx.save_for_backward(key)
-        ctx.args = (rate, site)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        nat.call("rpx_dropout", _ptr(_aligned(x)), _dtype_code(x.dtype), x.numel(), _ptr(key),
-                 site, threshold, _ptr(out), _stream(x.device))
-        return out
+        ctx.args = (rate, threshold, site)
+        return _launch(x, key, threshold, site)
 
     @staticmethod
     def backward(ctx, grad):
         (key,) = ctx.saved_tensors
-        rate, site = ctx.args
+        rate, threshold, site = ctx.args
+        if (not torch.is_grad_enabled() and eager_calls() and plain_tensor(grad)
+                and on_current_device(grad)):
+            return _launch(grad, key, threshold, site), None, None, None, None
         return dropout(grad, rate, key, site), None, None, None, None
 
 
@@ -123,7 +143,10 @@ def dropout(value: torch.Tensor, rate: float, key: torch.Tensor, site: int = 0) 
     check_key(key, site, value.device)
     if (eager_calls() and plain_tensor(value) and plain_tensor(key) and on_current_device(value)
             and value.dtype in (BF16, F32) and value.layout == torch.strided):
-        return DropoutFn.apply(value, key.contiguous(), rate, threshold, int(site))
+        key = key.contiguous()
+        if torch.is_grad_enabled() and value.requires_grad:
+            return DropoutFn.apply(value, key, rate, threshold, int(site))
+        return _launch(value, key, threshold, int(site))
     return dropped(value.to(_wide(value.dtype)), key, threshold, int(site)).to(value.dtype)
 
 

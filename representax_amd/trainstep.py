@@ -46,7 +46,8 @@ from .bank import active_adapter_rows, adapter_rows
 from .components import Linear
 from .config import PrecisionConfig
 from .mlp import gelu_mlp, shared_input_projections, swiglu_mlp
-from .norms import LayerNorm, RMSNorm, add_norm, attention_heads
+from .norms import LayerNorm, RMSNorm, add_norm, attention_heads, block_norm
+from .philox import DropoutKeys
 from .precision import (active_compute_views, active_policy, compute_views, precision_context,
                         resolve_precision_policy)
 
@@ -65,6 +66,9 @@ class BertConfig:
     norm_epsilon: float = 1e-12
     initializer_range: float = 0.02
     pad_token_id: int = 0
+    # of a sublayer's output before the residual sum, while training and given a
+    # key (an extension: the reference's encoders have none)
+    hidden_dropout: float = 0.0
 
     @property
     def head_dimension(self) -> int:
@@ -203,10 +207,20 @@ class BertLayer(torch.nn.Module):
         self.attention_norm = LayerNorm(config.hidden_size, config.norm_epsilon, device)
         self.mlp = BertMLP(config, key + 4, device)
         self.output_norm = LayerNorm(config.hidden_size, config.norm_epsilon, device)
+        self.dropout = config.hidden_dropout
 
-    def forward(self, hidden: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
-        _, hidden = add_norm(self.attention_norm, hidden, self.attention(hidden, bias))
-        return add_norm(self.output_norm, hidden, self.mlp(hidden))[1]
+    def forward(self, hidden: torch.Tensor, bias: torch.Tensor | None,
+                key: torch.Tensor | None = None, site: int = 0) -> torch.Tensor:
+        if key is None or not self.training or self.dropout == 0:
+            _, hidden = add_norm(self.attention_norm, hidden, self.attention(hidden, bias))
+            return add_norm(self.output_norm, hidden, self.mlp(hidden))[1]
+        _, hidden = block_norm(self.attention_norm, hidden, self.attention(hidden, bias),
+                               rate=self.dropout, key=key, site=site)
+        return block_norm(self.output_norm, hidden, self.mlp(hidden), rate=self.dropout, key=key,
+                          site=site + 1)[1]
+
+
+HIDDEN_SITE = 1 << 16  # of the first layer's hidden dropouts, past those of adapter banks
 
 
 class BertEncoder(torch.nn.Module):
@@ -233,8 +247,10 @@ class BertEncoder(torch.nn.Module):
         self.remat = "none"
 
     def hidden_states(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None,
-                      compute_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """``attention_mask`` None means every position is a real token."""
+                      compute_dtype: torch.dtype = torch.bfloat16,
+                      key: torch.Tensor | None = None) -> torch.Tensor:
+        """``attention_mask`` None means every position is a real token; ``key``
+        (``DropoutKeys.next``) draws the hidden dropout, if there is one."""
 
         s = input_ids.shape[1]
         hidden = (self.word[input_ids] + self.position[:s][None]
@@ -244,13 +260,14 @@ class BertEncoder(torch.nn.Module):
         if attention_mask is not None:
             bias = torch.zeros(attention_mask.shape, dtype=torch.float32, device=hidden.device)
             bias = bias.masked_fill(~attention_mask.bool(), float("-inf"))[:, None, None, :]
-        for layer in self.layers:
-            hidden = run_layer(layer, self.remat, hidden, bias)
+        for i, layer in enumerate(self.layers):
+            hidden = run_layer(layer, self.remat, hidden, bias, key, HIDDEN_SITE + 2 * i)
         return hidden
 
     def encode(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None,
-               compute_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        hidden = self.hidden_states(input_ids, attention_mask, compute_dtype).float()
+               compute_dtype: torch.dtype = torch.bfloat16,
+               key: torch.Tensor | None = None) -> torch.Tensor:
+        hidden = self.hidden_states(input_ids, attention_mask, compute_dtype, key).float()
         if attention_mask is None:
             pooled = hidden.mean(1)
         else:
@@ -463,6 +480,7 @@ class MNRTrainStep:
     masters' float32 gradient by one concatenation (the transpose of the
     cast): two kernels per step instead of a cast per parameter use and an
     add per gradient.
+    A model with hidden dropout draws from a new key each step (``self.keys``).
     ``capture()`` records forward, backward and the update into one HIP graph
     over static input buffers; ``__call__`` replays it (or runs eagerly
     before capture).
@@ -514,6 +532,9 @@ class MNRTrainStep:
         self.loss = torch.zeros((), dtype=torch.float32, device=device)
         self.grad_norm = torch.zeros((), dtype=torch.float32, device=device)
         self.finite = torch.ones((), dtype=torch.bool, device=device)
+        self.keys = None
+        if getattr(model.config, "hidden_dropout", 0.0) > 0:
+            self.keys = DropoutKeys(seed, device)
         self._backup = None
         self.graph = None
 
@@ -528,7 +549,8 @@ class MNRTrainStep:
             self.flat_c.copy_(self.flat)
         with precision_context(self.policy), compute_views(self.views):
             ids = torch.cat([self.query_ids, self.document_ids], 0)
-            emb = self.model.encode(ids)
+            emb = (self.model.encode(ids) if self.keys is None
+                   else self.model.encode(ids, key=self.keys.next()))
             b = self.query_ids.shape[0]
             loss = mnr_loss(emb[:b], emb[b:], self.scale)
         loss.backward()

@@ -10,7 +10,7 @@ import torch.nn.functional as F
 
 import representax_amd as rx
 from representax_amd import _native as nat
-from representax_amd.dropout import dropped
+from representax_amd.philox import dropped
 from representax_amd.norms import _rows_per_gate
 
 F64 = torch.float64

@@ -12,7 +12,7 @@ import torch
 import representax_amd as rx
 from oracle import dropout as odrop
 from representax_amd import _native as nat
-from representax_amd.dropout import dropout_threshold, dropped, kept
+from representax_amd.philox import dropout_threshold, dropped, kept
 
 
 # counter, key and result of the generator's authors' known answers
