@@ -221,6 +221,9 @@ def bank_linear(x: torch.Tensor, packed: torch.Tensor, scale_bits: torch.Tensor,
               None if bias is None else _u16(bias).contiguous(), scalings.contiguous(), plan.buffer,
               key)
     _on_device(x2d, lora_a, lora_b, *frozen)
+    if torch.is_grad_enabled() and (scalings.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
+        raise ValueError("scalings and bias are constants of a bank: they get no gradients")
     if torch.is_grad_enabled() and (x2d.requires_grad or lora_a.requires_grad
                                     or lora_b.requires_grad):
         y = BankLinearFn.apply(x2d, lora_a, lora_b, *frozen, cfg)

@@ -22,7 +22,9 @@ struct BankTile {
 // What a batch's plan holds, in one int32 buffer.
 struct BankPlan {
   const int32_t* rows;         // [m] a row's adapter, -1: none
-  const int32_t* order;        // [m] the rows by adapter, in their own order within one
+  const int32_t* order;        // [m] the rows by adapter, in their own order within one, and
+                               // those without one last
+  const int32_t* sorted;       // [m] the adapter of each position of that order
   const int32_t* first;        // [adapters + 1] an adapter's first position
   const int32_t* chunk_first;  // [adapters + 1] its first chunk
   const BankTile* tiles;       // of `tile` rows each, `tile_count` records

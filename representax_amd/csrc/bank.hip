@@ -74,7 +74,7 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanWaves = kPlanThreads / 64;
 
 struct PlanOut {
-  int32_t *rows, *order, *first, *chunk_first;
+  int32_t *rows, *order, *sorted, *first, *chunk_first;
   BankTile *tiles, *chunks;
 };
 
@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     k_bank_plan(const I* __restrict__ index, BankPlan plan, PlanOut out, unsigned int* err) {
   constexpr int kMax = static_cast<int>(kBankMaxAdapters);
   __shared__ int32_t count[kPlanWaves][kMax];
+  __shared__ int32_t none[kPlanWaves];  // rows without an adapter
   __shared__ int32_t scan[3][kMax + 1];  // positions, tiles and chunks before an adapter
   __shared__ int32_t wave_sum[kPlanWaves][3];
   const int tid = threadIdx.x;
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   const int adapters = static_cast<int>(plan.adapters);
   const int m = static_cast<int>(plan.m);
   for (int i = tid; i < kPlanWaves * kMax; i += kPlanThreads) count[i / kMax][i % kMax] = 0;
+  if (tid < kPlanWaves) none[tid] = 0;
   __syncthreads();
   const int64_t share = ceil_div(ceil_div(m, kPlanWaves), 64) * 64;
   const int64_t begin = share * wave < m ? share * wave : m;
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     bad |= e < -1 || e >= adapters;
     const int32_t v = e < 0 || e >= adapters ? -1 : static_cast<int32_t>(e);
     out.rows[r] = v;
-    if (v >= 0) atomicAdd(&count[wave][v], 1);
+    atomicAdd(v >= 0 ? &count[wave][v] : &none[wave], 1);
   }
   if (bad && err != nullptr) atomicOr(err, kDevErrBankIndex);
   __syncthreads();
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     out.first[e] = scan[0][e];
     out.chunk_first[e] = scan[2][e];
   }
-  // each wave's places within an adapter; rows without one go last, in any place
+  // each wave's places within an adapter, and among the rows without one
   for (int e = tid; e < adapters; e += kPlanThreads) {
     int32_t s = scan[0][e];
     for (int w = 0; w < kPlanWaves; ++w) {
@@ -161,20 +163,33 @@ __global__ void __launch_bounds__(kPlanThreads)
       s += n;
     }
   }
+  if (tid == 0) {
+    int32_t s = scan[0][adapters];
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int32_t n = none[w];
+      none[w] = s;
+      s += n;
+    }
+  }
   __syncthreads();
   for (int64_t r0 = begin; r0 < end; r0 += 64) {
     const int64_t r = r0 + lane;
-    const int32_t e = r < end ? out.rows[r] : -1;
-    uint64_t left = __ballot(e >= 0);
+    const int32_t e = r < end ? out.rows[r] : -2;
+    uint64_t left = __ballot(e >= -1);
     while (left != 0) {
       const int leader = __builtin_ctzll(left);
       const int32_t mine = __shfl(e, leader, 64);
       const uint64_t same = __ballot(e == mine);
       int32_t base = 0;
-      if (lane == leader) base = atomicAdd(&count[wave][mine], __popcll(same));
+      if (lane == leader)
+        base = atomicAdd(mine >= 0 ? &count[wave][mine] : &none[wave],
+                         static_cast<int32_t>(__popcll(same)));
       base = __shfl(base, leader, 64);
-      if (e == mine)
-        out.order[base + __popcll(same & ((1ull << lane) - 1))] = static_cast<int32_t>(r);
+      if (e == mine) {
+        const int32_t at = base + __popcll(same & ((1ull << lane) - 1));
+        out.order[at] = static_cast<int32_t>(r);
+        out.sorted[at] = e;
+      }
       left &= ~same;
     }
   }
@@ -679,13 +694,14 @@ BankPlan bank_plan(void* buffer, int64_t m, int64_t adapters) {
     at += (count + 3) / 4 * 4;  // 16-byte pieces
     return here;
   };
-  const int64_t rows = take(m), order = take(m), first = take(adapters + 1),
+  const int64_t rows = take(m), order = take(m), sorted = take(m), first = take(adapters + 1),
                 chunk_first = take(adapters + 1), tiles = take(4 * p.tile_count),
                 chunks = take(4 * p.chunk_count);
   p.words = at;
   if (w == nullptr) return p;
   p.rows = w + rows;
   p.order = w + order;
+  p.sorted = w + sorted;
   p.first = w + first;
   p.chunk_first = w + chunk_first;
   p.tiles = reinterpret_cast<const BankTile*>(w + tiles);
@@ -695,9 +711,10 @@ BankPlan bank_plan(void* buffer, int64_t m, int64_t adapters) {
 
 hipError_t launch_bank_plan(const void* index, int index_bytes, const BankPlan& plan,
                             hipStream_t stream) {
-  const PlanOut out{const_cast<int32_t*>(plan.rows),        const_cast<int32_t*>(plan.order),
-                    const_cast<int32_t*>(plan.first),       const_cast<int32_t*>(plan.chunk_first),
-                    const_cast<BankTile*>(plan.tiles),      const_cast<BankTile*>(plan.chunks)};
+  const PlanOut out{const_cast<int32_t*>(plan.rows),  const_cast<int32_t*>(plan.order),
+                    const_cast<int32_t*>(plan.sorted), const_cast<int32_t*>(plan.first),
+                    const_cast<int32_t*>(plan.chunk_first), const_cast<BankTile*>(plan.tiles),
+                    const_cast<BankTile*>(plan.chunks)};
   if (index_bytes == 8)
     hipLaunchKernelGGL(k_bank_plan<int64_t>, dim3(1), dim3(kPlanThreads), 0, stream,
                        static_cast<const int64_t*>(index), plan, out, device_error_word());

@@ -107,7 +107,8 @@ LowRankEpilogue bank_epilogue(const Bank& b, const uint16_t* h, const uint16_t* 
   epi.cols_sj = 1;
   epi.rank = b.rank;
   epi.act = kActBank;
-  epi.adapter_rows = b.plan.rows;
+  epi.row_order = b.plan.order;
+  epi.row_adapters = b.plan.sorted;
   epi.adapter_scales = b.scalings;
   epi.adapter_stride = columns * b.rank;
   return epi;

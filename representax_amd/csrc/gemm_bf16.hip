@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       const int trow = 8 * j + (lane >> 3);
       int64_t r = m0 + trow;
       r = r < M ? r : M - 1;
+      if constexpr (ACT == kActBank) r = epi.row_order[r];
       src[i] = reinterpret_cast<const uint8_t*>(A + r * lda) + (((lane & 7) ^ swz(trow)) << 4);
     } else if constexpr (T4) {
       if (j < A_SEGS + P_SEGS) {
@@ -592,6 +593,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       const int trow = 8 * (wave + d * NW) + (lane >> 3);
       int64_t r = m0 + trow;
       r = r < M ? r : M - 1;
+      if constexpr (ACT == kActBank) r = epi.row_order[r];
       aoff[d] = static_cast<uint32_t>(r * lda * 2 + (((lane & 7) ^ swz(trow)) << 4));
     }
     uint32_t a_off[FM][4], b_off[FN][4];
@@ -910,6 +912,12 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   // no LDS DMA may still be in flight when the waves leave the loop
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
+  // where the output's row m is
+  auto out_row = [&](int64_t m) -> int64_t {
+    if constexpr (BANK) return epi.row_order[m];
+    return m;
+  };
+
   // Epilogue --------------------------------------------------------------
   // y = bf16(bf16(acc) + bf16(bf16(t) * scale)) (+ bias, rounded again), the
   // reference's rounding points, where t = C R^T is one more 32x32x16 MFMA
@@ -933,8 +941,8 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     // Lane's row frow of each 32-row block has its own adapter: for the adapters of a
     // block's rows in turn, t = C R_e^T for all of them, added (scaled, in f32) where the
     // row is its: by a branch, so that no value of another adapter reaches a row. The
-    // fragments of one adapter stay while blocks have no other (the rows of a request
-    // are consecutive); of several, those of GA are loaded together.
+    // fragments of one adapter stay while blocks have no other (its rows are neighbours);
+    // of several, those of GA are loaded together.
     constexpr int GA = kMaxJB * FN > 2 ? 2 : 4;
     bf16x8_t ga[GA][kMaxJB][FN];
     auto load_adapter = [&](int g, int e) {
@@ -970,11 +978,11 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
       const int64_t m = mw + fm * 32 + frow;
-      mine[fm] = m < M ? epi.adapter_rows[m] : -1;
+      mine[fm] = m < M ? epi.row_adapters[m] : -1;
     }
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
-      const int64_t m = mw + fm * 32 + frow;
+      const int64_t m = mine[fm] >= 0 ? out_row(mw + fm * 32 + frow) : 0;
 #pragma unroll
       for (int jb = 0; jb < kMaxJB; ++jb) {
         const int64_t jl = jb * 16 + half * 8;
@@ -1117,7 +1125,8 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (int it = 0; it < ITS; ++it) {
           const int idx = it * NT + tid;
-          *reinterpret_cast<u32x4_t*>(out + (m0 + idx / CPR) * ldc + n0 + 8 * (idx % CPR)) = v[it];
+          *reinterpret_cast<u32x4_t*>(out + out_row(m0 + idx / CPR) * ldc + n0 +
+                                      8 * (idx % CPR)) = v[it];
         }
         return;
       }
@@ -1127,7 +1136,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
         const int64_t n = n0 + 8 * (idx % CPR);
         if (m >= M || n >= N) continue;
         const u32x4_t v = *reinterpret_cast<const u32x4_t*>(smem + (idx / CPR) * P + (idx % CPR) * 16);
-        uint16_t* d = out + m * ldc + n;
+        uint16_t* d = out + out_row(m) * ldc + n;
         if (vec_out && n + 7 < N) {
           *reinterpret_cast<u32x4_t*>(d) = v;
         } else {
@@ -1146,7 +1155,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
           for (int vg = 0; vg < 4; ++vg) {
             const int64_t nb = nw + fn * 32 + 8 * vg + 4 * half;
-            uint16_t* dst = out + m * ldc + nb;
+            uint16_t* dst = out + out_row(m) * ldc + nb;
             if (vec_out && nb + 3 < N) {
               *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{ypk[fn][fm][2 * vg], ypk[fn][fm][2 * vg + 1]};
             } else {

@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (j < A_SEGS) {
         int r = tm * BM + trow;
         r = r < M ? r : M - 1;
+        if constexpr (ACT == kActBank) r = epi.row_order[r];
         off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(lda_bytes) + chunk;
       } else {
         int r = tn * BN + trow;
@@ -262,15 +263,16 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
     // BANK: the rows' adapters, and the adapter whose fragments rf holds, at first that
     // of the sub-tile's first row
-    int mine[BANK ? FM : 1];
+    int mine[BANK ? FM : 1], place[BANK ? FM : 1];  // and where its rows are
     int cur = 0;
     if constexpr (BANK) {
-      cur = epi.adapter_rows[mw < M ? mw : M - 1];
+      cur = epi.row_adapters[mw < M ? mw : M - 1];
       cur = cur < 0 ? 0 : cur;
     }
     auto load_cols = [&](int fm) {
       int r = mw + fm * 32 + (el & 31);
       r = r < M ? r : M - 1;
+      if constexpr (BANK) r = place[fm];
       const uint32_t at = static_cast<uint32_t>(r) * static_cast<uint32_t>(2 * epi.cols_sm) + (el >> 5) * 16;
       if constexpr (BANK) {
         // ranks of 8 and 24 end in the middle of a 16-rank block
@@ -330,7 +332,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int fm = 0; fm < FM; ++fm) {
           const int r = mw + fm * 32 + (el & 31);
-          mine[fm] = epi.adapter_rows[r < M ? r : M - 1];
+          mine[fm] = epi.row_adapters[r < M ? r : M - 1];
+          place[fm] = epi.row_order[r < M ? r : M - 1];
           if (r >= M) mine[fm] = -1;
         }
         load_rows(0, cur);
@@ -516,6 +519,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + r * (TN * 2) +
                                                             (stage_chunk<CPR>(r, c) << 4));
         u32x4_t o = v, o2{0u, 0u, 0u, 0u};
+        int row_at = 0;
+        if constexpr (BANK) row_at = __shfl(place[fm], r, 64);
         if constexpr (ACT != kActNone && !BANK) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -536,7 +541,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
         if (inside || piece_ok(fm, it)) {
           const uint32_t po = piece_off(it);
-          *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(out) + at + po) = o;
+          if constexpr (BANK)
+            *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(out) + 2 * nw + 16 * c +
+                                        static_cast<int64_t>(row_at) * ld2) = o;
+          else
+            *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(out) + at + po) = o;
           if constexpr (FWD)
             *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(epi.pre_out) + at + po) = v;
           if constexpr (TWO)

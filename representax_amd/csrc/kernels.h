@@ -52,10 +52,13 @@ struct LowRankEpilogue {
   const uint16_t* aux2 = nullptr;  // up (SiLU-mul backward)
   uint16_t* pre_out = nullptr;     // v itself (forward modes)
   uint16_t* out2 = nullptr;        // d gate (SiLU-mul backward)
-  // kActBank: row m's R is rows + adapter_rows[m] * adapter_stride (none where it is
-  // negative) and its scale adapter_scales[adapter_rows[m]], and the sum of product,
-  // term and bias is rounded once. C's columns past the rank are not read.
-  const int32_t* adapter_rows = nullptr;
+  // kActBank: the product's row m is row row_order[m] of A, of C and of the output, so
+  // that the rows of an adapter are neighbours. Its R is rows + row_adapters[m] *
+  // adapter_stride (none where that is negative), its scale adapter_scales[
+  // row_adapters[m]], and the sum of product, term and bias is rounded once. C's columns
+  // past the rank are not read.
+  const int32_t* row_order = nullptr;
+  const int32_t* row_adapters = nullptr;
   const float* adapter_scales = nullptr;
   int64_t adapter_stride = 0;
 };

@@ -326,6 +326,15 @@ def test_two_streams():
             assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
+def test_gradients_of_constants_are_refused():
+    case = Case(9, 64, 32, 8, 2, "rows", bias=True)
+    case.s.requires_grad_(True)
+    with pytest.raises(ValueError, match="constants"):
+        case.call()
+    with torch.no_grad():
+        case.call()
+
+
 def test_a_second_derivative_is_refused():
     case = Case(9, 64, 32, 8, 2, "rows")
     x = case.x.requires_grad_(True)

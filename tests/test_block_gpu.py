@@ -147,6 +147,22 @@ def test_masters_in_float32_keep_float32_gradients():
     _check((7, 31, 320), BF16, "rms", "rms", (320,), 0.0, weight_dtype=F32)
 
 
+def test_a_layer_norm_takes_its_masters_in_the_values_type():
+    x, u = (torch.randn(9, 264, device=DEV).to(BF16) for _ in range(2))
+    masters, views = (_module("layer", 264, F32, 3) for _ in range(2))
+    with torch.no_grad():
+        for p in views.parameters():
+            p.copy_(p.to(BF16))
+    x.requires_grad_(True)
+    got, want = (rx.block_norm(m, x, u, post=m) for m in (masters, views))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    grads = [torch.autograd.grad(out, [x, *m.parameters()], (u, u))
+             for out, m in ((got, masters), (want, views))]
+    for a, b in zip(*grads):
+        assert torch.equal(a, b) and a.dtype in (BF16, F32)
+
+
 @pytest.mark.parametrize("dt,dh", [(True, False), (False, True)])
 def test_one_output_used(dt, dh):
     _check((6, 40, 136), BF16, "layer", "rms", (6, 1, 136), 0.3, dt=dt, dh=dh)
