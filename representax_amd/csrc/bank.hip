@@ -65,12 +65,14 @@ __device__ __forceinline__ u32x4_t masked8(u32x4_t v, const PhiloxCall& call, ui
 }
 
 // ---------------------------------------------------------------------------
-// The plan: a stable counting sort in one workgroup. Wave w takes the w-th eighth
-// of the rows; counts of (wave, adapter) give each its places, and within 64 rows
-// a ballot gives each row its rank, so the order is the rows' own. 16384 rows of
-// eight adapters: 24 us, once a batch.
+// The plan: a stable counting sort in one workgroup. Wave w takes the w-th share of
+// the rows; counts of (wave, adapter) give each its places, and within 64 rows one
+// ballot for each bit of an adapter's number gives every lane the lanes of its own, so
+// the order is the rows' own. Once a batch: 16384 rows of 8, 48 and 1024 adapters 18, 19
+// and 28 us (60, 191 and 319 with the lanes of each adapter in turn), 2^20 rows of 64 1.6
+// ms; a plan of several workgroups would need three launches.
 // ---------------------------------------------------------------------------
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 
 struct PlanOut {
@@ -98,30 +100,36 @@ __global__ void __launch_bounds__(kPlanThreads)
   const int64_t begin = share * wave < m ? share * wave : m;
   const int64_t end = begin + share < m ? begin + share : m;
   bool bad = false;
-  for (int64_t r = begin + lane; r < end; r += 64) {
-    const int64_t e = static_cast<int64_t>(index[r]);
-    bad |= e < -1 || e >= adapters;
-    const int32_t v = e < 0 || e >= adapters ? -1 : static_cast<int32_t>(e);
-    out.rows[r] = v;
-    atomicAdd(v >= 0 ? &count[wave][v] : &none[wave], 1);
+  constexpr int kAhead = 4;  // loads in flight
+  for (int64_t r0 = begin; r0 < end; r0 += 64 * kAhead) {
+    int64_t e[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + 64 * i + lane;
+      e[i] = static_cast<int64_t>(index[r < end ? r : end - 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + 64 * i + lane;
+      if (r >= end) continue;
+      bad |= e[i] < -1 || e[i] >= adapters;
+      const int32_t v = e[i] < 0 || e[i] >= adapters ? -1 : static_cast<int32_t>(e[i]);
+      out.rows[r] = v;
+      atomicAdd(v >= 0 ? &count[wave][v] : &none[wave], 1);
+    }
   }
   if (bad && err != nullptr) atomicOr(err, kDevErrBankIndex);
   __syncthreads();
-  // exclusive sums over the adapters of their rows, tiles and chunks: two adapters
-  // a thread, over the lanes, then over the waves
-  int32_t v[2][3];
+  // exclusive sums over the adapters of their rows, tiles and chunks: an adapter a
+  // thread, over the lanes, then over the waves
+  static_assert(kPlanThreads >= kMax, "an adapter a thread");
   int32_t run[3] = {0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = 2 * tid + i;
+  if (tid < adapters) {
     int32_t n = 0;
-    if (e < adapters)
-      for (int w = 0; w < kPlanWaves; ++w) n += count[w][e];
-    v[i][0] = n;
-    v[i][1] = (n + plan.tile - 1) / plan.tile;
-    v[i][2] = (n + plan.chunk - 1) / plan.chunk;
-#pragma unroll
-    for (int q = 0; q < 3; ++q) run[q] += v[i][q];
+    for (int w = 0; w < kPlanWaves; ++w) n += count[w][tid];
+    run[0] = n;
+    run[1] = (n + plan.tile - 1) / plan.tile;
+    run[2] = (n + plan.chunk - 1) / plan.chunk;
   }
   int32_t before[3];
 #pragma unroll
@@ -140,14 +148,10 @@ __global__ void __launch_bounds__(kPlanThreads)
   for (int q = 0; q < 3; ++q) {
     int32_t s = before[q];
     for (int w = 0; w < wave; ++w) s += wave_sum[w][q];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = 2 * tid + i;
-      if (e <= adapters && e <= kMax) scan[q][e] = s;
-      s += v[i][q];
+    if (tid < adapters) {
+      scan[q][tid] = s;
+      if (tid == adapters - 1) scan[q][adapters] = s + run[q];
     }
-    // adapter kMax's entry is the end of the last thread's
-    if (tid == kPlanThreads - 1 && adapters == kMax) scan[q][kMax] = s;
   }
   __syncthreads();
   for (int e = tid; e <= adapters; e += kPlanThreads) {
@@ -172,25 +176,29 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
   }
   __syncthreads();
+  // bits of an adapter's number plus one; -1 (no adapter) has none set
+  const int bits = 32 - __builtin_clz(static_cast<unsigned>(adapters));
+  int32_t next = begin + lane < end ? out.rows[begin + lane] : -1;
   for (int64_t r0 = begin; r0 < end; r0 += 64) {
     const int64_t r = r0 + lane;
-    const int32_t e = r < end ? out.rows[r] : -2;
-    uint64_t left = __ballot(e >= -1);
-    while (left != 0) {
-      const int leader = __builtin_ctzll(left);
-      const int32_t mine = __shfl(e, leader, 64);
-      const uint64_t same = __ballot(e == mine);
+    const int32_t e = next;
+    next = r + 64 < end ? out.rows[r + 64] : -1;
+    uint64_t same = __ballot(r < end);  // the lanes of this lane's adapter
+    for (int i = 0; i < bits; ++i) {
+      const bool set = ((e + 1) >> i) & 1;
+      const uint64_t with = __ballot(set);
+      same &= set ? with : ~with;
+    }
+    if (r < end) {
+      const int leader = __builtin_ctzll(same);
       int32_t base = 0;
       if (lane == leader)
-        base = atomicAdd(mine >= 0 ? &count[wave][mine] : &none[wave],
+        base = atomicAdd(e >= 0 ? &count[wave][e] : &none[wave],
                          static_cast<int32_t>(__popcll(same)));
       base = __shfl(base, leader, 64);
-      if (e == mine) {
-        const int32_t at = base + __popcll(same & ((1ull << lane) - 1));
-        out.order[at] = static_cast<int32_t>(r);
-        out.sorted[at] = e;
-      }
-      left &= ~same;
+      const int32_t at = base + __popcll(same & ((1ull << lane) - 1));
+      out.order[at] = static_cast<int32_t>(r);
+      out.sorted[at] = e;
     }
   }
   // the records, with the adapter found by halving
@@ -219,6 +227,8 @@ __global__ void __launch_bounds__(kPlanThreads)
 // ---------------------------------------------------------------------------
 // h = drop(x) A_e^T, and dh = g B_e with B_e^T in A_e's place: one workgroup per
 // 16 G rows of an adapter, whose four waves take a quarter of K each and meet in LDS.
+// Bound by the rows' bytes: 16384 rows of 6144, 201 MB, in 52 (rank 32) and 56 us (rank
+// 16), 3.7 TB/s where a copy reaches 5.1; of 2048 with dropout 20.
 // ---------------------------------------------------------------------------
 struct ShrinkArgs {
   const uint16_t* x;
@@ -330,7 +340,8 @@ __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
 // out += s_e drop(h B_e^T), also dx += s_e drop(dh A_e) with A_e^T in B_e's place:
 // a wave has 16 rows of one adapter and 64 columns. Row r of MFMA i is column
 // 16 (r / 4) + 4 i + r % 4, so that the four give a lane 16 consecutive columns of
-// its row.
+// its row. Only where the product's epilogue does not add the term: ranks above 32 and
+// the shapes off the matrix-core products. A pass over y: 16384 x 2048 34 us.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
   const uint16_t* h;
@@ -414,7 +425,9 @@ __global__ void __launch_bounds__(256) k_bank_expand(ExpandArgs a) {
 // The adapters' gradients: a workgroup takes a chunk of one adapter's rows and
 // 128 columns of x (or g), [64 rows x 128 columns] at a time into LDS, from where
 // transposing reads feed the matrix cores; the chunks' f32 sums are joined in
-// order by a second launch, which also scales and rounds them.
+// order by a second launch, which also scales and rounds them. Bound by HBM: 16384 rows,
+// 2048 -> 6144, rank 16: 62 us for 269 MB (x, g, h and dh, 53 us at a copy's rate), the
+// joining 9.
 // ---------------------------------------------------------------------------
 constexpr int kGradRows = 64;
 constexpr int kGradColumns = 128;
@@ -434,6 +447,7 @@ struct GradPair {
   int stride, rank;
   const BankTile* chunks;
   const int32_t* order;
+  int64_t chunk_count;
   Dropout drop;
 };
 
@@ -462,11 +476,15 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
   __shared__ __align__(16) uint16_t sx[kGradRows * PX];
   __shared__ __align__(16) uint16_t sh[kGradRows * PH];
   __shared__ int32_t rows[kMaxChunk];
-  const BankTile chunk = a.chunks[blockIdx.y];
+  const int64_t blocks = a.part[0].blocks + a.part[1].blocks;
+  const int64_t number = block_of_grid() / blocks;
+  const int block = static_cast<int>(block_of_grid() % blocks);
+  if (number >= a.chunk_count) return;
+  const BankTile chunk = a.chunks[number];
   if (chunk.adapter < 0) return;
-  const int which = static_cast<int>(blockIdx.x) < a.part[0].blocks ? 0 : 1;
+  const int which = block < a.part[0].blocks ? 0 : 1;
   const GradArgs& g = a.part[which];
-  const int64_t p0 = static_cast<int64_t>(blockIdx.x - (which ? a.part[0].blocks : 0)) * kGradColumns;
+  const int64_t p0 = static_cast<int64_t>(block - (which ? a.part[0].blocks : 0)) * kGradColumns;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
@@ -541,12 +559,11 @@ __global__ void __launch_bounds__(256) k_bank_gradients(GradPair a) {
     }
   }
   constexpr int R = 16 * RB;
-  float* out = g.partials + static_cast<int64_t>(blockIdx.y) * g.p * R;
+  float* out = g.partials + number * g.p * R;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-{
+    for (int rb = 0; rb < RB; ++rb) {
       // lane: ranks 16 rb + 4 (lane >> 4) + v of column c
       const int64_t c = p0 + 32 * wave + 16 * i + (lane & 15);
       const int j = 16 * rb + 4 * (lane >> 4);
@@ -777,6 +794,7 @@ hipError_t launch_bank_gradients(const BankAdapterGradients& p, const BankPlan& 
   a.rank = static_cast<int>(p.rank);
   a.chunks = plan.chunks;
   a.order = plan.order;
+  a.chunk_count = plan.chunk_count;
   a.drop = p.drop;
   j.chunk_first = plan.chunk_first;
   j.scalings = p.scalings;
@@ -795,10 +813,10 @@ hipError_t launch_bank_gradients(const BankAdapterGradients& p, const BankPlan& 
     j.part[1] = JoinArgs{at, p.n * r, p.n, r, p.rank, p.n, 1.0f, p.d_b, p.b_dtype};
     j.blocks[1] = ceil_div(p.n * p.rank, 256);
   }
-  const int blocks = a.part[0].blocks + a.part[1].blocks;
+  const int64_t blocks = a.part[0].blocks + a.part[1].blocks;
   if (blocks == 0) return hipSuccess;
   if (plan.chunk_count > 0) {
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(plan.chunk_count));
+    const dim3 grid = grid_of(blocks * plan.chunk_count);
     const bool drop = p.d_a != nullptr && drops(p.drop), whole = p.k % 8 == 0 && p.n % 8 == 0;
     if (rb == 1) RPX_BANK_LAUNCH(k_bank_gradients, 1);
     else if (rb == 2) RPX_BANK_LAUNCH(k_bank_gradients, 2);
