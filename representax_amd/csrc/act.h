@@ -20,6 +20,7 @@ enum ActMode : int {
   kActSiluMulBwd = 4,  // out = v * silu(gate) (d up), out2 = v * up * silu'(gate) (d gate)
   kActAddBwd = 5,      // out = v + z: an input gradient added to the one accumulated so far
   kActBank = 6,        // no transform: the low-rank term is that of each row's own adapter
+  kActBankDrop = 7,    // the same, the term through a dropout
 };
 
 constexpr float kInvSqrt2 = 0.70710678118654752440f;

@@ -333,10 +333,13 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
       RPX_HIP(launch_int4_dequant_t(b.w.packed, b.w.scales, s.wt, b.n, b.k, b.w.packed_cols,
                                     b.w.n_groups, b.w.group, n64, st),
               "rpx_bank_backward: weight");
-      // a dropout's mask lies on the adapters' part alone: a pass after the product
-      const bool fused = b.drop.threshold >= 65536u && b.rank <= 32;
-      const LowRankEpilogue epi =
-          fused ? bank_epilogue(b, s.dh, s.at, b.k) : LowRankEpilogue{};
+      // a dropout's mask lies on the adapters' part alone; the epilogue applies it there
+      const bool fused = b.rank <= 32;
+      LowRankEpilogue epi = fused ? bank_epilogue(b, s.dh, s.at, b.k) : LowRankEpilogue{};
+      if (fused && b.drop.threshold < 65536u) {
+        epi.act = kActBankDrop;
+        epi.drop = b.drop;
+      }
       RPX_HIP(launch_gemm_bf16(ga, n64, s.wt, n64, b.m, b.k, n64, dx, b.k, epi, st),
               "rpx_bank_backward: dx");
       expand = !fused;

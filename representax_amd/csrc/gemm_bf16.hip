@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       const int trow = 8 * j + (lane >> 3);
       int64_t r = m0 + trow;
       r = r < M ? r : M - 1;
-      if constexpr (ACT == kActBank) r = epi.row_order[r];
+      if constexpr (ACT == kActBank || ACT == kActBankDrop) r = epi.row_order[r];
       src[i] = reinterpret_cast<const uint8_t*>(A + r * lda) + (((lane & 7) ^ swz(trow)) << 4);
     } else if constexpr (T4) {
       if (j < A_SEGS + P_SEGS) {
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   // idx = it * NT + tid of the tile) before the last K slice so that their
   // latency overlaps it; that slice runs outside the loop so the loop itself
   // does not carry their registers.
-  constexpr bool BANK = ACT == kActBank;
+  constexpr bool BANK = ACT == kActBank || ACT == kActBankDrop;
   constexpr bool PLAIN = ACT == kActNone || BANK;  // the rounded outputs are the results
   constexpr bool AUX_OPS = !PLAIN && ACT != kActGeluFwd;
   constexpr bool TWO_OPS = ACT == kActSiluMulBwd;
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       const int trow = 8 * (wave + d * NW) + (lane >> 3);
       int64_t r = m0 + trow;
       r = r < M ? r : M - 1;
-      if constexpr (ACT == kActBank) r = epi.row_order[r];
+      if constexpr (ACT == kActBank || ACT == kActBankDrop) r = epi.row_order[r];
       aoff[d] = static_cast<uint32_t>(r * lda * 2 + (((lane & 7) ^ swz(trow)) << 4));
     }
     uint32_t a_off[FM][4], b_off[FN][4];
@@ -958,6 +958,10 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
         }
       }
     };
+    constexpr bool DROP = ACT == kActBankDrop;
+    PhiloxCall call{};
+    if constexpr (DROP) call = philox_call(epi.drop);
+    uint32_t kept[FN];  // of the block's values
     auto add_adapter = [&](int g, int fm, bool own, float scale) {
 #pragma unroll
       for (int fn = 0; fn < FN; ++fn) {
@@ -969,8 +973,10 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
           t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga[g][jb][fn], cf[jb][fm], t, 0, 0, 0);
         if (own) {
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            acc[fn][fm][v] = __builtin_fmaf(scale, t[v], acc[fn][fm][v]);
+          for (int v = 0; v < 16; ++v) {
+            const float add = DROP ? dropout_masked(t[v], kept[fn], v) : t[v];
+            acc[fn][fm][v] = __builtin_fmaf(scale, add, acc[fn][fm][v]);
+          }
         }
       }
     };
@@ -994,6 +1000,13 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
       uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
+      if constexpr (DROP) {
+        const int64_t row = left != 0 ? out_row(mw + fm * 32 + frow < M ? mw + fm * 32 + frow : 0) : 0;
+#pragma unroll
+        for (int fn = 0; fn < FN; ++fn)
+          if (left != 0)
+            kept[fn] = dropout_block(call, epi.drop.threshold, row * N + nw + 32 * fn, half);
+      }
       while (left != 0) {
         int e[GA];
 #pragma unroll
@@ -1005,7 +1018,9 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
         cur = e[0];
 #pragma unroll
         for (int g = 0; g < GA; ++g)
-          if (e[g] >= 0) add_adapter(g, fm, mine[fm] == e[g], epi.adapter_scales[e[g]]);
+          if (e[g] >= 0)
+            add_adapter(g, fm, mine[fm] == e[g],
+                        epi.adapter_scales[e[g]] * (DROP ? epi.drop.scale : 1.0f));
       }
     }
   } else if (jblocks > 0) {
@@ -1353,6 +1368,9 @@ hipError_t run_gemm_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
   if constexpr (JB > 0 && !(BM == 256 && BN == 256)) {
     if constexpr (BK != kBInt4T && JB <= 2) {
       if (epi.act == kActBank) return RPX_RUN_ACT(kActBank);
+      if constexpr (BK == kBBf16) {
+        if (epi.act == kActBankDrop) return RPX_RUN_ACT(kActBankDrop);
+      }
     }
     if constexpr (BK == kBInt4 || BK == kBInt4L) {
       if (epi.act == kActGeluFwd) return RPX_RUN_ACT(kActGeluFwd);

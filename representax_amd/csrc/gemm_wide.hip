@@ -19,7 +19,7 @@
 // its outputs 32 rows at a time in its own few KB of LDS behind the two
 // stages, so the epilogue needs no workgroup barrier and leaves the pipeline
 // stages alone. The epilogue's arithmetic is not hidden (one workgroup per
-// CU), so its registers are: no kernel below spills more than 3 (with 40-140
+// CU), so its registers are: no kernel below without banks spills more than 3 (with 40-140
 // spilled the gated forward took 553 us instead of 423).
 //
 // Measured against k_gemm_nt's tiles, kernel traces, us (the forward's
@@ -29,6 +29,9 @@
 //   16384 x 6144 <- 2048, gated dx    641 -> 453
 //   32768 x 3072 <- 768, rank 16      GELU forward 285 -> 238, GELU dx 316 -> 254
 //   32768 x 768 <- 3072               forward 174 -> 134, dx 166 -> 134
+// With each row's own adapter in the epilogue and rows taken in a plan's order:
+//   16384 x 2048 <- 6144, rank 32     343; with a dropout on the term, rank 16, 336
+// (a mask's bits and four adapters' fragments together spilled 69 registers: two then).
 // The MFMA sequence of an output (which k go into which MFMA, and the order)
 // is k_gemm_nt's, so the outputs are the same bit for bit.
 #include <atomic>
@@ -124,7 +127,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (j < A_SEGS) {
         int r = tm * BM + trow;
         r = r < M ? r : M - 1;
-        if constexpr (ACT == kActBank) r = epi.row_order[r];
+        if constexpr (ACT == kActBank || ACT == kActBankDrop) r = epi.row_order[r];
         off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(lda_bytes) + chunk;
       } else {
         int r = tn * BN + trow;
@@ -193,7 +196,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   // bf16(t) * scale is already a bf16 value when scale = 2^k, k >= 0
   const bool scale_exact = (sbits & 0x807FFFFFu) == 0 && sbits >= 0x3F800000u && sbits < 0x7F800000u;
   // (the backward epilogues carry no bias)
-  constexpr bool BANK = ACT == kActBank;
+  constexpr bool BANK = ACT == kActBank || ACT == kActBankDrop;
+  constexpr bool DROP = ACT == kActBankDrop;
   const bool has_bias = (ACT == kActNone || BANK || ACT == kActGeluFwd || ACT == kActSiluMulFwd) && epi.bias != nullptr;
   const bool bias_vec = (reinterpret_cast<uintptr_t>(epi.bias) & 7) == 0;
   constexpr int kJB = JB > 0 ? JB : 1;
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
             reinterpret_cast<const uint8_t*>(epi.cols) + at + jb * 32);
     };
     // the fragments of up to GA adapters, ga[0] those of `cur`
-    constexpr int GA = JB > 1 ? 2 : 4;
+    constexpr int GA = JB > 1 || DROP ? 2 : 4;
     bf16x8_t ga[BANK ? GA : 1][kJB][FN];
     auto load_rows = [&](int g, int e) {
       const uint8_t* rows = reinterpret_cast<const uint8_t*>(epi.rows + e * epi.adapter_stride);
@@ -413,6 +417,18 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         // the adapters of the block's rows, GA at a time: their terms for all rows, kept
         // where the row is its, by a branch (no value of another adapter reaches a row)
         uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
+        uint32_t kept[FN];  // of the block's values
+        if constexpr (DROP) {
+          const PhiloxCall call = philox_call(epi.drop);
+#pragma unroll
+          for (int fn = 0; fn < FN; ++fn) {
+            __builtin_amdgcn_sched_barrier(0);
+            kept[fn] = 0;
+            if (left != 0)
+              kept[fn] = dropout_block(call, epi.drop.threshold,
+                                       static_cast<int64_t>(place[fm]) * N + nw + 32 * fn, el >> 5);
+          }
+        }
         while (left != 0) {
           int e[GA];
 #pragma unroll
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
           for (int g = 0; g < GA; ++g) {
             if (e[g] < 0) continue;
-            const float scale = epi.adapter_scales[e[g]];
+            const float scale = epi.adapter_scales[e[g]] * (DROP ? epi.drop.scale : 1.0f);
             const bool own = mine[fm] == e[g];
 #pragma unroll
             for (int fn = 0; fn < FN; ++fn) {
@@ -439,8 +455,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
                                                              0, 0);
               if (own) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v)
-                  acc[fn][fm][v] = __builtin_fmaf(scale, lr[v], acc[fn][fm][v]);
+                for (int v = 0; v < 16; ++v) {
+                  const float add = DROP ? dropout_masked(lr[v], kept[fn], v) : lr[v];
+                  acc[fn][fm][v] = __builtin_fmaf(scale, add, acc[fn][fm][v]);
+                }
               }
             }
           }
@@ -628,6 +646,7 @@ hipError_t run_wide_act(const uint16_t* a, int64_t lda, const uint16_t* b, int64
     case kActSiluMulBwd: return RPX_WIDE(kActSiluMulBwd);
     case kActAddBwd: return RPX_WIDE(kActAddBwd);
     case kActBank: return RPX_WIDE(kActBank);
+    case kActBankDrop: return RPX_WIDE(kActBankDrop);
     default: return hipErrorInvalidValue;
   }
 #undef RPX_WIDE
@@ -670,7 +689,7 @@ int wide_plan(int64_t m, int64_t n, int64_t k, int knob, int act, bool dequant) 
   const double t192 = first + ceil_div(tm * ceil_div(n, 192), 256) * (1.30 * s + 5.0);
   const double other =
       10.0 + 2.0 * static_cast<double>(m) * n * k / 0.93e9 * (1.0 + 200.0 / static_cast<double>(k));
-  const double margin = act == kActNone || act == kActAddBwd || act == kActBank ? 0.95 : 0.90;
+  const double margin = act == kActNone || act == kActAddBwd || act >= kActBank ? 0.95 : 0.90;
   const double t = t256 <= t192 ? t256 : t192;
   if (t >= margin * other) return 0;
   return t256 <= t192 ? kTileWide_256x256 : kTileWide_256x192;
@@ -695,7 +714,8 @@ bool wide_gemm_ok(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb
          m < (int64_t{1} << 31) - 256 && n < (int64_t{1} << 31) - 256 &&
          ceil_div(m, 256) * ceil_div(n, 192) < (int64_t{1} << 30) &&
          (epi.rank == 16 || epi.rank == 32 || (epi.rank == 0 && epi.act == kActNone) ||
-          (epi.act == kActBank && (epi.rank == 8 || epi.rank == 24) && epi.adapter_stride % 8 == 0)) &&
+          ((epi.act == kActBank || epi.act == kActBankDrop) &&
+           (epi.rank == 8 || epi.rank == 24) && epi.adapter_stride % 8 == 0)) &&
          (epi.rank == 0 || (epi.rows_sj == 1 && epi.cols_sj == 1 && epi.rows_sn % 8 == 0 &&
                             epi.cols_sm % 8 == 0 && m * epi.cols_sm * 2 < lim &&
                             n * epi.rows_sn * 2 < lim)) &&

@@ -60,6 +60,7 @@ struct LowRankEpilogue {
   const int32_t* row_order = nullptr;
   const int32_t* row_adapters = nullptr;
   const float* adapter_scales = nullptr;
+  Dropout drop{nullptr, 0, 65536u, 1.0f};  // kActBankDrop: of the term, over the output's elements
   int64_t adapter_stride = 0;
 };
 

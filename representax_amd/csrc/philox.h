@@ -91,4 +91,38 @@ __device__ __forceinline__ void dropout8(const PhiloxCall& call, const Dropout& 
   for (int j = 0; j < 8; ++j) v[j] = dropout_kept(bits, j, d.threshold) ? v[j] * d.scale : 0.0f;
 }
 
+// v, or zero where bit `bit` of the mask is clear: as bits, so that a NaN goes too.
+__device__ __forceinline__ float dropout_masked(float v, uint32_t mask, int bit) {
+  const int32_t all = static_cast<int32_t>(mask << (31 - bit)) >> 31;
+  return __builtin_bit_cast(float, __builtin_bit_cast(int32_t, v) & all);
+}
+
+// Which of a lane's 16 values of a 32 x 32 matrix-core block are kept: its row begins
+// (at the block's first column) at element `first`, a multiple of 8, and register v
+// holds column 8 (v / 4) + 4 (lane / 32) + v % 4: bit v. The two lanes of a row take two
+// of its four counters each and exchange what the other needs.
+__device__ __forceinline__ uint32_t dropout_block(const PhiloxCall& call, uint32_t threshold,
+                                                  int64_t first, int half) {
+  const uint64_t at = (static_cast<uint64_t>(first) >> 3) + 2 * half;
+  uint32_t mask = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4_t w = philox(call, at + i);
+    // columns 8 i + and 8 (i + 2) +: this lane's two words of each
+    const u32x2_t a =
+        __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false));
+    const u32x2_t b =
+        __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int v = 4 * (i + 2 * k);
+      mask |= static_cast<uint32_t>((a[k] & 0xFFFFu) < threshold) << v;
+      mask |= static_cast<uint32_t>((a[k] >> 16) < threshold) << (v + 1);
+      mask |= static_cast<uint32_t>((b[k] & 0xFFFFu) < threshold) << (v + 2);
+      mask |= static_cast<uint32_t>((b[k] >> 16) < threshold) << (v + 3);
+    }
+  }
+  return mask;
+}
+
 }  // namespace rpx

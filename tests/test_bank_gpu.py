@@ -150,10 +150,55 @@ def test_many_rows_and_adapters():
     Case(700, 128, 64, 8, 1024, "rows").check()
 
 
+@pytest.mark.parametrize("tile", [0, 18, 19])
+@pytest.mark.parametrize("rank", [5, 8, 16, 24, 32])
+@pytest.mark.parametrize("index", ["rows", "runs"])
+def test_dropout_in_every_product(tile, rank, index):
+    """The planners' tiles for these sizes, and both of the large products'."""
+
+    case = Case(600, 512, 456, rank, 5, index, rate=0.3)
+    with ops.tuning(int4_tile=tile, bf16_tile=tile):
+        case.check()
+
+
 def test_the_large_products():
     """Sizes that take the products over a bf16 copy of the weight."""
 
     Case(4500, 2048, 2048, 16, 4, "runs", group=64).check()
+
+
+def test_more_rows_than_a_grid_axis_and_32_bits_reach():
+    """2^24 rows are 65536 chunks of the gradients' sums; y has over 2^32 bytes."""
+
+    m, k, n, rank, adapters = (1 << 24) + 300, 64, 136, 4, 3
+    g = torch.Generator().manual_seed(8)
+    packed, scales, w = _weight(n, k, None, g)
+    x, dy = (torch.randn((m, c), device=DEV, dtype=BF16) for c in (k, n))
+    a = torch.randn((adapters, rank, k), device=DEV).to(BF16) / 8
+    b = torch.randn((adapters, n, rank), device=DEV).to(BF16)
+    s = torch.ones(adapters, device=DEV)
+    index = torch.arange(m, device=DEV, dtype=torch.int32) * 7 % (adapters + 1) - 1
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = rx.bank_linear(x, packed, scales, a, b, s, rx.adapter_plan(index, adapters))
+    dx, da, db = torch.autograd.grad(y, leaves, dy)
+    x, a, b, y = x.detach(), a.detach().to(F64), b.detach().to(F64), y.detach()
+    rows = torch.cat([torch.randint(0, m, (2000,), generator=g), torch.arange(m - 300, m)]).to(DEV)
+    e = index[rows].long().clamp_min(0)
+    on = (index[rows] >= 0).to(F64)[:, None]
+    xr, gr = x[rows].to(F64), dy[rows].to(F64)
+    h, dh = (xr[:, None] * a[e]).sum(2), (gr[..., None] * b[e]).sum(1)
+    assert _err(y[rows], xr @ w.t() + on * (h[:, None] * b[e]).sum(2)) <= 3 * STEP
+    assert _err(dx[rows], gr @ w + on * (dh[..., None] * a[e]).sum(1)) <= 3 * STEP
+    want_a, want_b = torch.zeros_like(a), torch.zeros_like(b)
+    for part in torch.arange(m, device=DEV).split(1 << 21):
+        for i in range(adapters):
+            at = part[index[part] == i]
+            xs, gs = x[at].to(F64), dy[at].to(F64)
+            want_a[i] += (gs @ b[i]).t() @ xs
+            want_b[i] += gs.t() @ (xs @ a[i].t())
+    # sums of 4 million terms of either sign: those of the rounded h and dh differ by their
+    # roundings' random walk, as the terms themselves do
+    assert _err(da, want_a) <= 2 * STEP and _err(db, want_b) <= 2 * STEP
 
 
 @pytest.mark.parametrize("m", [3, 40, 500])
