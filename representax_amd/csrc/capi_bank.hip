@@ -118,6 +118,19 @@ int wide_tile(const Bank& b) {
   return wide_plan(b.m, b.n, b.k, tune(kTuneInt4Tile), kActBank, true);
 }
 
+// Products that dequantize the weight first and run over the copy: the wide tiles; more
+// groups than the 64 KB of a tile's scales in LDS hold; and long sums in one round of 64-row
+// tiles, whose 64-column slices take 0.37 us over bf16 and 0.58 over packed weights, while
+// the copy costs 2 us and 0.67 more for every million of weights (and the host 4). Total us
+// with rank 16 and groups of 64, packed / copied: 6144 -> 2048 at 1000 rows 71 / 64, 8192 ->
+// 1024 90 / 72, 4096 -> 1024 50 / 44, 14336 -> 4096 at 333 rows 145 / 135.
+bool copied(const Bank& b) {
+  if (wide_tile(b) != 0 || b.w.n_groups > 256) return true;
+  const double k = static_cast<double>(b.k), weights = k * static_cast<double>(b.n);
+  return ceil_div(b.m, 64) * ceil_div(b.n, 128) <= 256 &&
+         (0.58 - 0.37) * k / 64 > 6.0 + 0.67e-6 * weights;
+}
+
 struct ForwardScratch {
   float* sums = nullptr;    // partial sums of h, or the base product of the generic path
   uint16_t* h = nullptr;
@@ -147,7 +160,7 @@ void forward_scratch(A& arena, const Bank& b, bool h_given, ForwardScratch* s) {
   if (!h_given) s->h = halves(b.m * stride);
   if (!fast(b))
     s->sums = floats(b.m * b.n);
-  else if (wide_tile(b) != 0)
+  else if (copied(b))
     s->weight = halves(b.n * b.k);
 }
 
@@ -257,20 +270,24 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
     const int tile = wide_tile(b);
     const bool fused =
         narrow && wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi);
-    if (tile != 0 &&
-        (fused || wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, base))) {
+    const bool wide =
+        tile != 0 && (fused || wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, base));
+    const bool copy = copied(b);
+    if (copy)
       RPX_HIP(launch_int4_dequant(b.w.packed, b.w.scales, s.weight, b.n, b.k, b.w.packed_cols,
                                   b.w.n_groups, b.w.group, st),
               "rpx_bank_forward: weight");
+    if (wide)
       RPX_HIP(launch_gemm_wide(tile, b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n,
                                fused ? epi : base, st),
               "rpx_bank_forward: product");
-      if (fused) return kOk;
-    } else {
+    else if (copy)
+      RPX_HIP(launch_gemm_bf16(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi, st),
+              "rpx_bank_forward: product");
+    else
       RPX_HIP(launch_gemm_int4(b.x, b.k, b.w, b.m, b.n, b.k, y, b.n, epi, st),
               "rpx_bank_forward: product");
-      if (narrow) return kOk;
-    }
+    if (wide ? fused : narrow) return kOk;
   } else {
     RPX_HIP(launch_generic_gemm(b.x, kBF16, b.k, 1, nullptr, kBF16, 0, 0, &b.w, false, b.m, b.n, b.k,
                                 s.sums, st),

@@ -1430,6 +1430,21 @@ hipError_t dispatch_int4(const uint16_t* a, int64_t lda, const Int4Operand& w, i
   if (cfg == kTileI4_256x128s2)
     return run_gemm<256, 128, 1, 4, 2, 2, kBInt4>(a, lda, nullptr, 0, w, m, n, k, out, ldc, epi,
                                                 stream);
+  if (cfg == kTileAuto && epi.act == kActBank) {
+    // Products of a few hundred rows are bound by their longest workgroup's slices (0.58 us
+    // a 64-column slice for 64 rows, 0.68 for 128, 1.0 for 256): the smallest tile that
+    // gives a CU one workgroup. Total us of 64 / 128 / 256 rows a tile with rank 16 and
+    // groups of 64: 6144 -> 2048 at 1000 rows 71 / 78 / 103, at 2000 rows 97 / 87 / 109, at
+    // 4000 180 / 134 / 128; 2048 -> 2048 at 1000 rows 29 / 34 / 46, 2048 -> 6144 at 333
+    // 37 / 35 / 49.
+    const int64_t across = ceil_div(n, 128);
+    if (ceil_div(m, 64) * across <= 256)
+      return run_gemm<64, 128, 1, 4, 3, 2, kBInt4>(a, lda, nullptr, 0, w, m, n, k, out, ldc, epi,
+                                                   stream);
+    if (ceil_div(m, 128) * across <= 256)
+      return run_gemm<128, 128, 1, 4, 2, 3, kBInt4>(a, lda, nullptr, 0, w, m, n, k, out, ldc, epi,
+                                                    stream);
+  }
   if (cfg < kTileI4_256x128 || cfg > kTileI4_64x128) {
     // Long reductions over outputs that split into whole 192-column tiles,
     // at least one round of them: the 256 x 192 tile that dequantizes each

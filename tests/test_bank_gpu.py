@@ -138,6 +138,19 @@ def test_shapes(m, k, n, group):
     Case(m, k, n, 8, 4, "rows", group=group, bias=True).check()
 
 
+@pytest.mark.parametrize("rank", [8, 40])
+def test_more_groups_than_a_tile_keeps(rank):
+    """1024 scales a row."""
+
+    Case(300, 32768, 72, rank, 3, "rows", group=32, bias=True).check()
+
+
+# one tile a CU of 64 and of 128 rows, and more
+@pytest.mark.parametrize("m", [257, 700, 1500])
+def test_tiles_of_a_few_hundred_rows(m):
+    Case(m, 1024, 2056, 16, 5, "runs", group=32).check()
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (50, 256, 72), (300, 256, 64), (90, 77, 30),
                                    (4500, 256, 128)])
 def test_dropout(m, k, n):
