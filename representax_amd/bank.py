@@ -106,7 +106,7 @@ def _bank_fields(x2d, packed, scale_bits, bias, a, b, scalings, plan, key, cfg):
 
 
 def _forward(x2d, a, b, packed, scale_bits, bias, scalings, plan, key, cfg, need_h):
-    device = _on_device(x2d, a, b, packed, scale_bits, bias, scalings, plan, key)
+    device = x2d.device
     fields = _bank_fields(x2d, packed, scale_bits, bias, a, b, scalings, plan, key, cfg)
     m = x2d.shape[0]
     y = torch.empty((m, packed.shape[0]), dtype=BF16, device=device)
@@ -205,8 +205,8 @@ def bank_linear(x: torch.Tensor, packed: torch.Tensor, scale_bits: torch.Tensor,
         raise ValueError("x must be [..., K]")
     k = x.shape[-1]
     n, e, _ = _check_bank(k, packed, scale_bits, lora_a, lora_b, scalings, group_size, bias)
-    lead = x.shape[:-1]
-    x2d = _aligned(x.reshape(-1, k))
+    flat = x.dim() == 2
+    x2d = _aligned(x if flat else x.reshape(-1, k))
     if plan.rows != x2d.shape[0] or plan.adapters != e:
         raise ValueError(f"the plan is one of {plan.rows} rows and {plan.adapters} adapters, x has "
                          f"{x2d.shape[0]} rows and the bank {e} adapters")
@@ -221,18 +221,17 @@ def bank_linear(x: torch.Tensor, packed: torch.Tensor, scale_bits: torch.Tensor,
               None if bias is None else _u16(bias).contiguous(), scalings.contiguous(), plan.buffer,
               key)
     _on_device(x2d, lora_a, lora_b, *frozen)
-    if torch.is_grad_enabled() and (scalings.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
+    grad = torch.is_grad_enabled()
+    if grad and (scalings.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("scalings and bias are constants of a bank: they get no gradients")
-    if torch.is_grad_enabled() and (x2d.requires_grad or lora_a.requires_grad
-                                    or lora_b.requires_grad):
+    if grad and (x2d.requires_grad or lora_a.requires_grad or lora_b.requires_grad):
         y = BankLinearFn.apply(x2d, lora_a, lora_b, *frozen, cfg)
     else:
-        a, b = (lora_a, lora_b)
+        a, b = lora_a, lora_b
         if a.dtype != BF16 or b.dtype != BF16:
             a, b = cast_many((a, b), BF16)
         y, _ = _forward(x2d, _aligned(a), _aligned(b), *frozen, cfg, False)
-    return y.reshape(*lead, n)
+    return y if flat else y.reshape(*x.shape[:-1], n)
 
 
 # ---------------------------------------------------------------------------
