@@ -445,6 +445,8 @@ def _rows_per_gate(gate: torch.Tensor, shape) -> int | None:
     go by leading axes."""
 
     lead = shape[:-1]
+    if gate.shape == shape[-1:]:
+        return math.prod(lead)
     g = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
     if g[-1] != shape[-1]:
         return None
@@ -465,7 +467,7 @@ def _parts(norm: torch.nn.Module | None):
     return kind, norm.weight, norm.bias if kind == nat.NORM_LAYER else None, norm.eps
 
 
-def _block_kernel(value, update, gate, weights, key) -> bool:
+def _block_kernel(value, update, gate, rows_per_gate, weights, key) -> bool:
     shape = value.shape
     size = shape[-1]
     index = value.get_device()
@@ -482,8 +484,7 @@ def _block_kernel(value, update, gate, weights, key) -> bool:
                 return False
     return ((key is None or plain_tensor(key))
             and (gate is None or (plain_tensor(gate) and gate.get_device() == index
-                                  and gate.dtype in (BF16, F32)
-                                  and _rows_per_gate(gate, shape) is not None)))
+                                  and gate.dtype in (BF16, F32) and rows_per_gate is not None)))
 
 
 def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.Tensor, *,
@@ -529,15 +530,14 @@ def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.
     kind, weight, bias, eps = before
     post_kind, post_weight, post_bias, post_eps = after
     cfg = {"kind": kind, "eps": eps, "post_kind": post_kind, "post_eps": post_eps,
-           "scale": float(scale), "threshold": threshold, "site": int(site), "rows_per_gate": 1}
+           "scale": float(scale), "threshold": threshold, "site": int(site),
+           "rows_per_gate": _rows_per_gate(gate, shape) if eager and gate is not None else 1}
     weights = (weight, bias, post_weight, post_bias)
-    if not (eager and _block_kernel(value, update, gate, weights, key)):
+    if not (eager and _block_kernel(value, update, gate, cfg["rows_per_gate"], weights, key)):
         return _block_expression(value, update, gate, *weights, key, cfg)
     value, update = value.contiguous(), update.contiguous()
     weight, bias, post_weight, post_bias = (None if w is None else w.contiguous() for w in weights)
-    if gate is not None:
-        cfg["rows_per_gate"] = _rows_per_gate(gate, value.shape)
-        gate = gate.contiguous()
+    gate = None if gate is None else gate.contiguous()
     key = None if key is None else key.contiguous()
     operands = (value, update, gate, weight, bias, post_weight, post_bias, key, cfg)
     if torch.is_grad_enabled():
