@@ -67,3 +67,39 @@ def test_a_captured_train_step_draws_a_new_key_each_replay():
         # the same steps: the optimizer's own kernels may differ in a rounding
         torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
     torch.testing.assert_close(eager.flat, captured.flat, rtol=1e-4, atol=1e-6)
+
+
+def test_a_captured_step_of_banks_with_every_dropout():
+    """Adapters of two tasks in one batch, their dropout and the hidden one, layers run
+    again in the backward: the captured step is the eager one, replay after replay, with
+    eager work between."""
+
+    index = torch.arange(8, device=DEV).repeat_interleave(16) % 3 - 1  # 4 queries, 4 documents
+    plan = rx.adapter_plan(index, 2)
+    key = torch.tensor([11, 0], device=DEV)
+    steps = []
+    for _ in range(2):
+        models = [_model(0.1), _model(0.1)]
+        with torch.no_grad():
+            for p in rx.lora_parameters(models[1]):
+                p.neg_()
+        steps.append(MNRTrainStep(rx.bank_quantized_lora(models, dropout=0.2).train(), batch=4,
+                                  sequence=16))
+    eager, captured = steps
+    with rx.adapter_rows(plan, key):
+        captured.capture(warmup=2)
+        for _ in range(2):
+            eager()
+    before, losses = captured.flat.detach().clone(), []
+    for step in range(1, 4):
+        key.copy_(torch.tensor([11, step], device=DEV))  # the adapters' masks of this step
+        with rx.adapter_rows(plan, key):
+            a = eager().clone()
+        b = captured().clone()
+        torch.cuda.synchronize()
+        # the same steps: the optimizer's own kernels may differ in a rounding
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
+        losses.append(float(b))
+    assert len(set(losses)) == 3 and bool(captured.finite)
+    torch.testing.assert_close(eager.flat, captured.flat, rtol=1e-4, atol=1e-6)
+    assert not torch.equal(before, captured.flat)
