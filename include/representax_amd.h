@@ -809,8 +809,9 @@ int rpx_block_backward(const rpx_block* block, const rpx_block_gradients* gradie
  *   y[i] = x[i] W_b^T + bias + s_e (dropout(x[i]) A_e^T) B_e^T
  * in bf16 with f32 sums (QuantizedLoRALinear.__call__, adapters.py:158-182, for
  * each row with its own adapter; one rounding of y instead of the reference's
- * three). h = dropout(x) A_e^T and its gradient are rounded to bf16, also where
- * they are f32 sums within a call.
+ * three). h = dropout(x) A_e^T and its gradient are rounded to bf16 where they
+ * are operands of matrix products; up to 64 rows, and up to 256 of few columns,
+ * y takes h as f32 sums.
  * ------------------------------------------------------------------------- */
 
 /* The rows of a batch sorted by adapter, for every projection that the batch

@@ -14,7 +14,8 @@ place of the adapters of several models over one base, and ``adapter_rows`` says
 which adapter each row of the calls inside it takes.
 
 The arithmetic is bf16 products with float32 sums and one rounding of y; h and
-its gradient, the operands of the second products, are rounded to bf16.
+its gradient are rounded to bf16 where they are operands of matrix products (for
+few rows, y takes h as float32 sums).
 """
 
 from __future__ import annotations

@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(256) k_bank_few_finish(FewArgs a) {
 #pragma unroll
     for (int i = 0; i < kMaxSlices; ++i) s += v[i];
     hs[at / a.stride][at % a.stride] = s;
-    if (p.h != nullptr && blockIdx.x == 0 && r < m) p.h[r * a.stride + at % a.stride] = f32_to_bf16(s);
+    if (p.h != nullptr && blockIdx.x == 0 && r < m && p.plan.rows[r] >= 0)
+      p.h[r * a.stride + at % a.stride] = f32_to_bf16(s);
   }
   __syncthreads();
   if (!in) return;
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) k_bank_one(FewArgs a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) s += hred[w][i][j];
     hs[i][j] = s;
-    if (p.h != nullptr && blockIdx.x == 0 && i < m && j < a.stride)
+    if (p.h != nullptr && blockIdx.x == 0 && i < m && j < a.stride && own[i] >= 0)
       p.h[i * a.stride + j] = j < rank ? f32_to_bf16(s) : 0;
   }
   __syncthreads();

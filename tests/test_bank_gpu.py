@@ -1,10 +1,11 @@
 """Adapters of many requests against their definition in float64 (GPU).
 
-y, dx: one rounding to bf16 of float32 sums (2^-9 of a value at most, relative to
-the norm less), on top of the rounding of h (dh) to bf16, whose independent errors of
-at most 2^-9 each enter the adapter's term, a part of y, as a norm does: together at
-most 2^-9 (1 + 1) where the adapter's term is as large as y (the tests' scalings make
-it about that). The calls that add the term to a base product already rounded (or
+One rounding to bf16 is off by at most 2^-8 of a value; over many values of spread
+significands x in [1, 2) its norm is 2^-7 / sqrt(12) against sqrt(mean x^2) = sqrt(7 / 3),
+2^-9.4 of theirs: STEP = 2^-9 a rounding. y, dx: one rounding of float32 sums, on top of
+the rounding of h (dh) to bf16, whose independent errors of 2^-9 each enter the
+adapter's term, a part of y, as a norm does: together at most 2^-9 (1 + 1) where the
+adapter's term is as large as y (the tests' scalings make it about that). The calls that add the term to a base product already rounded (or
 round that base first) add one rounding of each: 2^-9 (1 + 1 + 1) in all. dA, dB: sums
 of products with h or dh: 2^-9 (1 + 1) with bf16 gradients, 2^-9 with float32 ones.
 """
@@ -17,7 +18,7 @@ import torch
 import representax_amd as rx
 from oracle import dropout as odrop
 from representax_amd import _native as nat
-from representax_amd import ops
+from representax_amd import bank, ops
 from representax_amd.bank import AdapterPlan
 from representax_amd.trainstep import BertConfig, build_int4lora_encoder
 from tests.helpers import kernel_names
@@ -228,6 +229,28 @@ def test_no_adapter_and_one(m, index):
     if index < 0:
         got = case.train()
         assert not got[2].any() and not got[3].any()
+
+
+@pytest.mark.parametrize("m", [1, 2, 13, 40, 333, 4500])
+def test_rows_of_h_without_an_adapter_are_left(m):
+    case = Case(m, 128, 64, 4, 2, "rows")
+    case.index[m // 2] = -1
+    plan = rx.adapter_plan(case.index, 2)
+    y = torch.empty((m, 64), dtype=BF16, device=DEV)
+    h = torch.full((m, 8), 77.0, dtype=BF16, device=DEV)
+    cfg = {"group": 0, "site": 0, "threshold": 65536}
+    fields = bank._bank_fields(case.x, case.packed, case.scales, None, case.a, case.b, case.s,
+                               plan.buffer, None, cfg)
+    need = nat.bank_call("forward_workspace", fields, 1)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    nat.bank_call("forward", fields, y.data_ptr(), h.data_ptr(), ws.data_ptr(), need,
+                  torch.cuda.current_stream().cuda_stream)
+    none = case.index < 0
+    assert (h[none] == 77).all() and not h[~none][:, 4:].any()
+    e = case.index.long().clamp_min(0)
+    want = (case.x.to(F64)[:, None] * case.a.to(F64)[e]).sum(2)
+    # one rounding
+    assert bool(none.all()) or _err(h[~none][:, :4], want[~none]) <= STEP * 2
 
 
 def test_no_rows():

@@ -1,7 +1,8 @@
 """The boundary between two blocks against its definition in float64 (GPU).
 
-A value rounded once to bf16 is off by at most 2^-9 of itself where numbers are
-halfway at most (half a step, 2^-8 / 2 relative), and by far less in norm; the
+A value rounded once to bf16 is off by at most half a step, 2^-8 of itself; over many
+values the errors' norm is 2^-7 / sqrt(12) = 1.16 * 2^-9 of theirs where all significands
+are near 1, and less where they spread. The
 float32 sums before it (of at most 8192 values, statistics and the products of
 the gradients) add less than 2^-15. Gradients of the update come through a
 bf16 t: the same t as the definition's here, since the tests take it from the
