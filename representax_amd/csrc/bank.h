@@ -10,7 +10,7 @@ namespace rpx {
 
 constexpr int64_t kBankMaxAdapters = 1024;
 constexpr int64_t kBankMaxRank = 64;
-constexpr int64_t kBankSkinnyRows = 256;
+constexpr int64_t kBankSkinnyRows = 1024;
 
 // Rows of one adapter: positions [pos, end) of the plan's order.
 struct BankTile {

@@ -1,19 +1,23 @@
 // A projection of few rows, each with its own adapter of a bank, over the packed INT4
 // weight:
 //   y[m, n] = sum_k x[m, k] W[n, k] + bias[n] + s_e sum_j h[m, j] B_e[n, j].
-// Bound by launches and latency, then by the packed weight's bytes. Two launches, with
-// everything that is long in the first:
+// Bound by launches and latency, then by the packed weight's bytes, and from some 100
+// rows on by the reads of x in LDS. Two launches, with everything that is long in the first:
 //
-//   k_bank_few: workgroups for h = drop(x) A_e^T (16 rows of one adapter and a slice of
-//     K each) beside workgroups for x W^T (16 columns, up to 64 rows and a slice of K
-//     each). The latter read their packed rows once, dequantize them, bf16(q s), into
-//     matrix-core operands and multiply them with all their rows of x; eight waves take
-//     128-column chunks in turn and meet in LDS. Both leave f32 partial sums.
+//   k_bank_few (to 16 rows), k_bank_mid: workgroups for h = drop(x) A_e^T (16 rows of one
+//     adapter and a slice of K each) beside workgroups for x W^T, which read their packed
+//     rows once for 16 or 64 rows of x, dequantize them, bf16(q s), into matrix-core
+//     operands and multiply them. Both leave f32 partial sums.
 //   k_bank_few_finish: adds the partial sums in slice order, bias and adapter term, and
 //     rounds once.
 //
 // One or two rows with a small A (up to 64 KB) take one launch, in which every workgroup
 // computes h itself (A comes from L2): 768 -> 768, one row 5.5 us against 8.3.
+//
+// us, both launches, rank 16, groups of 64, at 1 (2048 -> 6144: one launch) / 13 / 17 / 64 /
+// 100 / 200 / 333 rows: 2048 -> 6144 6 / 12 / 12 / 14.6 / 20, 6144 -> 2048 10 / 11 / 14 / 16 / 18 /
+// 26 / 34, 2048 -> 2048 7 / 9.4 / 9.7 / 11 / 12.5 / 16 / 21, 768 -> 768 5.6 / 8.6 / 9.0 / 9.4 / 9.5 /
+// 9.8 / 10.4.
 #include "bank.h"
 
 namespace rpx {
@@ -32,29 +36,6 @@ __device__ __forceinline__ u32x4_t keep(u32x4_t v, bool ok) {
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                  __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-}
-
-// The values of register i of lanes 16 p .. 16 p + 15 change places with those of
-// register p of lanes 16 i .. 16 i + 15.
-__device__ __forceinline__ u32x4_t transposed(u32x4_t v) {
-  auto swap32 = [](uint32_t& a, uint32_t& b) {
-    const u32x2_t t =
-        __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(a, b, false, false));
-    a = t[0];
-    b = t[1];
-  };
-  auto swap16 = [](uint32_t& a, uint32_t& b) {
-    const u32x2_t t =
-        __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a, b, false, false));
-    a = t[0];
-    b = t[1];
-  };
-  uint32_t w0 = v[0], w1 = v[1], w2 = v[2], w3 = v[3];
-  swap32(w0, w2);
-  swap32(w1, w3);
-  swap16(w0, w1);
-  swap16(w2, w3);
-  return u32x4_t{w0, w1, w2, w3};
 }
 
 // Eight nibbles as bf16(q s): with u = nibble ^ 8, q s = fma(u, s, -8 s) is exact.
@@ -78,29 +59,26 @@ struct FewArgs {
   // h: blocks [0, h_blocks), tile-major, h_slices slices of h_slice columns
   int h_blocks, h_slices, h_slice;
   float* h_sums;  // [h_slices][m][stride]
-  // products: column blocks fastest, then slices of `chunks` chunks, then rows
+  // products: column blocks fastest, then slices of `chunks` chunks of 128, then rows
   int columns, slices, chunks;
   float* sums;  // [slices][m][n]
 };
 
-// This lane's chunks' loads and products: step s of chunk c multiplies k = 128 c + 32 s +
-// 8 part + [0, 8) (NATURAL), or 128 c + 32 part + 8 s + [0, 8), which spares the codes and
-// the scale their change of places between the lanes of a row; x then comes as 16 bytes
-// of every 64. With up to 16 rows the latter is faster (13 rows, 6144 -> 2048: by 0.3 us),
-// with more the former (32 rows, 2048 -> 6144: by 2.6 us).
-template <int MT, int U>
+// This lane's chunks' loads and products: step s of chunk c multiplies k = 128 c + 32 part +
+// 8 s + [0, 8), so that a lane's 16 bytes of codes and one scale serve four steps; x
+// comes as 16 bytes of every 64.
+template <int U>
 struct FewProduct {
-  static constexpr bool NATURAL = MT > 1;
   const uint8_t* packed;
   const uint16_t* scales;
-  const uint16_t* xrow[MT];
+  const uint16_t* xrow;
   int k_end, group_shift, part;
   bool grouped;
-  u32x4_t wq[U], xf[U][4][MT];
+  u32x4_t wq[U], xf[U][4];
   uint32_t ws[U];
-  f32x4_t acc[MT];
+  f32x4_t acc{0.f, 0.f, 0.f, 0.f};
 
-  __device__ __forceinline__ FewProduct(const FewArgs& a, int64_t n0, int row0, int lane) {
+  __device__ __forceinline__ FewProduct(const FewArgs& a, int64_t n0, int lane) {
     const BankSkinny& p = a.p;
     const int r = lane & 15;
     part = lane >> 4;
@@ -110,13 +88,7 @@ struct FewProduct {
     grouped = p.w.n_groups > 1;
     group_shift = a.group_shift;
     k_end = static_cast<int>(p.k);
-    const int m = static_cast<int>(p.m);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int row = row0 + 16 * mt + r;
-      xrow[mt] = p.x + static_cast<int64_t>(row < m ? row : m - 1) * p.k + (NATURAL ? 8 * part : 0);
-      acc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
+    xrow = p.x + static_cast<int64_t>(r < p.m ? r : p.m - 1) * p.k;
   }
   // unconditional: what lies past K's end is read from its beginning and not used
   __device__ __forceinline__ void load(int c0, int step) {
@@ -127,34 +99,20 @@ struct FewProduct {
       wq[u] = ld16(packed + piece / 2);
       ws[u] = scales[grouped ? piece >> group_shift : 0];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = (c0 + step * u) * 128 + 32 * s;
-        const int at = NATURAL ? (k < k_end ? k : 0) : piece + 8 * s;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) xf[u][s][mt] = ld16(xrow[mt] + at);
-      }
+      for (int s = 0; s < 4; ++s) xf[u][s] = ld16(xrow + piece + 8 * s);
     }
   }
-  __device__ __forceinline__ bool in(int c0, int step, int u, int s) const {
-    return (c0 + step * u) * 128 + (NATURAL ? 32 * s : 32 * part) < k_end;
+  __device__ __forceinline__ bool in(int c0, int step, int u) const {
+    return (c0 + step * u) * 128 + 32 * part < k_end;
   }
   __device__ __forceinline__ void multiply(int c0, int step) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      u32x4_t codes = wq[u];
-      u32x4_t scale{ws[u], ws[u], ws[u], ws[u]};
-      if constexpr (NATURAL) {
-        codes = transposed(codes);
-        scale = transposed(scale);
-      }
+      const bool ok = in(c0, step, u);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bool ok = in(c0, step, u, s);
-        u32x4_t w = dequant8(codes[s], bf16_to_f32(static_cast<uint16_t>(scale[s])));
-        w = keep(w, ok);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt] = mfma(w, keep(xf[u][s][mt], ok), acc[mt]);
-      }
+      for (int s = 0; s < 4; ++s)
+        acc = mfma(keep(dequant8(wq[u][s], bf16_to_f32(static_cast<uint16_t>(ws[u]))), ok),
+                   keep(xf[u][s], ok), acc);
     }
   }
 };
@@ -233,11 +191,11 @@ __device__ __forceinline__ void few_shrink(const FewArgs& a, int block, float* l
   }
 }
 
-// MT: tiles of 16 rows a product's workgroup takes. U: chunks a wave has in flight.
-template <int MT, int U, int RB, bool DROP>
+// Up to 16 rows: 16 columns and a slice of K a workgroup, whose waves take chunks of 128
+// in turn, U in flight, and meet in LDS.
+template <int U, int RB, bool DROP>
 __global__ void __launch_bounds__(kThreads) k_bank_few(FewArgs a) {
-  constexpr int kLds = kWaves * 256 * (MT > RB ? MT : RB);
-  __shared__ float lds[kLds];
+  __shared__ float lds[kWaves * 256 * RB];
   int block = blockIdx.x;
   if (block < a.h_blocks) {
     few_shrink<RB, DROP>(a, block, lds);
@@ -246,9 +204,7 @@ __global__ void __launch_bounds__(kThreads) k_bank_few(FewArgs a) {
   block -= a.h_blocks;
   const BankSkinny& p = a.p;
   const int64_t n0 = static_cast<int64_t>(block % a.columns) * 16;
-  const int rest = block / a.columns;
-  const int slice = rest % a.slices;
-  const int row0 = rest / a.slices * 16 * MT;
+  const int slice = block / a.columns;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -257,27 +213,135 @@ __global__ void __launch_bounds__(kThreads) k_bank_few(FewArgs a) {
   const int c0 = slice * a.chunks;
   int c1 = c0 + a.chunks;
   c1 = c1 < all ? c1 : all;
-  FewProduct<MT, U> f(a, n0, row0, lane);
+  FewProduct<U> f(a, n0, lane);
   f.k_end = c1 * 128 < f.k_end ? c1 * 128 : f.k_end;
   for (int c = c0 + wave; c < c1; c += kWaves * U) {
     f.load(c, kWaves);
     f.multiply(c, kWaves);
   }
-  // lane: columns n0 + 4 part + v of row 16 mt + (lane & 15)
+  // lane: columns n0 + 4 part + v of row (lane & 15)
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-      lds[(wave * MT + mt) * 256 + (lane & 15) * 16 + 4 * (lane >> 4) + v] = f.acc[mt][v];
+  for (int v = 0; v < 4; ++v) lds[wave * 256 + (lane & 15) * 16 + 4 * (lane >> 4) + v] = f.acc[v];
   __syncthreads();
+  if (tid >= 256) return;
+  const int row = tid / 16;
+  const int64_t col = n0 + tid % 16;
+  float s = 0.0f;
 #pragma unroll
-  for (int at = tid; at < MT * 256; at += kThreads) {
-    const int row = row0 + at / 16;
-    const int64_t col = n0 + at % 16;
-    float s = 0.0f;
+  for (int w = 0; w < kWaves; ++w) s += lds[w * 256 + tid];
+  if (row < m && col < p.n) a.sums[(static_cast<int64_t>(slice) * m + row) * p.n + col] = s;
+}
+
+// More rows: 64 of them, 128 columns and a slice of K a workgroup. A wave has 16 columns
+// and all rows, whose columns of x the workgroup keeps in LDS, 256 at a time in two
+// buffers; the next ones' loads, and the codes', run under the products. (32 columns a
+// wave halve the reads of LDS, but with their registers spilled to keep two workgroups a
+// CU 100 rows of 2048 -> 6144 took 25 us against 19.)
+constexpr int kMidRows = 64;
+constexpr int kMidStage = 256;
+constexpr int kMidPitch = kMidStage + 8;  // rows 4 banks apart
+
+template <int RB, bool DROP>
+__global__ void __launch_bounds__(kThreads) k_bank_mid(FewArgs a) {
+  constexpr int MT = kMidRows / 16;
+  constexpr int XV = kMidRows * kMidStage / 8 / kThreads;  // 16-byte pieces a thread
+  __shared__ __align__(16) uint16_t xs[2][kMidRows * kMidPitch];
+  static_assert(sizeof(xs) >= sizeof(float) * kWaves * 256 * RB, "h's partial sums meet there too");
+  int block = blockIdx.x;
+  if (block < a.h_blocks) {
+    few_shrink<RB, DROP>(a, block, reinterpret_cast<float*>(&xs[0][0]));
+    return;
+  }
+  block -= a.h_blocks;
+  const BankSkinny& p = a.p;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15;
+  const int part = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(block % a.columns) * (16 * kWaves) + wave * 16;
+  const int rest = block / a.columns;
+  const int slice = rest % a.slices;
+  const int row0 = rest / a.slices * kMidRows;
+  const int m = static_cast<int>(p.m);
+  const int k_begin = slice * a.chunks * 128;
+  int k_end = k_begin + a.chunks * 128;
+  k_end = k_end < p.k ? k_end : static_cast<int>(p.k);
+  const int64_t wrow = n0 + r < p.n ? n0 + r : p.n - 1;
+  const uint8_t* packed = p.w.packed + wrow * p.w.packed_cols;
+  const uint16_t* scales = p.w.scales + wrow * p.w.n_groups;
+  const uint16_t* xrow[XV];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += lds[w * MT * 256 + at];
-    if (row < m && col < p.n) a.sums[(static_cast<int64_t>(slice) * m + row) * p.n + col] = s;
+  for (int i = 0; i < XV; ++i) {
+    const int row = row0 + (tid + kThreads * i) / (kMidStage / 8);
+    xrow[i] = p.x + static_cast<int64_t>(row < m ? row : m - 1) * p.k;
+  }
+  const bool grouped = p.w.n_groups > 1;
+  const int kx = tid % (kMidStage / 8) * 8;
+  u32x4_t xr[XV], wq[2], wc[2];
+  uint32_t ws[2], wsc[2];
+  // what lies past the slice's end is read from its beginning and not used
+  auto load = [&](int kb) {
+    const int k = kb + kx;
+#pragma unroll
+    for (int i = 0; i < XV; ++i) xr[i] = ld16(xrow[i] + (k < k_end ? k : k_begin));
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int mine = kb + 128 * c + 32 * part;
+      const int piece = mine < k_end ? mine : k_begin;
+      wq[c] = ld16(packed + piece / 2);
+      ws[c] = scales[grouped ? piece >> a.group_shift : 0];
+    }
+  };
+  f32x4_t acc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  load(k_begin);
+  int buffer = 0;
+  for (int kb = k_begin; kb < k_end; kb += kMidStage) {
+    uint16_t* x = xs[buffer];
+#pragma unroll
+    for (int i = 0; i < XV; ++i)
+      *reinterpret_cast<u32x4_t*>(x + (tid + kThreads * i) / (kMidStage / 8) * kMidPitch + kx) =
+          keep(xr[i], kb + kx < k_end);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      wc[c] = wq[c];
+      wsc[c] = ws[c];
+    }
+    __syncthreads();
+    if (kb + kMidStage < k_end) load(kb + kMidStage);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const bool ok = kb + 128 * c + 32 * part < k_end;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const u32x4_t w =
+            keep(dequant8(wc[c][s], bf16_to_f32(static_cast<uint16_t>(wsc[c]))), ok);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          acc[mt] = mfma(w,
+                         *reinterpret_cast<const u32x4_t*>(x + (16 * mt + r) * kMidPitch + 128 * c +
+                                                           32 * part + 8 * s),
+                         acc[mt]);
+      }
+    }
+    buffer ^= 1;
+  }
+  // lane: columns n0 + 4 part + v of row 16 mt + r
+  const int64_t col = n0 + 4 * part;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = row0 + 16 * mt + r;
+    if (row >= m) continue;
+    float* out = a.sums + (static_cast<int64_t>(slice) * m + row) * p.n + col;
+    if (col + 4 <= p.n) {
+      __builtin_memcpy(out, &acc[mt], 16);
+    } else {
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (col + v < p.n) out[v] = acc[mt][v];
+    }
   }
 }
 
@@ -371,7 +435,7 @@ __global__ void __launch_bounds__(kThreads) k_bank_one(FewArgs a) {
   for (int i = 0; i < kOneRows; ++i)
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) hacc[i][rb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  FewProduct<1, U> f(a, n0, 0, lane);
+  FewProduct<U> f(a, n0, lane);
   for (int c = wave; c < chunks; c += kWaves * U) {
     f.load(c, kWaves);
 #pragma unroll
@@ -396,15 +460,15 @@ __global__ void __launch_bounds__(kThreads) k_bank_one(FewArgs a) {
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const bool ok = f.in(c, kWaves, u, s);
+            const bool ok = f.in(c, kWaves, u);
             hacc[i][rb] = mfma(keep(af[u][rb][s], ok && 16 * rb + r < rank),
-                               keep(f.xf[u][s][0], ok), hacc[i][rb]);
+                               keep(f.xf[u][s], ok), hacc[i][rb]);
           }
     }
     f.multiply(c, kWaves);
   }
 #pragma unroll
-  for (int v = 0; v < 4; ++v) red[wave][r * 16 + 4 * part + v] = f.acc[0][v];
+  for (int v = 0; v < 4; ++v) red[wave][r * 16 + 4 * part + v] = f.acc[v];
 #pragma unroll
   for (int i = 0; i < kOneRows; ++i)
 #pragma unroll
@@ -447,8 +511,10 @@ bool one_launch(const BankSkinny& p, const Dropout& drop) {
          p.m * p.rank * p.k * 2 <= kOneBytes;
 }
 
-// The split of a call over workgroups. Slices of K of at least 16 chunks (two a wave)
-// bring the products to about two workgroups a CU.
+// The rows that k_bank_few takes (13 rows of 6144 -> 2048 11.0 us, 13.6 in k_bank_mid).
+constexpr int64_t kFewRows = 16;
+
+// The split of a call over workgroups.
 FewArgs plan_few(const BankSkinny& p, const Dropout& drop) {
   FewArgs a{};
   a.p = p;
@@ -460,45 +526,64 @@ FewArgs plan_few(const BankSkinny& p, const Dropout& drop) {
   a.h_slice = static_cast<int>(ceil_div(ceil_div(p.k, a.h_slices), 64) * 64);
   a.h_slices = static_cast<int>(ceil_div(p.k, a.h_slice));
   a.h_blocks = static_cast<int>(p.plan.tile_count * a.h_slices);
-  a.columns = static_cast<int>(ceil_div(p.n, 16));
   const int64_t all = ceil_div(p.k, 128);
-  const int64_t rows = ceil_div(p.m, p.m <= 16 ? 16 : (p.m <= 32 ? 32 : 64));
-  int64_t s = 512 / (a.columns * rows);
-  const int64_t most = all / 16 < kMaxSlices ? all / 16 : kMaxSlices;
+  int64_t s, most;
+  if (p.m > kFewRows) {
+    // two workgroups a CU of slices of eight chunks and more, one of shorter ones, whose
+    // partial sums weigh more (100 rows of 2048 -> 6144 in two slices 19.2 us, in four 21.0;
+    // 333 of 6144 -> 2048 in two 37.7, in five 32.7), down to one stage where there are few
+    // (64 rows of 768 -> 768 in one slice 13.1, in three 9.4)
+    a.columns = static_cast<int>(ceil_div(p.n, 16 * kWaves));
+    const int64_t tiles = a.columns * ceil_div(p.m, kMidRows);
+    const int64_t two = 512 / tiles < all / 8 ? 512 / tiles : all / 8;
+    s = 256 / tiles > two ? 256 / tiles : two;
+    most = all / 2;
+  } else {
+    // about two workgroups a CU, slices of at least 16 chunks (two a wave)
+    a.columns = static_cast<int>(ceil_div(p.n, 16));
+    s = 512 / a.columns;
+    most = all / 16;
+  }
+  most = most < kMaxSlices ? most : kMaxSlices;
   s = s > most ? most : s;
   s = s < 1 ? 1 : s;
   a.chunks = static_cast<int>(ceil_div(all, s));
+  if (p.m > kFewRows) a.chunks += a.chunks & 1;  // whole stages
   a.slices = static_cast<int>(ceil_div(all, a.chunks));
   return a;
 }
 
-template <int MT, int U>
-void few(const FewArgs& a, unsigned blocks, hipStream_t stream) {
-  const bool drop = a.drop.threshold < 65536u;
-#define RPX_FEW(RB)                                                                            \
-  if (drop)                                                                                    \
-    hipLaunchKernelGGL((k_bank_few<MT, U, RB, true>), dim3(blocks), dim3(kThreads), 0, stream, \
-                       a);                                                                     \
-  else                                                                                         \
-    hipLaunchKernelGGL((k_bank_few<MT, U, RB, false>), dim3(blocks), dim3(kThreads), 0, stream, a)
+void partial_sums(const FewArgs& a, unsigned blocks, hipStream_t stream) {
+  const bool drop = a.drop.threshold < 65536u, few = a.p.m <= kFewRows;
+#define RPX_SUMS(RB)                                                                             \
+  if (few && drop)                                                                               \
+    hipLaunchKernelGGL((k_bank_few<2, RB, true>), dim3(blocks), dim3(kThreads), 0, stream, a);   \
+  else if (few)                                                                                  \
+    hipLaunchKernelGGL((k_bank_few<2, RB, false>), dim3(blocks), dim3(kThreads), 0, stream, a);  \
+  else if (drop)                                                                                 \
+    hipLaunchKernelGGL((k_bank_mid<RB, true>), dim3(blocks), dim3(kThreads), 0, stream, a);      \
+  else                                                                                           \
+    hipLaunchKernelGGL((k_bank_mid<RB, false>), dim3(blocks), dim3(kThreads), 0, stream, a)
   if (a.p.rank <= 16) {
-    RPX_FEW(1);
+    RPX_SUMS(1);
   } else if (a.p.rank <= 32) {
-    RPX_FEW(2);
+    RPX_SUMS(2);
   } else {
-    RPX_FEW(4);
+    RPX_SUMS(4);
   }
-#undef RPX_FEW
+#undef RPX_SUMS
 }
 
 }  // namespace
 
-// Up to 64 rows, and up to 256 of few columns: each block of 64 rows costs the whole
-// weight's dequantization again, while the tiles of the larger products cost 0.7 us a
-// 64-column slice of K however few there are (256 rows, 6144 -> 2048: 58 us here, 79
-// there; 2048 -> 6144: 63 and 45).
+// Up to 64 rows, and up to 1024 of few columns: each 64 rows cost the whole weight's
+// dequantization and their reads of x from LDS again, 0.37 to 0.49 us for every million of
+// weights, while the tiles of the larger products cost 0.58 us and more a 64-column slice of
+// K however few there are. us here / there: 2048 -> 6144 at 128 rows 21 / 28, at 200 31 / 29;
+// 2048 -> 2048 at 500 rows 23 / 28, at 1000 35 / 30; 6144 -> 2048 at 333 rows 33 / 60, at 1000
+// 80 / 64; 768 -> 768 at 1000 rows 15 / 16.
 bool bank_skinny_ok(int64_t m, int64_t n, int64_t k, int64_t n_groups, int64_t group) {
-  return m >= 1 && (m <= 64 || (m <= kBankSkinnyRows && n * ceil_div(m, 64) <= 10240)) &&
+  return m >= 1 && (m <= 64 || (m <= kBankSkinnyRows && n * ceil_div(m, kMidRows) <= 18432)) &&
          k % 32 == 0 &&
          (n_groups == 1 || (group % 32 == 0 && (group & (group - 1)) == 0));
 }
@@ -523,12 +608,8 @@ hipError_t launch_bank_skinny(const BankSkinny& p, const Dropout& drop, float* p
   }
   a.sums = partials;
   a.h_sums = partials + a.slices * p.m * p.n;
-  const int64_t tile = p.m <= 16 ? 16 : (p.m <= 32 ? 32 : 64);
-  const unsigned blocks = static_cast<unsigned>(a.h_blocks + a.columns * a.slices *
-                                                                 ceil_div(p.m, tile));
-  if (tile == 16) few<1, 2>(a, blocks, stream);
-  else if (tile == 32) few<2, 2>(a, blocks, stream);
-  else few<4, 2>(a, blocks, stream);
+  const int64_t rows = p.m <= kFewRows ? 1 : ceil_div(p.m, kMidRows);
+  partial_sums(a, static_cast<unsigned>(a.h_blocks + a.columns * a.slices * rows), stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(k_bank_few_finish,

@@ -118,13 +118,13 @@ class Case:
 
 
 # rows about the ends of the tiles and of the few-row kernels
-@pytest.mark.parametrize("m", [1, 2, 4, 5, 16, 17, 33, 64, 65, 130, 333])
+@pytest.mark.parametrize("m", [1, 2, 4, 5, 16, 17, 33, 64, 65, 130, 333, 1024, 1025])
 @pytest.mark.parametrize("index", ["rows", "runs"])
 def test_rows(m, index):
     Case(m, 256, 192, 16, 5, index, group=64, bias=m % 2 == 0).check()
 
 
-@pytest.mark.parametrize("m", [3, 40, 200])
+@pytest.mark.parametrize("m", [3, 40, 200, 1100])
 @pytest.mark.parametrize("rank", [1, 4, 8, 12, 16, 24, 32, 33, 48, 64])
 def test_ranks(m, rank):
     Case(m, 128, 136, rank, 3, "rows").check()
@@ -139,15 +139,23 @@ def test_shapes(m, k, n, group):
     Case(m, k, n, 8, 4, "rows", group=group, bias=True).check()
 
 
-@pytest.mark.parametrize("rank", [8, 40])
-def test_more_groups_than_a_tile_keeps(rank):
+@pytest.mark.parametrize("m,rank", [(300, 8), (1100, 8), (1100, 40)])
+def test_more_groups_than_a_tile_keeps(m, rank):
     """1024 scales a row."""
 
-    Case(300, 32768, 72, rank, 3, "rows", group=32, bias=True).check()
+    Case(m, 32768, 72, rank, 3, "rows", group=32, bias=True).check()
+
+
+# the ends of slices, stages and columns of up to 1024 rows
+@pytest.mark.parametrize("m", [16, 17, 64, 65, 321])
+@pytest.mark.parametrize("k,n,group", [(32, 33, None), (160, 131, 32), (288, 3, None),
+                                       (2080, 129, None), (4128, 257, None)])
+def test_few_rows_of_odd_columns(m, k, n, group):
+    Case(m, k, n, 12, 4, "rows", group=group, bias=True, rate=0.2).check()
 
 
 # one tile a CU of 64 and of 128 rows, and more
-@pytest.mark.parametrize("m", [257, 700, 1500])
+@pytest.mark.parametrize("m", [257, 700, 1300, 1500])
 def test_tiles_of_a_few_hundred_rows(m):
     Case(m, 1024, 2056, 16, 5, "runs", group=32).check()
 
@@ -170,7 +178,7 @@ def test_many_rows_and_adapters():
 def test_dropout_in_every_product(tile, rank, index):
     """The planners' tiles for these sizes, and both of the large products'."""
 
-    case = Case(600, 512, 456, rank, 5, index, rate=0.3)
+    case = Case(1100, 512, 456, rank, 5, index, rate=0.3)
     with ops.tuning(int4_tile=tile, bf16_tile=tile):
         case.check()
 
@@ -262,7 +270,7 @@ def test_no_rows():
     assert case.call().shape == (0, 32)
 
 
-@pytest.mark.parametrize("m", [4, 60, 600])
+@pytest.mark.parametrize("m", [4, 60, 600, 1200])
 def test_adapters_do_not_reach_each_others_rows(m):
     """Infinities and NaN of one adapter (and of its rows) stay with its rows, and
     their gradients with it."""
@@ -282,7 +290,7 @@ def test_adapters_do_not_reach_each_others_rows(m):
         assert torch.equal(got[i][[0, 2]], clean[i][[0, 2]])
 
 
-@pytest.mark.parametrize("m,rate", [(40, 0.0), (700, 0.2)])
+@pytest.mark.parametrize("m,rate", [(10, 0.1), (40, 0.0), (700, 0.2), (1300, 0.2)])
 def test_the_same_bits_every_time_and_in_every_order(m, rate):
     case = Case(m, 256, 128, 16, 4, "rows")
     case.rate = rate
