@@ -12,6 +12,8 @@ of products with h or dh: 2^-9 (1 + 1) with bf16 gradients, 2^-9 with float32 on
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -413,6 +415,28 @@ def test_two_streams():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_threads_on_streams_of_their_own():
+    cases = [Case(m, 256, 192, 16, 4, "rows", group=64, seed=m) for m in (2, 13, 100, 1100)]
+    want = [case.train() for case in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(case, expected):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got = case.train()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, expected)):
+                    wrong.append(case.x.shape)
+
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_gradients_of_constants_are_refused():
