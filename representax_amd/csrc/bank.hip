@@ -589,6 +589,7 @@ struct JoinArgs {
 };
 struct JoinPair {
   JoinArgs part[2];
+  int64_t adapters;
   int64_t blocks[2];  // workgroups an adapter
   const int32_t* chunk_first;
   const float* scalings;
@@ -597,6 +598,7 @@ struct JoinPair {
 __global__ void __launch_bounds__(256) k_bank_join(JoinPair a) {
   const int64_t per = a.blocks[0] + a.blocks[1];
   const int64_t e = block_of_grid() / per;
+  if (e >= a.adapters) return;  // a grid of several rows has more workgroups than adapters
   int64_t b = block_of_grid() % per;
   const int which = b < a.blocks[0] ? 0 : 1;
   if (which) b -= a.blocks[0];
@@ -796,6 +798,7 @@ hipError_t launch_bank_gradients(const BankAdapterGradients& p, const BankPlan& 
   a.order = plan.order;
   a.chunk_count = plan.chunk_count;
   a.drop = p.drop;
+  j.adapters = plan.adapters;
   j.chunk_first = plan.chunk_first;
   j.scalings = p.scalings;
   float* at = partials;
