@@ -289,12 +289,16 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
               "rpx_bank_forward: product");
     if (wide ? fused : narrow) return kOk;
   } else {
+    // the terms meet the float32 sums, and their total is rounded
     RPX_HIP(launch_generic_gemm(b.x, kBF16, b.k, 1, nullptr, kBF16, 0, 0, &b.w, false, b.m, b.n, b.k,
                                 s.sums, st),
             "rpx_bank_forward: base product");
-    RPX_HIP(launch_bank_store(s.sums, b.bias, b.m, b.n, y, st), "rpx_bank_forward: base product");
+    RPX_HIP(launch_bank_expand(h, b.b, b.rank, b.n, b.scalings, b.plan, kNoDropout, s.sums, kF32, st),
+            "rpx_bank_forward: up-projections");
+    RPX_HIP(launch_bank_store(s.sums, b.bias, b.m, b.n, y, st), "rpx_bank_forward: y");
+    return kOk;
   }
-  RPX_HIP(launch_bank_expand(h, b.b, b.rank, b.n, b.scalings, b.plan, kNoDropout, y, st),
+  RPX_HIP(launch_bank_expand(h, b.b, b.rank, b.n, b.scalings, b.plan, kNoDropout, y, kBF16, st),
           "rpx_bank_forward: up-projections");
   return kOk;
 }
@@ -364,10 +368,14 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
       RPX_HIP(launch_generic_gemm(g, kBF16, b.n, 1, nullptr, kBF16, 0, 0, &b.w, true, b.m, b.k, b.n,
                                   s.base, st),
               "rpx_bank_backward: dx");
+      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, s.base, kF32,
+                                 st),
+              "rpx_bank_backward: dx of the adapters");
       RPX_HIP(launch_bank_store(s.base, nullptr, b.m, b.k, dx, st), "rpx_bank_backward: dx");
+      expand = false;
     }
     if (expand)
-      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, dx, st),
+      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, dx, kBF16, st),
               "rpx_bank_backward: dx of the adapters");
   }
   if (da || db) {
