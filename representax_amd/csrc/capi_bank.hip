@@ -131,10 +131,15 @@ bool copied(const Bank& b) {
          (0.58 - 0.37) * k / 64 > 6.0 + 0.67e-6 * weights;
 }
 
+// The wide tiles read whole pieces of eight ranks: B of another rank is copied to rows of
+// them, with zeros behind (h has those zeros too).
+bool padded(const Bank& b) { return wide_tile(b) != 0 && b.rank <= 32 && b.rank % 8 != 0; }
+
 struct ForwardScratch {
   float* sums = nullptr;    // partial sums of h, or the base product of the generic path
   uint16_t* h = nullptr;
   uint16_t* weight = nullptr;
+  uint16_t* b = nullptr;
 };
 
 template <typename A>
@@ -162,6 +167,7 @@ void forward_scratch(A& arena, const Bank& b, bool h_given, ForwardScratch* s) {
     s->sums = floats(b.m * b.n);
   else if (copied(b))
     s->weight = halves(b.n * b.k);
+  if (fast(b) && padded(b)) s->b = halves(b.adapters * b.n * stride);
 }
 
 struct BackwardScratch {
@@ -262,24 +268,28 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
   RPX_HIP(launch_bank_shrink(b.x, b.k, b.a, b.rank, b.plan, b.drop, h, st),
           "rpx_bank_forward: down-projections");
   if (fast(b)) {
-    // Ranks above 32, and in the wide tiles those that are no multiple of 8, follow the
-    // base product in a pass of their own.
+    // Ranks above 32 follow the base product in a pass of their own.
     const bool narrow = b.rank <= 32;
-    LowRankEpilogue epi = narrow ? bank_epilogue(b, h, b.b, b.n) : LowRankEpilogue{}, base;
-    epi.bias = base.bias = b.bias;
+    LowRankEpilogue epi = narrow ? bank_epilogue(b, h, b.b, b.n) : LowRankEpilogue{};
+    epi.bias = b.bias;
+    if (padded(b)) {
+      const int64_t stride = bank_rank_stride(b.rank);
+      RPX_HIP(launch_bank_pad(b.b, b.adapters * b.n, b.rank, s.b, stride, st),
+              "rpx_bank_forward: adapters");
+      epi.rows = s.b;
+      epi.rows_sn = epi.rank = stride;
+      epi.adapter_stride = b.n * stride;
+    }
     const int tile = wide_tile(b);
-    const bool fused =
-        narrow && wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi);
     const bool wide =
-        tile != 0 && (fused || wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, base));
+        tile != 0 && wide_gemm_ok(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi);
     const bool copy = copied(b);
     if (copy)
       RPX_HIP(launch_int4_dequant(b.w.packed, b.w.scales, s.weight, b.n, b.k, b.w.packed_cols,
                                   b.w.n_groups, b.w.group, st),
               "rpx_bank_forward: weight");
     if (wide)
-      RPX_HIP(launch_gemm_wide(tile, b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n,
-                               fused ? epi : base, st),
+      RPX_HIP(launch_gemm_wide(tile, b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi, st),
               "rpx_bank_forward: product");
     else if (copy)
       RPX_HIP(launch_gemm_bf16(b.x, b.k, s.weight, b.k, b.m, b.n, b.k, y, b.n, epi, st),
@@ -287,7 +297,7 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
     else
       RPX_HIP(launch_gemm_int4(b.x, b.k, b.w, b.m, b.n, b.k, y, b.n, epi, st),
               "rpx_bank_forward: product");
-    if (wide ? fused : narrow) return kOk;
+    if (narrow) return kOk;
   } else {
     // the terms meet the float32 sums, and their total is rounded
     RPX_HIP(launch_generic_gemm(b.x, kBF16, b.k, 1, nullptr, kBF16, 0, 0, &b.w, false, b.m, b.n, b.k,

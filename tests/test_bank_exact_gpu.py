@@ -85,3 +85,23 @@ class Exact:
     (100, 100, 72, 40, None), (300, 77, 40, 64, None)])
 def test_shapes_off_the_matrix_core_products(m, k, n, rank, group, rate):
     Exact(m, k, n, rank, group).check(rate)
+
+
+# 256- and 192-column tiles of the large products, and the planners' own
+@pytest.mark.parametrize("tile", [0, 18, 19])
+@pytest.mark.parametrize("rank", [1, 4, 8, 12, 13, 16, 20, 24, 28, 32])
+def test_ranks_in_the_large_products(tile, rank):
+    with ops.tuning(int4_tile=tile, bf16_tile=tile):
+        for rate in (0.0, 0.5):
+            Exact(1100, 512, 456, rank, 64).check(rate)
+
+
+def test_a_small_rank_at_sizes_that_take_the_large_products():
+    Exact(4500, 2048, 2048, 4, 64).check(0.0)
+
+
+@pytest.mark.parametrize("m", [1, 2, 13, 64, 100, 333])
+@pytest.mark.parametrize("rank", [3, 16, 32])
+def test_few_rows(m, rank):
+    Exact(m, 256, 200, rank, 64).check(0.0)
+    Exact(m, 2048, 2056, rank, 64).check(0.5)
