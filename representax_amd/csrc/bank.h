@@ -47,10 +47,10 @@ hipError_t launch_bank_shrink(const uint16_t* x, int64_t k, const uint16_t* w, i
                               const BankPlan& plan, const Dropout& drop, uint16_t* h,
                               hipStream_t stream);
 // out[m, n] += s[adapter(m)] drop(sum_j h[m, j] w[adapter(m), n, j]); w [adapters, n, rank],
-// out of `dtype`.
+// out f32.
 hipError_t launch_bank_expand(const uint16_t* h, const uint16_t* w, int64_t rank, int64_t n,
                               const float* scalings, const BankPlan& plan, const Dropout& drop,
-                              void* out, int dtype, hipStream_t stream);
+                              float* out, hipStream_t stream);
 // Both gradients of the adapters:
 //   d_a[e, j, k] = s_e sum_{m of e} dh[m, j] drop(x[m, k]),
 //   d_b[e, n, j] = s_e sum_{m of e} g[m, n] h[m, j].

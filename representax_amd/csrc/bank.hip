@@ -340,8 +340,8 @@ __global__ void __launch_bounds__(256) k_bank_shrink(ShrinkArgs a) {
 // out += s_e drop(h B_e^T), also dx += s_e drop(dh A_e) with A_e^T in B_e's place:
 // a wave has 16 rows of one adapter and 64 columns. Row r of MFMA i is column
 // 16 (r / 4) + 4 i + r % 4, so that the four give a lane 16 consecutive columns of
-// its row. Only where the product's epilogue does not add the term: ranks above 32 and
-// the shapes off the matrix-core products. A pass over y: 16384 x 2048 34 us.
+// its row. Only for the shapes off the matrix-core products, whose base product it finds
+// as f32 sums; elsewhere the product's epilogue adds the term.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
   const uint16_t* h;
@@ -353,11 +353,11 @@ struct ExpandArgs {
   const BankTile* tiles;
   const int32_t* order;
   Dropout drop;
-  void* out;  // of T
+  float* out;
 };
 
-// T: Bf16 or float. KB: 32-rank blocks. WHOLE: n is a multiple of eight.
-template <typename T, int KB, bool DROP, bool WHOLE>
+// KB: 32-rank blocks. WHOLE: n is a multiple of eight.
+template <int KB, bool DROP, bool WHOLE>
 __global__ void __launch_bounds__(256) k_bank_expand(ExpandArgs a) {
   const BankTile tile = a.tiles[blockIdx.x];
   if (tile.adapter < 0) return;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(256) k_bank_expand(ExpandArgs a) {
       const int64_t c = c0 + 8 * q;
       if (c >= a.n) continue;
       const int count = clamp8(a.n - c);
-      T* at = static_cast<T*>(a.out) + row * a.n + c;
+      float* at = a.out + row * a.n + c;
       float v[8];
       load_row8<WHOLE>(at, count, v);
       u32x4_t bits{};
@@ -770,19 +770,14 @@ hipError_t launch_bank_shrink(const uint16_t* x, int64_t k, const uint16_t* w, i
 
 hipError_t launch_bank_expand(const uint16_t* h, const uint16_t* w, int64_t rank, int64_t n,
                               const float* scalings, const BankPlan& plan, const Dropout& dropout,
-                              void* out, int dtype, hipStream_t stream) {
+                              float* out, hipStream_t stream) {
   if (plan.m <= 0 || n <= 0) return hipSuccess;
   const ExpandArgs a{h, static_cast<int>(bank_rank_stride(rank)), w, static_cast<int>(rank), n,
                      scalings, plan.tiles, plan.order, dropout, out};
   const dim3 grid(static_cast<unsigned>(plan.tile_count), static_cast<unsigned>(ceil_div(n, 256)));
   const bool drop = drops(dropout), whole = n % 8 == 0;
-  if (dtype == kBF16) {
-    if (rank <= 32) RPX_BANK_LAUNCH(k_bank_expand, Bf16, 1);
-    else RPX_BANK_LAUNCH(k_bank_expand, Bf16, 2);
-  } else {
-    if (rank <= 32) RPX_BANK_LAUNCH(k_bank_expand, float, 1);
-    else RPX_BANK_LAUNCH(k_bank_expand, float, 2);
-  }
+  if (rank <= 32) RPX_BANK_LAUNCH(k_bank_expand, 1);
+  else RPX_BANK_LAUNCH(k_bank_expand, 2);
   return hipGetLastError();
 }
 

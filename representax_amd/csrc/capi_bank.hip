@@ -133,7 +133,7 @@ bool copied(const Bank& b) {
 
 // The wide tiles read whole pieces of eight ranks: B of another rank is copied to rows of
 // them, with zeros behind (h has those zeros too).
-bool padded(const Bank& b) { return wide_tile(b) != 0 && b.rank <= 32 && b.rank % 8 != 0; }
+bool padded(const Bank& b) { return wide_tile(b) != 0 && b.rank % 8 != 0; }
 
 struct ForwardScratch {
   float* sums = nullptr;    // partial sums of h, or the base product of the generic path
@@ -268,9 +268,7 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
   RPX_HIP(launch_bank_shrink(b.x, b.k, b.a, b.rank, b.plan, b.drop, h, st),
           "rpx_bank_forward: down-projections");
   if (fast(b)) {
-    // Ranks above 32 follow the base product in a pass of their own.
-    const bool narrow = b.rank <= 32;
-    LowRankEpilogue epi = narrow ? bank_epilogue(b, h, b.b, b.n) : LowRankEpilogue{};
+    LowRankEpilogue epi = bank_epilogue(b, h, b.b, b.n);
     epi.bias = b.bias;
     if (padded(b)) {
       const int64_t stride = bank_rank_stride(b.rank);
@@ -297,19 +295,15 @@ int rpx_bank_forward(const rpx_bank* bank, void* y_out, void* h_out, void* works
     else
       RPX_HIP(launch_gemm_int4(b.x, b.k, b.w, b.m, b.n, b.k, y, b.n, epi, st),
               "rpx_bank_forward: product");
-    if (narrow) return kOk;
   } else {
     // the terms meet the float32 sums, and their total is rounded
     RPX_HIP(launch_generic_gemm(b.x, kBF16, b.k, 1, nullptr, kBF16, 0, 0, &b.w, false, b.m, b.n, b.k,
                                 s.sums, st),
             "rpx_bank_forward: base product");
-    RPX_HIP(launch_bank_expand(h, b.b, b.rank, b.n, b.scalings, b.plan, kNoDropout, s.sums, kF32, st),
+    RPX_HIP(launch_bank_expand(h, b.b, b.rank, b.n, b.scalings, b.plan, kNoDropout, s.sums, st),
             "rpx_bank_forward: up-projections");
     RPX_HIP(launch_bank_store(s.sums, b.bias, b.m, b.n, y, st), "rpx_bank_forward: y");
-    return kOk;
   }
-  RPX_HIP(launch_bank_expand(h, b.b, b.rank, b.n, b.scalings, b.plan, kNoDropout, y, kBF16, st),
-          "rpx_bank_forward: up-projections");
   return kOk;
 }
 
@@ -350,7 +344,6 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
             "rpx_bank_backward: dh");
   }
   if (b.m > 0 && dx_wanted) {
-    bool expand = true;
     if (fast(b)) {
       const int64_t n64 = ceil_div(b.n, 64) * 64;
       const uint16_t* ga = g;
@@ -365,28 +358,21 @@ int rpx_bank_backward(const rpx_bank* bank, const void* grad, const void* h, voi
                                     b.w.n_groups, b.w.group, n64, st),
               "rpx_bank_backward: weight");
       // a dropout's mask lies on the adapters' part alone; the epilogue applies it there
-      const bool fused = b.rank <= 32;
-      LowRankEpilogue epi = fused ? bank_epilogue(b, s.dh, s.at, b.k) : LowRankEpilogue{};
-      if (fused && b.drop.threshold < 65536u) {
+      LowRankEpilogue epi = bank_epilogue(b, s.dh, s.at, b.k);
+      if (b.drop.threshold < 65536u) {
         epi.act = kActBankDrop;
         epi.drop = b.drop;
       }
       RPX_HIP(launch_gemm_bf16(ga, n64, s.wt, n64, b.m, b.k, n64, dx, b.k, epi, st),
               "rpx_bank_backward: dx");
-      expand = !fused;
     } else {
       RPX_HIP(launch_generic_gemm(g, kBF16, b.n, 1, nullptr, kBF16, 0, 0, &b.w, true, b.m, b.k, b.n,
                                   s.base, st),
               "rpx_bank_backward: dx");
-      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, s.base, kF32,
-                                 st),
+      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, s.base, st),
               "rpx_bank_backward: dx of the adapters");
       RPX_HIP(launch_bank_store(s.base, nullptr, b.m, b.k, dx, st), "rpx_bank_backward: dx");
-      expand = false;
     }
-    if (expand)
-      RPX_HIP(launch_bank_expand(s.dh, s.at, b.rank, b.k, b.scalings, b.plan, b.drop, dx, kBF16, st),
-              "rpx_bank_backward: dx of the adapters");
   }
   if (da || db) {
     const BankAdapterGradients p{b.x, g, static_cast<const uint16_t*>(h), s.dh, b.k, b.n, b.rank,

@@ -942,14 +942,17 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     // block's rows in turn, t = C R_e^T for all of them, added (scaled, in f32) where the
     // row is its: by a branch, so that no value of another adapter reaches a row. The
     // fragments of one adapter stay while blocks have no other (its rows are neighbours);
-    // of several, those of GA are loaded together.
-    constexpr int GA = kMaxJB * FN > 2 ? 2 : 4;
-    bf16x8_t ga[GA][kMaxJB][FN];
-    auto load_adapter = [&](int g, int e) {
+    // of several, those of GA are loaded together. Ranks above 32 come in halves, whose
+    // fragments take the same registers one after the other.
+    constexpr int HJB = kMaxJB > 2 ? 2 : kMaxJB;  // 16-rank blocks at a time
+    constexpr int HALVES = kMaxJB / HJB;
+    constexpr int GA = HJB * FN > 2 ? 2 : 4;
+    bf16x8_t ga[GA][HJB][FN];
+    auto load_adapter = [&](int g, int e, int h) {
       const uint16_t* rows = epi.rows + e * epi.adapter_stride;
 #pragma unroll
-      for (int jb = 0; jb < kMaxJB; ++jb) {
-        const int64_t jl = jb * 16 + half * 8;
+      for (int jb = 0; jb < HJB; ++jb) {
+        const int64_t jl = (h * HJB + jb) * 16 + half * 8;
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn) {
           const int64_t n = nw + fn * 32 + frow;
@@ -969,7 +972,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (int v = 0; v < 16; ++v) t[v] = 0.0f;
 #pragma unroll
-        for (int jb = 0; jb < kMaxJB; ++jb)
+        for (int jb = 0; jb < HJB; ++jb)
           t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga[g][jb][fn], cf[jb][fm], t, 0, 0, 0);
         if (own) {
 #pragma unroll
@@ -986,41 +989,52 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       const int64_t m = mw + fm * 32 + frow;
       mine[fm] = m < M ? epi.row_adapters[m] : -1;
     }
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm) {
+    auto load_cols = [&](int fm, int h) {
       const int64_t m = mine[fm] >= 0 ? out_row(mw + fm * 32 + frow) : 0;
 #pragma unroll
-      for (int jb = 0; jb < kMaxJB; ++jb) {
-        const int64_t jl = jb * 16 + half * 8;
+      for (int jb = 0; jb < HJB; ++jb) {
+        const int64_t jl = (h * HJB + jb) * 16 + half * 8;
         cf[jb][fm] = load8_j(epi.cols + (mine[fm] >= 0 ? m * epi.cols_sm + jl : 0), 1,
                              mine[fm] >= 0 ? valid8(epi.rank, jl) : 0);
       }
+    };
+    if constexpr (HALVES == 1) {
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm) load_cols(fm, 0);
     }
     int cur = -1;  // the adapter whose fragments ga[0] holds
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
-      uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
+      const uint32_t all = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
       if constexpr (DROP) {
-        const int64_t row = left != 0 ? out_row(mw + fm * 32 + frow < M ? mw + fm * 32 + frow : 0) : 0;
+        const int64_t row = all != 0 ? out_row(mw + fm * 32 + frow < M ? mw + fm * 32 + frow : 0) : 0;
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn)
-          if (left != 0)
+          if (all != 0)
             kept[fn] = dropout_block(call, epi.drop.threshold, row * N + nw + 32 * fn, half);
       }
-      while (left != 0) {
-        int e[GA];
 #pragma unroll
-        for (int g = 0; g < GA; ++g) {
-          e[g] = left != 0 ? __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left)) : -1;
-          left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e[g]));
-          if (e[g] >= 0 && !(g == 0 && e[0] == cur)) load_adapter(g, e[g]);
+      for (int h = 0; h < HALVES; ++h) {
+        if constexpr (HALVES > 1) {
+          load_cols(fm, h);
+          cur = -1;
         }
-        cur = e[0];
+        uint32_t left = all;
+        while (left != 0) {
+          int e[GA];
 #pragma unroll
-        for (int g = 0; g < GA; ++g)
-          if (e[g] >= 0)
-            add_adapter(g, fm, mine[fm] == e[g],
-                        epi.adapter_scales[e[g]] * (DROP ? epi.drop.scale : 1.0f));
+          for (int g = 0; g < GA; ++g) {
+            e[g] = left != 0 ? __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left)) : -1;
+            left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e[g]));
+            if (e[g] >= 0 && !(g == 0 && e[0] == cur)) load_adapter(g, e[g], h);
+          }
+          cur = e[0];
+#pragma unroll
+          for (int g = 0; g < GA; ++g)
+            if (e[g] >= 0)
+              add_adapter(g, fm, mine[fm] == e[g],
+                          epi.adapter_scales[e[g]] * (DROP ? epi.drop.scale : 1.0f));
+        }
       }
     }
   } else if (jblocks > 0) {
@@ -1366,7 +1380,7 @@ hipError_t run_gemm_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
   run_gemm_act<BM, BN, WM, WN, NS, WPE, BK, JB, ACT>(a, lda, b, ldb, w, m, n, k, out, ldc, epi, stream)
   if (epi.act == kActNone) return RPX_RUN_ACT(kActNone);
   if constexpr (JB > 0 && !(BM == 256 && BN == 256)) {
-    if constexpr (BK != kBInt4T && JB <= 2) {
+    if constexpr (BK != kBInt4T) {
       if (epi.act == kActBank) return RPX_RUN_ACT(kActBank);
       if constexpr (BK == kBBf16) {
         if (epi.act == kActBankDrop) return RPX_RUN_ACT(kActBankDrop);

@@ -32,6 +32,9 @@
 // With each row's own adapter in the epilogue and rows taken in a plan's order:
 //   16384 x 2048 <- 6144, rank 32     343; with a dropout on the term, rank 16, 336
 // (a mask's bits and four adapters' fragments together spilled 69 registers: two then).
+// Ranks 33 to 64 take the fragments' registers in halves, one adapter's at a time (two
+// spilled 74): a whole call of 16384 x 2048 <- 6144 at rank 32 / 64 435 / 460, of
+// 16384 x 6144 <- 2048 421 / 490.
 // The MFMA sequence of an output (which k go into which MFMA, and the order)
 // is k_gemm_nt's, so the outputs are the same bit for bit.
 #include <atomic>
@@ -200,7 +203,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   constexpr bool DROP = ACT == kActBankDrop;
   const bool has_bias = (ACT == kActNone || BANK || ACT == kActGeluFwd || ACT == kActSiluMulFwd) && epi.bias != nullptr;
   const bool bias_vec = (reinterpret_cast<uintptr_t>(epi.bias) & 7) == 0;
-  constexpr int kJB = JB > 0 ? JB : 1;
+  // 16-rank blocks at a time: the epilogue has registers for two, so a bank's ranks above
+  // 32 come in halves, one after the other
+  constexpr int kJB = JB > 2 ? 2 : (JB > 0 ? JB : 1);
+  constexpr int kHalves = JB > 2 ? JB / 2 : 1;
+  static_assert(kHalves == 1 || BANK, "ranks above 32 are a bank's alone");
 
   for (int t = first; t < tiles; t += grid) {
 #pragma unroll
@@ -273,31 +280,33 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       cur = epi.row_adapters[mw < M ? mw : M - 1];
       cur = cur < 0 ? 0 : cur;
     }
-    auto load_cols = [&](int fm) {
-      int r = mw + fm * 32 + (el & 31);
+    // of block i / kHalves of 32 rows, half i % kHalves of the rank
+    auto load_cols = [&](int i) {
+      int r = mw + i * 32 + (el & 31);
       r = r < M ? r : M - 1;
-      if constexpr (BANK) r = place[fm];
+      if constexpr (BANK) r = place[i / kHalves];
       const uint32_t at = static_cast<uint32_t>(r) * static_cast<uint32_t>(2 * epi.cols_sm) + (el >> 5) * 16;
       if constexpr (BANK) {
-        // ranks of 8 and 24 end in the middle of a 16-rank block
+        // ranks that are no multiple of 16 end in the middle of a 16-rank block
 #pragma unroll
         for (int jb = 0; jb < kJB; ++jb) {
-          const bool in = jb * 16 + (el >> 5) * 8 < epi.rank;
+          const int block = (i % kHalves) * kJB + jb;
+          const bool in = block * 16 + (el >> 5) * 8 < epi.rank;
           const u32x4_t v = *reinterpret_cast<const u32x4_t*>(
-              reinterpret_cast<const uint8_t*>(epi.cols) + at + (in ? jb * 32 : -(el >> 5) * 16));
-          cf[fm & 1][jb] = as_bf16x8(in ? v : u32x4_t{0u, 0u, 0u, 0u});
+              reinterpret_cast<const uint8_t*>(epi.cols) + at + (in ? block * 32 : -(el >> 5) * 16));
+          cf[i & 1][jb] = as_bf16x8(in ? v : u32x4_t{0u, 0u, 0u, 0u});
         }
         return;
       }
 #pragma unroll
       for (int jb = 0; jb < kJB; ++jb)
-        cf[fm & 1][jb] = *reinterpret_cast<const bf16x8_t*>(
+        cf[i & 1][jb] = *reinterpret_cast<const bf16x8_t*>(
             reinterpret_cast<const uint8_t*>(epi.cols) + at + jb * 32);
     };
     // the fragments of up to GA adapters, ga[0] those of `cur`
-    constexpr int GA = JB > 1 || DROP ? 2 : 4;
+    constexpr int GA = kHalves > 1 ? 1 : (kJB > 1 || DROP ? 2 : 4);
     bf16x8_t ga[BANK ? GA : 1][kJB][FN];
-    auto load_rows = [&](int g, int e) {
+    auto load_rows = [&](int g, int e, int h) {
       const uint8_t* rows = reinterpret_cast<const uint8_t*>(epi.rows + e * epi.adapter_stride);
 #pragma unroll
       for (int fn = 0; fn < FN; ++fn) {
@@ -306,7 +315,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         const uint32_t at = static_cast<uint32_t>(n) * static_cast<uint32_t>(2 * epi.rows_sn);
 #pragma unroll
         for (int jb = 0; jb < kJB; ++jb) {
-          const int j = jb * 16 + (el >> 5) * 8;
+          const int j = (h * kJB + jb) * 16 + (el >> 5) * 8;
           const u32x4_t v =
               *reinterpret_cast<const u32x4_t*>(rows + at + (j < epi.rank ? 2 * j : 0));
           ga[g][jb][fn] = as_bf16x8(j < epi.rank ? v : u32x4_t{0u, 0u, 0u, 0u});
@@ -340,7 +349,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           place[fm] = epi.row_order[r < M ? r : M - 1];
           if (r >= M) mine[fm] = -1;
         }
-        load_rows(0, cur);
+        load_rows(0, cur, 0);
         load_cols(0);
       } else if constexpr (JB > 0) {
 #pragma unroll
@@ -410,54 +419,64 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     // which would spill.
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
-      if constexpr (JB > 0) {
+      if constexpr (JB > 0 && !BANK) {
         if (fm + 1 < FM) load_cols(fm + 1);
       }
       if constexpr (BANK) {
         // the adapters of the block's rows, GA at a time: their terms for all rows, kept
         // where the row is its, by a branch (no value of another adapter reaches a row)
-        uint32_t left = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
+        const uint32_t all = static_cast<uint32_t>(__ballot(mine[fm] >= 0));
         uint32_t kept[FN];  // of the block's values
-        if constexpr (DROP) {
-          const PhiloxCall call = philox_call(epi.drop);
 #pragma unroll
-          for (int fn = 0; fn < FN; ++fn) {
-            __builtin_amdgcn_sched_barrier(0);
-            kept[fn] = 0;
-            if (left != 0)
-              kept[fn] = dropout_block(call, epi.drop.threshold,
-                                       static_cast<int64_t>(place[fm]) * N + nw + 32 * fn, el >> 5);
+        for (int h = 0; h < kHalves; ++h) {
+          const int i = fm * kHalves + h;
+          if (i + 1 < FM * kHalves) load_cols(i + 1);
+          if constexpr (DROP) {
+            if (h == 0) {
+              const PhiloxCall call = philox_call(epi.drop);
+#pragma unroll
+              for (int fn = 0; fn < FN; ++fn) {
+                __builtin_amdgcn_sched_barrier(0);
+                kept[fn] = 0;
+                if (all != 0)
+                  kept[fn] = dropout_block(call, epi.drop.threshold,
+                                           static_cast<int64_t>(place[fm]) * N + nw + 32 * fn,
+                                           el >> 5);
+              }
+            }
           }
-        }
-        while (left != 0) {
-          int e[GA];
+          if (kHalves > 1 && i > 0) cur = -1;  // ga[0] holds the other half
+          uint32_t left = all;
+          while (left != 0) {
+            int e[GA];
 #pragma unroll
-          for (int g = 0; g < GA; ++g) {
-            e[g] = left != 0 ? __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left)) : -1;
-            left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e[g]));
-            if (e[g] >= 0 && !(g == 0 && e[0] == cur)) load_rows(g, e[g]);
-          }
-          cur = e[0];
+            for (int g = 0; g < GA; ++g) {
+              e[g] = left != 0 ? __builtin_amdgcn_readlane(mine[fm], __builtin_ctz(left)) : -1;
+              left &= ~static_cast<uint32_t>(__ballot(mine[fm] == e[g]));
+              if (e[g] >= 0 && !(g == 0 && e[0] == cur)) load_rows(g, e[g], h);
+            }
+            cur = e[0];
 #pragma unroll
-          for (int g = 0; g < GA; ++g) {
-            if (e[g] < 0) continue;
-            const float scale = epi.adapter_scales[e[g]] * (DROP ? epi.drop.scale : 1.0f);
-            const bool own = mine[fm] == e[g];
+            for (int g = 0; g < GA; ++g) {
+              if (e[g] < 0) continue;
+              const float scale = epi.adapter_scales[e[g]] * (DROP ? epi.drop.scale : 1.0f);
+              const bool own = mine[fm] == e[g];
 #pragma unroll
-            for (int fn = 0; fn < FN; ++fn) {
-              __builtin_amdgcn_sched_barrier(0);
-              f32x16_t lr;
+              for (int fn = 0; fn < FN; ++fn) {
+                __builtin_amdgcn_sched_barrier(0);
+                f32x16_t lr;
 #pragma unroll
-              for (int v = 0; v < 16; ++v) lr[v] = 0.0f;
+                for (int v = 0; v < 16; ++v) lr[v] = 0.0f;
 #pragma unroll
-              for (int jb = 0; jb < kJB; ++jb)
-                lr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga[g][jb][fn], cf[fm & 1][jb], lr, 0,
-                                                             0, 0);
-              if (own) {
+                for (int jb = 0; jb < kJB; ++jb)
+                  lr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga[g][jb][fn], cf[i & 1][jb], lr, 0,
+                                                               0, 0);
+                if (own) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                  const float add = DROP ? dropout_masked(lr[v], kept[fn], v) : lr[v];
-                  acc[fn][fm][v] = __builtin_fmaf(scale, add, acc[fn][fm][v]);
+                  for (int v = 0; v < 16; ++v) {
+                    const float add = DROP ? dropout_masked(lr[v], kept[fn], v) : lr[v];
+                    acc[fn][fm][v] = __builtin_fmaf(scale, add, acc[fn][fm][v]);
+                  }
                 }
               }
             }
@@ -660,7 +679,9 @@ hipError_t run_wide_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
     return run_wide<BN, WM, WN, 0, kActNone>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
   if (epi.rank <= 16)
     return run_wide_act<BN, WM, WN, 1>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
-  return run_wide_act<BN, WM, WN, 2>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
+  if (epi.rank <= 32)
+    return run_wide_act<BN, WM, WN, 2>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
+  return run_wide<BN, WM, WN, 4, kActBank>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
 }
 
 }  // namespace
@@ -707,15 +728,19 @@ bool wide_gemm_ok(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb
   // 32-bit row offsets of the operands; 16-byte pieces everywhere; a LoRA
   // term of rank 16 or 32 with unit stride: two 16-rank blocks are what the
   // epilogue has registers for (48 and 64 would spill), and its loads read whole
-  // blocks, so other ranks, also below 16, stay with k_gemm_nt, which pads them
+  // blocks, so other ranks, also below 16, stay with k_gemm_nt, which pads them.
+  // A bank's term is read in pieces of eight ranks, 32 ranks at a time: every
+  // multiple of 8 up to 64, and up to 32 where the epilogue also makes a
+  // dropout's bits (more spilled 120 registers)
   const int64_t lim = int64_t{1} << 32;
   return m > 0 && n > 0 && k > 0 && k % kBK == 0 && lda % 8 == 0 && ldb % 8 == 0 && n % 8 == 0 &&
          ldc % 8 == 0 && (ptrs & 15) == 0 && m * lda * 2 < lim && n * ldb * 2 < lim &&
          m < (int64_t{1} << 31) - 256 && n < (int64_t{1} << 31) - 256 &&
          ceil_div(m, 256) * ceil_div(n, 192) < (int64_t{1} << 30) &&
          (epi.rank == 16 || epi.rank == 32 || (epi.rank == 0 && epi.act == kActNone) ||
-          ((epi.act == kActBank || epi.act == kActBankDrop) &&
-           (epi.rank == 8 || epi.rank == 24) && epi.adapter_stride % 8 == 0)) &&
+          ((epi.act == kActBank || epi.act == kActBankDrop) && epi.rank % 8 == 0 &&
+           epi.rank >= 8 && epi.rank <= (epi.act == kActBank ? 64 : 32) &&
+           epi.adapter_stride % 8 == 0)) &&
          (epi.rank == 0 || (epi.rows_sj == 1 && epi.cols_sj == 1 && epi.rows_sn % 8 == 0 &&
                             epi.cols_sm % 8 == 0 && m * epi.cols_sm * 2 < lim &&
                             n * epi.rows_sn * 2 < lim)) &&

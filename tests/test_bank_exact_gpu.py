@@ -105,3 +105,26 @@ def test_a_small_rank_at_sizes_that_take_the_large_products():
 def test_few_rows(m, rank):
     Exact(m, 256, 200, rank, 64).check(0.0)
     Exact(m, 2048, 2056, rank, 64).check(0.5)
+
+
+@pytest.mark.parametrize("rank", [33, 40, 47, 48, 56, 64])
+def test_ranks_above_32(rank):
+    for m, k, n, group, tile in [(1100, 512, 456, 64, 0), (1100, 512, 456, 64, 18),
+                                 (1100, 512, 456, 64, 19), (4500, 256, 264, None, 0),
+                                 (100, 256, 33, 64, 0), (700, 1024, 2056, 32, 0)]:
+        with ops.tuning(int4_tile=tile, bf16_tile=tile):
+            for rate in (0.0, 0.5):
+                Exact(m, k, n, rank, group).check(rate)
+
+
+# every tile of packed weights (y) and of copied ones (dx) that has activation epilogues
+@pytest.mark.parametrize("rank", [16, 32, 64])
+@pytest.mark.parametrize("int4,bf16", [(1, 4), (2, 5), (3, 6), (10, 9), (11, 13), (12, 0), (17, 0)])
+def test_every_tile(int4, bf16, rank):
+    with ops.tuning(int4_tile=int4, bf16_tile=bf16):
+        for rate in (0.0, 0.5):
+            Exact(1100, 384, 392, rank, 64).check(rate)
+
+
+def test_rank_64_at_sizes_that_take_the_large_products():
+    Exact(4500, 2048, 2048, 64, 64).check(0.0)
