@@ -420,9 +420,12 @@ class BlockNormFn(torch.autograd.Function):
         if not _kernel_gradients(dt, dh):
             again = torch.is_grad_enabled()
             with torch.enable_grad():
-                outs = _block_expression(*inputs, key, ctx.cfg)
+                # views, so that an input's gradient is its own place's alone: not also what
+                # reaches it through another that was made from it, or is the same tensor
+                places = [None if v is None else v.view_as(v) for v in inputs]
+                outs = _block_expression(*places, key, ctx.cfg)
             pairs = [(o, g) for o, g in zip(outs, (dt, dh)) if g is not None]
-            leaves = [v for v, need in zip(inputs, wanted) if need]
+            leaves = [v for v, need in zip(places, wanted) if need]
             grads = iter(torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs],
                                              create_graph=again, allow_unused=True))
             return (*(next(grads) if need else None for need in wanted), *none)

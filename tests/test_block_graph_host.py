@@ -1,0 +1,74 @@
+"""Gradients of ``block_norm``'s autograd node that are themselves differentiated, with the
+kernel's forward replaced by the torch expression (CPU)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import representax_amd as rx
+from representax_amd import norms
+
+F64 = torch.float64
+
+
+@pytest.fixture
+def node(monkeypatch):
+    """Calls take the autograd node, as bf16 and float32 device values do."""
+
+    def forward(*operands):
+        with torch.no_grad():
+            return norms._block_expression(*operands)
+
+    monkeypatch.setattr(norms, "_block_kernel", lambda *a: True)
+    monkeypatch.setattr(norms, "_block_forward", forward)
+
+
+def _parts():
+    g = torch.Generator().manual_seed(2)
+    draw = lambda *s: torch.randn(*s, generator=g, dtype=F64)
+    norm, w, x = rx.RMSNorm(12, 1e-6).double(), draw(12, 12), draw(3, 5, 12)
+    with torch.no_grad():
+        norm.weight.copy_(draw(12))
+    return norm, w.requires_grad_(True), x.requires_grad_(True)
+
+
+def _layer(norm, w, x):
+    """A block whose update and gate come from its stream, one norm before and after it."""
+
+    return rx.block_norm(norm, x, torch.sin(x @ w), post=norm, gate=torch.tanh(x[:, :1] * 2),
+                         scale=0.5, rate=0.25, key=torch.tensor([4, 2]), site=1)
+
+
+def _loss(out):
+    return (out[0] ** 2).sum() + (out[1] ** 3).sum()
+
+
+@pytest.mark.parametrize("call", [_layer, lambda norm, w, x: rx.block_norm(norm, x @ w, x @ w),
+                                  lambda norm, w, x: (lambda v: rx.block_norm(norm, v, v))(x @ w)])
+def test_gradients_that_keep_their_graph(node, call, monkeypatch):
+    norm, w, x = _parts()
+    leaves = (x, w, norm.weight)
+    out = call(norm, w, x)
+    assert type(out[0].grad_fn).__name__ == "BlockNormFnBackward"
+    got = torch.autograd.grad(_loss(out), leaves, create_graph=True)
+    again = torch.autograd.grad(sum((v ** 2).sum() for v in got), leaves)
+    monkeypatch.setattr(norms, "_block_kernel", lambda *a: False)
+    out = call(norm, w, x)
+    want = torch.autograd.grad(_loss(out), leaves, create_graph=True)
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b)
+    for a, b in zip(again, torch.autograd.grad(sum((v ** 2).sum() for v in want), leaves)):
+        torch.testing.assert_close(a, b)
+
+
+def test_batched_gradients(node):
+    norm, w, x = _parts()
+    t, _ = rx.block_norm(norm, x, x @ w, post=norm)
+    rows = torch.eye(4, t.numel(), dtype=F64).view(4, *t.shape)
+    got = torch.autograd.grad(t, (x, w, norm.weight), rows, is_grads_batched=True,
+                              retain_graph=True)
+    for i in range(4):
+        for a, b in zip(got, torch.autograd.grad(t, (x, w, norm.weight), rows[i],
+                                                 create_graph=True)):
+            torch.testing.assert_close(a[i], b)
