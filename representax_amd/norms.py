@@ -357,19 +357,60 @@ def _block_expression(x, u, gate, weight, bias, post_weight, post_bias, key, cfg
     """The torch expression of ``block_norm``: what the kernels compute, in
     float32 (float64 for float64 values) with t and h rounded to the values' type."""
 
-    wide = torch.promote_types(x.dtype, F32)
+    update = _update_expression(u, gate, post_weight, post_bias, key, cfg, x.dtype)
+    t = (x.to(update.dtype) + update).to(x.dtype)
+    return t, None if weight is None else _normed_expression(t, weight, bias, cfg)
+
+
+def _update_expression(u, gate, post_weight, post_bias, key, cfg, dtype):
+    """What is added to the stream, in wide values."""
+
+    wide = torch.promote_types(dtype, F32)
     p = u.to(wide)
     if post_weight is not None:
-        p = _expression_norm(cfg["post_kind"], p, post_weight, post_bias, cfg["post_eps"], x.dtype)
+        p = _expression_norm(cfg["post_kind"], p, post_weight, post_bias, cfg["post_eps"], dtype)
     if gate is not None:
         p = gate.to(wide) * p
     if cfg["threshold"] < 65536:
         p = dropped(p, key, cfg["threshold"], cfg["site"])
-    t = (x.to(wide) + cfg["scale"] * p).to(x.dtype)
-    if weight is None:
-        return t, None
-    h = _expression_norm(cfg["kind"], t.to(wide), weight, bias, cfg["eps"], x.dtype)
-    return t, h.to(x.dtype)
+    return cfg["scale"] * p
+
+
+def _normed_expression(t, weight, bias, cfg):
+    wide = torch.promote_types(t.dtype, F32)
+    return _expression_norm(cfg["kind"], t.to(wide), weight, bias, cfg["eps"], t.dtype).to(t.dtype)
+
+
+def _expression_gradients(ctx, inputs, wanted, key, t, dt, dh):
+    """The gradients of ``block_norm`` by torch operations, from t and u as the kernels
+    have them, where they are differentiated themselves (or batched, or traced)."""
+
+    again = torch.is_grad_enabled()
+
+    def gradients(out, places, needs, grad):
+        found = [v for v, need in zip(places, needs) if need]
+        if not found:
+            return [None] * len(places)
+        found = iter(torch.autograd.grad(out, found, grad, create_graph=again))
+        return [next(found) if need else None for need in needs]
+
+    with torch.enable_grad():
+        # views, so that an input's gradient is its own place's alone: not also what
+        # reaches it through another that was made from it, or is the same tensor
+        u, gate, weight, bias, post_weight, post_bias, t = (
+            None if v is None else v.view_as(v) for v in (*inputs, t))
+        if dh is not None:
+            d, dw, db = gradients(_normed_expression(t, weight, bias, ctx.cfg), (t, weight, bias),
+                                  (True, *wanted[3:5]), dh)
+            d = d if dt is None else dt + d
+        else:
+            d = dt
+            dw, db = (torch.zeros_like(v) if need else None
+                      for v, need in zip((weight, bias), wanted[3:5]))
+        update = _update_expression(u, gate, post_weight, post_bias, key, ctx.cfg, t.dtype)
+        du, dg, dpw, dpb = gradients(update, (u, gate, post_weight, post_bias),
+                                     (*wanted[1:3], *wanted[5:7]), d.to(update.dtype))
+    return d if wanted[0] else None, du, dg, dw, db, dpw, dpb
 
 
 def _block_fields(x, u, gate, weight, bias, post_weight, post_bias, key, cfg, like, t, h):
@@ -405,34 +446,24 @@ class BlockNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         t, h = _block_forward(x, u, gate, weight, bias, post_weight, post_bias, key, cfg)
         ctx.cfg = cfg
-        # x is read only where the expressions are differentiated instead
-        ctx.save_for_backward(x, u, gate, weight, bias, post_weight, post_bias, key, t)
+        # not x: t has it, and the kernels do not read it
+        ctx.save_for_backward(u, gate, weight, bias, post_weight, post_bias, key, t)
         return t, h
 
     @staticmethod
     def backward(ctx, dt, dh):
         *inputs, key, t = ctx.saved_tensors
-        x, u, gate, weight, bias, post_weight, post_bias = inputs
+        u, gate, weight, bias, post_weight, post_bias = inputs
         wanted = ctx.needs_input_grad[:7]
         none = (None, None)
         if dt is None and dh is None:
             return (None,) * 9
         if not _kernel_gradients(dt, dh):
-            again = torch.is_grad_enabled()
-            with torch.enable_grad():
-                # views, so that an input's gradient is its own place's alone: not also what
-                # reaches it through another that was made from it, or is the same tensor
-                places = [None if v is None else v.view_as(v) for v in inputs]
-                outs = _block_expression(*places, key, ctx.cfg)
-            pairs = [(o, g) for o, g in zip(outs, (dt, dh)) if g is not None]
-            leaves = [v for v, need in zip(places, wanted) if need]
-            grads = iter(torch.autograd.grad([o for o, _ in pairs], leaves, [g for _, g in pairs],
-                                             create_graph=again, allow_unused=True))
-            return (*(next(grads) if need else None for need in wanted), *none)
+            return (*_expression_gradients(ctx, inputs, wanted, key, t, dt, dh), *none)
         _on_device(dt, dh, u)
         dt = None if dt is None else dt.contiguous()
         dh = None if dh is None else dh.contiguous()
-        outs = [torch.empty_like(v) if need else None for v, need in zip(inputs, wanted)]
+        outs = [torch.empty_like(v) if need else None for v, need in zip((t, *inputs), wanted)]
         fields = _block_fields(None, u, gate, weight, bias, post_weight, post_bias, key, ctx.cfg,
                                u, t, None)
         grads = (_ptr(dt), _ptr(dh), *map(_ptr, outs))

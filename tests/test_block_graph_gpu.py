@@ -53,3 +53,29 @@ def test_gradients_that_keep_their_graph():
             assert float((v.detach().to(F64) - c.detach()).norm() / c.detach().norm()) < 2.0 ** -12
     for a, b in zip(again, want2):
         assert float((a.to(F64) - b).norm() / b.norm()) < 2.0 ** -12
+
+
+def test_the_stream_may_change_after_the_call():
+    norm, w, x = _parts()
+    want = torch.autograd.grad(_loss(rx.block_norm(norm, x * 1, x @ w)), (x, w))
+    value = x * 1
+    out = rx.block_norm(norm, value, x @ w)
+    with torch.no_grad():
+        value.add_(1)
+    for a, b in zip(torch.autograd.grad(_loss(out), (x, w)), want):
+        assert torch.equal(a, b)
+
+
+def test_the_stream_is_not_kept():
+    """Of a boundary the graph keeps t and the update, not the stream before it."""
+
+    norm = rx.RMSNorm(2048, 1e-6, DEV)
+    u = torch.randn(512, 2048, device=DEV, requires_grad=True)
+    value = torch.randn_like(u).requires_grad_(True) * 1
+    t, h = rx.block_norm(norm, value, u)
+    before = torch.cuda.memory_allocated()
+    size = value.numel() * 4
+    del value
+    assert before - torch.cuda.memory_allocated() >= size
+    (t + h).sum().backward()
+    assert u.grad is not None

@@ -72,3 +72,36 @@ def test_batched_gradients(node):
         for a, b in zip(got, torch.autograd.grad(t, (x, w, norm.weight), rows[i],
                                                  create_graph=True)):
             torch.testing.assert_close(a[i], b)
+
+
+@pytest.mark.parametrize("kept", [False, True])
+def test_the_stream_may_change_after_the_call(node, kept):
+    """The backward reads t and the update alone."""
+
+    norm, w, x = _parts()
+    want = torch.autograd.grad(_loss(rx.block_norm(norm, x * 1, x @ w)), (x, w))
+    value = x * 1
+    out = rx.block_norm(norm, value, x @ w)
+    with torch.no_grad():
+        value.add_(1)
+    got = torch.autograd.grad(_loss(out), (x, w), create_graph=kept)
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b)
+
+
+def test_one_output_and_frozen_parts_that_keep_their_graph(node, monkeypatch):
+    norm, w, x = _parts()
+    norm.requires_grad_(False)
+
+    def grads(kernel):
+        monkeypatch.setattr(norms, "_block_kernel", lambda *a: kernel)
+        out = []
+        for pick in (0, 1):
+            t = rx.block_norm(norm, x, torch.sin(x @ w), post=norm)[pick]
+            first = torch.autograd.grad((t ** 3).sum(), (x, w), create_graph=True)
+            out += [*first, *torch.autograd.grad(sum((v ** 2).sum() for v in first), (x, w))]
+        t = rx.block_norm(norm, x.detach(), (x @ w).detach(), gate=w[0])[1]
+        return [*out, *torch.autograd.grad((t ** 3).sum(), w, create_graph=True)]
+
+    for a, b in zip(grads(True), grads(False)):
+        torch.testing.assert_close(a, b)
