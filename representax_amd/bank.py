@@ -27,13 +27,15 @@ from contextvars import ContextVar
 from typing import Iterator, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from .adapters import QuantizedLoRALinear, _set_module
 from .philox import check_key, dropout_threshold
-from .ops import (BF16, F32, _aligned, _as, _check_extent, _dtype_code, _on_device, _ptr, _stream,
-                  _u16, _workspace, cast_many, group_arg, on_current_device)
+from .ops import (BF16, F32, _aligned, _as, _check_extent, _dtype_code, _has_storage, _on_device,
+                  _ptr, _stream, _u16, _workspace, cast_many, eager_calls, group_arg,
+                  on_current_device)
 from .precision import active_compute_dtype, activation_inputs, compute_operands
 from .sharding import constrain_activation
 
@@ -49,6 +51,21 @@ def _on(device: torch.device, t: torch.Tensor):
     """Launches go to the current device: make it the tensors'."""
 
     return _HERE if on_current_device(t) else torch.cuda.device(device)
+
+
+def _check_unwatched(what: str, *tensors: torch.Tensor | None) -> None:
+    """A launch is in no trace, and has no batching rule and no forward derivative: where
+    one of them is asked for, it is refused rather than left out."""
+
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what} cannot be traced")
+    for t in tensors:
+        if t is None:
+            continue
+        if not _has_storage(t):
+            raise RuntimeError(f"{what} takes no tensors of function transforms (vmap, jvp, grad)")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 class AdapterPlan:
@@ -79,6 +96,8 @@ def adapter_plan(index, adapters: int, device=None) -> AdapterPlan:
         index = index.to(torch.int32) if index.numel() == 0 else index
     if index.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"adapter index must be int32 or int64, got {index.dtype}")
+    if not eager_calls():
+        _check_unwatched("adapter_plan", index)
     if index.numel() > MAX_ROWS:
         raise ValueError(f"a plan has at most {MAX_ROWS} rows, got {index.numel()}")
     if not index.is_cuda:
@@ -139,6 +158,8 @@ class BankLinearFn(torch.autograd.Function):
     def backward(ctx, grad):
         x2d, a, b, packed, scale_bits, scalings, plan, key, h = ctx.saved_tensors
         need_x, need_a, need_b = ctx.needs_input_grad[:3]
+        if not eager_calls() or not _has_storage(grad):
+            _check_unwatched("the gradient of bank_linear", grad)
         grad = _aligned(_as(grad, BF16))
         device = _on_device(grad, x2d)
         fields = _bank_fields(x2d, packed, scale_bits, None, a, b, scalings, plan, key, ctx.cfg)
@@ -198,8 +219,11 @@ def bank_linear(x: torch.Tensor, packed: torch.Tensor, scale_bits: torch.Tensor,
 
     bf16 activations; gradients reach x, A and B (once: there is no second
     derivative). Adapters without rows get gradients of zero. One adapter's values
-    never reach another's rows."""
+    never reach another's rows. Traces, function transforms (``torch.func``) and
+    forward-mode derivatives are refused."""
 
+    if not eager_calls():
+        _check_unwatched("bank_linear", x, packed, scale_bits, lora_a, lora_b, scalings, bias, key)
     if x.dtype != BF16:
         raise TypeError(f"bank_linear takes bfloat16 activations, got {x.dtype}")
     if x.dim() < 1:
