@@ -308,6 +308,16 @@ class QuantizedLoRABank(torch.nn.Module):
         self.lora_b = torch.nn.Parameter(lora_b)
         self.dropout, self.site = float(dropout), int(site)
 
+    def _apply(self, fn, recurse: bool = True):
+        """Moves with the module; a cast of its floating-point values is not for
+        ``scalings``, which are no weights (an adapter has a number there)."""
+
+        scalings = self.scalings
+        super()._apply(fn, recurse)
+        if self.scalings.dtype != F32:
+            self.scalings = scalings.to(self.scalings.device)
+        return self
+
     @classmethod
     def from_adapters(cls, adapters: Sequence[QuantizedLoRALinear], *, dropout: float = 0.0,
                       site: int = 0) -> "QuantizedLoRABank":
