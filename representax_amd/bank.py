@@ -36,7 +36,8 @@ from .philox import check_key, dropout_threshold
 from .ops import (BF16, F32, _aligned, _as, _check_extent, _dtype_code, _has_storage, _on_device,
                   _ptr, _stream, _u16, _workspace, cast_many, eager_calls, group_arg,
                   on_current_device)
-from .precision import active_compute_dtype, activation_inputs, compute_operands
+from .precision import (active_compute_dtype, activation_inputs, compute_operands,
+                        compute_parameter_dtype)
 from .sharding import constrain_activation
 
 MAX_ADAPTERS = 1024
@@ -286,7 +287,12 @@ class QuantizedLoRABank(torch.nn.Module):
     """One packed INT4 base projection with several adapters: the leaves of
     ``QuantizedLoRALinear`` with ``lora_a [E, r, K]`` and ``lora_b [E, N, r]``, and
     ``scalings [E]``. Called under ``adapter_rows``. ``dropout`` is the rate on the
-    adapters' input while training, ``site`` the number of its masks in a step."""
+    adapters' input while training, ``site`` the number of its masks in a step.
+
+    It computes in bfloat16, where the linear it stands for has other arithmetic too:
+    float32 activations, and float32 masters without a precision policy (which the
+    linear promotes to float32), are refused, and under an fp8 policy a bank's products
+    stay bfloat16."""
 
     def __init__(self, *, packed_weight: torch.Tensor, scale_bits: torch.Tensor,
                  bias_bits: torch.Tensor | None, lora_a: torch.Tensor, lora_b: torch.Tensor,
@@ -375,6 +381,10 @@ class QuantizedLoRABank(torch.nn.Module):
         value = activation_inputs(value)
         if active_compute_dtype(value.dtype) != BF16:
             raise TypeError("a bank computes in bfloat16: enter a bfloat16 precision policy")
+        if compute_parameter_dtype(self.lora_a) != BF16:
+            raise TypeError("float32 adapters outside a precision policy are promoted to float32, "
+                            "and a bank computes in bfloat16: enter a bfloat16 precision policy, or "
+                            "keep the adapters in bfloat16")
         rate = self.dropout if self.training else 0.0
         a, b = compute_operands(self.lora_a, self.lora_b)
         y = bank_linear(value.to(BF16), self.packed_weight, self.scale_bits, a, b, self.scalings,
@@ -391,7 +401,10 @@ class QuantizedLoRABank(torch.nn.Module):
 def bank_quantized_lora(models: Sequence[torch.nn.Module], *, dropout: float = 0.0):
     """One model with a bank in the place of every ``QuantizedLoRALinear``: adapter i
     of each is that of ``models[i]``. The models have one base; everything else is
-    the first one's. Each bank has a ``site`` of its own."""
+    the first one's. Each bank has a ``site`` of its own. Banks compute in bfloat16
+    (``QuantizedLoRABank``), and each is called by itself: the layers' fused calls
+    (``gelu_mlp``, ``swiglu_mlp``, ``shared_input_projections``) are those of linears
+    with one adapter."""
 
     models = list(models)
     if not models:

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import representax_amd as rx
+from representax_amd import bank as bank_module
 from tests.test_bank_host import _adapter
 
 BF16 = torch.bfloat16
@@ -26,3 +27,38 @@ def test_scalings_stay_float32(cast):
     assert "scalings" in dict(model[0].named_buffers())
     assert torch.equal(model.state_dict()["0.scalings"], want)
     assert model.to("meta")[0].scalings.device.type == "meta"
+
+
+@pytest.fixture
+def taken(monkeypatch):
+    """The types of A that banks call with, in the launch's place."""
+
+    types = []
+
+    def call(x, packed, scale_bits, lora_a, *rest, **options):
+        types.append(lora_a.dtype)
+        return x.new_zeros(*x.shape[:-1], packed.shape[0])
+
+    monkeypatch.setattr(bank_module, "bank_linear", call)
+    return types
+
+
+def test_what_a_bank_computes_in(taken):
+    bank = rx.QuantizedLoRABank.from_adapters([_adapter(0)])
+    plan = rx.AdapterPlan(torch.empty(64, dtype=torch.uint8), 5, 1)
+    x = torch.zeros(5, 64, dtype=BF16)
+    policy = lambda config: rx.precision_context(rx.resolve_precision_policy(config))
+    with rx.adapter_rows(plan):
+        # the linear promotes these to float32
+        with pytest.raises(TypeError, match="promoted to float32"):
+            bank(x)
+        with pytest.raises(TypeError, match="bfloat16"):
+            bank(x.float())
+        with rx.precision_context(rx.FP32_POLICY), pytest.raises(TypeError, match="bfloat16"):
+            bank(x)
+        assert not taken
+        for config in (rx.PrecisionConfig.bfloat16_mixed(), rx.PrecisionConfig.float8_mixed()):
+            with policy(config):
+                assert bank(x).dtype == BF16 and bank(x.float()).dtype == BF16
+        assert bank.to(BF16)(x).dtype == BF16
+    assert taken == [torch.float32] * 4 + [BF16]
