@@ -474,6 +474,11 @@ class BlockNormFn(torch.autograd.Function):
         return (*outs, *none)
 
 
+def _broadcasts(gate, shape) -> bool:
+    return (len(gate) <= len(shape)
+            and all(g in (1, n) for g, n in zip(reversed(gate), reversed(shape))))
+
+
 def _rows_per_gate(gate: torch.Tensor, shape) -> int | None:
     """How many consecutive rows share a row of the gate; None where it does not
     go by leading axes."""
@@ -543,8 +548,7 @@ def block_norm(norm: torch.nn.Module | None, value: torch.Tensor, update: torch.
     if update.shape != shape or not shape:
         raise ValueError(f"update {tuple(update.shape)} must have the shape of value "
                          f"{tuple(value.shape)}")
-    if gate is not None and gate.shape != shape[-1:] and (
-            torch.broadcast_shapes(gate.shape, shape) != shape):
+    if gate is not None and gate.shape != shape[-1:] and not _broadcasts(gate.shape, shape):
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over {tuple(value.shape)}")
     threshold = dropout_threshold(rate)
     if threshold < 65536:

@@ -105,3 +105,23 @@ def test_one_output_and_frozen_parts_that_keep_their_graph(node, monkeypatch):
 
     for a, b in zip(grads(True), grads(False)):
         torch.testing.assert_close(a, b)
+
+
+@pytest.mark.parametrize("gate", [(4, 8), (2, 2, 1, 8), (3,), (0, 8), (2, 8)])
+def test_gates_that_do_not_broadcast_are_refused(gate):
+    x = torch.zeros(2, 3, 8)
+    with pytest.raises(ValueError, match="broadcast"):
+        rx.block_norm(None, x, x, gate=torch.zeros(gate))
+
+
+@pytest.mark.parametrize("gate", [(), (1,), (8,), (3, 1), (2, 1, 8), (1, 3, 8), (2, 3, 8)])
+def test_gates_that_broadcast(gate):
+    x, u = torch.randn(2, 3, 8), torch.randn(2, 3, 8)
+    k = torch.randn(gate)
+    torch.testing.assert_close(rx.block_norm(None, x, u, gate=k)[0], x + k * u)
+
+
+def test_gates_over_empty_rows():
+    x = torch.zeros(0, 3, 8)
+    for gate in ((8,), (1, 1, 8), (0, 1, 8)):
+        assert rx.block_norm(None, x, x, gate=torch.zeros(gate))[0].shape == x.shape
