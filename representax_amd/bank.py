@@ -409,18 +409,26 @@ def bank_quantized_lora(models: Sequence[torch.nn.Module], *, dropout: float = 0
     models = list(models)
     if not models:
         raise ValueError("bank_quantized_lora needs at least one model")
-    paths = [n for n, m in models[0].named_modules() if isinstance(m, QuantizedLoRALinear)]
+    # a module that a model has in several places is in the list under each of them
+    def places(model):
+        return [n for n, m in model.named_modules(remove_duplicate=False)
+                if isinstance(m, QuantizedLoRALinear)]
+
+    paths = places(models[0])
     if not paths:
         raise ValueError("the models have no QuantizedLoRALinear modules")
     for other in models[1:]:
-        if paths != [n for n, m in other.named_modules() if isinstance(m, QuantizedLoRALinear)]:
+        if paths != places(other):
             raise ValueError("the models have their adapters in different places")
     target = copy.deepcopy(models[0])
-    for site, path in enumerate(paths):
-        bank = QuantizedLoRABank.from_adapters([m.get_submodule(path) for m in models],
-                                               dropout=dropout, site=site)
-        bank.train(target.training)
-        target = _set_module(target, path, bank)
+    banks: dict[tuple[int, ...], QuantizedLoRABank] = {}
+    for path in paths:
+        adapters = [m.get_submodule(path) for m in models]
+        key = tuple(map(id, adapters))
+        if key not in banks:
+            banks[key] = QuantizedLoRABank.from_adapters(adapters, dropout=dropout, site=len(banks))
+            banks[key].train(target.training)
+        target = _set_module(target, path, banks[key])
     return target
 
 

@@ -62,3 +62,24 @@ def test_what_a_bank_computes_in(taken):
                 assert bank(x).dtype == BF16 and bank(x.float()).dtype == BF16
         assert bank.to(BF16)(x).dtype == BF16
     assert taken == [torch.float32] * 4 + [BF16]
+
+
+class _Pair(torch.nn.Module):
+    def __init__(self, first, second):
+        super().__init__()
+        self.first, self.inner = first, torch.nn.ModuleList([second])
+
+
+def test_an_adapter_in_two_places_is_one_bank():
+    """Left where it was, the second place would serve every row the first model's adapter."""
+
+    shared = [_adapter(i) for i in range(2)]
+    banked = rx.bank_quantized_lora([_Pair(a, a) for a in shared])
+    assert isinstance(banked.first, rx.QuantizedLoRABank) and banked.inner[0] is banked.first
+    assert [torch.equal(banked.first.lora_a[i], a.lora_a) for i, a in enumerate(shared)] == [True] * 2
+    # one model has it twice, the other two of them: two banks
+    apart = rx.bank_quantized_lora([_Pair(shared[0], shared[0]), _Pair(shared[1], _adapter(5))])
+    assert apart.inner[0] is not apart.first and [apart.first.site, apart.inner[0].site] == [0, 1]
+    assert torch.equal(apart.inner[0].lora_a[1], _adapter(5).lora_a)
+    with pytest.raises(ValueError, match="different places"):
+        rx.bank_quantized_lora([_Pair(shared[0], shared[0]), _Pair(shared[1], torch.nn.GELU())])
