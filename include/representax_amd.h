@@ -124,13 +124,14 @@ int rpx_get_tuning(int knob);
 
 /* Kernels with bounded cross-block waits (the one-launch skinny-M forward)
  * raise a bit in a per-device error word when a wait expires; that call's
- * outputs then hold NaN instead of hanging. This takes the current device's
+ * outputs then hold NaN instead of hanging. A plan raises one for an index
+ * outside its bank. This takes the current device's
  * word with one atomic exchange (queued on `stream`, after the work already
  * there; a bit raised later by another stream's kernel stays for the next
  * check), synchronizes `stream`, and returns RPX_ERR_DEVICE (with a
  * message naming the kernel) if any bit was set; flags_out (host, may be
  * NULL) receives the bits: 1 = skinny M <= 64 adapter arrivals, 2 = skinny
- * M <= 4 adapter partials. Synchronizes, so it must not be called during graph
+ * M <= 4 adapter partials, 4 = adapter index. Synchronizes, so it must not be called during graph
  * capture. No reference counterpart (XLA's kernels have no cross-block waits). */
 int rpx_check_device_errors(void* stream, uint32_t* flags_out);
 
@@ -808,10 +809,12 @@ int rpx_block_backward(const rpx_block* block, const rpx_block_gradients* gradie
  * takes the adapter e = index[i] of a bank of `adapters`, or none where it is -1:
  *   y[i] = x[i] W_b^T + bias + s_e (dropout(x[i]) A_e^T) B_e^T
  * in bf16 with f32 sums (QuantizedLoRALinear.__call__, adapters.py:158-182, for
- * each row with its own adapter; one rounding of y instead of the reference's
- * three). h = dropout(x) A_e^T and its gradient are rounded to bf16 where they
- * are operands of matrix products; up to 64 rows, and up to 256 of few columns,
- * y takes h as f32 sums.
+ * each row with its own adapter; base product, term and bias meet in f32 and y is
+ * rounded once, where the reference rounds three times; dx likewise). h =
+ * dropout(x) A_e^T and its gradient are rounded to bf16 where they are operands of
+ * matrix products. Few rows' y takes h as f32 sums: up to 64 rows, and up to 1024
+ * while n * ceil(m / 64) <= 18432, of k a multiple of 32 and groups that are a power
+ * of two of 32 or more.
  * ------------------------------------------------------------------------- */
 
 /* The rows of a batch sorted by adapter, for every projection that the batch

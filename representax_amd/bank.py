@@ -13,9 +13,9 @@ adapters at once, with the gradients of x, A and B.
 place of the adapters of several models over one base, and ``adapter_rows`` says
 which adapter each row of the calls inside it takes.
 
-The arithmetic is bf16 products with float32 sums and one rounding of y; h and
-its gradient are rounded to bf16 where they are operands of matrix products (for
-few rows, y takes h as float32 sums).
+The arithmetic is bf16 products with float32 sums and one rounding of y and of dx;
+h and its gradient are rounded to bf16 where they are operands of matrix products
+(for few rows, y takes h as float32 sums).
 """
 
 from __future__ import annotations

@@ -284,7 +284,8 @@ class tuning:
 def check_device_errors(device: torch.device | None = None) -> int:
     """Synchronize the current stream and raise ``DeviceError`` if a kernel
     reported an expired bounded wait since the last check (its outputs then
-    hold NaN); returns the raw bits otherwise (0)."""
+    hold NaN), or a plan an adapter's number outside the bank (its row ran
+    without one); returns the raw bits otherwise (0)."""
 
     nat.load()
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import representax_amd as rx
+from representax_amd import ops
 
 pytestmark = pytest.mark.gpu
 DEV, F32, F64 = "cuda:0", torch.float32, torch.float64
@@ -79,3 +80,15 @@ def test_the_stream_is_not_kept():
     assert before - torch.cuda.memory_allocated() >= size
     (t + h).sum().backward()
     assert u.grad is not None
+
+
+def test_workspaces_are_released_and_made_again():
+    norm, w, x = _parts()
+    first = torch.autograd.grad(_loss(_layer(norm, w, x)), (x, w, norm.weight))
+    stream = torch.cuda.current_stream()
+    assert (x.get_device(), stream.cuda_stream) in ops._WORKSPACES
+    stream.synchronize()
+    ops.release_workspaces()
+    assert not ops._WORKSPACES
+    second = torch.autograd.grad(_loss(_layer(norm, w, x)), (x, w, norm.weight))
+    assert ops._WORKSPACES and all(torch.equal(a, b) for a, b in zip(first, second))
