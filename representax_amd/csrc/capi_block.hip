@@ -106,7 +106,7 @@ int rpx_dropout(const void* x, int dtype, int64_t count, const int64_t* key, int
   Dropout d;
   RPX_TRY(check_dropout(key, site, threshold, who, &d));
   if (count == 0) return kOk;
-  if (x == nullptr || out == nullptr || key == nullptr) return fail_invalid(who + ": null pointer");
+  if (x == nullptr || out == nullptr) return fail_invalid(who + ": null pointer");
   if (!aligned16_all({x, out})) return fail_invalid(who + ": pointers must be 16-byte aligned");
   RPX_HIP(launch_dropout(x, dtype, count, d, out, static_cast<hipStream_t>(stream)), "rpx_dropout");
   return kOk;

@@ -19,7 +19,8 @@ __global__ void __launch_bounds__(kThreads)
   const int n = count - first < 8 ? static_cast<int>(count - first) : 8;
   float v[8];
   load_row8<false>(x + first, n, v);
-  dropout8<true>(philox_call(d), d, first, v);
+  // no dropout: there may be no key
+  if (d.threshold < 65536u) dropout8<true>(philox_call(d), d, first, v);
   store_row8<false>(out + first, n, v);
 }
 
