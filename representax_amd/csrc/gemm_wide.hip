@@ -34,7 +34,9 @@
 // (a mask's bits and four adapters' fragments together spilled 69 registers: two then).
 // Ranks 33 to 64 take the fragments' registers in halves, one adapter's at a time (two
 // spilled 74): a whole call of 16384 x 2048 <- 6144 at rank 32 / 64 435 / 460, of
-// 16384 x 6144 <- 2048 421 / 490.
+// 16384 x 6144 <- 2048 421 / 490. With a mask's bits these ranks spill 115 and 123
+// registers, in the epilogue, and are still ahead of k_gemm_nt's tiles: a whole
+// dx of 16384 x 6144 <- 2048, rank 64 530 / 590, of 16384 x 2048 <- 6144 469 / 510.
 // The MFMA sequence of an output (which k go into which MFMA, and the order)
 // is k_gemm_nt's, so the outputs are the same bit for bit.
 #include <atomic>
@@ -681,7 +683,9 @@ hipError_t run_wide_jb(const uint16_t* a, int64_t lda, const uint16_t* b, int64_
     return run_wide_act<BN, WM, WN, 1>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
   if (epi.rank <= 32)
     return run_wide_act<BN, WM, WN, 2>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
-  return run_wide<BN, WM, WN, 4, kActBank>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
+  if (epi.act == kActBank)
+    return run_wide<BN, WM, WN, 4, kActBank>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
+  return run_wide<BN, WM, WN, 4, kActBankDrop>(a, lda, b, ldb, m, n, k, out, ldc, epi, stream);
 }
 
 }  // namespace
@@ -730,8 +734,7 @@ bool wide_gemm_ok(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb
   // epilogue has registers for (48 and 64 would spill), and its loads read whole
   // blocks, so other ranks, also below 16, stay with k_gemm_nt, which pads them.
   // A bank's term is read in pieces of eight ranks, 32 ranks at a time: every
-  // multiple of 8 up to 64, and up to 32 where the epilogue also makes a
-  // dropout's bits (more spilled 120 registers)
+  // multiple of 8 up to 64
   const int64_t lim = int64_t{1} << 32;
   return m > 0 && n > 0 && k > 0 && k % kBK == 0 && lda % 8 == 0 && ldb % 8 == 0 && n % 8 == 0 &&
          ldc % 8 == 0 && (ptrs & 15) == 0 && m * lda * 2 < lim && n * ldb * 2 < lim &&
@@ -739,7 +742,7 @@ bool wide_gemm_ok(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb
          ceil_div(m, 256) * ceil_div(n, 192) < (int64_t{1} << 30) &&
          (epi.rank == 16 || epi.rank == 32 || (epi.rank == 0 && epi.act == kActNone) ||
           ((epi.act == kActBank || epi.act == kActBankDrop) && epi.rank % 8 == 0 &&
-           epi.rank >= 8 && epi.rank <= (epi.act == kActBank ? 64 : 32) &&
+           epi.rank >= 8 && epi.rank <= 64 &&
            epi.adapter_stride % 8 == 0)) &&
          (epi.rank == 0 || (epi.rows_sj == 1 && epi.cols_sj == 1 && epi.rows_sn % 8 == 0 &&
                             epi.cols_sm % 8 == 0 && m * epi.cols_sm * 2 < lim &&
